@@ -14,7 +14,7 @@ from pathlib import Path
 import torch  # noqa: F401  (must be loaded before the library; see module doc)
 
 LIB_PATH = Path(__file__).resolve().parent / "libafterimage_decode.so"
-ABI_VERSION = 11
+ABI_VERSION = 12
 MAX_TENSORS = 32
 
 AIMG_OK = 0
@@ -22,6 +22,9 @@ AIMG_ERR_INVALID_ARGUMENT = 1
 AIMG_ERR_BAD_TABLE = 2
 AIMG_ERR_HIP = 3
 AIMG_ERR_UNSUPPORTED = 4
+
+AIMG_BF16 = 0
+AIMG_FP16 = 1
 
 
 class NativeError(RuntimeError):
@@ -51,6 +54,21 @@ class AimgTensor(ctypes.Structure):
         ("n_chunks", ctypes.c_int32),
     ]
 
+
+class AimgHeads(ctypes.Structure):
+    """Mirror of ``aimg_heads``."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("n_rows", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+    ]
+
+
+_HEADS = ctypes.POINTER(AimgHeads)
 
 _lib = None
 _lock = threading.Lock()
@@ -91,6 +109,9 @@ _SIGNATURES = [
     ("aimg_pack_chunked", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)]),
+    ("aimg_prompt_attention", ctypes.c_int,
+     [_HEADS, _HEADS, _HEADS, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
+      ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]),
 ]
 
 EXPORTED_SYMBOLS = tuple(name for name, _, _ in _SIGNATURES)

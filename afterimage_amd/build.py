@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -60,22 +61,26 @@ def build(verbose: bool = False) -> Path:
     BUILD_DIR.mkdir(exist_ok=True)
     hipcc = _hipcc()
     inc = ["-I", str(INCLUDE), "-I", str(CSRC)]
-    dev_obj = BUILD_DIR / "aimg_decode.o"
+    hip = [(CSRC / f"{name}.hip", BUILD_DIR / f"{name}.o")
+           for name in ("aimg_decode", "aimg_attention")]
     host_obj = BUILD_DIR / "aimg_host.o"
     cpu_obj = BUILD_DIR / "aimg_cpu.o"
     steps = [
-        [hipcc, "-c", *HIP_FLAGS, *inc, str(CSRC / "aimg_decode.hip"), "-o", str(dev_obj)],
+        *([hipcc, "-c", *HIP_FLAGS, *inc, str(src), "-o", str(obj)] for src, obj in hip),
         ["g++", "-c", *HOST_FLAGS, *inc, str(CSRC / "aimg_host.cpp"), "-o", str(host_obj)],
         ["g++", "-c", *HOST_FLAGS, *inc, str(CSRC / "aimg_cpu.cpp"), "-o", str(cpu_obj)],
     ]
     torch_lib = _torch_lib_dir()
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    steps.append(["g++", "-shared", "-pthread", "-o", str(tmp), str(dev_obj), str(host_obj),
-                  str(cpu_obj), f"-L{torch_lib}", "-l:libamdhip64.so", "-Wl,--no-undefined"])
+    steps.append(["g++", "-shared", "-pthread", "-o", str(tmp), *(str(obj) for _, obj in hip),
+                  str(host_obj), str(cpu_obj), f"-L{torch_lib}", "-l:libamdhip64.so", "-Wl,--no-undefined"])
     for cmd in steps:
         if verbose:
             print(" ".join(cmd), flush=True)
-        _run(cmd)
+    # The objects side by side, then the link.
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        list(pool.map(_run, steps[:-1]))
+    _run(steps[-1])
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

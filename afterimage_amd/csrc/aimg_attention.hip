@@ -1,0 +1,563 @@
+// Attention of packed prompts, and of drafted tokens over a paged cache (gfx950).
+//
+// For a query row q with the keys j it sees,
+//   s_j = c q.k_j,  m = max_j s_j,  l = sum_j 2^(s_j - m),  o = sum_j 2^(s_j - m) v_j / l,
+// with c = scale * log2(e), in one pass over the keys: m, l and o are kept in
+// fp32 and o and l are multiplied by 2^(m_old - m_new) where m rises. A row
+// that sees no key gives zeros.
+//
+// Products. Keys are the rows and queries the columns of S^T = K Q^T
+// (v_mfma_f32_32x32x16): a lane then holds 16 of 32 scores of ONE query, so
+// the maximum and the sum are lane sums and one exchange of the wave's halves,
+// and the probabilities are already laid out as the second operand of
+// O^T = V^T P^T. The key order inside a step of 16 is the one S^T leaves them
+// in (the sum over keys does not depend on it); V^T comes out of LDS through
+// the transposing read (ds_read_b64_tr_b16) in that order. No probability
+// passes through LDS or another lane.
+//
+// Rounding. q, k, v enter the products as they are; scores, m, l and o are
+// fp32. Probabilities are rounded once to the inputs' type for the second
+// product (l sums them unrounded), and the result once at the end.
+//
+// Rows of K and V go to LDS with asynchronous 16-byte loads, two tiles in
+// turn; their 16-byte pieces are permuted within a row (by the row's index) so
+// that neither read meets a bank twice.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "afterimage_decode.h"
+#include "aimg_internal.h"
+
+namespace aimg {
+namespace {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
+struct Bf16 {
+    static constexpr uint32_t kInf = 0x7F80u, kOne = 0x3F80u;
+    static __device__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    static __device__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+    }
+};
+
+struct Fp16 {
+    static constexpr uint32_t kInf = 0x7C00u, kOne = 0x3C00u;
+    static __device__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+    }
+};
+
+// A maximum is raised only where it grew by more than this (in powers of
+// two): below it the probabilities stay under 2^8, far inside the range of
+// both types and of the fp32 sums, and o and l need no multiplication.
+constexpr float kRise = 8.0f;
+constexpr float kLog2E = 1.44269504088896340736f;
+constexpr int kMaxDim = 256;
+constexpr int64_t kMaxRowStride = 1 << 24;  // 64 rows stay within 32-bit byte offsets
+
+// Rows of a tile in LDS: row r of kBytes bytes, its 16-byte piece x at place
+// x ^ key_place(r) or x ^ value_place(r).
+// Keys are read 16 bytes a lane, one row a lane: 16 rows (8 of 128 bytes) at
+// one x cover all banks. Values are read by four rows and two neighbouring
+// pieces at a time (four pieces for two groups of lanes): {0,6,10,12} takes
+// pairs to four places of 32 bytes mod 128 and fours to four of 64 mod 256.
+template <int DP>
+struct Rows {
+    static constexpr int kBytes = DP * 2;
+    static constexpr int kPieces = DP / 8;
+    static constexpr int kPerLoad = 64 / kPieces;  // rows of one load of 64 lanes
+    static __device__ int key_place(int r) { return r & (DP == 64 ? 7 : 15); }
+    static __device__ int value_place(int r) {
+        r &= 3;
+        return DP == 64 ? 2 * r : 4 * r ^ 2 * ((r ^ r >> 1) & 1);
+    }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The larger of a lane's value and that of the same query in the wave's other half.
+__device__ __forceinline__ float max_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+__device__ __forceinline__ float add_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+__device__ __forceinline__ void load_to_lds(const void* from, lds_char* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// x where bit `at` of bits is set, -inf otherwise: two instructions, and no lane mask in scalar registers.
+__device__ __forceinline__ float seen_or(uint32_t bits, int at, float x) {
+    const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), at, 1));
+    return __uint_as_float((__float_as_uint(x) & all) | (0xFF800000u & ~all));
+}
+
+// Waits until at most kLeft of the wave's vector memory loads are in flight.
+template <int kLeft>
+__device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt((kLeft & 15) | (kLeft >> 4) << 14 | 0x0F70);
+    asm volatile("" ::: "memory");
+}
+
+// One wave's softmax state and output of QT tiles of 32 queries.
+template <typename T, int DP, int QT>
+struct State {
+    static constexpr int kSteps = DP / 16;   // steps of the first product
+    static constexpr int kBlocks = DP / 32;  // blocks of output columns
+    s16x8 q[QT][kSteps];
+    f32x16 o[QT][kBlocks];
+    float m[QT], l[QT];
+
+    __device__ void clear() {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) o[t][d] = f32x16{0};
+        }
+    }
+
+    // A lane's query row (dim elements, the rest zero), in the layout of the second operand.
+    __device__ void load_query(int t, const uint16_t* row, int dim, int half) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const int x = 8 * (2 * k + half);
+            const s16x8 v = *reinterpret_cast<const s16x8*>(row + (x < dim ? x : 0));
+            q[t][k] = x < dim ? v : s16x8{0};
+        }
+    }
+
+    // The next 32 * NSUB keys, their rows at `keys` and `values` in LDS.
+    // kMasked: allow[t][u] has bit r set where the lane's query of tile t sees
+    // key 32 u + r; every key is seen otherwise.
+    template <int NSUB, bool kMasked>
+    __device__ __forceinline__ void step(const lds_char* keys, const lds_char* values, float c, int lane,
+                                         const uint32_t (&allow)[QT][NSUB]) {
+        typedef Rows<DP> R;
+        const int half = lane >> 5;
+        f32x16 s[QT][NSUB];
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u) {
+            const int r = lane & 31;
+            const lds_char* const row = keys + (32 * u + r) * R::kBytes;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const s16x8 a = *reinterpret_cast<const __attribute__((address_space(3))) s16x8*>(
+                    row + (((2 * k + half) ^ R::key_place(r)) << 4));
+#pragma unroll
+                for (int t = 0; t < QT; ++t) s[t][u] = T::mfma(a, q[t][k], k == 0 ? f32x16{0} : s[t][u]);
+            }
+        }
+        s16x8 p[QT][NSUB][2];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            if (kMasked) {
+#pragma unroll
+                for (int u = 0; u < NSUB; ++u) {
+                    const uint32_t bits = allow[t][u] >> (4 * half);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[t][u][i] = seen_or(bits, 8 * (i / 4) + i % 4, s[t][u][i]);
+                }
+            }
+            float top = s[t][0][0];
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][u][i]);
+            top = max_halves(top);
+            const bool rise = (top - m[t]) * c > kRise;  // false where both are -inf
+            if (__any(rise)) {
+                const float to = rise ? top : m[t];
+                const float by = rise ? exp2_fast((m[t] - to) * c) : 1.0f;
+                m[t] = to;
+                l[t] *= by;
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[t][d][i] *= by;
+            }
+            const float mc = m[t] == -INFINITY ? 0.0f : m[t] * c;
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < NSUB; ++u) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[t][u][i] = exp2_fast(fmaf(s[t][u][i], c, -mc));
+                    sum += s[t][u][i];
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    u32x4 w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = T::pack(s[t][u][8 * k + 2 * i], s[t][u][8 * k + 2 * i + 1]);
+                    p[t][u][k] = __builtin_bit_cast(s16x8, w);
+                }
+            }
+            l[t] += sum;
+        }
+        const int r = (lane & 15) >> 2;
+        const lds_char* const first = values + (4 * half + r) * R::kBytes + (lane & 1) * 8;
+        const int piece = (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
+        uint32_t odd = 0;
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int d = 0; d < kBlocks; ++d) {
+                    s16x8 a = value(first, piece, r, u, k, d);
+                    if (kMasked) a = finite(a, odd);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) o[t][d] = T::mfma(a, p[t][u][k], o[t][d]);
+                }
+        if (kMasked && __any(odd != 0)) add_infinite<NSUB>(first, piece, r, half, allow);
+    }
+
+    // V^T of keys 32 u + 16 k + {0..3, 8..11} (+ 4 in the upper half) and block d of columns.
+    __device__ __forceinline__ s16x8 value(const lds_char* first, int piece, int r, int u, int k, int d) {
+        typedef Rows<DP> R;
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        lds_char* const at = const_cast<lds_char*>(first) + (32 * u + 16 * k) * R::kBytes + (((4 * d + piece) ^ R::value_place(r)) << 4);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 8 * R::kBytes));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+
+    // A masked key has probability 0, but 0 * inf is not 0: infinities and
+    // NaNs of V leave the product where keys are masked...
+    static __device__ __forceinline__ s16x8 finite(s16x8 a, uint32_t& odd) {
+        u32x4 w = __builtin_bit_cast(u32x4, a);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // Adding the exponent's lowest bit to it carries into the sign's place where all its bits are set.
+            const uint32_t x = ((w[i] & T::kInf * 0x10001u) + (T::kInf & (0u - T::kInf)) * 0x10001u) & 0x80008000u;
+            odd |= x;
+            w[i] &= ~((x - (x >> 15)) | x);
+        }
+        return __builtin_bit_cast(s16x8, w);
+    }
+
+    // ...and come back for the queries that see them: a product of ones counts
+    // the visible keys with +inf or NaN, and one those with -inf or NaN.
+    template <int NSUB>
+    __device__ __forceinline__ void add_infinite(const lds_char* first, int piece, int r, int half, const uint32_t (&allow)[QT][NSUB]) {
+        for (int sign = 0; sign < 2; ++sign) {
+#pragma unroll
+            for (int d = 0; d < kBlocks; ++d) {
+                f32x16 n[QT];
+#pragma unroll
+                for (int t = 0; t < QT; ++t) n[t] = f32x16{0};
+#pragma unroll
+                for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const s16x8 v = value(first, piece, r, u, k, d);
+                        s16x8 a;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t x = static_cast<uint16_t>(v[i]);
+                            const bool nan = (x & 0x7FFFu) > T::kInf;
+                            a[i] = nan || x == (T::kInf | (sign ? 0x8000u : 0u)) ? static_cast<short>(T::kOne) : 0;
+                        }
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) {
+                            s16x8 b;
+                            const uint32_t bits = allow[t][u] >> (4 * half + 16 * k);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) b[i] = (bits >> (8 * (i / 4) + i % 4)) & 1u ? static_cast<short>(T::kOne) : 0;
+                            n[t] = T::mfma(a, b, n[t]);
+                        }
+                    }
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[t][d][i] += n[t][i] > 0.0f ? (sign ? -INFINITY : INFINITY) : 0.0f;
+            }
+        }
+    }
+};
+
+// Bits 0..31 of the keys k0.. that a row sees which sees keys 0..end-1.
+__device__ __forceinline__ uint32_t first_bits(int32_t n) {
+    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
+// One lane's columns 8 * (i / 4) + 4 * half + i % 4 of block d, written as four elements at a time.
+template <typename T>
+__device__ __forceinline__ void store_four(uint16_t* to, float a, float b, float c, float d) {
+    uint2 w;
+    w.x = T::pack(a, b);
+    w.y = T::pack(c, d);
+    *reinterpret_cast<uint2*>(to) = w;
+}
+
+// --------------------------------------------------------------------------
+// Packed prompts.
+// --------------------------------------------------------------------------
+
+struct PromptArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    float* lse;
+    const int32_t *q_offsets, *k_offsets;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // strides in elements
+    int32_t n_seqs, heads, kv_heads, dim, n_q, n_k, n_slots;
+    float c, scale;
+};
+
+__device__ __forceinline__ int32_t bounded(int32_t x, int32_t most) { return x < 0 ? 0 : x > most ? most : x; }
+
+constexpr int kPromptKeys = 64;
+
+// Workgroup: one head, 32 * QT * NW query rows of one sequence, four or more
+// waves that share the tiles of K and V.
+// Slots: sequence b's tiles of rows start at slot offset[b] / rows + b, a place
+// that needs no sums over the sequences before it; slots past a sequence's
+// rows are empty. Later slots, whose rows see more keys, start first.
+template <typename T, int DP, int QT, int NW>
+__global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_kernel(const PromptArgs A) {
+    typedef Rows<DP> R;
+    constexpr int KT = DP <= 128 ? kPromptKeys : 32;
+    constexpr int NSUB = KT / 32;
+    constexpr int BM = 32 * QT * NW;
+    constexpr int kTile = KT * R::kBytes;            // bytes of a tile of K, and of V
+    constexpr int kLoads = kTile / 1024 / NW;        // loads a wave makes of either
+    __shared__ __attribute__((aligned(1024))) char lds[4 * kTile];
+    lds_char* const shared = (lds_char*)lds;
+
+    const int hid = blockIdx.x % A.heads;
+    const int slot = A.n_slots - 1 - static_cast<int>(blockIdx.x / A.heads);
+    // Consecutive workgroups take the key/value heads in turn: with eight of
+    // them an XCD keeps to one head, whose keys and values stay in its L2.
+    const int kvh = hid % A.kv_heads;
+    const int head = kvh * (A.heads / A.kv_heads) + hid / A.kv_heads;
+    int lo = 0, hi = A.n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (bounded(A.q_offsets[mid], A.n_q) / BM + mid <= slot) lo = mid; else hi = mid - 1;
+    }
+    const int q_begin = bounded(A.q_offsets[lo], A.n_q), q_end = bounded(A.q_offsets[lo + 1], A.n_q);
+    const int k_begin = bounded(A.k_offsets[lo], A.n_k), k_end = bounded(A.k_offsets[lo + 1], A.n_k);
+    const int q_len = q_end - q_begin, k_len = k_end > k_begin ? k_end - k_begin : 0;
+    const int row0 = (slot - (q_begin / BM + lo)) * BM;
+    if (row0 < 0 || row0 >= q_len) return;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = lane >> 5;
+    const int shift = k_len - q_len;  // row i sees keys 0 .. i + shift
+    const int wave_row = row0 + wave * 32 * QT;
+
+    State<T, DP, QT> st;
+    st.clear();
+    int32_t sees[QT];  // keys that the lane's rows see
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = wave_row + 32 * t + (lane & 31);
+        const int at = row < q_len ? row : q_len - 1;
+        st.load_query(t, A.q + (q_begin + at) * A.q_row + head * A.q_head, A.dim, half);
+        const int n = at + 1 + shift;
+        sees[t] = n < 0 ? 0 : n;
+    }
+    const int wg_last = row0 + BM < q_len ? row0 + BM : q_len;
+    const int keys_wg = wg_last + shift < 0 ? 0 : wg_last + shift;  // keys that some row here sees
+    const int wave_last = wave_row + 32 * QT < q_len ? wave_row + 32 * QT : q_len;
+    const int keys_wave = wave_row >= q_len || wave_last + shift < 0 ? 0 : wave_last + shift;
+
+    const uint16_t* const k_base = A.k + k_begin * A.k_row + kvh * A.k_head;
+    const uint16_t* const v_base = A.v + k_begin * A.v_row + kvh * A.v_head;
+    const int pieces = A.dim / 8 - 1;  // the last 16-byte piece of a row; pieces past it repeat it
+    const int lane_row = lane / R::kPieces, lane_piece = lane % R::kPieces;
+    const uint32_t k_bytes = static_cast<uint32_t>(2 * A.k_row), v_bytes = static_cast<uint32_t>(2 * A.v_row);
+    auto load_tile = [&](int k0, lds_char* to) {
+        // Rows past the last key repeat it; no row sees them.
+        const int last = k_len - 1 - k0;
+        const bool whole = last >= KT - 1;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int load = wave * kLoads + i;
+            const int r0 = load * R::kPerLoad, r = r0 + lane_row;
+            const int kx = lane_piece ^ R::key_place(r), vx = lane_piece ^ R::value_place(r);
+            const uint32_t kp = (kx < pieces ? kx : pieces) * 16, vp = (vx < pieces ? vx : pieces) * 16;
+            const int from0 = whole ? r0 : 0;
+            const uint32_t from = whole ? lane_row : (r < last ? r : last);
+            const char* const kb = reinterpret_cast<const char*>(k_base + (k0 + from0) * A.k_row);
+            const char* const vb = reinterpret_cast<const char*>(v_base + (k0 + from0) * A.v_row);
+            load_to_lds(kb + (from * k_bytes + kp), to + load * 1024);
+            load_to_lds(vb + (from * v_bytes + vp), to + kTile + load * 1024);
+        }
+    };
+    if (keys_wg > 0) load_tile(0, shared);
+    wait_loads<0>();
+    __syncthreads();
+    int k0 = 0;
+    uint32_t at = 0;  // the tile's place in LDS
+    // Tiles that every row of the workgroup sees whole, then those it needs
+    // masks for. The two places are passed as restrict pointers: the compiler
+    // then knows that reads of a tile need not wait for the loads of the next.
+    for (; k0 + KT <= row0 + 1 + shift; k0 += KT, at ^= 2 * kTile) {
+        auto tile = [&](lds_char* __restrict__ next, const lds_char* __restrict__ now) __attribute__((always_inline)) {
+            if (k0 + KT < keys_wg) load_tile(k0 + KT, next);
+            const uint32_t all[QT][NSUB] = {};
+            st.template step<NSUB, false>(now, now + kTile, A.c, lane, all);
+        };
+        tile(shared + (at ^ 2 * kTile), shared + at);
+        wait_loads<0>();
+        __syncthreads();
+    }
+    for (; k0 < keys_wg; k0 += KT, at ^= 2 * kTile) {
+        auto tile = [&](lds_char* __restrict__ next, const lds_char* __restrict__ now) __attribute__((always_inline)) {
+            if (k0 + KT < keys_wg) load_tile(k0 + KT, next);
+            if (k0 < keys_wave) {
+                uint32_t allow[QT][NSUB];
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int u = 0; u < NSUB; ++u) allow[t][u] = first_bits(sees[t] - k0 - 32 * u);
+                st.template step<NSUB, true>(now, now + kTile, A.c, lane, allow);
+            }
+        };
+        tile(shared + (at ^ 2 * kTile), shared + at);
+        wait_loads<0>();
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int row = wave_row + 32 * t + (lane & 31);
+        const float l = add_halves(st.l[t]);
+        if (row >= q_len) continue;
+        const float by = l == 0.0f ? 0.0f : 1.0f / l;
+        uint16_t* const to = A.out + (q_begin + row) * A.out_row + head * A.out_head;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int x = 32 * d + 8 * i + 4 * half;
+                const f32x16& o = st.o[t][d];
+                if (x < A.dim) store_four<T>(to + x, o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
+            }
+        if (A.lse != nullptr && half == 0)
+            A.lse[static_cast<int64_t>(q_begin + row) * A.heads + head] = l == 0.0f ? -INFINITY : st.m[t] * A.scale + logf(l);
+    }
+}
+
+template <typename T, int DP>
+int launch_prompt(PromptArgs& A, hipStream_t s) {
+    constexpr int QT = 1, NW = 4, BM = 32 * QT * NW;
+    A.n_slots = A.n_q / BM + A.n_seqs;
+    const int64_t groups = static_cast<int64_t>(A.n_slots) * A.heads;
+    if (groups > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "prompt attention: too many rows times heads");
+    hipLaunchKernelGGL((prompt_kernel<T, DP, QT, NW>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess)
+        return fail(AIMG_ERR_HIP, std::string("kernel launch failed: ") + hipGetErrorString(err));
+    return AIMG_OK;
+}
+
+}  // namespace
+}  // namespace aimg
+
+namespace {
+
+// The checks every attention shares: type, element counts, strides that keep
+// 16-byte pieces aligned.
+int check_heads(const aimg_heads* x, const char* name, bool written = false) {
+    using aimg::fail;
+    const std::string n(name);
+    if (x == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, n + " is null");
+    if (x->n_rows < 0 || x->n_rows > INT32_MAX || x->heads < 1 || x->dim < 1)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, n + ": n_rows must be in 0..2^31-1, heads and dim at least 1");
+    if (x->dim % 8 != 0 || x->dim > aimg::kMaxDim)
+        return fail(AIMG_ERR_UNSUPPORTED, n + ": dim must be a multiple of 8 up to " + std::to_string(aimg::kMaxDim) + ", got " + std::to_string(x->dim));
+    if (x->n_rows == 0) return AIMG_OK;
+    if (x->data == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, n + ": null data");
+    if (x->row_stride < 0 || x->head_stride < 0 || (!written && x->row_stride > aimg::kMaxRowStride))
+        return fail(AIMG_ERR_UNSUPPORTED, n + ": strides must not be negative, a row's at most 2^24 elements");
+    const int64_t unit = written ? 4 : 8;
+    if (reinterpret_cast<uintptr_t>(x->data) % (2 * unit) != 0 || x->row_stride % unit != 0 || x->head_stride % unit != 0)
+        return fail(AIMG_ERR_UNSUPPORTED, n + ": needs a " + std::to_string(2 * unit) + "-byte aligned pointer and strides of whole " +
+                                              std::to_string(2 * unit) + " bytes");
+    return AIMG_OK;
+}
+
+template <typename Launch>
+int by_type(int type, int dim, Launch launch) {
+    if (type == AIMG_BF16) return launch(aimg::Bf16{}, dim);
+    if (type == AIMG_FP16) return launch(aimg::Fp16{}, dim);
+    return aimg::fail(AIMG_ERR_UNSUPPORTED, "type must be AIMG_BF16 or AIMG_FP16, got " + std::to_string(type));
+}
+
+int check_scale(float scale) {
+    if (!(scale > 0.0f) || std::isinf(scale)) return aimg::fail(AIMG_ERR_INVALID_ARGUMENT, "scale must be a positive number");
+    return AIMG_OK;
+}
+
+}  // namespace
+
+extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, const aimg_heads* v, const aimg_heads* out,
+                                     const int32_t* q_offsets, const int32_t* k_offsets, int n_seqs, int type,
+                                     float scale, float* lse, void* stream) {
+    using aimg::fail;
+    int rc = check_heads(q, "q");
+    if (rc == AIMG_OK) rc = check_heads(k, "k");
+    if (rc == AIMG_OK) rc = check_heads(v, "v");
+    if (rc == AIMG_OK) rc = check_heads(out, "out", true);
+    if (rc == AIMG_OK) rc = check_scale(scale);
+    if (rc != AIMG_OK) return rc;
+    if (k->n_rows != v->n_rows || k->heads != v->heads || k->dim != q->dim || v->dim != q->dim)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "k and v must have the same rows and heads, and q's dim");
+    if (out->n_rows != q->n_rows || out->heads != q->heads || out->dim != q->dim)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "out must have q's shape");
+    if (q->heads % k->heads != 0)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "q's heads must be a multiple of k's");
+    if (n_seqs < 0) return fail(AIMG_ERR_INVALID_ARGUMENT, "n_seqs must be >= 0");
+    if (n_seqs == 0 || q->n_rows == 0) return AIMG_OK;
+    if (q_offsets == nullptr || k_offsets == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "null offsets");
+    aimg::PromptArgs a{};
+    a.q = static_cast<const uint16_t*>(q->data);
+    a.k = static_cast<const uint16_t*>(k->data);
+    a.v = static_cast<const uint16_t*>(v->data);
+    a.out = static_cast<uint16_t*>(out->data);
+    a.lse = lse;
+    a.q_offsets = q_offsets;
+    a.k_offsets = k_offsets;
+    a.q_row = q->row_stride, a.q_head = q->head_stride;
+    a.k_row = k->row_stride, a.k_head = k->head_stride;
+    a.v_row = v->row_stride, a.v_head = v->head_stride;
+    a.out_row = out->row_stride, a.out_head = out->head_stride;
+    a.n_seqs = n_seqs, a.heads = q->heads, a.kv_heads = k->heads, a.dim = q->dim;
+    a.n_q = static_cast<int32_t>(q->n_rows), a.n_k = static_cast<int32_t>(k->n_rows);
+    a.c = scale * aimg::kLog2E, a.scale = scale;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return by_type(type, q->dim, [&](auto t, int dim) {
+        typedef decltype(t) T;
+        if (dim <= 64) return aimg::launch_prompt<T, 64>(a, s);
+        if (dim <= 128) return aimg::launch_prompt<T, 128>(a, s);
+        return aimg::launch_prompt<T, 256>(a, s);
+    });
+}

@@ -262,6 +262,44 @@ int aimg_pack_chunked(const uint8_t* symbols, int64_t n, const uint32_t* code_of
                       const uint8_t* len_of, int32_t chunk_size, uint8_t* out,
                       int64_t out_cap, int32_t* chunk_nbytes, int64_t* total);
 
+/* ------------------------------------------------------------------------- */
+/* Attention.                                                                */
+/* The products between the projections of a decoder layer and its output    */
+/* projection (the reference leaves them to the model's own forward pass).   */
+/* Elements are bf16 or fp16; scores, softmax statistics and sums are fp32.  */
+/* ------------------------------------------------------------------------- */
+
+#define AIMG_BF16 0
+#define AIMG_FP16 1
+
+/* Rows of heads: element (row, head, x) is data[row * row_stride + head *
+ * head_stride + x], strides in elements. dim is a multiple of 8 up to 256.
+ * Inputs need 16-byte aligned data and strides of whole 16 bytes, outputs 8. */
+typedef struct aimg_heads {
+    void* data;          /* device                                    */
+    int64_t n_rows;
+    int64_t row_stride;
+    int64_t head_stride;
+    int32_t heads;
+    int32_t dim;
+} aimg_heads;
+
+/*
+ * Causal attention of n_seqs packed prompts: rows q_offsets[b] ..
+ * q_offsets[b+1] - 1 of q (int32[n_seqs + 1], device) attend over rows
+ * k_offsets[b] .. of k and v. The last query row sees every key, the one
+ * before it all but the last, and so on (a prompt that continues a context
+ * has more keys than rows); a row that sees no key gives zeros. Head h of q
+ * reads head h / (q->heads / k->heads) of k and v.
+ * out has q's shape; rows outside every sequence are not written. lse: NULL,
+ * or float[q->n_rows][q->heads] (device) for log(sum(exp(scale * q.k))), -inf
+ * for a row that sees no key. scale > 0. Offsets outside the rows are bounded
+ * to them; keys that a row does not see never reach it, whatever they hold.
+ */
+int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, const aimg_heads* v, const aimg_heads* out,
+                          const int32_t* q_offsets, const int32_t* k_offsets, int n_seqs, int type,
+                          float scale, float* lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
