@@ -68,7 +68,51 @@ class AimgHeads(ctypes.Structure):
     ]
 
 
+class AimgPages(ctypes.Structure):
+    """Mirror of ``aimg_pages``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("slot_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("table_stride", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("max_seqs", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
+class AimgCache(ctypes.Structure):
+    """Mirror of ``aimg_cache``."""
+
+    _fields_ = [
+        ("pool", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("held", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("n_layers", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("dim", ctypes.c_int32),
+        ("max_seqs", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
 _HEADS = ctypes.POINTER(AimgHeads)
+_CACHE = ctypes.POINTER(AimgCache)
+_SIZE = ctypes.POINTER(ctypes.c_size_t)
+_PAGES = ctypes.POINTER(AimgPages)
 
 _lib = None
 _lock = threading.Lock()
@@ -112,6 +156,31 @@ _SIGNATURES = [
     ("aimg_prompt_attention", ctypes.c_int,
      [_HEADS, _HEADS, _HEADS, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
       ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]),
+    ("aimg_tree_workspace_nbytes", ctypes.c_int,
+     [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
+      ctypes.POINTER(ctypes.c_size_t)]),
+    ("aimg_tree_attention", ctypes.c_int,
+     [_HEADS, _PAGES, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
+      ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+      ctypes.c_void_p]),
+    ("aimg_tree_masks", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
+    ("aimg_cache_append", ctypes.c_int,
+     [_CACHE, ctypes.c_int, _HEADS, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    ("aimg_cache_advance", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    ("aimg_cache_reserve", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    ("aimg_cache_release", ctypes.c_int, [_CACHE, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    ("aimg_cache_fork_workspace_nbytes", ctypes.c_int, [_CACHE, ctypes.c_int, _SIZE]),
+    ("aimg_cache_fork", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    ("aimg_cache_commit", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+      ctypes.c_void_p]),
+    ("aimg_cache_compact_workspace_nbytes", ctypes.c_int, [_CACHE, _SIZE]),
+    ("aimg_cache_compact", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
 ]
 
 EXPORTED_SYMBOLS = tuple(name for name, _, _ in _SIGNATURES)

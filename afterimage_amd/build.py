@@ -33,6 +33,11 @@ HIP_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
+# Accumulators of the matrix instructions stay in ordinary vector registers
+# where they fit, for the softmax between the two products works on them (kernels
+# of one workgroup a CU were given the other half of the file, and moved 64
+# registers to and fro in every step).
+ATTENTION_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 HOST_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-Wall", "-pthread"]
 
 
@@ -61,18 +66,18 @@ def build(verbose: bool = False) -> Path:
     BUILD_DIR.mkdir(exist_ok=True)
     hipcc = _hipcc()
     inc = ["-I", str(INCLUDE), "-I", str(CSRC)]
-    hip = [(CSRC / f"{name}.hip", BUILD_DIR / f"{name}.o")
-           for name in ("aimg_decode", "aimg_attention")]
+    hip = [(CSRC / f"{name}.hip", BUILD_DIR / f"{name}.o", flags)
+           for name, flags in (("aimg_decode", []), ("aimg_attention", ATTENTION_FLAGS), ("aimg_cache", []))]
     host_obj = BUILD_DIR / "aimg_host.o"
     cpu_obj = BUILD_DIR / "aimg_cpu.o"
     steps = [
-        *([hipcc, "-c", *HIP_FLAGS, *inc, str(src), "-o", str(obj)] for src, obj in hip),
+        *([hipcc, "-c", *HIP_FLAGS, *flags, *inc, str(src), "-o", str(obj)] for src, obj, flags in hip),
         ["g++", "-c", *HOST_FLAGS, *inc, str(CSRC / "aimg_host.cpp"), "-o", str(host_obj)],
         ["g++", "-c", *HOST_FLAGS, *inc, str(CSRC / "aimg_cpu.cpp"), "-o", str(cpu_obj)],
     ]
     torch_lib = _torch_lib_dir()
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    steps.append(["g++", "-shared", "-pthread", "-o", str(tmp), *(str(obj) for _, obj in hip),
+    steps.append(["g++", "-shared", "-pthread", "-o", str(tmp), *(str(obj) for _, obj, _ in hip),
                   str(host_obj), str(cpu_obj), f"-L{torch_lib}", "-l:libamdhip64.so", "-Wl,--no-undefined"])
     for cmd in steps:
         if verbose:

@@ -27,6 +27,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "afterimage_decode.h"
 #include "aimg_internal.h"
@@ -479,6 +480,424 @@ int launch_prompt(PromptArgs& A, hipStream_t s) {
     return AIMG_OK;
 }
 
+// --------------------------------------------------------------------------
+// Drafted tokens over a paged cache.
+// --------------------------------------------------------------------------
+
+struct TreeArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    float* lse;
+    const int32_t *table, *lengths, *seqs, *offsets;
+    const uint64_t* masks;
+    float* part_o;    // [split][row * heads + head][DP]
+    float2* part_ml;  // [split][row * heads + head]: c * maximum, sum
+    int64_t q_row, q_head, out_row, out_head, page_stride, slot_stride, kv_head_stride;  // in elements
+    int32_t table_stride, max_pages, n_slots, n_pages, page_size, n_seqs, heads, kv_heads, dim, n_q, words;
+    int32_t max_drafts, chunk, n_splits, row_blocks;
+    uint32_t magic;   // 2^32 / page_size, for divisions by it
+    float c, scale;
+};
+
+// key / page_size and key % page_size. The product is off by less than one
+// either way (key below 2^31, magic at most 1 below or above 2^32 / page_size).
+__device__ __forceinline__ void page_of(const TreeArgs& A, int32_t key, int32_t& page, int32_t& slot) {
+    int32_t p = static_cast<int32_t>(__umulhi(static_cast<uint32_t>(key), A.magic));
+    int32_t r = key - p * A.page_size;
+    if (r < 0) --p, r += A.page_size;
+    if (r >= A.page_size) ++p, r -= A.page_size;
+    page = p, slot = r;
+}
+
+// A sequence of the call: its drafted rows and the positions it holds. What
+// the arrays say is bounded to the buffers.
+struct Drafted {
+    int32_t row, n, context, end;  // first row of q, drafted tokens, positions before and with them
+    const int32_t* pages;
+};
+
+__device__ __forceinline__ Drafted drafted(const TreeArgs& A, int b) {
+    Drafted d;
+    d.row = bounded(A.offsets[b], A.n_q);
+    const int32_t last = bounded(A.offsets[b + 1], A.n_q);
+    d.n = bounded(last - d.row, A.max_drafts);
+    const int32_t slot = A.seqs[b];
+    const bool known = slot >= 0 && slot < A.n_slots;
+    const int64_t most = static_cast<int64_t>(A.max_pages) * A.page_size;
+    if (d.n > most) d.n = static_cast<int32_t>(most);
+    d.context = known ? bounded(A.lengths[slot], static_cast<int32_t>(most - d.n)) : 0;
+    d.end = known ? d.context + d.n : 0;
+    d.pages = A.table + static_cast<int64_t>(known ? slot : 0) * A.table_stride;
+    return d;
+}
+
+// Bits of the keys k0 .. k0 + 31 that drafted token t (row of q: row) sees.
+__device__ __forceinline__ uint32_t seen_keys(const TreeArgs& A, const Drafted& D, int row, int t, int k0) {
+    const int32_t j = k0 - D.context;  // drafted index of the first key, negative: so many keys of context
+    if (j <= -32) return ~0u;
+    const int32_t at = j < 0 ? 0 : j;
+    uint32_t bits;
+    if (A.masks == nullptr) {
+        bits = first_bits(t + 1 - at);
+    } else {
+        const int32_t w = at >> 6, sh = at & 63;
+        const uint64_t* const m = A.masks + static_cast<int64_t>(row) * A.words;
+        uint64_t v = w < A.words ? m[w] >> sh : 0;
+        if (sh > 32 && w + 1 < A.words) v |= m[w + 1] << (64 - sh);
+        bits = static_cast<uint32_t>(v) & first_bits(D.n - at);
+    }
+    return j < 0 ? bits << -j | first_bits(-j) : bits;
+}
+
+// One call's rows of a (sequence, key/value head): drafted token t and head g
+// of the group are row t * group + g, so a key and value are read once for all
+// of them. kShared: NW waves with 32 * QT rows each share tiles of K and V.
+// Otherwise the waves hold the same 32 * QT rows and take tiles in turn, each
+// into its own part of LDS with no barrier in the loop, and join their sums at
+// the end: one token's group (5 rows of 32 here) leaves the matrix cores idle,
+// but the bytes in flight, not the products, bound it.
+// kWhole: a tile never crosses a page, so it has one base address.
+template <typename T, int DP, int QT, int NW, bool kShared, bool kWhole>
+__global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_kernel(const TreeArgs A) {
+    typedef Rows<DP> R;
+    constexpr int KT = kShared && DP <= 128 ? 64 : 32;
+    constexpr int NSUB = KT / 32;
+    constexpr int kTile = KT * R::kBytes;
+    constexpr int kLoads = kTile / 1024 / (kShared ? NW : 1);  // loads a wave makes of K, and of V
+    constexpr int BM = 32 * QT * (kShared ? NW : 1);
+    constexpr int kRow = DP + 4;  // floats of a row of sums in LDS: 16 bytes more than a multiple of all banks
+    constexpr int kSums = kShared ? 0 : NW * 32 * QT * (kRow * 4 + 8);
+    constexpr int kTiles = 4 * kTile * (kShared ? 1 : NW);
+    __shared__ __attribute__((aligned(1024))) char lds[kTiles > kSums ? kTiles : kSums];
+
+    const int group = A.heads / A.kv_heads;
+    int id = blockIdx.x;
+    const int kvh = id % A.kv_heads;
+    id /= A.kv_heads;
+    const int split = id % A.n_splits;
+    id /= A.n_splits;
+    const int block = id % A.row_blocks, b = id / A.row_blocks;
+    const Drafted D = drafted(A, b);
+    const int rows = D.n * group;
+    if (block * BM >= rows) return;
+    const int lo = split * A.chunk;
+    // The last part takes what a sequence holds beyond the longest one planned for.
+    const int hi = split == A.n_splits - 1 || D.end - lo < A.chunk ? D.end : lo + A.chunk;
+    if (split > 0 && lo >= hi) return;  // the join knows how many parts a sequence has
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = lane >> 5;
+    lds_char* const mine = (lds_char*)lds + (kShared ? 0 : wave * 4 * kTile);
+
+    State<T, DP, QT> st;
+    st.clear();
+    int token[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        int r = block * BM + (kShared ? wave * 32 * QT : 0) + 32 * t + (lane & 31);
+        r = r < rows ? r : rows - 1;
+        token[t] = r / group;
+        st.load_query(t, A.q + (D.row + token[t]) * A.q_row + (kvh * group + r % group) * A.q_head, A.dim, half);
+    }
+
+    const int pieces = A.dim / 8 - 1;
+    const int lane_row = lane / R::kPieces, lane_piece = lane % R::kPieces;
+    const uint32_t row_bytes = static_cast<uint32_t>(2 * A.slot_stride);
+    const int64_t head_at = kvh * A.kv_head_stride;
+    const int load0 = kShared ? wave * kLoads : 0;
+    // A lane holds the number of page `first_page` + lane of the sequence, for
+    // 64 pages at a time: a tile's page numbers then come out of a register,
+    // and no load of the loop waits for another.
+    int32_t first_page = 0, held = 0;
+    auto hold = [&](int32_t page) __attribute__((always_inline)) {
+        first_page = page;
+        const int32_t at = page + lane < A.max_pages ? page + lane : A.max_pages - 1;
+        const int32_t id = D.pages[at];
+        held = static_cast<uint32_t>(id) < static_cast<uint32_t>(A.n_pages) ? id : 0;
+    };
+    // Keys past the last one repeat it; no row sees them.
+    auto issue = [&](int k0, lds_char* to) __attribute__((always_inline)) {
+        const int last = D.end - 1 - k0 < KT - 1 ? D.end - 1 - k0 : KT - 1;
+        int32_t page, first, page_end, unused;
+        page_of(A, k0, page, first);
+        page_of(A, k0 + last, page_end, unused);
+        if (page_end >= first_page + 64) hold(page);
+        int64_t tile_at = 0;
+        if (kWhole)
+            tile_at = 2 * (__builtin_amdgcn_readlane(held, page - first_page) * A.page_stride + first * A.slot_stride + head_at);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int load = load0 + i;
+            const int r = load * R::kPerLoad + lane_row;
+            const int kx = lane_piece ^ R::key_place(r), vx = lane_piece ^ R::value_place(r);
+            const uint32_t kp = (kx < pieces ? kx : pieces) * 16, vp = (vx < pieces ? vx : pieces) * 16;
+            const int from = r < last ? r : last;
+            if (kWhole) {
+                load_to_lds(reinterpret_cast<const char*>(A.k) + tile_at + (from * row_bytes + kp), to + load * 1024);
+                load_to_lds(reinterpret_cast<const char*>(A.v) + tile_at + (from * row_bytes + vp), to + kTile + load * 1024);
+            } else {
+                int32_t p, slot;
+                page_of(A, k0 + from, p, slot);
+                const int64_t id = __builtin_amdgcn_ds_bpermute(4 * (p - first_page), held);
+                const int64_t at = 2 * (id * A.page_stride + slot * A.slot_stride + head_at);
+                load_to_lds(reinterpret_cast<const char*>(A.k) + at + kp, to + load * 1024);
+                load_to_lds(reinterpret_cast<const char*>(A.v) + at + vp, to + kTile + load * 1024);
+            }
+        }
+    };
+
+    constexpr int kStep = kShared ? KT : KT * NW;
+    int k0 = lo + (kShared ? 0 : wave * KT);
+    uint32_t at = 0;
+    if (k0 < hi) {
+        int32_t page, unused;
+        page_of(A, k0, page, unused);
+        hold(page);
+        issue(k0, mine);
+    }
+    if (kShared) {
+        wait_loads<0>();
+        __syncthreads();
+    }
+    // Two tiles in turn.
+    auto tile = [&](auto masked, lds_char* __restrict__ next, const lds_char* __restrict__ now) __attribute__((always_inline)) {
+        constexpr bool kMasked = decltype(masked)::value;
+        const bool more = k0 + kStep < hi;
+        if (more) issue(k0 + kStep, next);
+        if (!kShared) {
+            // All but the 2 * kLoads loads just issued, the next tile's, have
+            // arrived. The tile's reads take their place from the wait, so
+            // that none can move before it.
+            uint32_t zero = 0;
+            if (more) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(zero) : "n"(2 * kLoads) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" : "+v"(zero) : : "memory");
+            now += zero;
+        }
+        uint32_t allow[QT][NSUB] = {};
+        if (kMasked) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int u = 0; u < NSUB; ++u) allow[t][u] = seen_keys(A, D, D.row + token[t], token[t], k0 + 32 * u);
+        }
+        st.template step<NSUB, kMasked>(now, now + kTile, A.c, lane, allow);
+    };
+    for (; k0 + KT <= D.context && k0 < hi; k0 += kStep, at ^= 2 * kTile) {
+        tile(std::integral_constant<bool, false>{}, mine + (at ^ 2 * kTile), mine + at);
+        if (kShared) {
+            wait_loads<0>();
+            __syncthreads();
+        }
+    }
+    for (; k0 < hi; k0 += kStep, at ^= 2 * kTile) {
+        tile(std::integral_constant<bool, true>{}, mine + (at ^ 2 * kTile), mine + at);
+        if (kShared) {
+            wait_loads<0>();
+            __syncthreads();
+        }
+    }
+
+    const int64_t part = static_cast<int64_t>(split) * A.n_q * A.heads;
+    if (kShared) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int r = block * BM + wave * 32 * QT + 32 * t + (lane & 31);
+            const float l = add_halves(st.l[t]);
+            if (r >= rows) continue;
+            const int row = D.row + token[t], head = kvh * group + r % group;
+            const int64_t rh = static_cast<int64_t>(row) * A.heads + head;
+            const float by = A.n_splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            uint16_t* const to = A.out + row * A.out_row + head * A.out_head;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int x = 32 * d + 8 * i + 4 * half;
+                    const f32x16& o = st.o[t][d];
+                    if (A.n_splits > 1)
+                        *reinterpret_cast<float4*>(A.part_o + (part + rh) * DP + x) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    else if (x < A.dim)
+                        store_four<T>(to + x, o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
+                }
+            if (half == 0) {
+                if (A.n_splits > 1) A.part_ml[part + rh] = make_float2(st.m[t] * A.c, l);
+                else if (A.lse != nullptr) A.lse[rh] = l == 0.0f ? -INFINITY : st.m[t] * A.scale + logf(l);
+            }
+        }
+        return;
+    }
+
+    // The waves' sums, joined in LDS.
+    __syncthreads();
+    float* const sums = reinterpret_cast<float*>(lds);                       // [wave][row][kRow]
+    float2* const ml = reinterpret_cast<float2*>(sums + NW * 32 * QT * kRow);  // [wave][row]
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int r = wave * 32 * QT + 32 * t + (lane & 31);
+        const float l = add_halves(st.l[t]);
+        if (half == 0) ml[r] = make_float2(st.m[t] * A.c, l);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x16& o = st.o[t][d];
+                *reinterpret_cast<float4*>(sums + r * kRow + 32 * d + 8 * i + 4 * half) =
+                    make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            }
+    }
+    __syncthreads();
+    const int here = rows - block * BM < BM ? rows - block * BM : BM;
+    for (int i = threadIdx.x; i < here * (DP / 4); i += 64 * NW) {
+        const int r = i / (DP / 4), x = i % (DP / 4) * 4;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w * 32 * QT + r].x);
+        float l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float2 one = ml[w * 32 * QT + r];
+            if (one.x == -INFINITY) continue;  // a wave without a visible key
+            const float by = exp2_fast(one.x - top);
+            const float4 v = *reinterpret_cast<const float4*>(sums + (w * 32 * QT + r) * kRow + x);
+            l += one.y * by;
+            o.x += v.x * by, o.y += v.y * by, o.z += v.z * by, o.w += v.w * by;
+        }
+        const int row = D.row + (block * BM + r) / group, head = kvh * group + (block * BM + r) % group;
+        const int64_t rh = static_cast<int64_t>(row) * A.heads + head;
+        if (A.n_splits > 1) {
+            *reinterpret_cast<float4*>(A.part_o + (part + rh) * DP + x) = o;
+            if (x == 0) A.part_ml[part + rh] = make_float2(top, l);
+        } else {
+            const float by = l == 0.0f ? 0.0f : 1.0f / l;
+            if (x < A.dim) store_four<T>(A.out + row * A.out_row + head * A.out_head + x, o.x * by, o.y * by, o.z * by, o.w * by);
+            if (x == 0 && A.lse != nullptr) A.lse[rh] = l == 0.0f ? -INFINITY : top * (1.0f / kLog2E) + logf(l);
+        }
+    }
+}
+
+// The parts of each row joined in their order: a wave a row and head.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
+    const int64_t rh = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int64_t all = static_cast<int64_t>(A.n_q) * A.heads;
+    if (rh >= all) return;
+    const int row = static_cast<int>(rh / A.heads), head = static_cast<int>(rh % A.heads);
+    int lo = 0, hi = A.n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (bounded(A.offsets[mid], A.n_q) <= row) lo = mid; else hi = mid - 1;
+    }
+    const Drafted D = drafted(A, lo);
+    if (row < D.row || row >= D.row + D.n) return;
+    int parts = D.end > 0 ? (D.end - 1) / A.chunk + 1 : 1;
+    parts = parts < A.n_splits ? parts : A.n_splits;
+    constexpr int kEach = DP / 64;
+    float top = -INFINITY;
+    for (int s = lane; s < parts; s += 64) top = fmaxf(top, A.part_ml[s * all + rh].x);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    float l = 0.0f, o[kEach] = {};
+    for (int s0 = 0; s0 < parts; s0 += 64) {
+        const int s = s0 + lane;
+        float2 one = make_float2(-INFINITY, 0.0f);
+        if (s < parts) one = A.part_ml[s * all + rh];
+        const float by = one.x == -INFINITY ? 0.0f : exp2_fast(one.x - top);
+        float sum = one.y * by;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
+        l += sum;
+        const int n = parts - s0 < 64 ? parts - s0 : 64;
+        for (int i = 0; i < n; ++i) {
+            const float w = __shfl(by, i);
+            const float* const from = A.part_o + ((s0 + i) * all + rh) * DP + lane * kEach;
+#pragma unroll
+            for (int x = 0; x < kEach; ++x) o[x] += w == 0.0f ? 0.0f : from[x] * w;
+        }
+    }
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* const to = A.out + row * A.out_row + head * A.out_head;
+#pragma unroll
+    for (int x = 0; x < kEach; ++x)
+        if (lane * kEach + x < A.dim) to[lane * kEach + x] = static_cast<uint16_t>(T::pack(o[x] * by, 0.0f));
+    if (lane == 0 && A.lse != nullptr) A.lse[rh] = l == 0.0f ? -INFINITY : top * (1.0f / kLog2E) + logf(l);
+}
+
+// Ancestor bits of drafted tokens: token t's parent is an earlier drafted
+// token of its sequence, or any other number where it follows the context.
+__global__ __launch_bounds__(256) void tree_masks_kernel(const int32_t* parents, const int32_t* offsets, int n_seqs, int n, int words,
+                                                         uint64_t* masks) {
+    const int row = blockIdx.x * 256 + threadIdx.x;
+    if (row >= n) return;
+    int lo = 0, hi = n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (bounded(offsets[mid], n) <= row) lo = mid; else hi = mid - 1;
+    }
+    const int first = bounded(offsets[lo], n);
+    for (int w = 0; w < words; ++w) {
+        uint64_t bits = 0;
+        // Parents come before their children, so the walk goes down.
+        for (int t = row - first; t >= 0;) {
+            if (t >> 6 == w) bits |= uint64_t{1} << (t & 63);
+            const int up = parents[first + t];
+            t = up < t ? up : -1;
+        }
+        masks[static_cast<int64_t>(row) * words + w] = bits;
+    }
+}
+
+constexpr int kMinChunk = 128;   // keys of a part: a tile for each of four waves
+constexpr int kMaxChunk = 2048;
+constexpr int kPartsWanted = 2048;  // workgroups over which a call's keys are spread
+
+// Rows of a workgroup. Up to 32 or 64 rows of a (sequence, head) go to every
+// wave and the keys are dealt out to the waves; more rows are dealt out.
+int tree_rows(int dim, int64_t rows) { return rows <= 32 ? 32 : rows <= 64 && dim <= 128 ? 64 : 128; }
+
+// Keys of a part and how many parts the longest sequence has.
+void plan_parts(TreeArgs& A, int64_t max_context) {
+    const int64_t rows = static_cast<int64_t>(A.max_drafts) * (A.heads / A.kv_heads);
+    const int per = tree_rows(A.dim, rows);
+    A.row_blocks = static_cast<int32_t>((rows + per - 1) / per);
+    const int64_t longest = max_context + A.max_drafts;
+    const int64_t units = static_cast<int64_t>(A.n_seqs) * A.kv_heads * A.row_blocks;
+    int64_t chunk = longest * units / kPartsWanted;
+    chunk = (chunk + kMinChunk - 1) / kMinChunk * kMinChunk;
+    chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
+    A.chunk = static_cast<int32_t>(chunk);
+    A.n_splits = static_cast<int32_t>((longest + chunk - 1) / chunk);
+}
+
+int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+template <typename T, int DP, int QT, int NW, bool kShared>
+int launch_tree_as(TreeArgs& A, hipStream_t s) {
+    const int64_t groups = static_cast<int64_t>(A.n_seqs) * A.kv_heads * A.row_blocks * A.n_splits;
+    if (groups > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and keys");
+    constexpr int KT = kShared && DP <= 128 ? 64 : 32;
+    if (A.page_size % KT == 0)
+        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, true>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
+    else
+        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, false>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
+    if (A.n_splits > 1)
+        hipLaunchKernelGGL((tree_join_kernel<T, DP>), dim3(static_cast<uint32_t>((static_cast<int64_t>(A.n_q) * A.heads + 3) / 4)), dim3(256), 0, s, A);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess)
+        return fail(AIMG_ERR_HIP, std::string("kernel launch failed: ") + hipGetErrorString(err));
+    return AIMG_OK;
+}
+
+template <typename T, int DP>
+int launch_tree(TreeArgs& A, hipStream_t s) {
+    const int per = tree_rows(A.dim, static_cast<int64_t>(A.max_drafts) * (A.heads / A.kv_heads));
+    if (per == 32) return launch_tree_as<T, DP, 1, DP == 256 ? 2 : 4, false>(A, s);
+    if constexpr (DP < 256)
+        if (per == 64) return launch_tree_as<T, DP, 2, 4, false>(A, s);
+    return launch_tree_as<T, DP, 1, 4, true>(A, s);
+}
+
 }  // namespace
 }  // namespace aimg
 
@@ -502,6 +921,24 @@ int check_heads(const aimg_heads* x, const char* name, bool written = false) {
     if (reinterpret_cast<uintptr_t>(x->data) % (2 * unit) != 0 || x->row_stride % unit != 0 || x->head_stride % unit != 0)
         return fail(AIMG_ERR_UNSUPPORTED, n + ": needs a " + std::to_string(2 * unit) + "-byte aligned pointer and strides of whole " +
                                               std::to_string(2 * unit) + " bytes");
+    return AIMG_OK;
+}
+
+int check_pages(const aimg_pages* p) {
+    using aimg::fail;
+    if (p == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "pages is null");
+    if (p->n_pages < 1 || p->page_size < 1 || p->kv_heads < 1 || p->dim < 1 || p->max_seqs < 1 || p->max_pages < 1)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "pages: every size must be at least 1");
+    if (static_cast<int64_t>(p->max_pages) * p->page_size > INT32_MAX / 2)
+        return fail(AIMG_ERR_UNSUPPORTED, "pages: a sequence must hold fewer than 2^30 positions");
+    if (p->dim % 8 != 0 || p->dim > aimg::kMaxDim)
+        return fail(AIMG_ERR_UNSUPPORTED, "pages: dim must be a multiple of 8 up to " + std::to_string(aimg::kMaxDim));
+    if (p->k == nullptr || p->v == nullptr || p->page_table == nullptr || p->lengths == nullptr)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "pages: null pointer");
+    if ((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) % 16 != 0 || p->page_stride % 8 != 0 ||
+        p->slot_stride % 8 != 0 || p->head_stride % 8 != 0 || p->page_stride < 0 || p->head_stride < 0 || p->slot_stride < 0 ||
+        p->slot_stride > aimg::kMaxRowStride || p->table_stride < 0)
+        return fail(AIMG_ERR_UNSUPPORTED, "pages: needs 16-byte aligned pointers and strides of whole 16 bytes, a position's at most 2^24 elements");
     return AIMG_OK;
 }
 
@@ -560,4 +997,99 @@ extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, c
         if (dim <= 128) return aimg::launch_prompt<T, 128>(a, s);
         return aimg::launch_prompt<T, 256>(a, s);
     });
+}
+
+namespace {
+
+// What the sizes of one tree attention call imply; false where they are no such call.
+bool tree_sizes(aimg::TreeArgs& a, int n_seqs, int heads, int kv_heads, int dim, int max_drafts, int64_t max_context) {
+    if (n_seqs < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dim < 1 || max_drafts < 1 || max_context < 0 ||
+        max_context > INT32_MAX)
+        return false;
+    a.n_seqs = n_seqs, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.max_drafts = max_drafts;
+    aimg::plan_parts(a, max_context);
+    return true;
+}
+
+}  // namespace
+
+extern "C" int aimg_tree_workspace_nbytes(int64_t n_rows, int heads, int kv_heads, int dim, int n_seqs, int max_drafts,
+                                          int64_t max_context, size_t* nbytes) {
+    using aimg::fail;
+    if (nbytes == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "nbytes is null");
+    aimg::TreeArgs a{};
+    if (n_rows < 0 || n_rows > INT32_MAX || !tree_sizes(a, n_seqs, heads, kv_heads, dim, max_drafts, max_context) || dim > aimg::kMaxDim)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "tree attention: rows, heads, dim, n_seqs, max_drafts and max_context must be sizes of one call");
+    const int64_t rows = n_rows * heads * a.n_splits;
+    *nbytes = a.n_splits > 1 ? static_cast<size_t>(rows) * (4 * aimg::padded_dim(dim) + 8) : 0;
+    return AIMG_OK;
+}
+
+extern "C" int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_heads* out, const int32_t* seqs,
+                                   const int32_t* draft_offsets, int n_seqs, const int64_t* masks, int mask_words, int max_drafts,
+                                   int64_t max_context, int type, float scale, float* lse, void* workspace,
+                                   size_t workspace_nbytes, void* stream) {
+    using aimg::fail;
+    int rc = check_heads(q, "q");
+    if (rc == AIMG_OK) rc = check_heads(out, "out", true);
+    if (rc == AIMG_OK) rc = check_pages(pages);
+    if (rc == AIMG_OK) rc = check_scale(scale);
+    if (rc != AIMG_OK) return rc;
+    if (out->n_rows != q->n_rows || out->heads != q->heads || out->dim != q->dim)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "out must have q's shape");
+    if (q->dim != pages->dim || q->heads % pages->kv_heads != 0)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "q must have the pages' dim and a multiple of their heads");
+    aimg::TreeArgs a{};
+    if (!tree_sizes(a, n_seqs, q->heads, pages->kv_heads, q->dim, max_drafts, max_context))
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "n_seqs and max_context must be >= 0 (max_context below 2^31) and max_drafts >= 1");
+    if (masks != nullptr && mask_words < 1) return fail(AIMG_ERR_INVALID_ARGUMENT, "mask_words must be >= 1");
+    if (n_seqs == 0 || q->n_rows == 0) return AIMG_OK;
+    if (seqs == nullptr || draft_offsets == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "null seqs or draft_offsets");
+    const int64_t part_rows = q->n_rows * q->heads * a.n_splits;
+    const int dp = aimg::padded_dim(q->dim);
+    if (a.n_splits > 1 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+                           workspace_nbytes < static_cast<size_t>(part_rows) * (4 * dp + 8)))
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "the workspace is null, misaligned or below aimg_tree_workspace_nbytes");
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows * dp);
+    a.q = static_cast<const uint16_t*>(q->data);
+    a.k = static_cast<const uint16_t*>(pages->k);
+    a.v = static_cast<const uint16_t*>(pages->v);
+    a.out = static_cast<uint16_t*>(out->data);
+    a.lse = lse;
+    a.table = pages->page_table, a.lengths = pages->lengths, a.seqs = seqs, a.offsets = draft_offsets;
+    a.masks = reinterpret_cast<const uint64_t*>(masks);
+    a.words = mask_words;
+    a.q_row = q->row_stride, a.q_head = q->head_stride;
+    a.out_row = out->row_stride, a.out_head = out->head_stride;
+    a.page_stride = pages->page_stride, a.slot_stride = pages->slot_stride, a.kv_head_stride = pages->head_stride;
+    a.table_stride = pages->table_stride, a.max_pages = pages->max_pages, a.n_slots = pages->max_seqs;
+    a.n_pages = pages->n_pages, a.page_size = pages->page_size;
+    a.n_q = static_cast<int32_t>(q->n_rows);
+    a.magic = pages->page_size == 1 ? 0xFFFFFFFFu : static_cast<uint32_t>((uint64_t{1} << 32) / pages->page_size);
+    a.c = scale * aimg::kLog2E, a.scale = scale;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return by_type(type, q->dim, [&](auto t, int dim) {
+        typedef decltype(t) T;
+        if (dim <= 64) return aimg::launch_tree<T, 64>(a, s);
+        if (dim <= 128) return aimg::launch_tree<T, 128>(a, s);
+        return aimg::launch_tree<T, 256>(a, s);
+    });
+}
+
+extern "C" int aimg_tree_masks(const int32_t* parents, const int32_t* draft_offsets, int n_seqs, int64_t n_rows, int mask_words,
+                               int64_t* masks, void* stream) {
+    using aimg::fail;
+    if (n_seqs < 0 || n_rows < 0 || n_rows > INT32_MAX || mask_words < 1)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "n_seqs and n_rows must be >= 0 (n_rows below 2^31) and mask_words >= 1");
+    if (n_seqs == 0 || n_rows == 0) return AIMG_OK;
+    if (parents == nullptr || draft_offsets == nullptr || masks == nullptr)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "null pointer passed to aimg_tree_masks");
+    hipLaunchKernelGGL(aimg::tree_masks_kernel, dim3(static_cast<uint32_t>((n_rows + 255) / 256)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), parents, draft_offsets, n_seqs, static_cast<int>(n_rows), mask_words,
+                       reinterpret_cast<uint64_t*>(masks));
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess)
+        return fail(AIMG_ERR_HIP, std::string("kernel launch failed: ") + hipGetErrorString(err));
+    return AIMG_OK;
 }

@@ -300,6 +300,145 @@ int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, const aimg_h
                           const int32_t* q_offsets, const int32_t* k_offsets, int n_seqs, int type,
                           float scale, float* lse, void* stream);
 
+/* The keys and values of one layer in a paged cache: position j of sequence
+ * slot s is row j % page_size of page page_table[s * table_stride + j /
+ * page_size]; element x of head h there is k[page * page_stride + row *
+ * slot_stride + h * head_stride + x], and v's likewise (strides in elements,
+ * whole 16 bytes, the same for both). lengths[s] positions are held before the
+ * drafted ones. Page numbers outside 0..n_pages-1 read page 0. */
+typedef struct aimg_pages {
+    void* k;                      /* device */
+    void* v;                      /* device */
+    const int32_t* page_table;    /* device: [max_seqs][table_stride] */
+    const int32_t* lengths;       /* device: [max_seqs] */
+    int64_t page_stride;
+    int64_t slot_stride;
+    int64_t head_stride;
+    int32_t table_stride;
+    int32_t n_pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t dim;
+    int32_t max_seqs;
+    int32_t max_pages;            /* of a sequence (<= table_stride) */
+} aimg_pages;
+
+/*
+ * Attention of drafted tokens over a paged cache: the verification forward
+ * pass of a drafted tree, and plain decoding with one token a sequence. Rows
+ * draft_offsets[b] .. draft_offsets[b+1] - 1 of q (int32[n_seqs + 1], device;
+ * at most max_drafts rows each) are the drafted tokens of slot seqs[b]. Their
+ * keys and values are in the cache at positions lengths[slot], lengths[slot] +
+ * 1, ... Token t sees the positions before those, and drafted token j where
+ * bit j % 64 of masks[row * mask_words + j / 64] is set (masks NULL: the
+ * tokens up to itself). A row that sees nothing gives zeros; so do the rows of
+ * a slot outside 0..max_seqs-1.
+ * max_context: the longest lengths[slot] the caller expects; it only decides
+ * how the work is split. aimg_tree_workspace_nbytes gives the device scratch
+ * memory a call needs (16-byte aligned; 0: none), its contents mean nothing
+ * before or after. Parts are joined in their order: results do not vary
+ * between calls. lse: NULL or float[q->n_rows][q->heads], as above.
+ */
+int aimg_tree_workspace_nbytes(int64_t n_rows, int heads, int kv_heads, int dim, int n_seqs, int max_drafts,
+                               int64_t max_context, size_t* nbytes);
+int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_heads* out, const int32_t* seqs,
+                        const int32_t* draft_offsets, int n_seqs, const int64_t* masks, int mask_words, int max_drafts,
+                        int64_t max_context, int type, float scale, float* lse, void* workspace,
+                        size_t workspace_nbytes, void* stream);
+
+/*
+ * masks[row * mask_words + w] for n_rows drafted tokens from their parents:
+ * parents[row] is the index, within its sequence, of an earlier drafted token,
+ * and any other number for a token that follows the context directly. The bits
+ * are the token's own and its ancestors'.
+ */
+int aimg_tree_masks(const int32_t* parents, const int32_t* draft_offsets, int n_seqs, int64_t n_rows, int mask_words,
+                    int64_t* masks, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Pages of a key/value cache.                                               */
+/* The pool holds every layer's keys and values, [n_layers][2][n_pages]      */
+/* [kv_heads][page_size][dim] in elements of two bytes. Slot s of max_seqs   */
+/* holds held[s] pages, page_table[s][0 .. held[s]-1], for lengths[s]        */
+/* positions and those to come; refs[p] sequences hold page p, none a free   */
+/* one. All of it is device memory and every call works there, on `stream`.  */
+/* Positions at or past a length lie in pages that only their sequence holds: */
+/* fork shares full pages alone. A call names a slot once.                   */
+/* What a call finds wrong on the GPU it leaves undone and says in *status   */
+/* (bits, or-ed in): 1 no free pages (nothing was reserved or forked), 2 a   */
+/* sequence's row of the table or its pages end before the positions asked   */
+/* for, 4 a slot, page or source that does not exist.                        */
+/* ------------------------------------------------------------------------- */
+
+#define AIMG_CACHE_NO_PAGES 1
+#define AIMG_CACHE_ROW_FULL 2
+#define AIMG_CACHE_BAD_INDEX 4
+
+typedef struct aimg_cache {
+    void* pool;           /* 16-byte aligned; dim a multiple of 8 */
+    int32_t* page_table;  /* [max_seqs][max_pages] */
+    int32_t* lengths;     /* [max_seqs] */
+    int32_t* held;        /* [max_seqs] */
+    int32_t* refs;        /* [n_pages] */
+    int32_t* status;      /* [1] */
+    int32_t n_layers;
+    int32_t n_pages;
+    int32_t kv_heads;
+    int32_t page_size;
+    int32_t dim;
+    int32_t max_seqs;
+    int32_t max_pages;
+} aimg_cache;
+
+/* Writes rows offsets[b] .. offsets[b+1] - 1 of k and v into slot seqs[b]'s
+ * pages of one layer, from its length on. Lengths do not change. */
+int aimg_cache_append(const aimg_cache* cache, int layer, const aimg_heads* k, const aimg_heads* v, const int32_t* seqs,
+                      const int32_t* offsets, int n_seqs, void* stream);
+
+/* Adds offsets[b+1] - offsets[b] to slot seqs[b]'s length: the rows that every layer has appended. */
+int aimg_cache_advance(const aimg_cache* cache, const int32_t* seqs, const int32_t* offsets, int n_seqs, void* stream);
+
+/* Pages for tokens[b] positions past slot seqs[b]'s length, for all sequences
+ * or none: the lowest free pages, in the order of the call. At most 8192
+ * sequences a call, here and below. */
+int aimg_cache_reserve(const aimg_cache* cache, const int32_t* seqs, const int32_t* tokens, int n_seqs, void* stream);
+
+/* Empties the slots: their references go, pages without any are free. */
+int aimg_cache_release(const aimg_cache* cache, const int32_t* seqs, int n_seqs, void* stream);
+
+/*
+ * Slot dst[i] becomes a branch of slot src[i], whatever it held before, for
+ * all pairs at once (a source may be another pair's branch; src[i] == dst[i]
+ * stays as it is): it shares the source's full pages, and the rows of its last
+ * one, in every layer, are copied to a free page, the lowest ones in the
+ * order of the call. Pages that branches gave up are free after the call.
+ * Nothing changes where free pages are too few. Pages reserved past the
+ * source's length are not passed on.
+ */
+int aimg_cache_fork_workspace_nbytes(const aimg_cache* cache, int n_seqs, size_t* nbytes);
+int aimg_cache_fork(const aimg_cache* cache, const int32_t* src, const int32_t* dst, int n_seqs, void* workspace,
+                    size_t workspace_nbytes, void* stream);
+
+/*
+ * Keeps the accepted tokens of verified trees: rows lengths[slot] +
+ * accepted[b * max_accepted + i] of every layer become rows lengths[slot] + i,
+ * i < counts[b] <= max_accepted. Accepted indices rise (a path from the root,
+ * parents before children). new_lengths[slot] = lengths[slot] + counts[b]; it
+ * may be cache->lengths, and is written for the call's slots only.
+ */
+int aimg_cache_commit(const aimg_cache* cache, const int32_t* seqs, const int32_t* accepted, int max_accepted,
+                      const int32_t* counts, int n_seqs, int32_t* new_lengths, void* stream);
+
+/*
+ * Moves pages so that the *used pages in use are 0 .. *used - 1: the i-th one
+ * at or past *used goes to the i-th free one before it, in every layer.
+ * new_table and new_refs (which may be the cache's own) get the page table and
+ * the counts after the moves. The pages moved from keep their bytes.
+ */
+int aimg_cache_compact_workspace_nbytes(const aimg_cache* cache, size_t* nbytes);
+int aimg_cache_compact(const aimg_cache* cache, int32_t* new_table, int32_t* new_refs, int32_t* used, void* workspace,
+                       size_t workspace_nbytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
