@@ -646,6 +646,8 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         }
     };
 
+    // A wave whose rows are past the last only loads.
+    const bool active = !kShared || block * BM + wave * 32 * QT < rows;
     constexpr int kStep = kShared ? KT : KT * NW;
     int k0 = lo + (kShared ? 0 : wave * KT);
     uint32_t at = 0;
@@ -673,6 +675,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
             else asm volatile("s_waitcnt vmcnt(0)" : "+v"(zero) : : "memory");
             now += zero;
         }
+        if (!active) return;
         uint32_t allow[QT][NSUB] = {};
         if (kMasked) {
 #pragma unroll
@@ -776,13 +779,16 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
     }
 }
 
-// The parts of each row joined in their order: a wave a row and head.
+// The parts of a row and head joined in a fixed order: threads of DP / 4 hold a
+// row's columns, four each, and take parts in turn (eight at a time of 128
+// columns: with one row's thread after the other, a token over 32,000 positions
+// spent 100 of 145 us here); their sums meet in LDS.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
-    const int64_t rh = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int64_t all = static_cast<int64_t>(A.n_q) * A.heads;
-    if (rh >= all) return;
+    constexpr int kCols = DP / 4, kSides = 256 / kCols;
+    __shared__ float4 sums[kSides][kCols];
+    __shared__ float sides_l[kSides];
+    const int64_t rh = blockIdx.x, all = static_cast<int64_t>(A.n_q) * A.heads;
     const int row = static_cast<int>(rh / A.heads), head = static_cast<int>(rh % A.heads);
     int lo = 0, hi = A.n_seqs - 1;
     while (lo < hi) {
@@ -793,35 +799,46 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
     if (row < D.row || row >= D.row + D.n) return;
     int parts = D.end > 0 ? (D.end - 1) / A.chunk + 1 : 1;
     parts = parts < A.n_splits ? parts : A.n_splits;
-    constexpr int kEach = DP / 64;
+    const int lane = threadIdx.x & 63;
     float top = -INFINITY;
     for (int s = lane; s < parts; s += 64) top = fmaxf(top, A.part_ml[s * all + rh].x);
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-    float l = 0.0f, o[kEach] = {};
-    for (int s0 = 0; s0 < parts; s0 += 64) {
-        const int s = s0 + lane;
-        float2 one = make_float2(-INFINITY, 0.0f);
-        if (s < parts) one = A.part_ml[s * all + rh];
-        const float by = one.x == -INFINITY ? 0.0f : exp2_fast(one.x - top);
-        float sum = one.y * by;
+    const int side = threadIdx.x / kCols, col = threadIdx.x % kCols;
+    float l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = side; s0 < parts; s0 += 4 * kSides) {
+        float2 ml[4];
+        float4 v[4];
 #pragma unroll
-        for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
-        l += sum;
-        const int n = parts - s0 < 64 ? parts - s0 : 64;
-        for (int i = 0; i < n; ++i) {
-            const float w = __shfl(by, i);
-            const float* const from = A.part_o + ((s0 + i) * all + rh) * DP + lane * kEach;
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * kSides < parts ? s0 + i * kSides : s0;
+            ml[i] = A.part_ml[s * all + rh];
+            v[i] = *reinterpret_cast<const float4*>(A.part_o + (s * all + rh) * DP + 4 * col);
+        }
 #pragma unroll
-            for (int x = 0; x < kEach; ++x) o[x] += w == 0.0f ? 0.0f : from[x] * w;
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + i * kSides >= parts || ml[i].x == -INFINITY) continue;
+            const float by = exp2_fast(ml[i].x - top);
+            l += ml[i].y * by;
+            o.x += v[i].x * by, o.y += v[i].y * by, o.z += v[i].z * by, o.w += v[i].w * by;
         }
     }
-    const float by = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* const to = A.out + row * A.out_row + head * A.out_head;
+    sums[side][col] = o;
+    if (col == 0) sides_l[side] = l;
+    __syncthreads();
+    if (side != 0) return;
+    l = 0.0f, o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int x = 0; x < kEach; ++x)
-        if (lane * kEach + x < A.dim) to[lane * kEach + x] = static_cast<uint16_t>(T::pack(o[x] * by, 0.0f));
-    if (lane == 0 && A.lse != nullptr) A.lse[rh] = l == 0.0f ? -INFINITY : top * (1.0f / kLog2E) + logf(l);
+    for (int i = 0; i < kSides; ++i) {
+        const float4 v = sums[i][col];
+        l += sides_l[i];
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+    }
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    if (4 * col < A.dim)
+        store_four<T>(A.out + row * A.out_row + head * A.out_head + 4 * col, o.x * by, o.y * by, o.z * by, o.w * by);
+    if (col == 0 && A.lse != nullptr) A.lse[rh] = l == 0.0f ? -INFINITY : top * (1.0f / kLog2E) + logf(l);
 }
 
 // Ancestor bits of drafted tokens: token t's parent is an earlier drafted
@@ -848,9 +865,11 @@ __global__ __launch_bounds__(256) void tree_masks_kernel(const int32_t* parents,
     }
 }
 
-constexpr int kMinChunk = 128;   // keys of a part: a tile for each of four waves
-constexpr int kMaxChunk = 2048;
-constexpr int kPartsWanted = 2048;  // workgroups over which a call's keys are spread
+constexpr int kMinChunk = 512;      // keys of a part: fewer cost more in start-up and joining than they save
+constexpr int kMaxChunk = 8192;     // and most of them, so that a long sequence among short ones does not run alone
+constexpr int kMaxSharedChunk = 4096;
+constexpr int kSlots = 256;         // workgroups of dealt-out keys that run at a time, one a CU
+constexpr int kSharedParts = 2048;  // workgroups of shared tiles: two a CU, four rounds
 
 // Rows of a workgroup. Up to 32 or 64 rows of a (sequence, head) go to every
 // wave and the keys are dealt out to the waves; more rows are dealt out.
@@ -863,9 +882,17 @@ void plan_parts(TreeArgs& A, int64_t max_context) {
     A.row_blocks = static_cast<int32_t>((rows + per - 1) / per);
     const int64_t longest = max_context + A.max_drafts;
     const int64_t units = static_cast<int64_t>(A.n_seqs) * A.kv_heads * A.row_blocks;
-    int64_t chunk = longest * units / kPartsWanted;
-    chunk = (chunk + kMinChunk - 1) / kMinChunk * kMinChunk;
-    chunk = chunk < kMinChunk ? kMinChunk : chunk > kMaxChunk ? kMaxChunk : chunk;
+    int64_t chunk, most = kMaxChunk;
+    if (per <= 64) {
+        // One round of workgroups: 64 sequences of 2000-8000 positions take
+        // 220 us in one part each, 240-260 in two to four.
+        chunk = longest / (units > 0 && units < kSlots ? kSlots / units : 1) + 1;
+    } else {
+        chunk = longest * units / kSharedParts;
+        most = kMaxSharedChunk;
+    }
+    chunk = (chunk + 127) / 128 * 128;
+    chunk = chunk < kMinChunk ? kMinChunk : chunk > most ? most : chunk;
     A.chunk = static_cast<int32_t>(chunk);
     A.n_splits = static_cast<int32_t>((longest + chunk - 1) / chunk);
 }
@@ -875,14 +902,15 @@ int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 template <typename T, int DP, int QT, int NW, bool kShared>
 int launch_tree_as(TreeArgs& A, hipStream_t s) {
     const int64_t groups = static_cast<int64_t>(A.n_seqs) * A.kv_heads * A.row_blocks * A.n_splits;
-    if (groups > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and keys");
+    if (groups > INT32_MAX || static_cast<int64_t>(A.n_q) * A.heads > INT32_MAX)
+        return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and keys");
     constexpr int KT = kShared && DP <= 128 ? 64 : 32;
     if (A.page_size % KT == 0)
         hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, true>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
     else
         hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, false>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
     if (A.n_splits > 1)
-        hipLaunchKernelGGL((tree_join_kernel<T, DP>), dim3(static_cast<uint32_t>((static_cast<int64_t>(A.n_q) * A.heads + 3) / 4)), dim3(256), 0, s, A);
+        hipLaunchKernelGGL((tree_join_kernel<T, DP>), dim3(static_cast<uint32_t>(static_cast<int64_t>(A.n_q) * A.heads)), dim3(256), 0, s, A);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess)
         return fail(AIMG_ERR_HIP, std::string("kernel launch failed: ") + hipGetErrorString(err));

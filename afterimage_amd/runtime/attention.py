@@ -20,32 +20,62 @@ from .. import _native
 
 MAX_DIM = 256
 
+_current_device = torch._C._cuda_getDevice
+_stream_handle = torch._C._cuda_getCurrentRawStream
+
 _TYPES = {torch.bfloat16: _native.AIMG_BF16, torch.float16: _native.AIMG_FP16}
 
 
-def _heads(x: torch.Tensor, name: str, like: torch.Tensor | None = None, written: bool = False) -> _native.AimgHeads:
-    """The descriptor of rows of heads [n, heads, dim], any row and head
-    strides that keep whole 16-byte pieces aligned (8 where written)."""
-    if x.device.type != "cuda":
+# The calls are short (a few microseconds of GPU time for one token), so the
+# checks go by the cheapest question first: a device's index rather than the
+# device, shapes and strides taken apart once, descriptors built once a call.
+
+def _heads(x: torch.Tensor, name: str, dtype: torch.dtype, index: int, unit: int = 8) -> _native.AimgHeads:
+    """The descriptor of rows of heads [n, heads, dim] of this type on GPU
+    ``index``, any row and head strides that keep whole pieces of ``unit``
+    elements aligned."""
+    if x.get_device() != index or x.dtype is not dtype or x.dim() != 3:
+        _refuse(x, name, dtype, index)
+    n, heads, dim = x.shape
+    row, head, one = x.stride()
+    at = x.data_ptr()
+    if one != 1 or (row | head) % unit or at % (2 * unit) or dim % 8 or not 0 < dim <= MAX_DIM or heads < 1:
+        if dim < 1 or heads < 1 or dim % 8 or dim > MAX_DIM:
+            raise ValueError("%s: dim must be a multiple of 8 up to %d, got %d" % (name, MAX_DIM, dim))
+        raise ValueError("%s must be contiguous in its last dimension, its rows and heads on %d-byte boundaries"
+                         % (name, 2 * unit))
+    return _native.AimgHeads(at, n, row, head, heads, dim)
+
+
+def _refuse(x: torch.Tensor, name: str, dtype: torch.dtype, index: int) -> None:
+    if x.get_device() < 0:
         raise RuntimeError("attention runs on the GPU only; got %s on %s" % (name, x.device))
     if x.dim() != 3 or x.dtype not in _TYPES:
         raise ValueError("%s must be a bf16 or fp16 [rows, heads, dim] tensor" % name)
-    if like is not None and (x.dtype != like.dtype or x.device != like.device):
-        raise ValueError("%s must be %s on %s" % (name, like.dtype, like.device))
-    n, heads, dim = x.shape
-    row, head, one = x.stride()
-    if dim < 1 or heads < 1 or dim % 8 or dim > MAX_DIM:
-        raise ValueError("%s: dim must be a multiple of 8 up to %d, got %d" % (name, MAX_DIM, dim))
-    unit = 4 if written else 8
-    if one != 1 or row % unit or head % unit or x.data_ptr() % (2 * unit):
-        raise ValueError("%s must be contiguous in its last dimension, its rows and heads on %d-byte boundaries"
-                         % (name, 2 * unit))
-    return _native.AimgHeads(x.data_ptr(), n, row, head, heads, dim)
+    raise ValueError("%s must be %s on cuda:%d" % (name, dtype, index))
 
 
-def _offsets(x: torch.Tensor, name: str, device) -> int:
-    if x.dtype != torch.int32 or x.dim() != 1 or x.device != device or not x.is_contiguous():
-        raise ValueError("%s must be a contiguous 1-D int32 tensor on %s" % (name, device))
+def _query(q: torch.Tensor) -> tuple[_native.AimgHeads, int, int]:
+    """q's descriptor, its GPU and its type's number."""
+    index, kind = q.get_device(), _TYPES.get(q.dtype)
+    if kind is None or index < 0:
+        _refuse(q, "q", q.dtype, index)
+    return _heads(q, "q", q.dtype, index), index, kind
+
+
+def _result(q: torch.Tensor, qd: _native.AimgHeads, out: torch.Tensor | None, index: int) -> tuple[torch.Tensor, _native.AimgHeads]:
+    """The output tensor and its descriptor."""
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        return out, _native.AimgHeads(out.data_ptr(), qd.n_rows, qd.heads * qd.dim, qd.dim, qd.heads, qd.dim)
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape %s" % (tuple(q.shape),))
+    return out, _heads(out, "out", q.dtype, index, unit=4)
+
+
+def _offsets(x: torch.Tensor, name: str, index: int) -> int:
+    if x.dtype is not torch.int32 or x.dim() != 1 or x.get_device() != index or not x.is_contiguous():
+        raise ValueError("%s must be a contiguous 1-D int32 tensor on cuda:%d" % (name, index))
     return x.data_ptr()
 
 
@@ -59,9 +89,22 @@ def _scale(scale: float | None, dim: int) -> float:
 def _lse(lse: torch.Tensor | None, q: torch.Tensor) -> int | None:
     if lse is None:
         return None
-    if lse.dtype != torch.float32 or lse.device != q.device or lse.shape != q.shape[:2] or not lse.is_contiguous():
+    if lse.dtype is not torch.float32 or lse.device != q.device or lse.shape != q.shape[:2] or not lse.is_contiguous():
         raise ValueError("lse must be a contiguous fp32 [%d, %d] tensor on %s" % (*q.shape[:2], q.device))
     return lse.data_ptr()
+
+
+def launch(entry, index: int, *args) -> None:
+    """entry(*args, stream) with GPU ``index`` current, on its current stream.
+    (The handle itself: a torch.cuda.Stream object and a device context cost
+    2 us of a call.)"""
+    if _current_device() == index:
+        status = entry(*args, _stream_handle(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(*args, _stream_handle(index))
+    if status:
+        _native.check(status)
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
@@ -80,36 +123,26 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
 
     Returns out (q's shape and type; rows of no sequence are not written).
     lse, fp32 [rows, heads], receives log(sum(exp(scale * q.k))) when given."""
-    qd = _heads(q, "q")
-    kd, vd = _heads(k, "k", q), _heads(v, "v", q)
-    dev = q.device
-    if k.shape != v.shape or k.shape[2] != q.shape[2]:
+    qd, index, kind = _query(q)
+    kd, vd = _heads(k, "k", q.dtype, index), _heads(v, "v", q.dtype, index)
+    if kd.n_rows != vd.n_rows or kd.heads != vd.heads or kd.dim != qd.dim or vd.dim != qd.dim:
         raise ValueError("k and v must have one shape and q's dim, got %s, %s and %s"
                          % (tuple(k.shape), tuple(v.shape), tuple(q.shape)))
-    if q.shape[1] % k.shape[1]:
-        raise ValueError("q's %d heads must be a multiple of k's %d" % (q.shape[1], k.shape[1]))
-    q_at = _offsets(q_offsets, "q_offsets", dev)
-    if k_offsets is None:
-        if q.shape[0] != k.shape[0]:
-            raise ValueError("q has %d rows and k %d: k_offsets is needed" % (q.shape[0], k.shape[0]))
-        k_offsets, k_at = q_offsets, q_at
-    else:
-        k_at = _offsets(k_offsets, "k_offsets", dev)
+    if qd.heads % kd.heads:
+        raise ValueError("q's %d heads must be a multiple of k's %d" % (qd.heads, kd.heads))
+    q_at = _offsets(q_offsets, "q_offsets", index)
     n_seqs = q_offsets.shape[0] - 1
-    if n_seqs < 0 or k_offsets.shape[0] != n_seqs + 1:
+    if k_offsets is None:
+        if qd.n_rows != kd.n_rows:
+            raise ValueError("q has %d rows and k %d: k_offsets is needed" % (qd.n_rows, kd.n_rows))
+        k_at, n_keys = q_at, n_seqs
+    else:
+        k_at, n_keys = _offsets(k_offsets, "k_offsets", index), k_offsets.shape[0] - 1
+    if n_seqs < 0 or n_keys != n_seqs:
         raise ValueError("q_offsets and k_offsets must have one entry more than there are sequences, got %d and %d"
-                         % (q_offsets.shape[0], k_offsets.shape[0]))
-    scale = _scale(scale, q.shape[2])
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape:
-        raise ValueError("out must have q's shape %s" % (tuple(q.shape),))
-    od = _heads(out, "out", q, written=True)
-    lse_at = _lse(lse, q)
-    with torch.cuda.device(dev):
-        _native.check(_native.lib().aimg_prompt_attention(
-            ctypes.byref(qd), ctypes.byref(kd), ctypes.byref(vd), ctypes.byref(od), q_at, k_at, n_seqs,
-            _TYPES[q.dtype], scale, lse_at, torch.cuda.current_stream(dev).cuda_stream))
+                         % (n_seqs + 1, n_keys + 1))
+    out, od = _result(q, qd, out, index)
+    launch(_native.lib().aimg_prompt_attention, index, qd, kd, vd, od, q_at, k_at, n_seqs, kind, _scale(scale, qd.dim), _lse(lse, q))
     return out
 
 
@@ -119,25 +152,27 @@ def describe_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: tor
     page_size, dim] (any strides with a contiguous last dimension and whole
     16-byte pieces, the same for both) and of the int32 page table [max_seqs,
     max_pages] and lengths [max_seqs]."""
-    dev = k_pages.device
-    if dev.type != "cuda":
-        raise RuntimeError("the cache lives on the GPU only; got k_pages on %s" % dev)
+    index = k_pages.get_device()
+    if index < 0:
+        raise RuntimeError("the cache lives on the GPU only; got k_pages on %s" % k_pages.device)
     if k_pages.dim() != 4 or k_pages.dtype not in _TYPES:
         raise ValueError("k_pages must be a bf16 or fp16 [n_pages, kv_heads, page_size, dim] tensor")
-    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or v_pages.stride() != k_pages.stride() \
-            or v_pages.device != dev:
+    shape, strides = k_pages.shape, k_pages.stride()
+    if v_pages.shape != shape or v_pages.dtype is not k_pages.dtype or v_pages.stride() != strides or v_pages.get_device() != index:
         raise ValueError("v_pages must have k_pages' shape, type, strides and device")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.device != dev or page_table.stride(1) != 1:
-        raise ValueError("page_table must be an int32 [max_seqs, max_pages] tensor on %s, its rows contiguous" % dev)
-    if lengths.dtype != torch.int32 or lengths.shape != page_table.shape[:1] or lengths.device != dev \
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.get_device() != index or page_table.stride(1) != 1:
+        raise ValueError("page_table must be an int32 [max_seqs, max_pages] tensor on cuda:%d, its rows contiguous" % index)
+    max_seqs, max_pages = page_table.shape
+    if lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.shape[0] != max_seqs or lengths.get_device() != index \
             or not lengths.is_contiguous():
-        raise ValueError("lengths must be a contiguous int32 [%d] tensor on %s" % (page_table.shape[0], dev))
-    n_pages, kv_heads, page_size, dim = k_pages.shape
-    page, head, slot, one = k_pages.stride()
-    if one != 1 or page % 8 or head % 8 or slot % 8 or (k_pages.data_ptr() | v_pages.data_ptr()) % 16:
+        raise ValueError("lengths must be a contiguous int32 [%d] tensor on cuda:%d" % (max_seqs, index))
+    n_pages, kv_heads, page_size, dim = shape
+    page, head, slot, one = strides
+    k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
+    if one != 1 or (page | head | slot) % 8 or (k_at | v_at) % 16:
         raise ValueError("k_pages and v_pages must be contiguous in their last dimension, their rows on 16-byte boundaries")
-    return _native.AimgPages(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), page, slot, head,
-                             page_table.stride(0), n_pages, page_size, kv_heads, dim, page_table.shape[0], page_table.shape[1])
+    return _native.AimgPages(k_at, v_at, page_table.data_ptr(), lengths.data_ptr(), page, slot, head, page_table.stride(0), n_pages,
+                             page_size, kv_heads, dim, max_seqs, max_pages)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -174,45 +209,37 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
     Returns out (q's shape and type); lse as in prompt_attention. Results do
     not vary between calls."""
-    qd = _heads(q, "q")
-    dev = q.device
+    qd, index, kind = _query(q)
     pages = describe_pages(k_pages, v_pages, page_table, lengths)
-    if k_pages.dtype != q.dtype or k_pages.device != dev:
-        raise ValueError("k_pages must be %s on %s" % (q.dtype, dev))
-    if pages.dim != qd.dim or qd.heads % pages.kv_heads:
+    if k_pages.dtype is not q.dtype or k_pages.get_device() != index:
+        raise ValueError("k_pages must be %s on %s" % (q.dtype, q.device))
+    heads, kv_heads, dim = qd.heads, pages.kv_heads, qd.dim
+    if pages.dim != dim or heads % kv_heads:
         raise ValueError("q's dim %d must be the pages' %d, its %d heads a multiple of their %d"
-                         % (qd.dim, pages.dim, qd.heads, pages.kv_heads))
-    n_seqs = seqs.shape[0]
-    seqs_at, at = _offsets(seqs, "seqs", dev), _offsets(draft_offsets, "draft_offsets", dev)
+                         % (dim, pages.dim, heads, kv_heads))
+    seqs_at, at = _offsets(seqs, "seqs", index), _offsets(draft_offsets, "draft_offsets", index)
+    n_seqs, n = seqs.shape[0], qd.n_rows
     if draft_offsets.shape[0] != n_seqs + 1:
         raise ValueError("draft_offsets must have one entry more than seqs, got %d and %d" % (draft_offsets.shape[0], n_seqs))
     if max_drafts < 1:
         raise ValueError("max_drafts must be at least 1, got %d" % max_drafts)
     masks_at, words = None, 0
     if masks is not None:
-        if masks.dtype != torch.int64 or masks.dim() != 2 or masks.shape[0] != qd.n_rows or masks.device != dev \
+        if masks.dtype is not torch.int64 or masks.dim() != 2 or masks.shape[0] != n or masks.get_device() != index \
                 or not masks.is_contiguous() or masks.shape[1] * 64 < max_drafts:
-            raise ValueError("masks must be a contiguous int64 [%d, at least %d] tensor on %s"
-                             % (qd.n_rows, -(-max_drafts // 64), dev))
+            raise ValueError("masks must be a contiguous int64 [%d, at least %d] tensor on cuda:%d"
+                             % (n, -(-max_drafts // 64), index))
         masks_at, words = masks.data_ptr(), masks.shape[1]
     if max_context is None:
         max_context = pages.max_pages * pages.page_size
     elif max_context < 0:
         raise ValueError("max_context must not be negative, got %d" % max_context)
-    scale = _scale(scale, qd.dim)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape:
-        raise ValueError("out must have q's shape %s" % (tuple(q.shape),))
-    od = _heads(out, "out", q, written=True)
-    lse_at = _lse(lse, q)
-    nbytes = _tree_workspace_nbytes(qd.n_rows, qd.heads, pages.kv_heads, qd.dim, n_seqs, max_drafts, max_context)
-    with torch.cuda.device(dev):
-        work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        _native.check(_native.lib().aimg_tree_attention(
-            ctypes.byref(qd), ctypes.byref(pages), ctypes.byref(od), seqs_at, at, n_seqs, masks_at, words, max_drafts,
-            max_context, _TYPES[q.dtype], scale, lse_at, work.data_ptr() if nbytes else None, nbytes,
-            torch.cuda.current_stream(dev).cuda_stream))
+    out, od = _result(q, qd, out, index)
+    nbytes = _tree_workspace_nbytes(n, heads, kv_heads, dim, n_seqs, max_drafts, max_context)
+    # From torch's allocator on the current stream, which the launches use.
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+    launch(_native.lib().aimg_tree_attention, index, qd, pages, od, seqs_at, at, n_seqs, masks_at, words, max_drafts, max_context,
+           kind, _scale(scale, dim), _lse(lse, q), work, nbytes)
     return out
 
 
@@ -221,15 +248,13 @@ def tree_masks(parents: torch.Tensor, draft_offsets: torch.Tensor, max_drafts: i
     indices within the token's sequence, earlier than the token; any other
     number (-1) for a token that follows the context. A token sees itself
     and its ancestors. int64 [rows, ceil(max_drafts / 64)]."""
-    dev = parents.device
-    if dev.type != "cuda":
-        raise RuntimeError("attention runs on the GPU only; got parents on %s" % dev)
-    at, up = _offsets(draft_offsets, "draft_offsets", dev), _offsets(parents, "parents", dev)
+    index = parents.get_device()
+    if index < 0:
+        raise RuntimeError("attention runs on the GPU only; got parents on %s" % parents.device)
+    at, up = _offsets(draft_offsets, "draft_offsets", index), _offsets(parents, "parents", index)
     if max_drafts < 1 or draft_offsets.shape[0] < 1:
         raise ValueError("max_drafts must be at least 1 and draft_offsets not empty")
     n, words = parents.shape[0], -(-max_drafts // 64)
-    masks = torch.empty((n, words), dtype=torch.int64, device=dev)
-    with torch.cuda.device(dev):
-        _native.check(_native.lib().aimg_tree_masks(up, at, draft_offsets.shape[0] - 1, n, words, masks.data_ptr(),
-                                                    torch.cuda.current_stream(dev).cuda_stream))
+    masks = torch.empty((n, words), dtype=torch.int64, device=parents.device)
+    launch(_native.lib().aimg_tree_masks, index, up, at, draft_offsets.shape[0] - 1, n, words, masks.data_ptr())
     return masks

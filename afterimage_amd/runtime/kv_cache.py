@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from .. import _native
-from .attention import tree_attention
+from .attention import launch, tree_attention
 
 MAX_SEQS = 8192      # sequences of one call
 MAX_PAGES = (1 << 20) - 1
@@ -31,9 +31,9 @@ _PROBLEMS = ((1, "too few free pages"), (2, "positions past a sequence's pages o
              (4, "a slot, page or source that does not exist"))
 
 
-def _int32(x: torch.Tensor, name: str, shape: tuple, device) -> int:
-    if x.dtype != torch.int32 or tuple(x.shape) != tuple(shape) or x.device != device or not x.is_contiguous():
-        raise ValueError("%s must be a contiguous int32 %s tensor on %s" % (name, list(shape), device))
+def _int32(x: torch.Tensor, name: str, shape: tuple, index: int) -> int:
+    if x.dtype is not torch.int32 or x.get_device() != index or x.shape != shape or not x.is_contiguous():
+        raise ValueError("%s must be a contiguous int32 %s tensor on cuda:%d" % (name, list(shape), index))
     return x.data_ptr()
 
 
@@ -53,14 +53,14 @@ class PagedKVCache:
 
     def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, held: torch.Tensor,
                  refs: torch.Tensor, status: torch.Tensor):
-        dev = pool.device
-        if dev.type != "cuda":
-            raise RuntimeError("the cache lives on the GPU only; got the pool on %s" % dev)
+        index = pool.get_device()
+        if index < 0:
+            raise RuntimeError("the cache lives on the GPU only; got the pool on %s" % pool.device)
         if pool.dim() != 6 or pool.shape[1] != 2 or pool.dtype not in (torch.bfloat16, torch.float16) \
                 or not pool.is_contiguous() or pool.numel() == 0:
             raise ValueError("pool must be a contiguous bf16 or fp16 [n_layers, 2, n_pages, kv_heads, page_size, dim] tensor")
         if page_table.dim() != 2 or page_table.numel() == 0:
-            raise ValueError("page_table must be a contiguous int32 [max_seqs, max_pages] tensor on %s" % dev)
+            raise ValueError("page_table must be a contiguous int32 [max_seqs, max_pages] tensor on cuda:%d" % index)
         self.n_layers, _, self.n_pages, self.kv_heads, self.page_size, self.dim = pool.shape
         self.max_seqs, self.max_pages = page_table.shape
         if self.dim % 8 or pool.data_ptr() % 16:
@@ -68,17 +68,21 @@ class PagedKVCache:
         if self.n_pages > MAX_PAGES or self.max_pages * self.page_size >= 1 << 30:
             raise ValueError("pool: at most %d pages, and fewer than 2^30 positions a sequence" % MAX_PAGES)
         self._cache = _native.AimgCache(
-            pool.data_ptr(), _int32(page_table, "page_table", (self.max_seqs, self.max_pages), dev),
-            _int32(lengths, "lengths", (self.max_seqs,), dev), _int32(held, "held", (self.max_seqs,), dev),
-            _int32(refs, "refs", (self.n_pages,), dev), _int32(status, "status", (1,), dev),
+            pool.data_ptr(), _int32(page_table, "page_table", (self.max_seqs, self.max_pages), index),
+            _int32(lengths, "lengths", (self.max_seqs,), index), _int32(held, "held", (self.max_seqs,), index),
+            _int32(refs, "refs", (self.n_pages,), index), _int32(status, "status", (1,), index),
             self.n_layers, self.n_pages, self.kv_heads, self.page_size, self.dim, self.max_seqs, self.max_pages)
-        self._at = ctypes.byref(self._cache)
-        self.device = dev
+        self.device = pool.device
+        self._index = index
+        self._lib = _native.lib()
         self.pool, self.page_table, self.lengths, self.held, self.refs, self.status = \
             pool, page_table, lengths, held, refs, status
         nbytes = ctypes.c_size_t(0)
-        _native.check(_native.lib().aimg_cache_compact_workspace_nbytes(self._at, ctypes.byref(nbytes)))
-        self._compact_nbytes = nbytes.value
+        _native.check(self._lib.aimg_cache_compact_workspace_nbytes(self._cache, ctypes.byref(nbytes)))
+        # Scratch memory of the calls, kept: they change one cache and so run in order.
+        self._compact_work = torch.empty(nbytes.value, dtype=torch.uint8, device=self.device)
+        self._fork_work = torch.empty(0, dtype=torch.uint8, device=self.device)
+        self._used = torch.empty((), dtype=torch.int32, device=self.device)
 
     @classmethod
     def allocate(cls, n_layers: int, n_pages: int, page_size: int, kv_heads: int, dim: int, max_seqs: int, max_pages: int,
@@ -89,17 +93,14 @@ class PagedKVCache:
         pool = torch.empty((n_layers, 2, n_pages, kv_heads, page_size, dim), dtype=dtype, device=device)
         return cls(pool, ints(max_seqs, max_pages, value=-1), ints(max_seqs), ints(max_seqs), ints(n_pages), ints(1))
 
-    def _seqs(self, x: torch.Tensor, name: str = "seqs") -> int:
-        if x.dim() != 1 or x.shape[0] > MAX_SEQS:
-            raise ValueError("%s must be a 1-D tensor of at most %d slots" % (name, MAX_SEQS))
-        return _int32(x, name, x.shape, self.device)
-
-    def _call(self, entry: str, *args) -> None:
-        with torch.cuda.device(self.device):
-            _native.check(getattr(_native.lib(), entry)(self._at, *args, torch.cuda.current_stream(self.device).cuda_stream))
-
-    def _scratch(self, nbytes: int) -> torch.Tensor:
-        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+    def _seqs(self, x: torch.Tensor, name: str = "seqs") -> tuple[int, int]:
+        """The address and the number of a call's slots."""
+        if x.dtype is not torch.int32 or x.dim() != 1 or x.get_device() != self._index or not x.is_contiguous():
+            raise ValueError("%s must be a contiguous 1-D int32 tensor on cuda:%d" % (name, self._index))
+        n = x.shape[0]
+        if n > MAX_SEQS:
+            raise ValueError("%s: at most %d slots a call, got %d" % (name, MAX_SEQS, n))
+        return x.data_ptr(), n
 
     def keys(self, layer: int) -> torch.Tensor:
         """One layer's key pages [n_pages, kv_heads, page_size, dim]."""
@@ -111,15 +112,16 @@ class PagedKVCache:
     def reserve(self, seqs: torch.Tensor, tokens: torch.Tensor) -> None:
         """Pages for tokens[b] (int32) positions past slot seqs[b]'s length,
         for all slots or for none."""
-        at = self._seqs(seqs)
-        self._call("aimg_cache_reserve", at, _int32(tokens, "tokens", seqs.shape, self.device), seqs.shape[0])
+        at, n = self._seqs(seqs)
+        launch(self._lib.aimg_cache_reserve, self._index, self._cache, at, _int32(tokens, "tokens", (n,), self._index), n)
 
     def _rows(self, x: torch.Tensor, name: str) -> _native.AimgHeads:
-        if x.dim() != 3 or x.dtype != self.pool.dtype or x.device != self.device or tuple(x.shape[1:]) != (self.kv_heads, self.dim):
+        if x.dim() != 3 or x.dtype is not self.pool.dtype or x.get_device() != self._index \
+                or x.shape[1:] != (self.kv_heads, self.dim):
             raise ValueError("%s must be a %s [rows, %d, %d] tensor on %s"
                              % (name, self.pool.dtype, self.kv_heads, self.dim, self.device))
         row, head, one = x.stride()
-        if one != 1 or row % 8 or head % 8 or x.data_ptr() % 16:
+        if one != 1 or (row | head) % 8 or x.data_ptr() % 16:
             raise ValueError("%s must be contiguous in its last dimension, its rows and heads on 16-byte boundaries" % name)
         return _native.AimgHeads(x.data_ptr(), x.shape[0], row, head, x.shape[1], x.shape[2])
 
@@ -132,14 +134,14 @@ class PagedKVCache:
             raise ValueError("layer must be in 0..%d, got %d" % (self.n_layers - 1, layer))
         if k.shape != v.shape:
             raise ValueError("k and v must have one shape, got %s and %s" % (tuple(k.shape), tuple(v.shape)))
-        at, n = self._seqs(seqs), seqs.shape[0]
-        self._call("aimg_cache_append", layer, ctypes.byref(kd), ctypes.byref(vd), at,
-                   _int32(offsets, "offsets", (n + 1,), self.device), n)
+        at, n = self._seqs(seqs)
+        launch(self._lib.aimg_cache_append, self._index, self._cache, layer, kd, vd, at,
+               _int32(offsets, "offsets", (n + 1,), self._index), n)
 
     def advance(self, seqs: torch.Tensor, offsets: torch.Tensor) -> None:
         """Slot seqs[b]'s length grows by offsets[b + 1] - offsets[b], the rows that were appended."""
-        at, n = self._seqs(seqs), seqs.shape[0]
-        self._call("aimg_cache_advance", at, _int32(offsets, "offsets", (n + 1,), self.device), n)
+        at, n = self._seqs(seqs)
+        launch(self._lib.aimg_cache_advance, self._index, self._cache, at, _int32(offsets, "offsets", (n + 1,), self._index), n)
 
     def attend(self, layer: int, q: torch.Tensor, seqs: torch.Tensor, draft_offsets: torch.Tensor,
                masks: torch.Tensor | None = None, **options) -> torch.Tensor:
@@ -155,12 +157,13 @@ class PagedKVCache:
         length grows by counts[b]. The new lengths go to new_lengths (int32
         [max_seqs], the call's slots only) where given, in place otherwise.
         Returns the lengths written."""
-        at, n = self._seqs(seqs), seqs.shape[0]
+        at, n = self._seqs(seqs)
         if accepted.dim() != 2:
             raise ValueError("accepted must be a contiguous int32 [%d, most] tensor on %s" % (n, self.device))
+        most = accepted.shape[1]
         lengths = self.lengths if new_lengths is None else new_lengths
-        self._call("aimg_cache_commit", at, _int32(accepted, "accepted", (n, accepted.shape[1]), self.device), accepted.shape[1],
-                   _int32(counts, "counts", (n,), self.device), n, _int32(lengths, "new_lengths", (self.max_seqs,), self.device))
+        launch(self._lib.aimg_cache_commit, self._index, self._cache, at, _int32(accepted, "accepted", (n, most), self._index), most,
+               _int32(counts, "counts", (n,), self._index), n, _int32(lengths, "new_lengths", (self.max_seqs,), self._index))
         return lengths
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -169,15 +172,17 @@ class PagedKVCache:
         one slot stays). Branches share the source's full pages; the rows of its
         last page are copied to a free one. What a slot held before is given
         back after the copies."""
-        s, n = self._seqs(src, "src"), src.shape[0]
-        d = _int32(dst, "dst", (n,), self.device)
+        s, n = self._seqs(src, "src")
+        d = _int32(dst, "dst", (n,), self._index)
         nbytes = 4 * n * (2 + self.max_pages)
-        work = self._scratch(nbytes)
-        self._call("aimg_cache_fork", s, d, n, work.data_ptr() if n else None, nbytes)
+        if self._fork_work.shape[0] < nbytes:
+            self._fork_work = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        launch(self._lib.aimg_cache_fork, self._index, self._cache, s, d, n, self._fork_work.data_ptr(), nbytes)
 
     def release(self, seqs: torch.Tensor) -> None:
         """Empties the slots; pages that no other slot holds are free."""
-        self._call("aimg_cache_release", self._seqs(seqs), seqs.shape[0])
+        at, n = self._seqs(seqs)
+        launch(self._lib.aimg_cache_release, self._index, self._cache, at, n)
 
     def compact(self, new_table: torch.Tensor | None = None, new_refs: torch.Tensor | None = None) -> torch.Tensor:
         """Moves the pages in use to the front of the pool, in every layer,
@@ -186,10 +191,11 @@ class PagedKVCache:
         new_refs where given, in place otherwise."""
         table = self.page_table if new_table is None else new_table
         refs = self.refs if new_refs is None else new_refs
-        used = torch.empty((), dtype=torch.int32, device=self.device)
-        work = self._scratch(self._compact_nbytes)
-        self._call("aimg_cache_compact", _int32(table, "new_table", (self.max_seqs, self.max_pages), self.device),
-                   _int32(refs, "new_refs", (self.n_pages,), self.device), used.data_ptr(), work.data_ptr(), self._compact_nbytes)
+        used = torch.empty_like(self._used)
+        launch(self._lib.aimg_cache_compact, self._index, self._cache,
+               _int32(table, "new_table", (self.max_seqs, self.max_pages), self._index),
+               _int32(refs, "new_refs", (self.n_pages,), self._index), used.data_ptr(), self._compact_work.data_ptr(),
+               self._compact_work.shape[0])
         return used
 
     def check(self) -> None:

@@ -88,9 +88,11 @@ def test_tree_workspace_follows_the_sizes():
         assert lib.aimg_tree_workspace_nbytes(*sizes, ctypes.byref(n)) == OK
         return n.value
     assert nbytes(1, 40, 8, 128, 1, 1, 0) == 0
-    # A part for each 128 keys or more, a row of sums and two numbers each.
-    assert nbytes(1, 40, 8, 128, 1, 1, 1000) == 8 * 40 * (4 * 128 + 8)
-    assert nbytes(1, 40, 8, 96, 1, 1, 1000) == 8 * 40 * (4 * 128 + 8)
+    # A row of padded sums and two numbers for each part of a row and head.
+    parts, rest = divmod(nbytes(1, 40, 8, 128, 1, 1, 8000), 40 * (4 * 128 + 8))
+    assert parts > 1 and rest == 0
+    assert nbytes(3, 40, 8, 96, 1, 3, 8000) % (3 * 40 * (4 * 128 + 8)) == 0
+    assert nbytes(0, 40, 8, 128, 0, 1, 8000) == 0
     assert lib.aimg_tree_workspace_nbytes(1, 40, 7, 128, 1, 1, 0, ctypes.byref(n)) == BAD
     assert lib.aimg_tree_workspace_nbytes(1, 40, 8, 128, 1, 1, 0, None) == BAD
 
