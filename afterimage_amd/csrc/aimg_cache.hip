@@ -132,11 +132,10 @@ struct AppendArgs {
 // 16 bytes a thread, keys and values.
 __global__ __launch_bounds__(256) void append_kernel(const AppendArgs A) {
     const Cache& C = A.c;
-    const int32_t pieces = C.row_bytes / 16;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (i >= static_cast<int64_t>(A.n_rows) * C.kv_heads * pieces) return;
+    const uint32_t pieces = C.row_bytes / 16, i = blockIdx.x * 256u + threadIdx.x;  // fewer than 2^31 in all
     const int32_t x = static_cast<int32_t>(i % pieces);
     const int32_t head = static_cast<int32_t>(i / pieces % C.kv_heads), row = static_cast<int32_t>(i / pieces / C.kv_heads);
+    if (row >= A.n_rows) return;
     int lo = 0, hi = A.n_seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) / 2;
@@ -318,14 +317,32 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(const ForkArgs A) {
     if (tail == 0) return;
     const int32_t last = from[full];
     if (last < 0 || last >= C.n_pages) return;
-    // The tail's rows of every head and plane, 16 bytes a thread.
-    const int32_t bytes = tail * C.row_bytes, pieces = bytes / 16;
-    const int64_t all = static_cast<int64_t>(C.planes) * C.kv_heads * pieces;
-    for (int64_t j = static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x; j < all; j += static_cast<int64_t>(gridDim.y) * 256) {
-        const int32_t x = static_cast<int32_t>(j % pieces);
-        const int32_t ph = static_cast<int32_t>(j / pieces);
-        char* const base = C.pool + ph / C.kv_heads * C.plane_bytes + ph % C.kv_heads * C.head_bytes + x * 16;
-        put16(base + page * C.page_bytes, get16(base + last * C.page_bytes));
+    // The tail's rows of every head and plane, 16 bytes a thread and step: a
+    // thread keeps its place in a head's rows and steps over heads and planes,
+    // so it divides once (a division a step took longer than the bytes).
+    const uint32_t pieces = static_cast<uint32_t>(tail) * (C.row_bytes / 16);
+    const uint32_t heads = static_cast<uint32_t>(C.planes) * C.kv_heads, threads = gridDim.y * 256u;
+    const uint32_t t = blockIdx.y * 256u + threadIdx.x;
+    const int64_t away = (static_cast<int64_t>(page) - last) * C.page_bytes;
+    char* const base = C.pool + last * C.page_bytes;
+    const uint32_t step = pieces < threads ? threads / pieces : 1;
+    uint32_t x = pieces < threads ? t % pieces : t;
+    const uint32_t first = pieces < threads ? t / pieces : 0;
+    if (first >= step) return;
+    for (; x < pieces; x += threads) {
+        for (uint32_t h = first; h < heads; h += 4 * step) {
+            uint4 v[4];
+            char* at[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t ph = h + i * step < heads ? h + i * step : h;
+                at[i] = base + ph / C.kv_heads * C.plane_bytes + ph % C.kv_heads * C.head_bytes + x * 16u;
+                v[i] = get16(at[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (h + i * step < heads) put16(at[i] + away, v[i]);
+        }
     }
 }
 
@@ -383,10 +400,8 @@ __global__ __launch_bounds__(256) void commit_kernel(const CommitArgs A) {
         if (n == 0 && A.counts[b] > 0) tell(C, kRowFull);
         if (A.new_lengths != C.lengths) A.new_lengths[slot] = len + n;
     }
-    const int32_t pieces = C.row_bytes / 16;
-    const int64_t all = static_cast<int64_t>(C.planes) * C.kv_heads * pieces;
-    const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int32_t ph = static_cast<int32_t>(j / pieces);
+    const uint32_t pieces = C.row_bytes / 16, all = static_cast<uint32_t>(C.planes) * C.kv_heads * pieces;  // below 2^31
+    const uint32_t j = blockIdx.x * 256u + threadIdx.x, ph = j / pieces;
     char* const mine = C.pool + ph / C.kv_heads * C.plane_bytes + ph % C.kv_heads * C.head_bytes + j % pieces * 16;
     const int32_t* const row = C.table + static_cast<int64_t>(slot) * C.table_stride;
     const int64_t most = static_cast<int64_t>(held_of(C, slot)) * C.page_size;
@@ -534,6 +549,8 @@ int take(const aimg_cache* c, Cache& C, bool pool) {
     if (c->page_table == nullptr || c->lengths == nullptr || c->held == nullptr || c->refs == nullptr || c->status == nullptr ||
         (pool && c->pool == nullptr))
         return fail(AIMG_ERR_INVALID_ARGUMENT, "cache: null pointer");
+    if (2 * static_cast<int64_t>(c->n_layers) * c->kv_heads * (c->dim / 8) > INT32_MAX - 256)
+        return fail(AIMG_ERR_UNSUPPORTED, "cache: a position must be below 2^34 bytes in all layers");
     if (reinterpret_cast<uintptr_t>(c->pool) % 16 != 0) return fail(AIMG_ERR_UNSUPPORTED, "cache: the pool must be 16-byte aligned");
     C = Cache{static_cast<char*>(c->pool), c->page_table, c->lengths, c->held, c->refs, c->status,
               page * c->n_pages, page, 2 * static_cast<int64_t>(c->page_size) * c->dim,
@@ -579,7 +596,7 @@ extern "C" int aimg_cache_append(const aimg_cache* cache, int layer, const aimg_
     a.seqs = seqs, a.offsets = offsets, a.n_seqs = n_seqs, a.n_rows = static_cast<int32_t>(k->n_rows);
     a.layer_at = 2 * layer * a.c.plane_bytes;
     const int64_t work = k->n_rows * cache->kv_heads * (cache->dim / 8);
-    if (work > static_cast<int64_t>(INT32_MAX) * 256) return fail(AIMG_ERR_UNSUPPORTED, "too many rows");
+    if (work > INT32_MAX - 256) return fail(AIMG_ERR_UNSUPPORTED, "too many rows");
     hipLaunchKernelGGL(aimg::append_kernel, dim3(aimg::blocks(work, 256)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
     return aimg::launched();
 }
