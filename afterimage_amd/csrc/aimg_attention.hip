@@ -586,8 +586,10 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeArgs& A, const Drafted& 
 // into its own part of LDS with no barrier in the loop, and join their sums at
 // the end: one token's group (5 rows of 32 here) leaves the matrix cores idle,
 // but the bytes in flight, not the products, bound it.
-// kWhole: a tile never crosses a page, so it has one base address.
-template <typename T, int DP, int QT, int NW, bool kShared, bool kWhole>
+// kPages: what of a tile never crosses a page, and so has one base address: 2
+// the tile, 1 the rows of one load (2 to 8), 0 a row. (With addresses made lane
+// by lane for pages of 16, 54 trees over 139-2238 positions took 155 us.)
+template <typename T, int DP, int QT, int NW, bool kShared, int kPages>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_kernel(const TreeArgs A) {
     typedef Rows<DP> R;
     constexpr int KT = kShared && DP <= 128 ? 64 : 32;
@@ -642,26 +644,31 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         page_of(A, k0 + last, page_end, unused);
         if (page_end >= first_page + 64) hold(page);
         int64_t tile_at = 0;
-        if (kWhole)
+        if (kPages == 2)
             tile_at = 2 * (__builtin_amdgcn_readlane(held, page - first_page) * A.page_stride + first * A.slot_stride + head_at);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int load = load0 + i;
-            const int r = load * R::kPerLoad + lane_row;
+            const int r0 = load * R::kPerLoad, r = r0 + lane_row;
             const int kx = lane_piece ^ R::key_place(r), vx = lane_piece ^ R::value_place(r);
             const uint32_t kp = (kx < pieces ? kx : pieces) * 16, vp = (vx < pieces ? vx : pieces) * 16;
-            const int from = r < last ? r : last;
-            if (kWhole) {
-                load_to_lds(reinterpret_cast<const char*>(A.k) + tile_at + (from * row_bytes + kp), to + load * 1024);
-                load_to_lds(reinterpret_cast<const char*>(A.v) + tile_at + (from * row_bytes + vp), to + kTile + load * 1024);
-            } else {
+            int64_t at = tile_at;
+            uint32_t from = r < last ? r : last;
+            if (kPages == 1) {
+                const int row = r0 < last ? r0 : last;
+                int32_t p, slot;
+                page_of(A, k0 + row, p, slot);
+                at = 2 * (__builtin_amdgcn_readlane(held, p - first_page) * A.page_stride + slot * A.slot_stride + head_at);
+                from -= row;
+            } else if (kPages == 0) {
                 int32_t p, slot;
                 page_of(A, k0 + from, p, slot);
                 const int64_t id = __builtin_amdgcn_ds_bpermute(4 * (p - first_page), held);
-                const int64_t at = 2 * (id * A.page_stride + slot * A.slot_stride + head_at);
-                load_to_lds(reinterpret_cast<const char*>(A.k) + at + kp, to + load * 1024);
-                load_to_lds(reinterpret_cast<const char*>(A.v) + at + vp, to + kTile + load * 1024);
+                at = 2 * (id * A.page_stride + slot * A.slot_stride + head_at);
+                from = 0;
             }
+            load_to_lds(reinterpret_cast<const char*>(A.k) + at + (from * row_bytes + kp), to + load * 1024);
+            load_to_lds(reinterpret_cast<const char*>(A.v) + at + (from * row_bytes + vp), to + kTile + load * 1024);
         }
     };
 
@@ -730,6 +737,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
     }
 
     const int64_t part = static_cast<int64_t>(split) * A.n_q * A.heads;
+    const bool parted = A.n_splits > 1 && D.end > A.chunk;  // the join leaves sequences of one part alone
     if (kShared) {
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
@@ -738,7 +746,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
             if (r >= rows) continue;
             const int row = D.row + token[t], head = kvh * group + r % group;
             const int64_t rh = static_cast<int64_t>(row) * A.heads + head;
-            const float by = A.n_splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            const float by = parted ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             uint16_t* const to = A.out + row * A.out_row + head * A.out_head;
 #pragma unroll
             for (int d = 0; d < DP / 32; ++d)
@@ -746,13 +754,13 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
                 for (int i = 0; i < 4; ++i) {
                     const int x = 32 * d + 8 * i + 4 * half;
                     const f32x16& o = st.o[t][d];
-                    if (A.n_splits > 1)
+                    if (parted)
                         *reinterpret_cast<float4*>(A.part_o + (part + rh) * DP + x) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     else if (x < A.dim)
                         store_four<T>(to + x, o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
                 }
             if (half == 0) {
-                if (A.n_splits > 1) A.part_ml[part + rh] = make_float2(st.m[t] * A.c, l);
+                if (parted) A.part_ml[part + rh] = make_float2(st.m[t] * A.c, l);
                 else if (A.lse != nullptr) A.lse[rh] = l == 0.0f ? -INFINITY : st.m[t] * A.scale + logf(l);
             }
         }
@@ -797,7 +805,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         }
         const int row = D.row + (block * BM + r) / group, head = kvh * group + (block * BM + r) % group;
         const int64_t rh = static_cast<int64_t>(row) * A.heads + head;
-        if (A.n_splits > 1) {
+        if (parted) {
             *reinterpret_cast<float4*>(A.part_o + (part + rh) * DP + x) = o;
             if (x == 0) A.part_ml[part + rh] = make_float2(top, l);
         } else {
@@ -808,57 +816,78 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
     }
 }
 
-// The parts of a row and head joined in a fixed order: threads of DP / 4 hold a
-// row's columns, four each, and take parts in turn (eight at a time of 128
-// columns: with one row's thread after the other, a token over 32,000 positions
-// spent 100 of 145 us here); their sums meet in LDS.
-template <typename T, int DP>
+// The parts of a row and head joined in their order: DP / 4 threads hold a
+// row's columns, four each. kMany: all of a workgroup's threads take a row,
+// its parts in turn, and their sums meet in LDS (with the parts one after the
+// other, a token over 32,000 positions spent 100 of 145 us here). Otherwise
+// every DP / 4 threads take a row of their own: fewer, fuller workgroups.
+template <typename T, int DP, bool kMany>
 __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
     constexpr int kCols = DP / 4, kSides = 256 / kCols;
-    __shared__ float4 sums[kSides][kCols];
-    __shared__ float sides_l[kSides];
-    const int64_t rh = blockIdx.x, all = static_cast<int64_t>(A.n_q) * A.heads;
-    const int row = static_cast<int>(rh / A.heads), head = static_cast<int>(rh % A.heads);
+    constexpr int kTake = kMany ? kSides : 1;  // sides that share a row
+    __shared__ float4 sums[kMany ? kSides : 1][kCols];
+    __shared__ float sides_l[kMany ? kSides : 1];
     const int lane = threadIdx.x & 63;
-    const int lo = find_sequence(A.offsets, A.n_seqs, A.n_q, row, lane, [](int, int first) { return first; });
+    const int side = threadIdx.x / kCols, col = threadIdx.x % kCols;
+    const int64_t all = static_cast<int64_t>(A.n_q) * A.heads;
+    const int64_t rh = kMany ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kSides + side;
+    if (rh >= all) return;
+    const int row = static_cast<int>(rh / A.heads), head = static_cast<int>(rh % A.heads);
+    int lo;
+    if (kMany) {
+        lo = find_sequence(A.offsets, A.n_seqs, A.n_q, row, lane, [](int, int first) { return first; });
+    } else {
+        lo = 0;
+        for (int hi = A.n_seqs - 1; lo < hi;) {
+            const int mid = (lo + hi + 1) / 2;
+            if (bounded(A.offsets[mid], A.n_q) <= row) lo = mid; else hi = mid - 1;
+        }
+    }
     const Drafted D = drafted(A, lo);
-    if (row < D.row || row >= D.row + D.n) return;
-    int parts = D.end > 0 ? (D.end - 1) / A.chunk + 1 : 1;
+    if (row < D.row || row >= D.row + D.n || D.end <= A.chunk) return;
+    int parts = (D.end - 1) / A.chunk + 1;
     parts = parts < A.n_splits ? parts : A.n_splits;
     float top = -INFINITY;
-    for (int s = lane; s < parts; s += 64) top = fmaxf(top, A.part_ml[s * all + rh].x);
+    if (kMany) {
+        for (int s = lane; s < parts; s += 64) top = fmaxf(top, A.part_ml[s * all + rh].x);
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-    const int side = threadIdx.x / kCols, col = threadIdx.x % kCols;
+        for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    } else {
+        for (int s = col; s < parts; s += kCols) top = fmaxf(top, A.part_ml[s * all + rh].x);
+#pragma unroll
+        for (int x = 1; x < kCols; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    }
     float l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = side; s0 < parts; s0 += 4 * kSides) {
+    for (int s0 = kMany ? side : 0; s0 < parts; s0 += 4 * kTake) {
         float2 ml[4];
         float4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = s0 + i * kSides < parts ? s0 + i * kSides : s0;
+            const int s = s0 + i * kTake < parts ? s0 + i * kTake : s0;
             ml[i] = A.part_ml[s * all + rh];
             v[i] = *reinterpret_cast<const float4*>(A.part_o + (s * all + rh) * DP + 4 * col);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (s0 + i * kSides >= parts || ml[i].x == -INFINITY) continue;
+            if (s0 + i * kTake >= parts || ml[i].x == -INFINITY) continue;
             const float by = exp2_fast(ml[i].x - top);
             l += ml[i].y * by;
             o.x += v[i].x * by, o.y += v[i].y * by, o.z += v[i].z * by, o.w += v[i].w * by;
         }
     }
-    sums[side][col] = o;
-    if (col == 0) sides_l[side] = l;
-    __syncthreads();
-    if (side != 0) return;
-    l = 0.0f, o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (kMany) {
+        sums[side][col] = o;
+        if (col == 0) sides_l[side] = l;
+        __syncthreads();
+        if (side != 0) return;
+        l = 0.0f, o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-    for (int i = 0; i < kSides; ++i) {
-        const float4 v = sums[i][col];
-        l += sides_l[i];
-        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+        for (int i = 0; i < kTake; ++i) {
+            const float4 v = sums[i][col];
+            l += sides_l[i];
+            o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+        }
     }
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     if (4 * col < A.dim)
@@ -894,6 +923,7 @@ constexpr int kMinChunk = 512;      // keys of a part: fewer cost more in start-
 constexpr int kMaxChunk = 8192;     // and most of them, so that a long sequence among short ones does not run alone
 constexpr int kMaxSharedChunk = 4096;
 constexpr int kSlots = 256;         // workgroups of dealt-out keys that run at a time, one a CU
+constexpr int kFewParts = 16;       // at most so many are joined by DP / 4 threads a row
 constexpr int kSharedParts = 2048;  // workgroups of shared tiles: two a CU, four rounds
 
 // Rows of a workgroup. Up to 32 or 64 rows of a (sequence, head) go to every
@@ -930,12 +960,19 @@ int launch_tree_as(TreeArgs& A, hipStream_t s) {
     if (groups > INT32_MAX || static_cast<int64_t>(A.n_q) * A.heads > INT32_MAX)
         return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and keys");
     constexpr int KT = kShared && DP <= 128 ? 64 : 32;
+    const dim3 grid(static_cast<uint32_t>(groups)), block(64 * NW);
     if (A.page_size % KT == 0)
-        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, true>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
+        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 2>), grid, block, 0, s, A);
+    else if (A.page_size % Rows<DP>::kPerLoad == 0)
+        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 1>), grid, block, 0, s, A);
     else
-        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, false>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
-    if (A.n_splits > 1)
-        hipLaunchKernelGGL((tree_join_kernel<T, DP>), dim3(static_cast<uint32_t>(static_cast<int64_t>(A.n_q) * A.heads)), dim3(256), 0, s, A);
+        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 0>), grid, block, 0, s, A);
+    if (A.n_splits > kFewParts) {
+        hipLaunchKernelGGL((tree_join_kernel<T, DP, true>), dim3(static_cast<uint32_t>(A.n_q) * A.heads), dim3(256), 0, s, A);
+    } else if (A.n_splits > 1) {
+        constexpr int kRows = 1024 / DP;
+        hipLaunchKernelGGL((tree_join_kernel<T, DP, false>), dim3((static_cast<uint32_t>(A.n_q) * A.heads + kRows - 1) / kRows), dim3(256), 0, s, A);
+    }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess)
         return fail(AIMG_ERR_HIP, std::string("kernel launch failed: ") + hipGetErrorString(err));
