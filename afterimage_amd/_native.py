@@ -153,9 +153,11 @@ _SIGNATURES = [
     ("aimg_pack_chunked", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
       ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)]),
+    ("aimg_prompt_workspace_nbytes", ctypes.c_int,
+     [ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, _SIZE]),
     ("aimg_prompt_attention", ctypes.c_int,
      [_HEADS, _HEADS, _HEADS, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int,
-      ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p]),
+      ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     ("aimg_tree_workspace_nbytes", ctypes.c_int,
      [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
       ctypes.POINTER(ctypes.c_size_t)]),

@@ -338,9 +338,12 @@ struct PromptArgs {
     const uint16_t *q, *k, *v;
     uint16_t* out;
     float* lse;
+    float* part_o;    // [part][row * heads + head][DP], where keys are split
+    float2* part_ml;  // [part][row * heads + head]: c * maximum, sum
     const int32_t *q_offsets, *k_offsets;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // strides in elements
     int32_t n_seqs, heads, kv_heads, group, dim, n_q, n_k, n_slots;
+    int32_t chunk, n_splits;  // keys of a part, parts
     float c, scale;
 };
 
@@ -364,6 +367,7 @@ __device__ __forceinline__ int find_sequence(const int32_t* offsets, int n, int 
 }
 
 constexpr int kPromptKeys = 64;
+constexpr int kPromptRows = 128;  // of a workgroup
 
 // Workgroup: one sequence and key/value head, 32 * QT * NW rows of its group
 // of heads: row r is head r % group of position r / group. Rows of one position
@@ -374,6 +378,9 @@ constexpr int kPromptKeys = 64;
 // Slots: sequence b's tiles of rows start at slot first_row / rows + b, a place
 // that needs no sums over the sequences before it; slots past a sequence's
 // rows are empty. Later slots, whose rows see more keys, start first.
+// Parts: where a call has few rows and many keys (the next piece of a prompt
+// over a long context) each workgroup takes a part of its rows' keys, and
+// prompt_join_kernel joins them.
 template <typename T, int DP, int QT, int NW>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_kernel(const PromptArgs A) {
     typedef Rows<DP> R;
@@ -388,7 +395,8 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     // Consecutive workgroups take the key/value heads in turn: with eight of
     // them an XCD keeps to one head, whose keys and values stay in its L2.
     const int kvh = blockIdx.x % A.kv_heads;
-    const int slot = A.n_slots - 1 - static_cast<int>(blockIdx.x / A.kv_heads);
+    const int split = blockIdx.x / A.kv_heads % A.n_splits;
+    const int slot = A.n_slots - 1 - static_cast<int>(blockIdx.x / A.kv_heads / A.n_splits);
     const int group = A.group;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lo = find_sequence(A.q_offsets, A.n_seqs, A.n_q, slot, lane, [&](int b, int first) { return first * group / BM + b; });
@@ -405,7 +413,12 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     auto seen_by = [&](int row) { return row / group + 1 + shift < 0 ? 0 : row / group + 1 + shift; };
 
     const int keys_wg = seen_by((row0 + BM < rows ? row0 + BM : rows) - 1);  // keys that some row here sees
-    const int keys_wave = wave_row >= rows ? 0 : seen_by((wave_row + 32 * QT < rows ? wave_row + 32 * QT : rows) - 1);
+    const int begin = split * A.chunk;
+    if (split > 0 && begin >= keys_wg) return;
+    const bool parted = keys_wg > A.chunk;
+    const int end = keys_wg - begin < A.chunk ? keys_wg : begin + A.chunk;
+    int keys_wave = wave_row >= rows ? 0 : seen_by((wave_row + 32 * QT < rows ? wave_row + 32 * QT : rows) - 1);
+    keys_wave = keys_wave < end ? keys_wave : end;
 
     const uint16_t* const k_base = A.k + k_begin * A.k_row + kvh * A.k_head;
     const uint16_t* const v_base = A.v + k_begin * A.v_row + kvh * A.v_head;
@@ -430,7 +443,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
             load_to_lds(vb + (from * v_bytes + vp), to + kTile + load * 1024);
         }
     };
-    if (keys_wg > 0) load_tile(0, shared);
+    if (begin < end) load_tile(begin, shared);
     State<T, DP, QT> st;
     st.clear();
     int32_t sees[QT];  // keys that the lane's rows see
@@ -443,14 +456,14 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     }
     wait_loads<0>();
     __syncthreads();
-    int k0 = 0;
+    int k0 = begin;
     uint32_t at = 0;  // the tile's place in LDS
     // Tiles that every row of the workgroup sees whole, then those it needs
     // masks for. The two places are passed as restrict pointers: the compiler
     // then knows that reads of a tile need not wait for the loads of the next.
-    for (const int whole = row0 / group + 1 + shift; k0 + KT <= whole; k0 += KT, at ^= 2 * kTile) {
+    for (const int whole = row0 / group + 1 + shift; k0 + KT <= whole && k0 < end; k0 += KT, at ^= 2 * kTile) {
         auto tile = [&](lds_char* __restrict__ next, const lds_char* __restrict__ now) __attribute__((always_inline)) {
-            if (k0 + KT < keys_wg) load_tile(k0 + KT, next);
+            if (k0 + KT < end) load_tile(k0 + KT, next);
             const uint32_t all[QT][NSUB] = {};
             st.template step<NSUB, false>(now, now + kTile, A.c, lane, all);
         };
@@ -458,9 +471,9 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
         wait_loads<0>();
         __syncthreads();
     }
-    for (; k0 < keys_wg; k0 += KT, at ^= 2 * kTile) {
+    for (; k0 < end; k0 += KT, at ^= 2 * kTile) {
         auto tile = [&](lds_char* __restrict__ next, const lds_char* __restrict__ now) __attribute__((always_inline)) {
-            if (k0 + KT < keys_wg) load_tile(k0 + KT, next);
+            if (k0 + KT < end) load_tile(k0 + KT, next);
             if (k0 < keys_wave) {
                 uint32_t allow[QT][NSUB];
 #pragma unroll
@@ -481,7 +494,9 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
         const float l = add_halves(st.l[t]);
         if (r >= rows) continue;
         const int row = q_begin + r / group, head = kvh * group + r % group;
-        const float by = l == 0.0f ? 0.0f : 1.0f / l;
+        const int64_t rh = static_cast<int64_t>(row) * A.heads + head;
+        const int64_t part = static_cast<int64_t>(split) * A.n_q * A.heads + rh;
+        const float by = parted ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
         uint16_t* const to = A.out + row * A.out_row + head * A.out_head;
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d)
@@ -489,21 +504,108 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
             for (int i = 0; i < 4; ++i) {
                 const int x = 32 * d + 8 * i + 4 * half;
                 const f32x16& o = st.o[t][d];
-                if (x < A.dim) store_four<T>(to + x, o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
+                if (parted)
+                    *reinterpret_cast<float4*>(A.part_o + part * DP + x) = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                else if (x < A.dim)
+                    store_four<T>(to + x, o[4 * i] * by, o[4 * i + 1] * by, o[4 * i + 2] * by, o[4 * i + 3] * by);
             }
-        if (A.lse != nullptr && half == 0)
-            A.lse[static_cast<int64_t>(row) * A.heads + head] = l == 0.0f ? -INFINITY : st.m[t] * A.scale + logf(l);
+        if (half != 0) continue;
+        if (parted) A.part_ml[part] = make_float2(st.m[t] * A.c, l);
+        else if (A.lse != nullptr) A.lse[rh] = l == 0.0f ? -INFINITY : st.m[t] * A.scale + logf(l);
     }
+}
+
+// One row and head's parts in their order, by DP / 4 threads with four columns each.
+template <typename T, int DP>
+__device__ __forceinline__ void join_parts(const float* part_o, const float2* part_ml, int64_t all, int64_t rh, int parts, int col,
+                                           int dim, uint16_t* to, float* lse) {
+    constexpr int kCols = DP / 4;
+    float top = -INFINITY;
+    for (int s = col; s < parts; s += kCols) top = fmaxf(top, part_ml[s * all + rh].x);
+#pragma unroll
+    for (int x = 1; x < kCols; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    float l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s0 = 0; s0 < parts; s0 += 4) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i < parts ? s0 + i : s0;
+            ml[i] = part_ml[s * all + rh];
+            v[i] = *reinterpret_cast<const float4*>(part_o + (s * all + rh) * DP + 4 * col);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + i >= parts || ml[i].x == -INFINITY) continue;  // a part without a visible key
+            const float by = exp2_fast(ml[i].x - top);
+            l += ml[i].y * by;
+            o.x += v[i].x * by, o.y += v[i].y * by, o.z += v[i].z * by, o.w += v[i].w * by;
+        }
+    }
+    const float by = l == 0.0f ? 0.0f : 1.0f / l;
+    if (4 * col < dim) store_four<T>(to + 4 * col, o.x * by, o.y * by, o.z * by, o.w * by);
+    if (col == 0 && lse != nullptr) *lse = l == 0.0f ? -INFINITY : top * (1.0f / kLog2E) + logf(l);
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void prompt_join_kernel(const PromptArgs A) {
+    constexpr int kCols = DP / 4, kSides = 256 / kCols;
+    const int64_t all = static_cast<int64_t>(A.n_q) * A.heads;
+    const int64_t rh = static_cast<int64_t>(blockIdx.x) * kSides + threadIdx.x / kCols;
+    if (rh >= all) return;
+    const int row = static_cast<int>(rh / A.heads), head = static_cast<int>(rh % A.heads);
+    int lo = 0;
+    for (int hi = A.n_seqs - 1; lo < hi;) {
+        const int mid = (lo + hi + 1) / 2;
+        if (bounded(A.q_offsets[mid], A.n_q) <= row) lo = mid; else hi = mid - 1;
+    }
+    const int q_begin = bounded(A.q_offsets[lo], A.n_q), q_end = bounded(A.q_offsets[lo + 1], A.n_q);
+    const int k_begin = bounded(A.k_offsets[lo], A.n_k), k_end = bounded(A.k_offsets[lo + 1], A.n_k);
+    if (row < q_begin || row >= q_end) return;
+    const int q_len = q_end - q_begin, k_len = k_end > k_begin ? k_end - k_begin : 0;
+    // The keys of the row's workgroup decide its parts.
+    const int rows = q_len * A.group, r = (row - q_begin) * A.group + head % A.group;
+    const int row0 = r / kPromptRows * kPromptRows;
+    const int last = (row0 + kPromptRows < rows ? row0 + kPromptRows : rows) - 1;
+    const int keys = last / A.group + 1 + k_len - q_len;
+    if (keys <= A.chunk) return;
+    join_parts<T, DP>(A.part_o, A.part_ml, all, rh, (keys - 1) / A.chunk + 1, threadIdx.x % kCols, A.dim,
+                      A.out + row * A.out_row + head * A.out_head, A.lse != nullptr ? A.lse + rh : nullptr);
+}
+
+int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+// Keys of a part. Calls that fill the GPU with their rows alone, or whose
+// sequences have few keys, are not split (the join costs some 5 us).
+void plan_prompt(PromptArgs& A, int64_t n_rows, int64_t n_keys) {
+    const int64_t groups = (n_rows * A.group / kPromptRows + A.n_seqs) * A.kv_heads;
+    const int64_t each = A.n_seqs > 0 ? n_keys / A.n_seqs : 0;  // keys of a sequence, about
+    int64_t chunk = INT32_MAX / 2;
+    if (groups <= 384 && each > 1024) {
+        const int64_t parts = 1024 / (groups > 0 ? groups : 1);
+        chunk = each / parts > 512 ? each / parts : 512;
+        if (n_keys / chunk >= 64) chunk = n_keys / 64 + 1;  // sequences far longer than the others
+        chunk = (chunk + 63) / 64 * 64;
+    }
+    A.chunk = static_cast<int32_t>(chunk);
+    A.n_splits = n_keys > chunk ? static_cast<int32_t>((n_keys + chunk - 1) / chunk) : 1;
 }
 
 template <typename T, int DP>
 int launch_prompt(PromptArgs& A, hipStream_t s) {
     constexpr int QT = 1, NW = 4, BM = 32 * QT * NW;
+    static_assert(BM == kPromptRows, "the join goes by the same rows");
     const int64_t rows = static_cast<int64_t>(A.n_q) * A.group;
-    const int64_t groups = (rows / BM + A.n_seqs) * A.kv_heads;
+    const int64_t groups = (rows / BM + A.n_seqs) * A.kv_heads * A.n_splits;
     if (rows > INT32_MAX || groups > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "prompt attention: too many rows times heads");
     A.n_slots = static_cast<int32_t>(rows / BM + A.n_seqs);
     hipLaunchKernelGGL((prompt_kernel<T, DP, QT, NW>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
+    if (A.n_splits > 1) {
+        constexpr int kRows = 1024 / DP;
+        const int64_t all = static_cast<int64_t>(A.n_q) * A.heads;
+        hipLaunchKernelGGL((prompt_join_kernel<T, DP>), dim3(static_cast<uint32_t>((all + kRows - 1) / kRows)), dim3(256), 0, s, A);
+    }
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess)
         return fail(AIMG_ERR_HIP, std::string("kernel launch failed: ") + hipGetErrorString(err));
@@ -824,7 +926,6 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
 template <typename T, int DP, bool kMany>
 __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
     constexpr int kCols = DP / 4, kSides = 256 / kCols;
-    constexpr int kTake = kMany ? kSides : 1;  // sides that share a row
     __shared__ float4 sums[kMany ? kSides : 1][kCols];
     __shared__ float sides_l[kMany ? kSides : 1];
     const int lane = threadIdx.x & 63;
@@ -847,47 +948,43 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
     if (row < D.row || row >= D.row + D.n || D.end <= A.chunk) return;
     int parts = (D.end - 1) / A.chunk + 1;
     parts = parts < A.n_splits ? parts : A.n_splits;
-    float top = -INFINITY;
-    if (kMany) {
-        for (int s = lane; s < parts; s += 64) top = fmaxf(top, A.part_ml[s * all + rh].x);
-#pragma unroll
-        for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-    } else {
-        for (int s = col; s < parts; s += kCols) top = fmaxf(top, A.part_ml[s * all + rh].x);
-#pragma unroll
-        for (int x = 1; x < kCols; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
+    if constexpr (!kMany) {
+        join_parts<T, DP>(A.part_o, A.part_ml, all, rh, parts, col, A.dim, A.out + row * A.out_row + head * A.out_head,
+                          A.lse != nullptr ? A.lse + rh : nullptr);
+        return;
     }
+    float top = -INFINITY;
+    for (int s = lane; s < parts; s += 64) top = fmaxf(top, A.part_ml[s * all + rh].x);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
     float l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s0 = kMany ? side : 0; s0 < parts; s0 += 4 * kTake) {
+    for (int s0 = side; s0 < parts; s0 += 4 * kSides) {
         float2 ml[4];
         float4 v[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = s0 + i * kTake < parts ? s0 + i * kTake : s0;
+            const int s = s0 + i * kSides < parts ? s0 + i * kSides : s0;
             ml[i] = A.part_ml[s * all + rh];
             v[i] = *reinterpret_cast<const float4*>(A.part_o + (s * all + rh) * DP + 4 * col);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (s0 + i * kTake >= parts || ml[i].x == -INFINITY) continue;
+            if (s0 + i * kSides >= parts || ml[i].x == -INFINITY) continue;
             const float by = exp2_fast(ml[i].x - top);
             l += ml[i].y * by;
             o.x += v[i].x * by, o.y += v[i].y * by, o.z += v[i].z * by, o.w += v[i].w * by;
         }
     }
-    if (kMany) {
-        sums[side][col] = o;
-        if (col == 0) sides_l[side] = l;
-        __syncthreads();
-        if (side != 0) return;
-        l = 0.0f, o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int i = 0; i < kTake; ++i) {
-            const float4 v = sums[i][col];
-            l += sides_l[i];
-            o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
-        }
+    sums[side][col] = o;
+    if (col == 0) sides_l[side] = l;
+    __syncthreads();
+    if (side != 0) return;
+    l = 0.0f, o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < kSides; ++i) {
+        const float4 v = sums[i][col];
+        l += sides_l[i];
+        o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
     }
     const float by = l == 0.0f ? 0.0f : 1.0f / l;
     if (4 * col < A.dim)
@@ -952,7 +1049,6 @@ void plan_parts(TreeArgs& A, int64_t max_context) {
     A.n_splits = static_cast<int32_t>((longest + chunk - 1) / chunk);
 }
 
-int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 template <typename T, int DP, int QT, int NW, bool kShared>
 int launch_tree_as(TreeArgs& A, hipStream_t s) {
@@ -1046,9 +1142,23 @@ int check_scale(float scale) {
 
 }  // namespace
 
+extern "C" int aimg_prompt_workspace_nbytes(int64_t n_rows, int64_t n_keys, int heads, int kv_heads, int dim, int n_seqs,
+                                            size_t* nbytes) {
+    using aimg::fail;
+    if (nbytes == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "nbytes is null");
+    if (n_rows < 0 || n_rows > INT32_MAX || n_keys < 0 || n_keys > INT32_MAX || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 ||
+        dim < 1 || dim > aimg::kMaxDim || n_seqs < 0)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "prompt attention: rows, keys, heads, dim and n_seqs must be sizes of one call");
+    aimg::PromptArgs a{};
+    a.n_seqs = n_seqs, a.kv_heads = kv_heads, a.group = heads / kv_heads;
+    aimg::plan_prompt(a, n_rows, n_keys);
+    *nbytes = a.n_splits > 1 ? static_cast<size_t>(n_rows) * heads * a.n_splits * (4 * aimg::padded_dim(dim) + 8) : 0;
+    return AIMG_OK;
+}
+
 extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, const aimg_heads* v, const aimg_heads* out,
                                      const int32_t* q_offsets, const int32_t* k_offsets, int n_seqs, int type,
-                                     float scale, float* lse, void* stream) {
+                                     float scale, float* lse, void* workspace, size_t workspace_nbytes, void* stream) {
     using aimg::fail;
     int rc = check_heads(q, "q");
     if (rc == AIMG_OK) rc = check_heads(k, "k");
@@ -1080,6 +1190,14 @@ extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, c
     a.n_seqs = n_seqs, a.heads = q->heads, a.kv_heads = k->heads, a.group = q->heads / k->heads, a.dim = q->dim;
     a.n_q = static_cast<int32_t>(q->n_rows), a.n_k = static_cast<int32_t>(k->n_rows);
     a.c = scale * aimg::kLog2E, a.scale = scale;
+    aimg::plan_prompt(a, q->n_rows, k->n_rows);
+    const int64_t part_rows = q->n_rows * q->heads * a.n_splits;
+    const int dp = aimg::padded_dim(q->dim);
+    if (a.n_splits > 1 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+                           workspace_nbytes < static_cast<size_t>(part_rows) * (4 * dp + 8)))
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "the workspace is null, misaligned or below aimg_prompt_workspace_nbytes");
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows * dp);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return by_type(type, q->dim, [&](auto t, int dim) {
         typedef decltype(t) T;

@@ -107,6 +107,13 @@ def launch(entry, index: int, *args) -> None:
         _native.check(status)
 
 
+@functools.lru_cache(maxsize=1024)
+def _prompt_workspace_nbytes(n: int, n_keys: int, heads: int, kv_heads: int, dim: int, n_seqs: int) -> int:
+    nbytes = ctypes.c_size_t(0)
+    _native.check(_native.lib().aimg_prompt_workspace_nbytes(n, n_keys, heads, kv_heads, dim, n_seqs, ctypes.byref(nbytes)))
+    return nbytes.value
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                      k_offsets: torch.Tensor | None = None, *, scale: float | None = None,
                      out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
@@ -122,7 +129,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
     gives zeros. scale is 1 / sqrt(dim) when not given.
 
     Returns out (q's shape and type; rows of no sequence are not written).
-    lse, fp32 [rows, heads], receives log(sum(exp(scale * q.k))) when given."""
+    lse, fp32 [rows, heads], receives log(sum(exp(scale * q.k))) when given.
+    Results do not vary between calls."""
     qd, index, kind = _query(q)
     kd, vd = _heads(k, "k", q.dtype, index), _heads(v, "v", q.dtype, index)
     if kd.n_rows != vd.n_rows or kd.heads != vd.heads or kd.dim != qd.dim or vd.dim != qd.dim:
@@ -142,7 +150,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
         raise ValueError("q_offsets and k_offsets must have one entry more than there are sequences, got %d and %d"
                          % (n_seqs + 1, n_keys + 1))
     out, od = _result(q, qd, out, index)
-    launch(_native.lib().aimg_prompt_attention, index, qd, kd, vd, od, q_at, k_at, n_seqs, kind, _scale(scale, qd.dim), _lse(lse, q))
+    nbytes = _prompt_workspace_nbytes(qd.n_rows, kd.n_rows, qd.heads, kd.heads, qd.dim, n_seqs)
+    # From torch's allocator on the current stream, which the launches use.
+    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+    launch(_native.lib().aimg_prompt_attention, index, qd, kd, vd, od, q_at, k_at, n_seqs, kind, _scale(scale, qd.dim), _lse(lse, q),
+           work, nbytes)
     return out
 
 

@@ -295,10 +295,15 @@ typedef struct aimg_heads {
  * or float[q->n_rows][q->heads] (device) for log(sum(exp(scale * q.k))), -inf
  * for a row that sees no key. scale > 0. Offsets outside the rows are bounded
  * to them; keys that a row does not see never reach it, whatever they hold.
+ * aimg_prompt_workspace_nbytes gives the device scratch memory a call of these
+ * sizes needs (16-byte aligned; 0, for most: none): few rows over many keys are
+ * split along the keys and joined in order. Results do not vary between calls.
  */
+int aimg_prompt_workspace_nbytes(int64_t n_rows, int64_t n_keys, int heads, int kv_heads, int dim, int n_seqs,
+                                 size_t* nbytes);
 int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, const aimg_heads* v, const aimg_heads* out,
                           const int32_t* q_offsets, const int32_t* k_offsets, int n_seqs, int type,
-                          float scale, float* lse, void* stream);
+                          float scale, float* lse, void* workspace, size_t workspace_nbytes, void* stream);
 
 /* The keys and values of one layer in a paged cache: position j of sequence
  * slot s is row j % page_size of page page_table[s * table_stride + j /

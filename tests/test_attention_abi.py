@@ -32,7 +32,7 @@ def _cache(**more):
 def _prompt(q=None, k=None, v=None, out=None, at=64, n=1, kind=0, scale=1.0):
     q, k = q or _heads(), k or _heads()
     v, out = v or k, out or q
-    return _native.lib().aimg_prompt_attention(q, k, v, out, at, at, n, kind, scale, None, None)
+    return _native.lib().aimg_prompt_attention(q, k, v, out, at, at, n, kind, scale, None, None, 0, None)
 
 
 def _tree(q=None, pages=None, n=1, most=1, context=10, words=1, scale=1.0, at=64, kind=0, work=None, nbytes=0):
@@ -95,6 +95,22 @@ def test_tree_workspace_follows_the_sizes():
     assert nbytes(0, 40, 8, 128, 0, 1, 8000) == 0
     assert lib.aimg_tree_workspace_nbytes(1, 40, 7, 128, 1, 1, 0, ctypes.byref(n)) == BAD
     assert lib.aimg_tree_workspace_nbytes(1, 40, 8, 128, 1, 1, 0, None) == BAD
+
+
+def test_prompt_workspace_follows_the_sizes():
+    lib, n = _native.lib(), ctypes.c_size_t()
+
+    def nbytes(*sizes):
+        assert lib.aimg_prompt_workspace_nbytes(*sizes, ctypes.byref(n)) == OK
+        return n.value
+    # Rows that fill the GPU, or few keys: none. Few rows over many keys: a row of sums and two numbers a part.
+    assert nbytes(16384, 16384, 40, 8, 128, 1) == 0 and nbytes(77, 77, 16, 16, 64, 1) == 0 and nbytes(0, 0, 4, 2, 64, 0) == 0
+    parts, rest = divmod(nbytes(13, 8000, 8, 1, 96, 1), 13 * 8 * (4 * 128 + 8))
+    assert parts > 1 and rest == 0
+    assert lib.aimg_prompt_workspace_nbytes(13, 8000, 8, 3, 96, 1, ctypes.byref(n)) == BAD
+    q, k = _heads(n=13, heads=8), _heads(n=8000, heads=1)
+    assert lib.aimg_prompt_attention(q, k, k, q, 64, 64, 1, 0, 1.0, None, None, 0, None) == BAD
+    assert b"workspace" in lib.aimg_last_error()
 
 
 @pytest.mark.parametrize("more,code,message", [

@@ -46,6 +46,11 @@ SHAPES = [
     ([257, 100], [300, 100], 4, 2, 256),
     ([129], [400], 2, 1, 168),
     ([513, 40], [513, 1000], 40, 8, 128),
+    # Few rows over many keys: split along the keys.
+    ([13], [2900], 8, 1, 128),
+    ([1, 30, 7, 2], [1, 3000, 700, 5000], 10, 2, 64),
+    ([40, 9], [1400, 2600], 8, 4, 256),
+    ([150], [1600], 5, 1, 96),
 ]
 
 
