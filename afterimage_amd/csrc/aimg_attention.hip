@@ -65,9 +65,14 @@ struct Fp16 {
     }
 };
 
-// A maximum is raised only where it grew by more than this (in powers of
-// two): below it the probabilities stay under 2^8, far inside the range of
-// both types and of the fp32 sums, and o and l need no multiplication.
+// m need not be the maximum itself: any number near enough keeps 2^(s - m) in
+// range, and the quotient o / l is the same. It is set at a row's first visible
+// tile and then left alone while a lane's sum of 32 (or 16) probabilities
+// stays below kMostSum, so that each is far inside the range of both types; a
+// tile then needs no maximum and o and l no multiplication. Where the sum is
+// more, some probability is over 2^9 and the maximum is raised if it grew by
+// more than 2^kRise.
+constexpr float kMostSum = 16384.0f;
 constexpr float kRise = 8.0f;
 constexpr float kLog2E = 1.44269504088896340736f;
 constexpr int kMaxDim = 256;
@@ -185,39 +190,17 @@ struct State {
                     for (int i = 0; i < 16; ++i) s[t][u][i] = seen_or(bits, 8 * (i / 4) + i % 4, s[t][u][i]);
                 }
             }
-            float top = s[t][0][0];
-#pragma unroll
-            for (int u = 0; u < NSUB; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][u][i]);
-            top = max_halves(top);
-            const bool rise = (top - m[t]) * c > kRise;  // false where both are -inf
-            if (__any(rise)) {
-                const float to = rise ? top : m[t];
-                const float by = rise ? exp2_fast((m[t] - to) * c) : 1.0f;
-                m[t] = to;
-                l[t] *= by;
-#pragma unroll
-                for (int d = 0; d < kBlocks; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[t][d][i] *= by;
-            }
-            const float mc = m[t] == -INFINITY ? 0.0f : m[t] * c;
+            // The maximum is not needed where the probabilities against the
+            // one held stay in range: their sum, which is, tells.
             float sum = 0.0f;
-#pragma unroll
-            for (int u = 0; u < NSUB; ++u) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[t][u][i] = exp2_fast(fmaf(s[t][u][i], c, -mc));
-                    sum += s[t][u][i];
-                }
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    u32x4 w;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = T::pack(s[t][u][8 * k + 2 * i], s[t][u][8 * k + 2 * i + 1]);
-                    p[t][u][k] = __builtin_bit_cast(s16x8, w);
-                }
+            bool fits = false;
+            if (!__any(m[t] == -INFINITY)) {
+                sum = soften<NSUB>(s[t], p[t], c, m[t] * c);
+                fits = __all(sum <= kMostSum);
+            }
+            if (__builtin_expect(!fits, 0)) {
+                raise<NSUB>(t, s[t], c);
+                sum = soften<NSUB>(s[t], p[t], c, m[t] == -INFINITY ? 0.0f : m[t] * c);
             }
             l[t] += sum;
         }
@@ -237,6 +220,46 @@ struct State {
                     for (int t = 0; t < QT; ++t) o[t][d] = T::mfma(a, p[t][u][k], o[t][d]);
                 }
         if (kMasked && __any(odd != 0)) add_infinite<NSUB>(first, piece, r, half, allow);
+    }
+
+    // A lane's probabilities 2^(c s - mc), packed for the second product; returns their sum.
+    template <int NSUB>
+    static __device__ __forceinline__ float soften(const f32x16 (&s)[NSUB], s16x8 (&p)[NSUB][2], float c, float mc) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x = exp2_fast(fmaf(s[u][8 * k + 2 * i], c, -mc)), y = exp2_fast(fmaf(s[u][8 * k + 2 * i + 1], c, -mc));
+                    sum += x + y;
+                    w[i] = T::pack(x, y);
+                }
+                p[u][k] = __builtin_bit_cast(s16x8, w);
+            }
+        return sum;
+    }
+
+    // The maximum of tile t raised to that of its scores, the sums with it.
+    template <int NSUB>
+    __device__ __forceinline__ void raise(int t, const f32x16 (&s)[NSUB], float c) {
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+        top = max_halves(top);
+        const bool rise = (top - m[t]) * c > kRise;  // false where both are -inf
+        const float to = rise ? top : m[t];
+        const float by = rise ? exp2_fast((m[t] - to) * c) : 1.0f;
+        m[t] = to;
+        l[t] *= by;
+#pragma unroll
+        for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][d][i] *= by;
     }
 
     // V^T of keys 32 u + 16 k + {0..3, 8..11} (+ 4 in the upper half) and block d of columns.
@@ -381,7 +404,7 @@ constexpr int kPromptRows = 128;  // of a workgroup
 // Parts: where a call has few rows and many keys (the next piece of a prompt
 // over a long context) each workgroup takes a part of its rows' keys, and
 // prompt_join_kernel joins them.
-template <typename T, int DP, int QT, int NW>
+template <typename T, int DP, int QT, int NW, bool kParts>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_kernel(const PromptArgs A) {
     typedef Rows<DP> R;
     constexpr int KT = DP <= 128 ? kPromptKeys : 32;
@@ -395,8 +418,8 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     // Consecutive workgroups take the key/value heads in turn: with eight of
     // them an XCD keeps to one head, whose keys and values stay in its L2.
     const int kvh = blockIdx.x % A.kv_heads;
-    const int split = blockIdx.x / A.kv_heads % A.n_splits;
-    const int slot = A.n_slots - 1 - static_cast<int>(blockIdx.x / A.kv_heads / A.n_splits);
+    const int split = kParts ? blockIdx.x / A.kv_heads % A.n_splits : 0;
+    const int slot = A.n_slots - 1 - static_cast<int>(blockIdx.x / A.kv_heads / (kParts ? A.n_splits : 1));
     const int group = A.group;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lo = find_sequence(A.q_offsets, A.n_seqs, A.n_q, slot, lane, [&](int b, int first) { return first * group / BM + b; });
@@ -413,10 +436,10 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     auto seen_by = [&](int row) { return row / group + 1 + shift < 0 ? 0 : row / group + 1 + shift; };
 
     const int keys_wg = seen_by((row0 + BM < rows ? row0 + BM : rows) - 1);  // keys that some row here sees
-    const int begin = split * A.chunk;
+    const int begin = kParts ? split * A.chunk : 0;
     if (split > 0 && begin >= keys_wg) return;
-    const bool parted = keys_wg > A.chunk;
-    const int end = keys_wg - begin < A.chunk ? keys_wg : begin + A.chunk;
+    const bool parted = kParts && keys_wg > A.chunk;
+    const int end = !kParts || keys_wg - begin < A.chunk ? keys_wg : begin + A.chunk;
     int keys_wave = wave_row >= rows ? 0 : seen_by((wave_row + 32 * QT < rows ? wave_row + 32 * QT : rows) - 1);
     keys_wave = keys_wave < end ? keys_wave : end;
 
@@ -600,8 +623,11 @@ int launch_prompt(PromptArgs& A, hipStream_t s) {
     const int64_t groups = (rows / BM + A.n_seqs) * A.kv_heads * A.n_splits;
     if (rows > INT32_MAX || groups > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "prompt attention: too many rows times heads");
     A.n_slots = static_cast<int32_t>(rows / BM + A.n_seqs);
-    hipLaunchKernelGGL((prompt_kernel<T, DP, QT, NW>), dim3(static_cast<uint32_t>(groups)), dim3(64 * NW), 0, s, A);
-    if (A.n_splits > 1) {
+    const dim3 grid(static_cast<uint32_t>(groups)), block(64 * NW);
+    if (A.n_splits == 1) {
+        hipLaunchKernelGGL((prompt_kernel<T, DP, QT, NW, false>), grid, block, 0, s, A);
+    } else {
+        hipLaunchKernelGGL((prompt_kernel<T, DP, QT, NW, true>), grid, block, 0, s, A);
         constexpr int kRows = 1024 / DP;
         const int64_t all = static_cast<int64_t>(A.n_q) * A.heads;
         hipLaunchKernelGGL((prompt_join_kernel<T, DP>), dim3(static_cast<uint32_t>((all + kRows - 1) / kRows)), dim3(256), 0, s, A);
