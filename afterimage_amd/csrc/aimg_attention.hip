@@ -560,7 +560,7 @@ __device__ __forceinline__ void join_parts(const float* part_o, const float2* pa
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (s0 + i >= parts || ml[i].x == -INFINITY) continue;  // a part without a visible key
+            if (s0 + i >= parts || ml[i].y == 0.0f) continue;  // a part without a visible key (NaN scores leave a NaN sum)
             const float by = exp2_fast(ml[i].x - top);
             l += ml[i].y * by;
             o.x += v[i].x * by, o.y += v[i].y * by, o.z += v[i].z * by, o.w += v[i].w * by;
@@ -925,7 +925,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float2 one = ml[w * 32 * QT + r];
-            if (one.x == -INFINITY) continue;  // a wave without a visible key
+            if (one.y == 0.0f) continue;  // a wave without a visible key (NaN scores leave a NaN sum)
             const float by = exp2_fast(one.x - top);
             const float4 v = *reinterpret_cast<const float4*>(sums + (w * 32 * QT + r) * kRow + x);
             l += one.y * by;
@@ -996,7 +996,7 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (s0 + i * kSides >= parts || ml[i].x == -INFINITY) continue;
+            if (s0 + i * kSides >= parts || ml[i].y == 0.0f) continue;
             const float by = exp2_fast(ml[i].x - top);
             l += ml[i].y * by;
             o.x += v[i].x * by, o.y += v[i].y * by, o.z += v[i].z * by, o.w += v[i].w * by;

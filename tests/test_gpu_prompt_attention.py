@@ -101,6 +101,19 @@ def test_what_a_row_does_not_see_does_not_reach_it(bad, dtype):
     assert torch.equal(out[rest], clean[rest]) and bool(torch.isnan(out[at:200]).all())
 
 
+@pytest.mark.parametrize("rows,keys,heads,kv", [([40, 9], [40, 9], 4, 2), ([13], [2900], 8, 1), ([1, 30, 7], [1, 3000, 700], 10, 2)])
+def test_a_nan_query_gives_nan_and_no_other_row_does(rows, keys, heads, kv):
+    q, k, v = _case(rows, keys, heads, kv, 64, torch.bfloat16)
+    clean = prompt_attention(q, k, v, _offsets(rows), _offsets(keys))
+    q[5, 2, 30] = float("nan")
+    lse = torch.empty(q.shape[:2], device="cuda")
+    out = prompt_attention(q, k, v, _offsets(rows), _offsets(keys), lse=lse)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    hit[5, 2] = True
+    assert bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], clean[~hit])
+    assert torch.equal(torch.isnan(lse), hit[..., 0])
+
+
 def test_opposite_infinities_meet_in_a_masked_tile():
     q, k, v = _case([20], [20], 1, 1, 64, torch.bfloat16)
     v[3, 0, 7], v[5, 0, 7] = float("inf"), float("-inf")

@@ -168,6 +168,22 @@ def test_bad_values_of_an_unseen_draft(heads, kv, dtype):
     assert torch.equal(out[~hit], clean[~hit]) and bool(torch.isnan(out[hit]).all())
 
 
+@pytest.mark.parametrize("contexts,drafts,heads,kv", [([45, 20], [3, 4], 8, 2), ([3000, 200], [3, 4], 8, 2), ([14000], [2], 4, 4),
+                                                      ([2000, 90], [30, 9], 40, 8)])
+def test_a_nan_query_gives_nan_and_no_other_row_does(contexts, drafts, heads, kv):
+    """However a row's keys are split: with every score NaN no part has a maximum, and the sums still tell."""
+    c = Case(contexts, drafts, heads, kv, 128, 16, torch.bfloat16)
+    clean = c.run()
+    q = c.q.clone()
+    q[1, 2, 70] = float("nan")
+    lse = torch.empty(c.q.shape[:2], device="cuda")
+    out = c.run(q=q, lse=lse)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    hit[1, 2] = True
+    assert bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], clean[~hit])
+    assert torch.equal(torch.isnan(lse), hit[..., 0])
+
+
 def test_pages_of_another_layout_and_a_strided_table():
     """Positions outermost in a page, and a table that is part of a wider one."""
     c = Case([100, 260], [6, 2], 8, 4, 64, 32, torch.float16)
