@@ -1042,6 +1042,7 @@ __global__ __launch_bounds__(256) void tree_masks_kernel(const int32_t* parents,
     }
 }
 
+constexpr int64_t kMaxPositions = 1 << 30;  // of a sequence, by the checks of its pages
 constexpr int kMinChunk = 512;      // keys of a part: fewer cost more in start-up and joining than they save
 constexpr int kMaxChunk = 8192;     // and most of them, so that a long sequence among short ones does not run alone
 constexpr int kMaxSharedChunk = 4096;
@@ -1058,7 +1059,8 @@ void plan_parts(TreeArgs& A, int64_t max_context) {
     const int64_t rows = static_cast<int64_t>(A.max_drafts) * (A.heads / A.kv_heads);
     const int per = tree_rows(A.dim, rows);
     A.row_blocks = static_cast<int32_t>((rows + per - 1) / per);
-    const int64_t longest = max_context + A.max_drafts;
+    // No sequence holds more than 2^30 positions, so a part's first key is an int32.
+    const int64_t longest = max_context + A.max_drafts < kMaxPositions ? max_context + A.max_drafts : kMaxPositions;
     const int64_t units = static_cast<int64_t>(A.n_seqs) * A.kv_heads * A.row_blocks;
     int64_t chunk, most = kMaxChunk;
     if (per <= 64) {
@@ -1075,12 +1077,9 @@ void plan_parts(TreeArgs& A, int64_t max_context) {
     A.n_splits = static_cast<int32_t>((longest + chunk - 1) / chunk);
 }
 
-
 template <typename T, int DP, int QT, int NW, bool kShared>
 int launch_tree_as(TreeArgs& A, hipStream_t s) {
     const int64_t groups = static_cast<int64_t>(A.n_seqs) * A.kv_heads * A.row_blocks * A.n_splits;
-    if (groups > INT32_MAX || static_cast<int64_t>(A.n_q) * A.heads > INT32_MAX)
-        return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and keys");
     constexpr int KT = kShared && DP <= 128 ? 64 : 32;
     const dim3 grid(static_cast<uint32_t>(groups)), block(64 * NW);
     if (A.page_size % KT == 0)
@@ -1235,14 +1234,23 @@ extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, c
 
 namespace {
 
-// What the sizes of one tree attention call imply; false where they are no such call.
-bool tree_sizes(aimg::TreeArgs& a, int n_seqs, int heads, int kv_heads, int dim, int max_drafts, int64_t max_context) {
-    if (n_seqs < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dim < 1 || max_drafts < 1 || max_context < 0 ||
-        max_context > INT32_MAX)
-        return false;
-    a.n_seqs = n_seqs, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim, a.max_drafts = max_drafts;
+// What the sizes of one tree attention call imply.
+int tree_sizes(aimg::TreeArgs& a, int64_t n_rows, int n_seqs, int heads, int kv_heads, int dim, int max_drafts, int64_t max_context) {
+    using aimg::fail;
+    if (n_rows < 0 || n_rows > INT32_MAX || n_seqs < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dim < 1 ||
+        dim > aimg::kMaxDim || max_drafts < 1 || max_context < 0 || max_context > INT32_MAX)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "tree attention: n_seqs and max_context must be >= 0 (max_context below 2^31), max_drafts >= 1, "
+                                               "rows, heads and dim sizes of one call");
+    if (n_rows * heads > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many rows times heads");
+    a.n_seqs = n_seqs, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
+    a.max_drafts = max_drafts < n_rows ? max_drafts : n_rows > 0 ? static_cast<int32_t>(n_rows) : 1;  // no sequence has more
+    const int64_t blocks = (static_cast<int64_t>(a.max_drafts) * (heads / kv_heads) + 31) / 32;  // at least the row blocks
+    if (static_cast<int64_t>(n_seqs) * kv_heads > INT32_MAX / blocks)
+        return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and rows");
     aimg::plan_parts(a, max_context);
-    return true;
+    if (static_cast<int64_t>(n_seqs) * kv_heads * a.row_blocks > INT32_MAX / a.n_splits)
+        return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and keys");
+    return AIMG_OK;
 }
 
 }  // namespace
@@ -1252,8 +1260,8 @@ extern "C" int aimg_tree_workspace_nbytes(int64_t n_rows, int heads, int kv_head
     using aimg::fail;
     if (nbytes == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "nbytes is null");
     aimg::TreeArgs a{};
-    if (n_rows < 0 || n_rows > INT32_MAX || !tree_sizes(a, n_seqs, heads, kv_heads, dim, max_drafts, max_context) || dim > aimg::kMaxDim)
-        return fail(AIMG_ERR_INVALID_ARGUMENT, "tree attention: rows, heads, dim, n_seqs, max_drafts and max_context must be sizes of one call");
+    const int rc = tree_sizes(a, n_rows, n_seqs, heads, kv_heads, dim, max_drafts, max_context);
+    if (rc != AIMG_OK) return rc;
     const int64_t rows = n_rows * heads * a.n_splits;
     *nbytes = a.n_splits > 1 ? static_cast<size_t>(rows) * (4 * aimg::padded_dim(dim) + 8) : 0;
     return AIMG_OK;
@@ -1274,8 +1282,8 @@ extern "C" int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages,
     if (q->dim != pages->dim || q->heads % pages->kv_heads != 0)
         return fail(AIMG_ERR_INVALID_ARGUMENT, "q must have the pages' dim and a multiple of their heads");
     aimg::TreeArgs a{};
-    if (!tree_sizes(a, n_seqs, q->heads, pages->kv_heads, q->dim, max_drafts, max_context))
-        return fail(AIMG_ERR_INVALID_ARGUMENT, "n_seqs and max_context must be >= 0 (max_context below 2^31) and max_drafts >= 1");
+    rc = tree_sizes(a, q->n_rows, n_seqs, q->heads, pages->kv_heads, q->dim, max_drafts, max_context);
+    if (rc != AIMG_OK) return rc;
     if (masks != nullptr && mask_words < 1) return fail(AIMG_ERR_INVALID_ARGUMENT, "mask_words must be >= 1");
     if (n_seqs == 0 || q->n_rows == 0) return AIMG_OK;
     if (seqs == nullptr || draft_offsets == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "null seqs or draft_offsets");

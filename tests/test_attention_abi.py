@@ -97,6 +97,24 @@ def test_tree_workspace_follows_the_sizes():
     assert lib.aimg_tree_workspace_nbytes(1, 40, 8, 128, 1, 1, 0, None) == BAD
 
 
+def test_tree_sizes_at_their_limits():
+    """Contexts past what a sequence can hold plan no part past it, drafts past the rows no rows; sizes whose product is too large are refused."""
+    lib, n = _native.lib(), ctypes.c_size_t()
+
+    def nbytes(*sizes):
+        rc = lib.aimg_tree_workspace_nbytes(*sizes, ctypes.byref(n))
+        return n.value if rc == OK else rc
+
+    most = nbytes(1, 8, 8, 64, 1, 1, (1 << 30) - 1)
+    assert most > 0 and most == nbytes(1, 8, 8, 64, 1, 1, (1 << 31) - 1) == nbytes(1, 8, 8, 64, 1, (1 << 31) - 1, (1 << 31) - 1)
+    parts = most // (8 * (4 * 64 + 8))
+    assert (parts - 1) * 8192 < 1 << 30
+    assert nbytes(7, 40, 8, 64, 2, (1 << 31) - 1, 0) == nbytes(7, 40, 8, 64, 2, 7, 0)
+    for sizes in [(1 << 30, 8, 8, 64, 1, 1, 0), (1, 1 << 20, 1 << 20, 64, 1 << 20, 1, 0), (64, 1 << 20, 1, 64, 1 << 18, 64, 0),
+                  (1, 8, 8, 64, 1 << 20, 1, (1 << 30) - 1)]:
+        assert nbytes(*sizes) == UNSUPPORTED, sizes
+
+
 def test_prompt_workspace_follows_the_sizes():
     lib, n = _native.lib(), ctypes.c_size_t()
 
