@@ -289,7 +289,7 @@ struct State {
     // ...and come back for the queries that see them: a product of ones counts
     // the visible keys with +inf or NaN, and one those with -inf or NaN.
     // (Integer arithmetic on pairs throughout: as comparisons, this rare path
-    // spilled scalar registers, and a kernel that spills at all starts slower.)
+    // spilled scalar registers.)
     template <int NSUB>
     __device__ __forceinline__ void add_infinite(const lds_char* first, int piece, int r, int half, const uint32_t (&allow)[QT][NSUB]) {
         constexpr uint32_t kPair = 0x10001u, kTop = 0x8000u * kPair;

@@ -132,6 +132,47 @@ class Pair:
                     assert torch.equal(got, torch.stack([self.row(x, layer) for x in rows])), (s, layer)
 
 
+@pytest.mark.parametrize("free", [[12999], [4095, 4096, 8192, 12287], list(range(8190, 8200)), list(range(5)) + [9000, 9001], []])
+def test_pools_of_several_scans(free):
+    """More pages than a scan of them takes at a time, the free ones around its ends: the lowest are reserved and forked, or nothing is."""
+    n = 13000
+    c = PagedKVCache.allocate(1, n, 1, 1, 8, 4, 20)
+    refs = torch.ones(n, dtype=torch.int32)
+    refs[free] = 0
+    c.refs.copy_(refs)
+    more = len(free) // 2
+    c.reserve(_ints([2, 0]), _ints([more, len(free) - more]))
+    c.check()
+    assert c.page_table[2, :more].tolist() == free[:more] and c.page_table[0, :len(free) - more].tolist() == free[more:]
+    assert c.held.tolist() == [len(free) - more, 0, more, 0] and int(c.refs.min()) == 1
+    before = c.page_table.clone()
+    c.reserve(_ints([1, 3]), _ints([1, 0]))
+    with pytest.raises(RuntimeError, match="too few"):
+        c.check()
+    assert torch.equal(c.page_table, before) and int(c.refs.max()) == 1
+
+
+@pytest.mark.parametrize("free", [[12999], [0, 4096], list(range(4000, 4200)) + [12000], list(range(0, 13000, 3))])
+def test_pools_of_several_scans_are_compacted(free):
+    n = 13000
+    c = PagedKVCache.allocate(1, n, 1, 1, 8, 2, 13000)
+    in_use = sorted(set(range(n)) - set(free))
+    refs = torch.zeros(n, dtype=torch.int32)
+    refs[in_use] = torch.arange(1, len(in_use) + 1, dtype=torch.int32)
+    c.refs.copy_(refs)
+    c.page_table[1, :len(in_use)] = _ints(in_use)
+    c.pool[0, :, :, 0, 0] = (torch.arange(n, device="cuda") % 251)[None, :, None].to(c.pool.dtype)
+    assert int(c.compact()) == len(in_use)
+    low = [p for p in free if p < len(in_use)]
+    moves = dict(zip([p for p in in_use if p >= len(in_use)], low))
+    assert c.page_table[1, :len(in_use)].tolist() == [moves.get(p, p) for p in in_use]
+    where = torch.tensor([moves.get(p, p) for p in in_use])
+    want = torch.zeros(n, dtype=torch.int32)
+    want[where] = torch.arange(1, len(in_use) + 1, dtype=torch.int32)
+    assert torch.equal(c.refs.cpu(), want)
+    assert torch.equal(c.pool[0, 1, where.cuda(), 0, 0, 3].cpu(), (torch.tensor(in_use) % 251).to(c.pool.dtype))
+
+
 def test_reserve_append_advance():
     p = Pair()
     p.write([0, 3], [5, 1])
