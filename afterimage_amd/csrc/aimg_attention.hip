@@ -392,6 +392,14 @@ __device__ __forceinline__ int find_sequence(const int32_t* offsets, int n, int 
 constexpr int kPromptKeys = 64;
 constexpr int kPromptRows = 128;  // of a workgroup
 
+// Bound by the SIMDs' instruction issue: with two waves a SIMD the matrix
+// instructions hold 51% of its cycles and the softmax's ordinary ones 49%, LDS
+// reads 26% (no bank conflicts). 16384 rows, 40 heads of 8, dim 128: 2.54-2.68
+// ms by the box, 1030-1080 TFLOP/s of the products that are seen (a large
+// matrix product reaches 1224). 64 rows a wave: 896; the next tile's scores
+// computed beside this one's exponentials in one wave: 840; two groups of waves
+// taking products and softmax in turn: 887-947; 8 waves sharing a tile: 984;
+// tiles of 32 keys: 975 (when this form reached 1015-1045).
 // Workgroup: one sequence and key/value head, 32 * QT * NW rows of its group
 // of heads: row r is head r % group of position r / group. Rows of one position
 // see the same keys, so a workgroup's rows reach over few positions: the tiles
@@ -571,6 +579,7 @@ __device__ __forceinline__ void join_parts(const float* part_o, const float2* pa
     if (col == 0 && lse != nullptr) *lse = l == 0.0f ? -INFINITY : top * (1.0f / kLog2E) + logf(l);
 }
 
+// The parts of split prompts; a row's number of parts follows from its workgroup's keys.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptArgs A) {
     constexpr int kCols = DP / 4, kSides = 256 / kCols;
@@ -599,15 +608,20 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptArgs A) {
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
-// Keys of a part. Calls that fill the GPU with their rows alone, or whose
-// sequences have few keys, are not split (the join costs some 5 us).
+// Keys of a part. 512 workgroups run at a time; a call with up to half as many
+// splits its keys to fill them, where the keys are enough to pay for writing
+// and joining the parts' sums: 8 a workgroup of the call, and 512. (40 heads of
+// 8, dim 128, us with and without the split: 50 rows over 800 keys 17, 25; 50
+// over 12000 33, 257; 400 over 1500 33, 40; 400 over 800 29, 25 and so not
+// split; 800 over 3000 66, 71; 800 over 1500 45, 40 and so not split; 1100 over
+// 3000 101, 77. Twice as many parts: 400 over 3000 51, not 43.)
 void plan_prompt(PromptArgs& A, int64_t n_rows, int64_t n_keys) {
     const int64_t groups = (n_rows * A.group / kPromptRows + A.n_seqs) * A.kv_heads;
     const int64_t each = A.n_seqs > 0 ? n_keys / A.n_seqs : 0;  // keys of a sequence, about
     int64_t chunk = INT32_MAX / 2;
-    if (groups <= 384 && each > 1024) {
-        const int64_t parts = 1024 / (groups > 0 ? groups : 1);
-        chunk = each / parts > 512 ? each / parts : 512;
+    if (groups <= 256 && each > 512 && each > 8 * groups) {
+        const int64_t parts = 512 / (groups > 0 ? groups : 1);
+        chunk = each / parts > 256 ? each / parts : 256;
         if (n_keys / chunk >= 64) chunk = n_keys / 64 + 1;  // sequences far longer than the others
         chunk = (chunk + 63) / 64 * 64;
     }
@@ -714,6 +728,10 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeArgs& A, const Drafted& 
 // into its own part of LDS with no barrier in the loop, and join their sums at
 // the end: one token's group (5 rows of 32 here) leaves the matrix cores idle,
 // but the bytes in flight, not the products, bound it.
+// Bound by HBM where contexts are long: 16 trees of 4-16 tokens over 9000-65000
+// positions, 40 heads of 8, dim 128, read 1.73 GB in 325 us, 5.3 TB/s; 64
+// single tokens over 2000-8000 5.06 TB/s. 8 trees of 1-33 tokens over 700-6000
+// positions take 27 us, 3.7 TB/s: two rounds of short parts.
 // kPages: what of a tile never crosses a page, and so has one base address: 2
 // the tile, 1 the rows of one load (2 to 8), 0 a row. (With addresses made lane
 // by lane for pages of 16, 54 trees over 139-2238 positions took 155 us.)
@@ -948,7 +966,10 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
 // row's columns, four each. kMany: all of a workgroup's threads take a row,
 // its parts in turn, and their sums meet in LDS (with the parts one after the
 // other, a token over 32,000 positions spent 100 of 145 us here). Otherwise
-// every DP / 4 threads take a row of their own: fewer, fuller workgroups.
+// every DP / 4 threads take a row of their own: fewer, fuller workgroups (8
+// trees of 33 tokens over 700-6000 positions, 12 parts: 56 us in all, 65 with
+// a workgroup a row; a token over 32,000, 63 parts: 31 and 27 with one). Bound
+// by the latency of the sums' reads, 5 to 10 us a call.
 template <typename T, int DP, bool kMany>
 __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
     constexpr int kCols = DP / 4, kSides = 256 / kCols;
@@ -1019,7 +1040,9 @@ __global__ __launch_bounds__(256) void tree_join_kernel(const TreeArgs A) {
 }
 
 // Ancestor bits of drafted tokens: token t's parent is an earlier drafted
-// token of its sequence, or any other number where it follows the context.
+// token of its sequence, or any other number where it follows the context. A
+// thread walks up from its token, once for each word of its mask: the trees of
+// a call are some hundred tokens, one launch's latency.
 __global__ __launch_bounds__(256) void tree_masks_kernel(const int32_t* parents, const int32_t* offsets, int n_seqs, int n, int words,
                                                          uint64_t* masks) {
     const int row = blockIdx.x * 256 + threadIdx.x;
@@ -1043,15 +1066,27 @@ __global__ __launch_bounds__(256) void tree_masks_kernel(const int32_t* parents,
 }
 
 constexpr int64_t kMaxPositions = 1 << 30;  // of a sequence, by the checks of its pages
-constexpr int kMinChunk = 512;      // keys of a part: fewer cost more in start-up and joining than they save
-constexpr int kMaxChunk = 8192;     // and most of them, so that a long sequence among short ones does not run alone
+// Keys of a part. At least 512: with 256 two trees of 16 tokens over 20,000
+// positions take 55 us, not 47, with 1024 a tree of 64 over 2000 takes 33, not 25.
+constexpr int kMinChunk = 512;
+// And most of them, so that a long sequence among short ones does not run alone
+// (shared tiles, 16 trees over 9000-65000: 340 us, 427 with 8192).
+constexpr int kMaxChunk = 8192;
 constexpr int kMaxSharedChunk = 4096;
 constexpr int kSlots = 256;         // workgroups of dealt-out keys that run at a time, one a CU
 constexpr int kFewParts = 16;       // at most so many are joined by DP / 4 threads a row
-constexpr int kSharedParts = 2048;  // workgroups of shared tiles: two a CU, four rounds
+// Workgroups of shared tiles, were all sequences the longest: two a CU, four
+// rounds. Lengths that differ need the parts (16 trees of 18-33 tokens over
+// 200-8600 positions: 74 us, 86 with 1024, 116 with 512); trees of one length
+// would do with fewer (6 of 64 tokens over 8000: 122 us, 93 with 1024), which
+// the host, that knows the longest alone, cannot tell apart.
+constexpr int kSharedParts = 2048;
 
 // Rows of a workgroup. Up to 32 or 64 rows of a (sequence, head) go to every
-// wave and the keys are dealt out to the waves; more rows are dealt out.
+// wave and the keys are dealt out to the waves; more rows are dealt out. (32
+// trees of 12 tokens, 60 rows, over 3000 positions: 79 us, 106 with the rows
+// dealt out; 8 of them 31 and 30. 256 rows a workgroup: 8 trees of up to 33
+// tokens 42-58 us, not 36.)
 int tree_rows(int dim, int64_t rows) { return rows <= 32 ? 32 : rows <= 64 && dim <= 128 ? 64 : 128; }
 
 // Keys of a part and how many parts the longest sequence has.
