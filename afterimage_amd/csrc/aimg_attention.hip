@@ -393,7 +393,7 @@ constexpr int kPromptKeys = 64;
 constexpr int kPromptRows = 128;  // of a workgroup
 
 // Bound by the SIMDs' instruction issue: with two waves a SIMD the matrix
-// instructions hold 51% of its cycles and the softmax's ordinary ones 49%, LDS
+// instructions hold 52% of its cycles and the softmax's ordinary ones 45%, LDS
 // reads 26% (no bank conflicts). 16384 rows, 40 heads of 8, dim 128: 2.54-2.68
 // ms by the box, 1030-1080 TFLOP/s of the products that are seen (a large
 // matrix product reaches 1224). 64 rows a wave: 896; the next tile's scores

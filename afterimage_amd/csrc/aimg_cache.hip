@@ -307,7 +307,7 @@ __global__ __launch_bounds__(kScan) void fork_plan_kernel(const ForkArgs A) {
 // Workgroup (pair, share of its rows to copy). The first share of a pair also
 // counts its references and writes its new row beside the table: a pair's
 // source may be another pair's branch, so no row changes before all were read.
-// Bound by what it writes (96 branches, 16 planes of 8 heads of 128: 92.7 MB
+// Bound by what it writes (96 branches, 16 planes of 8 heads of 128: 95 MB
 // in 39.5 us; the sources' tails are read once and stay in the caches). Two,
 // four and eight times the rows a thread, or twice as many in flight, took
 // 0.2 to 2 us more.
