@@ -394,8 +394,8 @@ constexpr int kPromptRows = 128;  // of a workgroup
 
 // Bound by the SIMDs' instruction issue: with two waves a SIMD the matrix
 // instructions hold 52% of its cycles and the softmax's ordinary ones 45%, LDS
-// reads 26% (no bank conflicts). 16384 rows, 40 heads of 8, dim 128: 2.54-2.68
-// ms by the box, 1030-1080 TFLOP/s of the products that are seen (a large
+// reads 26% (no bank conflicts). 16384 rows, 40 heads of 8, dim 128: 2.54-2.79
+// ms by the card's clock, 986-1083 TFLOP/s of the products that are seen (a large
 // matrix product reaches 1224). 64 rows a wave: 896; the next tile's scores
 // computed beside this one's exponentials in one wave: 840; two groups of waves
 // taking products and softmax in turn: 887-947; 8 waves sharing a tile: 984;
