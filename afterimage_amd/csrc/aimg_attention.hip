@@ -1075,12 +1075,13 @@ constexpr int kMaxChunk = 8192;
 constexpr int kMaxSharedChunk = 4096;
 constexpr int kSlots = 256;         // workgroups of dealt-out keys that run at a time, one a CU
 constexpr int kFewParts = 16;       // at most so many are joined by DP / 4 threads a row
-// Workgroups of shared tiles, were all sequences the longest: two a CU, four
-// rounds. Lengths that differ need the parts (16 trees of 18-33 tokens over
-// 200-8600 positions: 74 us, 86 with 1024, 116 with 512); trees of one length
-// would do with fewer (6 of 64 tokens over 8000: 122 us, 93 with 1024), which
-// the host, that knows the longest alone, cannot tell apart.
-constexpr int kSharedParts = 2048;
+// Workgroups of shared tiles, were all sequences the longest: two a CU, two and
+// a half rounds. Lengths that differ need the parts (16 trees of 18-33 tokens
+// over 200-8600 positions: 62 us, 86 with 1024, 116 with 512, 74 with 2048);
+// trees of one length would do with fewer (6 of 64 tokens over 8000: 113 us, 93
+// with 1024, 125 with 2048), which the host, that knows the longest alone,
+// cannot tell apart.
+constexpr int kSharedParts = 1280;
 
 // Rows of a workgroup. Up to 32 or 64 rows of a (sequence, head) go to every
 // wave and the keys are dealt out to the waves; more rows are dealt out. (32
