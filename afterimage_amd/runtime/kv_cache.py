@@ -79,9 +79,8 @@ class PagedKVCache:
             pool, page_table, lengths, held, refs, status
         nbytes = ctypes.c_size_t(0)
         _native.check(self._lib.aimg_cache_compact_workspace_nbytes(self._cache, ctypes.byref(nbytes)))
-        # Scratch memory of the calls, kept: they change one cache and so run in order.
+        # Scratch memory of compact, of one size and so kept as long as the cache: calls change one cache and run in order.
         self._compact_work = torch.empty(nbytes.value, dtype=torch.uint8, device=self.device)
-        self._fork_work = torch.empty(0, dtype=torch.uint8, device=self.device)
         self._used = torch.empty((), dtype=torch.int32, device=self.device)
 
     @classmethod
@@ -175,9 +174,11 @@ class PagedKVCache:
         s, n = self._seqs(src, "src")
         d = _int32(dst, "dst", (n,), self._index)
         nbytes = 4 * n * (2 + self.max_pages)
-        if self._fork_work.shape[0] < nbytes:
-            self._fork_work = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        launch(self._lib.aimg_cache_fork, self._index, self._cache, s, d, n, self._fork_work.data_ptr(), nbytes)
+        # The call's own, from torch's allocator on the current stream: a buffer
+        # kept here would have to grow, and a captured graph or another stream
+        # may still use the smaller one.
+        work = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        launch(self._lib.aimg_cache_fork, self._index, self._cache, s, d, n, work.data_ptr(), nbytes)
 
     def release(self, seqs: torch.Tensor) -> None:
         """Empties the slots; pages that no other slot holds are free."""
