@@ -94,6 +94,14 @@ def _lse(lse: torch.Tensor | None, q: torch.Tensor) -> int | None:
     return lse.data_ptr()
 
 
+def _workspace(nbytes: int, q: torch.Tensor) -> torch.Tensor | None:
+    """Scratch memory from torch's allocator on the current stream, which the
+    launches use. The caller holds the tensor until they are made: the entries
+    release the interpreter's lock, and another thread on this stream would be
+    given memory that no tensor holds, for work that runs before them."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+
+
 def launch(entry, index: int, *args) -> None:
     """entry(*args, stream) with GPU ``index`` current, on its current stream.
     (The handle itself: a torch.cuda.Stream object and a device context cost
@@ -151,10 +159,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
                          % (n_seqs + 1, n_keys + 1))
     out, od = _result(q, qd, out, index)
     nbytes = _prompt_workspace_nbytes(qd.n_rows, kd.n_rows, qd.heads, kd.heads, qd.dim, n_seqs)
-    # From torch's allocator on the current stream, which the launches use.
-    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+    work = _workspace(nbytes, q)
     launch(_native.lib().aimg_prompt_attention, index, qd, kd, vd, od, q_at, k_at, n_seqs, kind, _scale(scale, qd.dim), _lse(lse, q),
-           work, nbytes)
+           work.data_ptr() if nbytes else None, nbytes)
     return out
 
 
@@ -248,10 +255,9 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         raise ValueError("max_context must not be negative, got %d" % max_context)
     out, od = _result(q, qd, out, index)
     nbytes = _tree_workspace_nbytes(n, heads, kv_heads, dim, n_seqs, max_drafts, max_context)
-    # From torch's allocator on the current stream, which the launches use.
-    work = torch.empty(nbytes, dtype=torch.uint8, device=q.device).data_ptr() if nbytes else None
+    work = _workspace(nbytes, q)
     launch(_native.lib().aimg_tree_attention, index, qd, pages, od, seqs_at, at, n_seqs, masks_at, words, max_drafts, max_context,
-           kind, _scale(scale, dim), _lse(lse, q), work, nbytes)
+           kind, _scale(scale, dim), _lse(lse, q), work.data_ptr() if nbytes else None, nbytes)
     return out
 
 

@@ -6,7 +6,8 @@ import weakref
 import pytest
 import torch
 
-from afterimage_amd.runtime import kv_cache
+from afterimage_amd import _native
+from afterimage_amd.runtime import attention, kv_cache
 
 
 class Recorder:
@@ -56,3 +57,24 @@ def test_a_larger_fork_takes_nothing_from_one_captured_before(cache, monkeypatch
     cache.fork(_ints(0, 0, 0, 0, 0), _ints(1, 2, 3, 4, 5))
     # The cache never held it (then torch's allocator decides, which knows of captures and streams), or holds it still.
     assert not kept or first() is not None
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """CPU tensors pass the attention calls' checks; their launches are recorded."""
+    monkeypatch.setattr(attention, "_query", lambda q: (attention._heads(q, "q", q.dtype, -1), -1, _native.AIMG_BF16))
+    monkeypatch.setattr(attention, "describe_pages", lambda k, v, table, lengths: _native.AimgPages(
+        kv_heads=k.shape[1], page_size=k.shape[2], dim=k.shape[3], max_pages=table.shape[1]))
+    return Recorder(monkeypatch, attention)
+
+
+def test_the_workspaces_of_split_attention_live_until_their_launch(on_cpu):
+    """A thread that allocates between the workspace and the launch must not be given the same memory."""
+    q, k = (torch.zeros(n, 1, 64, dtype=torch.bfloat16) for n in (3, 4000))
+    attention.prompt_attention(q, k, k, _ints(0, 3), _ints(0, 4000))
+    work, nbytes = on_cpu.launches[-1][0][-2:]
+    assert nbytes > 0 and on_cpu.living(work) is not None
+    pages = torch.zeros(300, 1, 16, 64, dtype=torch.bfloat16)
+    attention.tree_attention(q, pages, pages, _ints(*range(300)).view(1, 300), _ints(4000), _ints(0), _ints(0, 3), max_drafts=3)
+    work, nbytes = on_cpu.launches[-1][0][-2:]
+    assert nbytes > 0 and on_cpu.living(work) is not None
