@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void append_kernel(const AppendArgs A) {
     if (row < first || row >= A.offsets[lo + 1]) return;  // a row of no sequence
     const int32_t slot = A.seqs[lo];
     if (!known(C, slot)) return tell(C, kBadIndex);
-    const int64_t at = static_cast<int64_t>(length_of(C, slot)) + (row - first);
+    const int64_t at = static_cast<int64_t>(length_of(C, slot)) + row - first;  // first may be any int32
     const int64_t page = at / C.page_size;
     if (page >= held_of(C, slot)) return tell(C, kRowFull);
     const int32_t id = C.table[static_cast<int64_t>(slot) * C.table_stride + page];
