@@ -180,8 +180,10 @@ __global__ __launch_bounds__(256) void advance_kernel(const Cache C, const int32
     if (b >= n_seqs) return;
     const int32_t slot = seqs[b];
     if (!known(C, slot)) return tell(C, kBadIndex);
-    const int64_t to = static_cast<int64_t>(length_of(C, slot)) + offsets[b + 1] - offsets[b];
-    if (to < 0 || to > static_cast<int64_t>(held_of(C, slot)) * C.page_size) return tell(C, kRowFull);
+    // A length never falls: it could come to lie inside a page that another slot shares.
+    const int64_t more = static_cast<int64_t>(offsets[b + 1]) - offsets[b], to = length_of(C, slot) + more;
+    if (more < 0) return tell(C, kBadIndex);
+    if (to > static_cast<int64_t>(held_of(C, slot)) * C.page_size) return tell(C, kRowFull);
     C.lengths[slot] = static_cast<int32_t>(to);
 }
 

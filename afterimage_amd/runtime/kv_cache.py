@@ -28,7 +28,7 @@ MAX_SEQS = 8192      # sequences of one call
 MAX_PAGES = (1 << 20) - 1
 
 _PROBLEMS = ((1, "too few free pages"), (2, "positions past a sequence's pages or its row of the page table"),
-             (4, "a slot, page or source that does not exist"))
+             (4, "a slot, page, source or number of rows that does not exist"))
 
 
 def _int32(x: torch.Tensor, name: str, shape: tuple, index: int) -> int:

@@ -372,7 +372,7 @@ int aimg_tree_masks(const int32_t* parents, const int32_t* draft_offsets, int n_
 /* What a call finds wrong on the GPU it leaves undone and says in *status   */
 /* (bits, or-ed in): 1 no free pages (nothing was reserved or forked), 2 a   */
 /* sequence's row of the table or its pages end before the positions asked   */
-/* for, 4 a slot, page or source that does not exist.                        */
+/* for, 4 a slot, page, source or number of rows that does not exist.        */
 /* ------------------------------------------------------------------------- */
 
 #define AIMG_CACHE_NO_PAGES 1
@@ -400,7 +400,8 @@ typedef struct aimg_cache {
 int aimg_cache_append(const aimg_cache* cache, int layer, const aimg_heads* k, const aimg_heads* v, const int32_t* seqs,
                       const int32_t* offsets, int n_seqs, void* stream);
 
-/* Adds offsets[b+1] - offsets[b] to slot seqs[b]'s length: the rows that every layer has appended. */
+/* Adds offsets[b+1] - offsets[b] to slot seqs[b]'s length: the rows that every
+ * layer has appended (a difference below 0 is an error, 4). */
 int aimg_cache_advance(const aimg_cache* cache, const int32_t* seqs, const int32_t* offsets, int n_seqs, void* stream);
 
 /* Pages for tokens[b] positions past slot seqs[b]'s length, for all sequences

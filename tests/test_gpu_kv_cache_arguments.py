@@ -19,3 +19,18 @@ def test_append_with_offsets_far_below_zero(first):
         p.cache.check()
     assert torch.equal(p.cache.pool, before)
     p.check()
+
+
+@pytest.mark.parametrize("drop", [1, 2, 9, 1 << 30])
+def test_advance_does_not_shorten(drop):
+    """Offsets that fall are reported, so a length cannot come to lie inside a page that another slot shares."""
+    p = Pair()
+    p.write([0, 3], [9, 1])
+    p.fork([0], [1])
+    p.cache.advance(_ints([1]), _ints([drop, 0]))
+    with pytest.raises(RuntimeError, match="does not exist"):
+        p.cache.check()
+    p.check()
+    # The branch goes on, and its source keeps its rows.
+    p.write([1], [2])
+    p.check()
