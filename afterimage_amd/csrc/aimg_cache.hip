@@ -396,11 +396,10 @@ struct CommitArgs {
     int32_t n_seqs, most;  // most: entries of a row of accepted
 };
 
-// Accepted tokens of sequence b, 0 where they are not in its pages.
+// Accepted tokens of sequence b, 0 where there cannot be as many or they are not in its pages.
 __device__ __forceinline__ int32_t accepted_of(const CommitArgs& A, int b, int32_t slot) {
-    int32_t n = A.counts[b];
-    n = n < 0 ? 0 : n > A.most ? A.most : n;
-    if (n == 0) return 0;
+    const int32_t n = A.counts[b];
+    if (n <= 0 || n > A.most) return 0;
     const int32_t last = A.accepted[static_cast<int64_t>(b) * A.most + n - 1];
     const int64_t end = static_cast<int64_t>(length_of(A.c, slot)) + last;
     return last >= n - 1 && end < static_cast<int64_t>(held_of(A.c, slot)) * A.c.page_size ? n : 0;
@@ -424,7 +423,8 @@ __global__ __launch_bounds__(256) void commit_kernel(const CommitArgs A) {
     }
     const int32_t len = length_of(C, slot), n = accepted_of(A, b, slot);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
-        if (n == 0 && A.counts[b] > 0) tell(C, kRowFull);
+        const int32_t asked = A.counts[b];
+        if (n != asked) tell(C, asked < 0 || asked > A.most ? kBadIndex : kRowFull);
         if (A.new_lengths != C.lengths) A.new_lengths[slot] = len + n;
     }
     const uint32_t pieces = C.row_bytes / 16, all = static_cast<uint32_t>(C.planes) * C.kv_heads * pieces;  // below 2^31

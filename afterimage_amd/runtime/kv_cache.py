@@ -153,7 +153,8 @@ class PagedKVCache:
         """Keeps counts[b] drafted tokens of slot seqs[b], those of indices
         accepted[b, :counts[b]] (int32, rising: a path of the tree): in every
         layer their rows move to the positions from the length on, and the
-        length grows by counts[b]. The new lengths go to new_lengths (int32
+        length grows by counts[b] (0 to accepted's width; anything else is left
+        undone and recorded). The new lengths go to new_lengths (int32
         [max_seqs], the call's slots only) where given, in place otherwise.
         Returns the lengths written."""
         at, n = self._seqs(seqs)

@@ -428,9 +428,10 @@ int aimg_cache_fork(const aimg_cache* cache, const int32_t* src, const int32_t* 
 /*
  * Keeps the accepted tokens of verified trees: rows lengths[slot] +
  * accepted[b * max_accepted + i] of every layer become rows lengths[slot] + i,
- * i < counts[b] <= max_accepted. Accepted indices rise (a path from the root,
- * parents before children). new_lengths[slot] = lengths[slot] + counts[b]; it
- * may be cache->lengths, and is written for the call's slots only.
+ * i < counts[b] <= max_accepted (a count outside 0..max_accepted is an error,
+ * 4). Accepted indices rise (a path from the root, parents before children).
+ * new_lengths[slot] = lengths[slot] + counts[b]; it may be cache->lengths, and
+ * is written for the call's slots only.
  */
 int aimg_cache_commit(const aimg_cache* cache, const int32_t* seqs, const int32_t* accepted, int max_accepted,
                       const int32_t* counts, int n_seqs, int32_t* new_lengths, void* stream);

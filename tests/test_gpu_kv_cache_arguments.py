@@ -34,3 +34,27 @@ def test_advance_does_not_shorten(drop):
     # The branch goes on, and its source keeps its rows.
     p.write([1], [2])
     p.check()
+
+
+@pytest.mark.parametrize("count", [-1, -(1 << 31), 3, (1 << 31) - 1])
+@pytest.mark.parametrize("apart", [False, True])
+def test_commit_with_a_count_out_of_range(count, apart):
+    """No more than accepted's width, no less than 0: the sequence stays as it is, the others are committed."""
+    p = Pair()
+    p.write([0, 1], [6, 3])
+    p.cache.reserve(_ints([0, 1]), _ints([4, 4]))
+    p.model.reserve([0, 1], [4, 4])
+    numbers, _ = p.append([0, 1], [4, 4])
+    new = torch.full((7,), -9, dtype=torch.int32, device="cuda") if apart else None
+    p.cache.commit(_ints([0, 1]), _ints([[1, 3], [0, 2]]), _ints([count, 2]), new)
+    if apart:
+        assert new.tolist() == [6, 5, -9, -9, -9, -9, -9]
+        p.cache.lengths[:2] = new[:2]
+    p.model.rows[1] += [numbers[1][0], numbers[1][2]]
+    with pytest.raises(RuntimeError, match="does not exist"):
+        p.cache.check()
+    p.check()
+    # The drafted rows lie where they were appended.
+    p.cache.commit(_ints([0]), _ints([[0, 1, 2, 3]]), _ints([4]))
+    p.model.rows[0] += numbers[0]
+    p.check()
