@@ -361,12 +361,14 @@ struct PromptArgs {
     const uint16_t *q, *k, *v;
     uint16_t* out;
     float* lse;
-    float* part_o;    // [part][row * heads + head][DP], where keys are split
-    float2* part_ml;  // [part][row * heads + head]: c * maximum, sum
+    float* part_o;    // [place in the parts * heads + head][DP], where keys are split
+    float2* part_ml;  // [the same]: c * maximum, sum
     const int32_t *q_offsets, *k_offsets;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // strides in elements
     int32_t n_seqs, heads, kv_heads, group, dim, n_q, n_k, n_slots;
-    int32_t chunk, n_splits;  // keys of a part, parts
+    int32_t chunk, n_splits;  // keys of a part, parts of a sequence that holds every key
+    int32_t part_rows;        // rows of all parts that the workspace holds
+    bool all_fit;             // n_splits parts of every row
     float c, scale;
 };
 
@@ -392,6 +394,87 @@ __device__ __forceinline__ int find_sequence(const int32_t* offsets, int n, int 
 constexpr int kPromptKeys = 64;
 constexpr int kPromptRows = 128;  // of a workgroup
 
+// A sequence of a call, bounded to the buffers.
+struct Prompt {
+    int32_t q_begin, q_len, k_begin, k_len;
+};
+
+__device__ __forceinline__ Prompt prompt_of(const PromptArgs& A, int b) {
+    Prompt p;
+    p.q_begin = bounded(A.q_offsets[b], A.n_q), p.k_begin = bounded(A.k_offsets[b], A.n_k);
+    const int32_t q_len = bounded(A.q_offsets[b + 1], A.n_q) - p.q_begin, k_len = bounded(A.k_offsets[b + 1], A.n_k) - p.k_begin;
+    p.q_len = q_len > 0 ? q_len : 0, p.k_len = k_len > 0 ? k_len : 0;
+    return p;
+}
+
+// Split prompts: sequence b's keys are cut into parts_in(k_len, chunk) parts,
+// each a copy of the sequence's rows in the workspace, one sequence after the
+// other. (A call that is split has at most 256 sequences and 2^15 rows, by
+// plan_prompt, and a sequence at most 65 parts: sums of them fit 32 bits.)
+__device__ __forceinline__ int32_t parts_in(int32_t k_len, int32_t chunk) { return k_len > chunk ? (k_len - 1) / chunk + 1 : 1; }
+
+__device__ __forceinline__ int32_t part_rows_of(const Prompt& p, int32_t chunk) {
+    const int32_t parts = parts_in(p.k_len, chunk);
+    return parts > 1 ? p.q_len * parts : 0;
+}
+
+template <int kLanes>
+__device__ __forceinline__ int32_t sum_lanes(int32_t v) {
+#pragma unroll
+    for (int x = 1; x < kLanes; x *= 2) v += __shfl_xor(v, x);
+    return v;
+}
+
+// Keys of a part: the host's number, which goes by the average sequence,
+// doubled until every sequence's parts fit the workspace. kLanes neighbouring lanes call it together.
+template <int kLanes>
+__device__ __forceinline__ int32_t part_keys(const PromptArgs& A, int lane) {
+    int32_t chunk = A.chunk;
+    while (!A.all_fit) {
+        int32_t rows = 0;
+        for (int b = lane; b < A.n_seqs; b += kLanes) rows += part_rows_of(prompt_of(A, b), chunk);
+        if (sum_lanes<kLanes>(rows) <= A.part_rows) break;
+        chunk = chunk < 1 << 29 ? 2 * chunk : INT32_MAX;  // no sequence has more than INT32_MAX: the loop ends
+    }
+    return chunk;
+}
+
+// A workgroup of a split call: a tile of a sequence's rows and a part of its keys.
+struct PromptPart {
+    Prompt of;
+    int32_t tile, tiles, part, parts;
+    int32_t place;  // of the sequence's first row in the workspace
+};
+
+// The unit-th pair of a tile and a part, by a whole wave; false past the last.
+__device__ __forceinline__ bool find_part(const PromptArgs& A, int32_t chunk, int32_t unit, int lane, PromptPart& to) {
+    to.place = 0;
+    for (int b0 = 0; b0 < A.n_seqs; b0 += 64) {
+        const bool here = b0 + lane < A.n_seqs;
+        const Prompt p = prompt_of(A, here ? b0 + lane : A.n_seqs - 1);
+        const int32_t tiles = (p.q_len * A.group + kPromptRows - 1) / kPromptRows, parts = parts_in(p.k_len, chunk);
+        const int32_t units = here ? tiles * parts : 0, rows = here ? part_rows_of(p, chunk) : 0;
+        int32_t units_to = units, rows_to = rows;  // with the lanes before
+        for (int x = 1; x < 64 && x < A.n_seqs; x *= 2) {
+            const int32_t u = __shfl_up(units_to, x), r = __shfl_up(rows_to, x);
+            if (lane >= x) units_to += u, rows_to += r;
+        }
+        const uint64_t past = __ballot(units_to > unit);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            auto of = [at](int32_t x) { return __builtin_amdgcn_readlane(x, at); };
+            to.of = Prompt{of(p.q_begin), of(p.q_len), of(p.k_begin), of(p.k_len)};
+            to.tiles = of(tiles), to.parts = of(parts);
+            to.place += of(rows_to - rows);
+            const int32_t i = unit - of(units_to - units);
+            to.tile = i / to.parts, to.part = i % to.parts;
+            return true;
+        }
+        unit -= __builtin_amdgcn_readlane(units_to, 63), to.place += __builtin_amdgcn_readlane(rows_to, 63);
+    }
+    return false;
+}
+
 // Bound by the SIMDs' instruction issue: with two waves a SIMD the matrix
 // instructions hold 52% of its cycles and the softmax's ordinary ones 45%, LDS
 // reads 26% (no bank conflicts). 16384 rows, 40 heads of 8, dim 128: 2.54-2.79
@@ -411,7 +494,11 @@ constexpr int kPromptRows = 128;  // of a workgroup
 // rows are empty. Later slots, whose rows see more keys, start first.
 // Parts: where a call has few rows and many keys (the next piece of a prompt
 // over a long context) each workgroup takes a part of its rows' keys, and
-// prompt_join_kernel joins them.
+// prompt_join_kernel joins them. The sums lie one sequence after the other, so
+// that a short sequence has none for a long one's parts, and only pairs of a
+// tile and a part that exist are workgroups (32 prompts of 112 rows over 2112
+// keys, 8 heads of 1: 62 us and 67 MB; with the longest possible sequence's
+// parts for each row 93 us and 939 MB. Four small ones: 15.2 us, 14.5.)
 template <typename T, int DP, int QT, int NW, bool kParts>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_kernel(const PromptArgs A) {
     typedef Rows<DP> R;
@@ -426,17 +513,27 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     // Consecutive workgroups take the key/value heads in turn: with eight of
     // them an XCD keeps to one head, whose keys and values stay in its L2.
     const int kvh = blockIdx.x % A.kv_heads;
-    const int split = kParts ? blockIdx.x / A.kv_heads % A.n_splits : 0;
-    const int slot = A.n_slots - 1 - static_cast<int>(blockIdx.x / A.kv_heads / (kParts ? A.n_splits : 1));
     const int group = A.group;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lo = find_sequence(A.q_offsets, A.n_seqs, A.n_q, slot, lane, [&](int b, int first) { return first * group / BM + b; });
-    const int q_begin = bounded(A.q_offsets[lo], A.n_q), q_end = bounded(A.q_offsets[lo + 1], A.n_q);
-    const int k_begin = bounded(A.k_offsets[lo], A.n_k), k_end = bounded(A.k_offsets[lo + 1], A.n_k);
-    const int q_len = q_end - q_begin, k_len = k_end > k_begin ? k_end - k_begin : 0;
-    const int rows = q_len * group;
-    const int row0 = (slot - (q_begin * group / BM + lo)) * BM;
-    if (row0 < 0 || row0 >= rows) return;
+    int q_begin, q_len, k_begin, k_len, rows, row0;
+    int split = 0, chunk = 0, place = 0;
+    if constexpr (kParts) {
+        chunk = __builtin_amdgcn_readfirstlane(part_keys<64>(A, lane));
+        PromptPart p;
+        if (!find_part(A, chunk, static_cast<int32_t>(blockIdx.x / A.kv_heads), lane, p)) return;
+        q_begin = p.of.q_begin, q_len = p.of.q_len, k_begin = p.of.k_begin, k_len = p.of.k_len;
+        rows = q_len * group, row0 = (p.tiles - 1 - p.tile) * BM;
+        split = p.part, place = p.place;
+    } else {
+        const int slot = A.n_slots - 1 - static_cast<int>(blockIdx.x / A.kv_heads);
+        const int lo = find_sequence(A.q_offsets, A.n_seqs, A.n_q, slot, lane, [&](int b, int first) { return first * group / BM + b; });
+        const int q_end = bounded(A.q_offsets[lo + 1], A.n_q), k_end = bounded(A.k_offsets[lo + 1], A.n_k);
+        q_begin = bounded(A.q_offsets[lo], A.n_q), k_begin = bounded(A.k_offsets[lo], A.n_k);
+        q_len = q_end - q_begin, k_len = k_end > k_begin ? k_end - k_begin : 0;
+        rows = q_len * group;
+        row0 = (slot - (q_begin * group / BM + lo)) * BM;
+        if (row0 < 0 || row0 >= rows) return;
+    }
 
     const int half = lane >> 5;
     const int shift = k_len - q_len;  // position i sees keys 0 .. i + shift
@@ -444,10 +541,10 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     auto seen_by = [&](int row) { return row / group + 1 + shift < 0 ? 0 : row / group + 1 + shift; };
 
     const int keys_wg = seen_by((row0 + BM < rows ? row0 + BM : rows) - 1);  // keys that some row here sees
-    const int begin = kParts ? split * A.chunk : 0;
+    const int begin = kParts ? split * chunk : 0;  // at most k_len
     if (split > 0 && begin >= keys_wg) return;
-    const bool parted = kParts && keys_wg > A.chunk;
-    const int end = !kParts || keys_wg - begin < A.chunk ? keys_wg : begin + A.chunk;
+    const bool parted = kParts && keys_wg > chunk;
+    const int end = !kParts || keys_wg - begin < chunk ? keys_wg : begin + chunk;
     int keys_wave = wave_row >= rows ? 0 : seen_by((wave_row + 32 * QT < rows ? wave_row + 32 * QT : rows) - 1);
     keys_wave = keys_wave < end ? keys_wave : end;
 
@@ -526,7 +623,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
         if (r >= rows) continue;
         const int row = q_begin + r / group, head = kvh * group + r % group;
         const int64_t rh = static_cast<int64_t>(row) * A.heads + head;
-        const int64_t part = static_cast<int64_t>(split) * A.n_q * A.heads + rh;
+        const int64_t part = (place + split * q_len + r / group) * static_cast<int64_t>(A.heads) + head;
         const float by = parted ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
         uint16_t* const to = A.out + row * A.out_row + head * A.out_head;
 #pragma unroll
@@ -546,7 +643,8 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     }
 }
 
-// One row and head's parts in their order, by DP / 4 threads with four columns each.
+// One row and head's parts in their order, by DP / 4 threads with four columns
+// each: part s at s * all + rh.
 template <typename T, int DP>
 __device__ __forceinline__ void join_parts(const float* part_o, const float2* part_ml, int64_t all, int64_t rh, int parts, int col,
                                            int dim, uint16_t* to, float* lse) {
@@ -592,19 +690,28 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptArgs A) {
         const int mid = (lo + hi + 1) / 2;
         if (bounded(A.q_offsets[mid], A.n_q) <= row) lo = mid; else hi = mid - 1;
     }
-    const int q_begin = bounded(A.q_offsets[lo], A.n_q), q_end = bounded(A.q_offsets[lo + 1], A.n_q);
-    const int k_begin = bounded(A.k_offsets[lo], A.n_k), k_end = bounded(A.k_offsets[lo + 1], A.n_k);
-    if (row < q_begin || row >= q_end) return;
-    const int q_len = q_end - q_begin, k_len = k_end > k_begin ? k_end - k_begin : 0;
+    const Prompt p = prompt_of(A, lo);
+    if (row < p.q_begin || row >= p.q_begin + p.q_len) return;
+    const int col = threadIdx.x % kCols;
+    const int32_t chunk = part_keys<kCols>(A, col);
     // The keys of the row's workgroup decide its parts.
-    const int rows = q_len * A.group, r = (row - q_begin) * A.group + head % A.group;
+    const int rows = p.q_len * A.group, r = (row - p.q_begin) * A.group + head % A.group;
     const int row0 = r / kPromptRows * kPromptRows;
     const int last = (row0 + kPromptRows < rows ? row0 + kPromptRows : rows) - 1;
-    const int keys = last / A.group + 1 + k_len - q_len;
-    if (keys <= A.chunk) return;
-    join_parts<T, DP>(A.part_o, A.part_ml, all, rh, (keys - 1) / A.chunk + 1, threadIdx.x % kCols, A.dim,
-                      A.out + row * A.out_row + head * A.out_head, A.lse != nullptr ? A.lse + rh : nullptr);
+    const int keys = last / A.group + 1 + p.k_len - p.q_len;
+    if (keys <= chunk) return;
+    int32_t place = 0;
+    if (lo > 0) {
+        for (int b = col; b < lo; b += kCols) place += part_rows_of(prompt_of(A, b), chunk);
+        place = sum_lanes<kCols>(place);
+    }
+    place += row - p.q_begin;
+    join_parts<T, DP>(A.part_o, A.part_ml, static_cast<int64_t>(p.q_len) * A.heads, static_cast<int64_t>(place) * A.heads + head,
+                      (keys - 1) / chunk + 1, col, A.dim, A.out + row * A.out_row + head * A.out_head,
+                      A.lse != nullptr ? A.lse + rh : nullptr);
 }
+
+constexpr int64_t kPromptScratch = 64 << 20;  // bytes of split prompts' sums that need no further reason
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
@@ -618,7 +725,7 @@ int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 void plan_prompt(PromptArgs& A, int64_t n_rows, int64_t n_keys) {
     const int64_t groups = (n_rows * A.group / kPromptRows + A.n_seqs) * A.kv_heads;
     const int64_t each = A.n_seqs > 0 ? n_keys / A.n_seqs : 0;  // keys of a sequence, about
-    int64_t chunk = INT32_MAX / 2;
+    int64_t chunk = INT32_MAX;  // no call has more keys
     if (groups <= 256 && each > 512 && each > 8 * groups) {
         const int64_t parts = 512 / (groups > 0 ? groups : 1);
         chunk = each / parts > 256 ? each / parts : 256;
@@ -627,6 +734,16 @@ void plan_prompt(PromptArgs& A, int64_t n_rows, int64_t n_keys) {
     }
     A.chunk = static_cast<int32_t>(chunk);
     A.n_splits = n_keys > chunk ? static_cast<int32_t>((n_keys + chunk - 1) / chunk) : 1;
+    // Rows of parts: what one sequence needs with every key; of several, which
+    // are shorter, twice what they need if all are of one length, or 64 MiB.
+    // (The kernels take longer parts where that is too little: lengths are on
+    // the GPU. With as many rows as n_splits parts of every row, 32 prompts of
+    // 112 rows over 2112 keys took 939 MB for the 30 they use.)
+    const int64_t row = static_cast<int64_t>(A.kv_heads) * A.group * (4 * padded_dim(A.dim) + 8);
+    const int64_t even = 2 * n_rows * ((each + chunk - 1) / chunk), least = kPromptScratch / row;
+    const int64_t most = n_rows * A.n_splits, rows = even > least ? even : least;
+    A.part_rows = A.n_splits > 1 ? static_cast<int32_t>(most < rows ? most : rows) : 0;
+    A.all_fit = most <= rows;
 }
 
 template <typename T, int DP>
@@ -634,7 +751,14 @@ int launch_prompt(PromptArgs& A, hipStream_t s) {
     constexpr int QT = 1, NW = 4, BM = 32 * QT * NW;
     static_assert(BM == kPromptRows, "the join goes by the same rows");
     const int64_t rows = static_cast<int64_t>(A.n_q) * A.group;
-    const int64_t groups = (rows / BM + A.n_seqs) * A.kv_heads * A.n_splits;
+    // Split: a sequence's tiles are its rows / BM and one at most, in each of its
+    // parts; the parts are one for each chunk and sequence at most, their rows
+    // at most part_rows. Sequences of one part have the other tiles.
+    int64_t units = rows / BM + A.n_seqs;
+    if (A.n_splits > 1)
+        units = A.n_seqs == 1 ? (rows + BM - 1) / BM * A.n_splits
+                              : units + static_cast<int64_t>(A.part_rows) * A.group / BM + A.n_k / A.chunk + A.n_seqs;
+    const int64_t groups = units * A.kv_heads;
     if (rows > INT32_MAX || groups > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "prompt attention: too many rows times heads");
     A.n_slots = static_cast<int32_t>(rows / BM + A.n_seqs);
     const dim3 grid(static_cast<uint32_t>(groups)), block(64 * NW);
@@ -1211,9 +1335,9 @@ extern "C" int aimg_prompt_workspace_nbytes(int64_t n_rows, int64_t n_keys, int 
         dim < 1 || dim > aimg::kMaxDim || n_seqs < 0)
         return fail(AIMG_ERR_INVALID_ARGUMENT, "prompt attention: rows, keys, heads, dim and n_seqs must be sizes of one call");
     aimg::PromptArgs a{};
-    a.n_seqs = n_seqs, a.kv_heads = kv_heads, a.group = heads / kv_heads;
+    a.n_seqs = n_seqs, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim;
     aimg::plan_prompt(a, n_rows, n_keys);
-    *nbytes = a.n_splits > 1 ? static_cast<size_t>(n_rows) * heads * a.n_splits * (4 * aimg::padded_dim(dim) + 8) : 0;
+    *nbytes = static_cast<size_t>(a.part_rows) * heads * (4 * aimg::padded_dim(dim) + 8);
     return AIMG_OK;
 }
 
@@ -1252,7 +1376,7 @@ extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, c
     a.n_q = static_cast<int32_t>(q->n_rows), a.n_k = static_cast<int32_t>(k->n_rows);
     a.c = scale * aimg::kLog2E, a.scale = scale;
     aimg::plan_prompt(a, q->n_rows, k->n_rows);
-    const int64_t part_rows = q->n_rows * q->heads * a.n_splits;
+    const int64_t part_rows = static_cast<int64_t>(a.part_rows) * q->heads;
     const int dp = aimg::padded_dim(q->dim);
     if (a.n_splits > 1 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
                            workspace_nbytes < static_cast<size_t>(part_rows) * (4 * dp + 8)))
