@@ -392,6 +392,7 @@ __device__ __forceinline__ int find_sequence(const int32_t* offsets, int n, int 
 }
 
 constexpr int kPromptKeys = 64;
+constexpr int64_t kMostKeys = INT32_MAX - kPromptKeys;  // of a call: the first key after the last tile is an int32
 constexpr int kPromptRows = 128;  // of a workgroup
 
 // A sequence of a call, bounded to the buffers.
@@ -1320,6 +1321,11 @@ int by_type(int type, int dim, Launch launch) {
     return aimg::fail(AIMG_ERR_UNSUPPORTED, "type must be AIMG_BF16 or AIMG_FP16, got " + std::to_string(type));
 }
 
+int check_keys(int64_t n) {
+    if (n > aimg::kMostKeys) return aimg::fail(AIMG_ERR_UNSUPPORTED, "prompt attention: needs fewer than 2^31 - 64 rows of keys");
+    return AIMG_OK;
+}
+
 int check_scale(float scale) {
     if (!(scale > 0.0f) || std::isinf(scale)) return aimg::fail(AIMG_ERR_INVALID_ARGUMENT, "scale must be a positive number");
     return AIMG_OK;
@@ -1334,6 +1340,8 @@ extern "C" int aimg_prompt_workspace_nbytes(int64_t n_rows, int64_t n_keys, int 
     if (n_rows < 0 || n_rows > INT32_MAX || n_keys < 0 || n_keys > INT32_MAX || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 ||
         dim < 1 || dim > aimg::kMaxDim || n_seqs < 0)
         return fail(AIMG_ERR_INVALID_ARGUMENT, "prompt attention: rows, keys, heads, dim and n_seqs must be sizes of one call");
+    const int rc = check_keys(n_keys);
+    if (rc != AIMG_OK) return rc;
     aimg::PromptArgs a{};
     a.n_seqs = n_seqs, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = dim;
     aimg::plan_prompt(a, n_rows, n_keys);
@@ -1349,6 +1357,7 @@ extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, c
     if (rc == AIMG_OK) rc = check_heads(k, "k");
     if (rc == AIMG_OK) rc = check_heads(v, "v");
     if (rc == AIMG_OK) rc = check_heads(out, "out", true);
+    if (rc == AIMG_OK) rc = check_keys(k->n_rows);
     if (rc == AIMG_OK) rc = check_scale(scale);
     if (rc != AIMG_OK) return rc;
     if (k->n_rows != v->n_rows || k->heads != v->heads || k->dim != q->dim || v->dim != q->dim)

@@ -290,7 +290,8 @@ typedef struct aimg_heads {
  * k_offsets[b] .. of k and v. The last query row sees every key, the one
  * before it all but the last, and so on (a prompt that continues a context
  * has more keys than rows); a row that sees no key gives zeros. Head h of q
- * reads head h / (q->heads / k->heads) of k and v.
+ * reads head h / (q->heads / k->heads) of k and v, which have fewer than
+ * 2^31 - 64 rows.
  * out has q's shape; rows outside every sequence are not written. lse: NULL,
  * or float[q->n_rows][q->heads] (device) for log(sum(exp(scale * q.k))), -inf
  * for a row that sees no key. scale > 0. Offsets outside the rows are bounded

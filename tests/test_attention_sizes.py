@@ -25,3 +25,18 @@ def test_split_prompts_need_little_scratch_however_many_they_are(seqs, heads, kv
     # A single sequence's parts are known exactly: a row of sums and two numbers for each row, head and part.
     if seqs == 1:
         assert all(_prompt_nbytes(*size) % (size[0] * heads * row) == 0 for size in sizes)
+
+
+def _heads(n=4, heads=2, dim=64, data=1 << 20, row=None, head=None):
+    return _native.AimgHeads(data, n, heads * dim if row is None else row, dim if head is None else head, heads, dim)
+
+
+def test_keys_whose_tiles_would_pass_32_bits_are_refused():
+    """The first key of a tile and the tile's 64 stay below 2^31."""
+    lib, n = _native.lib(), ctypes.c_size_t()
+    for rows, prompt, nbytes in [((1 << 31) - 65, b"null offsets", _native.AIMG_OK), ((1 << 31) - 64, b"2^31 - 64", _native.AIMG_ERR_UNSUPPORTED),
+                                 ((1 << 31) - 1, b"2^31 - 64", _native.AIMG_ERR_UNSUPPORTED)]:
+        q, k = _heads(), _heads(n=rows, row=0)
+        assert lib.aimg_prompt_attention(q, k, k, q, None, None, 1, 0, 1.0, None, None, 0, None) != _native.AIMG_OK
+        assert prompt in lib.aimg_last_error(), rows
+        assert lib.aimg_prompt_workspace_nbytes(4, rows, 2, 2, 64, 1, ctypes.byref(n)) == nbytes, rows
