@@ -573,8 +573,10 @@ int take(const aimg_cache* c, Cache& C, bool pool) {
     if (c->dim % 8 != 0) return fail(AIMG_ERR_UNSUPPORTED, "cache: dim must be a multiple of 8");
     if (static_cast<int64_t>(c->max_pages) * c->page_size > INT32_MAX / 2)
         return fail(AIMG_ERR_UNSUPPORTED, "cache: a sequence must hold fewer than 2^30 positions");
+    // By division: the product of the three can pass 64 bits.
+    if (static_cast<int64_t>(c->kv_heads) * c->dim > INT32_MAX / 2 / c->page_size)
+        return fail(AIMG_ERR_UNSUPPORTED, "cache: a page must be below 2^31 bytes");
     const int64_t page = 2 * static_cast<int64_t>(c->kv_heads) * c->page_size * c->dim;
-    if (page > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "cache: a page must be below 2^31 bytes");
     if (c->page_table == nullptr || c->lengths == nullptr || c->held == nullptr || c->refs == nullptr || c->status == nullptr ||
         (pool && c->pool == nullptr))
         return fail(AIMG_ERR_INVALID_ARGUMENT, "cache: null pointer");

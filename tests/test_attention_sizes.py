@@ -40,3 +40,11 @@ def test_keys_whose_tiles_would_pass_32_bits_are_refused():
         assert lib.aimg_prompt_attention(q, k, k, q, None, None, 1, 0, 1.0, None, None, 0, None) != _native.AIMG_OK
         assert prompt in lib.aimg_last_error(), rows
         assert lib.aimg_prompt_workspace_nbytes(4, rows, 2, 2, 64, 1, ctypes.byref(n)) == nbytes, rows
+
+
+@pytest.mark.parametrize("page_size", [1 << 28, (1 << 29) + (1 << 28), (1 << 30) - 1])
+def test_pages_whose_bytes_pass_64_bits_are_refused(page_size):
+    lib = _native.lib()
+    c = _native.AimgCache(1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 1, 1, 1 << 20, page_size, 8 * 1023, 1, 1)
+    assert lib.aimg_cache_reserve(c, None, None, 0, None) == _native.AIMG_ERR_UNSUPPORTED
+    assert b"2^31 bytes" in lib.aimg_last_error()
