@@ -1277,7 +1277,8 @@ namespace {
 
 // The checks every attention shares: type, element counts, strides that keep
 // 16-byte pieces aligned.
-int check_heads(const aimg_heads* x, const char* name, bool written = false) {
+// most: of a row's stride.
+int check_heads(const aimg_heads* x, const char* name, int64_t most = INT64_MAX, bool written = false) {
     using aimg::fail;
     const std::string n(name);
     if (x == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, n + " is null");
@@ -1287,8 +1288,8 @@ int check_heads(const aimg_heads* x, const char* name, bool written = false) {
         return fail(AIMG_ERR_UNSUPPORTED, n + ": dim must be a multiple of 8 up to " + std::to_string(aimg::kMaxDim) + ", got " + std::to_string(x->dim));
     if (x->n_rows == 0) return AIMG_OK;
     if (x->data == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, n + ": null data");
-    if (x->row_stride < 0 || x->head_stride < 0 || (!written && x->row_stride > aimg::kMaxRowStride))
-        return fail(AIMG_ERR_UNSUPPORTED, n + ": strides must not be negative, a row's at most 2^24 elements");
+    if (x->row_stride < 0 || x->head_stride < 0) return fail(AIMG_ERR_UNSUPPORTED, n + ": strides must not be negative");
+    if (x->row_stride > most && x->n_rows > 1) return fail(AIMG_ERR_UNSUPPORTED, n + ": a row's stride must be at most 2^24 elements");
     const int64_t unit = written ? 4 : 8;
     if (reinterpret_cast<uintptr_t>(x->data) % (2 * unit) != 0 || x->row_stride % unit != 0 || x->head_stride % unit != 0)
         return fail(AIMG_ERR_UNSUPPORTED, n + ": needs a " + std::to_string(2 * unit) + "-byte aligned pointer and strides of whole " +
@@ -1354,9 +1355,9 @@ extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, c
                                      float scale, float* lse, void* workspace, size_t workspace_nbytes, void* stream) {
     using aimg::fail;
     int rc = check_heads(q, "q");
-    if (rc == AIMG_OK) rc = check_heads(k, "k");
-    if (rc == AIMG_OK) rc = check_heads(v, "v");
-    if (rc == AIMG_OK) rc = check_heads(out, "out", true);
+    if (rc == AIMG_OK) rc = check_heads(k, "k", aimg::kMaxRowStride);
+    if (rc == AIMG_OK) rc = check_heads(v, "v", aimg::kMaxRowStride);
+    if (rc == AIMG_OK) rc = check_heads(out, "out", INT64_MAX, true);
     if (rc == AIMG_OK) rc = check_keys(k->n_rows);
     if (rc == AIMG_OK) rc = check_scale(scale);
     if (rc != AIMG_OK) return rc;
@@ -1442,7 +1443,7 @@ extern "C" int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages,
                                    size_t workspace_nbytes, void* stream) {
     using aimg::fail;
     int rc = check_heads(q, "q");
-    if (rc == AIMG_OK) rc = check_heads(out, "out", true);
+    if (rc == AIMG_OK) rc = check_heads(out, "out", INT64_MAX, true);
     if (rc == AIMG_OK) rc = check_pages(pages);
     if (rc == AIMG_OK) rc = check_scale(scale);
     if (rc != AIMG_OK) return rc;

@@ -274,7 +274,8 @@ int aimg_pack_chunked(const uint8_t* symbols, int64_t n, const uint32_t* code_of
 
 /* Rows of heads: element (row, head, x) is data[row * row_stride + head *
  * head_stride + x], strides in elements. dim is a multiple of 8 up to 256.
- * Inputs need 16-byte aligned data and strides of whole 16 bytes, outputs 8. */
+ * Inputs need 16-byte aligned data and strides of whole 16 bytes, outputs 8.
+ * Rows of keys and values are at most 2^24 elements apart. */
 typedef struct aimg_heads {
     void* data;          /* device                                    */
     int64_t n_rows;
@@ -310,8 +311,9 @@ int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, const aimg_h
  * slot s is row j % page_size of page page_table[s * table_stride + j /
  * page_size]; element x of head h there is k[page * page_stride + row *
  * slot_stride + h * head_stride + x], and v's likewise (strides in elements,
- * whole 16 bytes, the same for both). lengths[s] positions are held before the
- * drafted ones. Page numbers outside 0..n_pages-1 read page 0. */
+ * whole 16 bytes, the same for both, slot_stride at most 2^24). lengths[s]
+ * positions are held before the drafted ones. Page numbers outside
+ * 0..n_pages-1 read page 0. */
 typedef struct aimg_pages {
     void* k;                      /* device */
     void* v;                      /* device */

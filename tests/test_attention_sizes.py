@@ -48,3 +48,13 @@ def test_pages_whose_bytes_pass_64_bits_are_refused(page_size):
     c = _native.AimgCache(1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 1, 1, 1 << 20, page_size, 8 * 1023, 1, 1)
     assert lib.aimg_cache_reserve(c, None, None, 0, None) == _native.AIMG_ERR_UNSUPPORTED
     assert b"2^31 bytes" in lib.aimg_last_error()
+
+
+def test_query_rows_may_be_any_distance_apart():
+    """Only rows of keys and values are read many at a time, by 32-bit offsets; a single row has no distance."""
+    lib = _native.lib()
+    far = (1 << 24) + 8
+    for q, k, message in [(_heads(row=1 << 40), _heads(), b"null offsets"), (_heads(), _heads(n=1, row=far), b"null offsets"),
+                          (_heads(), _heads(row=1 << 24), b"null offsets"), (_heads(), _heads(row=far), b"2^24")]:
+        assert lib.aimg_prompt_attention(q, k, k, q, None, None, 1, 0, 1.0, None, None, 0, None) != _native.AIMG_OK
+        assert message in lib.aimg_last_error()
