@@ -116,6 +116,20 @@ __device__ __forceinline__ void load_to_lds(const void* from, lds_char* to) {
                                      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
+// Keys narrower than DP elements: the pieces past a row's last, which hold a
+// copy of it, become zeros in rows row0 .. row0 + kRows - 1 of the tile, that
+// the wave itself has loaded. (An infinite element of the copy would meet the
+// query's zeros there and make the score NaN. Lanes that sit those loads out
+// instead, over places cleared once: 32 trees of dim 96 over 2000-8000
+// positions 130 us.)
+template <int DP, int kRows>
+__device__ __forceinline__ void clear_past(int dim, lds_char* keys, int row0, int lane) {
+    typedef Rows<DP> R;
+    const int r = row0 + lane % kRows;
+    for (int x = dim / 8 + lane / kRows; x < R::kPieces; x += 64 / kRows)
+        *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(keys + r * R::kBytes + ((x ^ R::key_place(r)) << 4)) = u32x4{0};
+}
+
 // x where bit `at` of bits is set, -inf otherwise: two instructions, and no lane mask in scalar registers.
 __device__ __forceinline__ float seen_or(uint32_t bits, int at, float x) {
     const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(bits), at, 1));
@@ -551,7 +565,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
 
     const uint16_t* const k_base = A.k + k_begin * A.k_row + kvh * A.k_head;
     const uint16_t* const v_base = A.v + k_begin * A.v_row + kvh * A.v_head;
-    const int pieces = A.dim / 8 - 1;  // the last 16-byte piece of a row; pieces past it repeat it
+    const int pieces = A.dim / 8 - 1;  // the last 16-byte piece of a row; pieces past it repeat it at first
     const int lane_row = lane / R::kPieces, lane_piece = lane % R::kPieces;
     const uint32_t k_bytes = static_cast<uint32_t>(2 * A.k_row), v_bytes = static_cast<uint32_t>(2 * A.v_row);
     auto load_tile = [&](int k0, lds_char* to) {
@@ -583,8 +597,12 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
         st.load_query(t, A.q + (q_begin + at / group) * A.q_row + (kvh * group + at % group) * A.q_head, A.dim, half);
         sees[t] = seen_by(at);
     }
-    wait_loads<0>();
-    __syncthreads();
+    auto arrived = [&](lds_char* to) __attribute__((always_inline)) {
+        wait_loads<0>();
+        if (A.dim < DP) clear_past<DP, KT / NW>(A.dim, to, wave * (KT / NW), lane);
+        __syncthreads();
+    };
+    arrived(shared);
     int k0 = begin;
     uint32_t at = 0;  // the tile's place in LDS
     // Tiles that every row of the workgroup sees whole, then those it needs
@@ -597,8 +615,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
             st.template step<NSUB, false>(now, now + kTile, A.c, lane, all);
         };
         tile(shared + (at ^ 2 * kTile), shared + at);
-        wait_loads<0>();
-        __syncthreads();
+        arrived(shared + (at ^ 2 * kTile));
     }
     for (; k0 < end; k0 += KT, at ^= 2 * kTile) {
         auto tile = [&](lds_char* __restrict__ next, const lds_char* __restrict__ now) __attribute__((always_inline)) {
@@ -613,8 +630,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
             }
         };
         tile(shared + (at ^ 2 * kTile), shared + at);
-        wait_loads<0>();
-        __syncthreads();
+        arrived(shared + (at ^ 2 * kTile));
     }
 
 #pragma unroll
@@ -964,12 +980,14 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         token[t] = r / group;
         st.load_query(t, A.q + (D.row + token[t]) * A.q_row + (kvh * group + r % group) * A.q_head, A.dim, half);
     }
-    if (kShared) {
+    auto arrived = [&](lds_char* to) __attribute__((always_inline)) {
         wait_loads<0>();
+        if (A.dim < DP) clear_past<DP, KT / NW>(A.dim, to, wave * (KT / NW), lane);
         __syncthreads();
-    }
+    };
+    if (kShared) arrived(mine);
     // Two tiles in turn.
-    auto tile = [&](auto masked, lds_char* __restrict__ next, const lds_char* __restrict__ now) __attribute__((always_inline)) {
+    auto tile = [&](auto masked, lds_char* __restrict__ next, lds_char* __restrict__ now) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked)::value;
         const bool more = k0 + kStep < hi;
         if (more) issue(k0 + kStep, next);
@@ -981,6 +999,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
             if (more) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(zero) : "n"(2 * kLoads) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" : "+v"(zero) : : "memory");
             now += zero;
+            if (A.dim < DP) clear_past<DP, KT>(A.dim, now, 0, lane);
         }
         if (!active) return;
         uint32_t allow[QT][NSUB] = {};
@@ -994,17 +1013,11 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
     };
     for (; k0 + KT <= D.context && k0 < hi; k0 += kStep, at ^= 2 * kTile) {
         tile(std::integral_constant<bool, false>{}, mine + (at ^ 2 * kTile), mine + at);
-        if (kShared) {
-            wait_loads<0>();
-            __syncthreads();
-        }
+        if (kShared) arrived(mine + (at ^ 2 * kTile));
     }
     for (; k0 < hi; k0 += kStep, at ^= 2 * kTile) {
         tile(std::integral_constant<bool, true>{}, mine + (at ^ 2 * kTile), mine + at);
-        if (kShared) {
-            wait_loads<0>();
-            __syncthreads();
-        }
+        if (kShared) arrived(mine + (at ^ 2 * kTile));
     }
 
     const int64_t part = static_cast<int64_t>(split) * A.n_q * A.heads;
