@@ -6,7 +6,8 @@ The reference leaves attention to the model's own forward pass
 products a program runs between the q/k/v projections whose weights it decodes
 and the output projection. Elements are bf16 or fp16; scores, softmax
 statistics and sums are fp32. Work is ordered on the current stream and nothing
-here synchronises.
+here synchronises. There is no backward pass: inputs that require a gradient are
+refused while gradients are recorded.
 """
 from __future__ import annotations
 
@@ -30,6 +31,12 @@ _TYPES = {torch.bfloat16: _native.AIMG_BF16, torch.float16: _native.AIMG_FP16}
 # checks go by the cheapest question first: a device's index rather than the
 # device, shapes and strides taken apart once, descriptors built once a call.
 
+def forward_only(x: torch.Tensor, name: str) -> None:
+    """Refuses a tensor whose gradient autograd would expect."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("%s requires a gradient, and attention has no backward pass: detach it, or call under torch.no_grad()" % name)
+
+
 def _heads(x: torch.Tensor, name: str, dtype: torch.dtype, index: int, unit: int = 8) -> _native.AimgHeads:
     """The descriptor of rows of heads [n, heads, dim] of this type on GPU
     ``index``, any row and head strides that keep whole pieces of ``unit``
@@ -44,6 +51,7 @@ def _heads(x: torch.Tensor, name: str, dtype: torch.dtype, index: int, unit: int
             raise ValueError("%s: dim must be a multiple of 8 up to %d, got %d" % (name, MAX_DIM, dim))
         raise ValueError("%s must be contiguous in its last dimension, its rows and heads on %d-byte boundaries"
                          % (name, 2 * unit))
+    forward_only(x, name)
     return _native.AimgHeads(at, n, row, head, heads, dim)
 
 
@@ -138,7 +146,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offset
 
     Returns out (q's shape and type; rows of no sequence are not written).
     lse, fp32 [rows, heads], receives log(sum(exp(scale * q.k))) when given.
-    Results do not vary between calls."""
+    Results do not vary between calls. No gradients: inputs that require one
+    are refused outside torch.no_grad()."""
     qd, index, kind = _query(q)
     kd, vd = _heads(k, "k", q.dtype, index), _heads(v, "v", q.dtype, index)
     if kd.n_rows != vd.n_rows or kd.heads != vd.heads or kd.dim != qd.dim or vd.dim != qd.dim:
@@ -226,10 +235,13 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     expect (all that the table can hold when not given), decides how the work is
     split, nothing else.
 
-    Returns out (q's shape and type); lse as in prompt_attention. Results do
-    not vary between calls."""
+    Returns out (q's shape and type; rows of no sequence, or past its first
+    max_drafts, are not written); lse as in prompt_attention. Results do not
+    vary between calls. No gradients, as there."""
     qd, index, kind = _query(q)
     pages = describe_pages(k_pages, v_pages, page_table, lengths)
+    forward_only(k_pages, "k_pages")
+    forward_only(v_pages, "v_pages")
     if k_pages.dtype is not q.dtype or k_pages.get_device() != index:
         raise ValueError("k_pages must be %s on %s" % (q.dtype, q.device))
     heads, kv_heads, dim = qd.heads, pages.kv_heads, qd.dim

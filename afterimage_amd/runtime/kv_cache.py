@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from .. import _native
-from .attention import launch, tree_attention
+from .attention import forward_only, launch, tree_attention
 
 MAX_SEQS = 8192      # sequences of one call
 MAX_PAGES = (1 << 20) - 1
@@ -122,6 +122,7 @@ class PagedKVCache:
         row, head, one = x.stride()
         if one != 1 or (row | head) % 8 or x.data_ptr() % 16:
             raise ValueError("%s must be contiguous in its last dimension, its rows and heads on 16-byte boundaries" % name)
+        forward_only(x, name)
         return _native.AimgHeads(x.data_ptr(), x.shape[0], row, head, x.shape[1], x.shape[2])
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, offsets: torch.Tensor) -> None:
