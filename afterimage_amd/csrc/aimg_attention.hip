@@ -205,15 +205,17 @@ struct State {
                 }
             }
             // The maximum is not needed where the probabilities against the
-            // one held stay in range: their sum, which is, tells.
+            // one held stay in range: their sum, which is, tells. A row's own
+            // sums (this lane's and that of the other half) decide for it
+            // alone, so its bits do not depend on the wave's other rows.
             float sum = 0.0f;
             bool fits = false;
-            if (!__any(m[t] == -INFINITY)) {
-                sum = soften<NSUB>(s[t], p[t], c, m[t] * c);
-                fits = __all(sum <= kMostSum);
+            if (!__all(m[t] == -INFINITY)) {
+                sum = soften<NSUB>(s[t], p[t], c, m[t] == -INFINITY ? 0.0f : m[t] * c);
+                fits = sum <= kMostSum && m[t] != -INFINITY;
             }
-            if (__builtin_expect(!fits, 0)) {
-                raise<NSUB>(t, s[t], c);
+            if (__builtin_expect(!__all(fits), 0)) {
+                raise<NSUB>(t, s[t], c, fits);
                 sum = soften<NSUB>(s[t], p[t], c, m[t] == -INFINITY ? 0.0f : m[t] * c);
             }
             l[t] += sum;
@@ -256,16 +258,16 @@ struct State {
         return sum;
     }
 
-    // The maximum of tile t raised to that of its scores, the sums with it.
+    // The maximum of tile t raised to that of its scores, the sums with it, for rows with a half that does not fit.
     template <int NSUB>
-    __device__ __forceinline__ void raise(int t, const f32x16 (&s)[NSUB], float c) {
+    __device__ __forceinline__ void raise(int t, const f32x16 (&s)[NSUB], float c, bool fits) {
         float top = s[0][0];
 #pragma unroll
         for (int u = 0; u < NSUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
         top = max_halves(top);
-        const bool rise = (top - m[t]) * c > kRise;  // false where both are -inf
+        const bool rise = max_halves(fits ? 0.0f : 1.0f) > 0.0f && (top - m[t]) * c > kRise;  // false where both are -inf
         const float to = rise ? top : m[t];
         const float by = rise ? exp2_fast((m[t] - to) * c) : 1.0f;
         m[t] = to;
