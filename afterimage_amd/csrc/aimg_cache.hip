@@ -329,6 +329,7 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(const ForkArgs A) {
             if (x < full) {
                 id = from[x];
                 if (id >= 0 && id < C.n_pages) atomicAdd(C.refs + id, 1);
+                else tell(C, kBadIndex);
             } else if (x == full && tail > 0) {
                 id = page;
                 atomicAdd(C.refs + id, 1);
@@ -342,7 +343,10 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(const ForkArgs A) {
     }
     if (tail == 0) return;
     const int32_t last = from[full];
-    if (last < 0 || last >= C.n_pages) return;
+    if (last < 0 || last >= C.n_pages) {
+        if (threadIdx.x == 0) tell(C, kBadIndex);
+        return;
+    }
     // The tail's rows of every head and plane, 16 bytes a thread and step: a
     // thread keeps its place in a head's rows and steps over heads and planes,
     // so it divides once (a division a step took longer than the bytes).
@@ -435,7 +439,10 @@ __global__ __launch_bounds__(256) void commit_kernel(const CommitArgs A) {
     auto place = [&](int64_t at) -> int64_t {
         if (at < 0 || at >= most) return -1;
         const int32_t id = row[at / C.page_size];
-        if (id < 0 || id >= C.n_pages) return -1;
+        if (id < 0 || id >= C.n_pages) {
+            tell(C, kBadIndex);
+            return -1;
+        }
         return id * C.page_bytes + at % C.page_size * C.row_bytes;
     };
     for (int32_t i0 = 0; i0 < n; i0 += kPath) {

@@ -375,7 +375,9 @@ int aimg_tree_masks(const int32_t* parents, const int32_t* draft_offsets, int n_
 /* What a call finds wrong on the GPU it leaves undone and says in *status   */
 /* (bits, or-ed in): 1 no free pages (nothing was reserved or forked), 2 a   */
 /* sequence's row of the table or its pages end before the positions asked   */
-/* for, 4 a slot, page, source or number of rows that does not exist.        */
+/* for, 4 a slot, page, source or number of rows that does not exist. (Rows  */
+/* of a table entry that is no page are neither copied nor moved; the rest   */
+/* of such a sequence is.)                                                   */
 /* ------------------------------------------------------------------------- */
 
 #define AIMG_CACHE_NO_PAGES 1

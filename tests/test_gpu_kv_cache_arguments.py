@@ -58,3 +58,30 @@ def test_commit_with_a_count_out_of_range(count, apart):
     p.cache.commit(_ints([0]), _ints([[0, 1, 2, 3]]), _ints([4]))
     p.model.rows[0] += numbers[0]
     p.check()
+
+
+@pytest.mark.parametrize("number", [-1, 40, 1 << 30])
+@pytest.mark.parametrize("entry", [0, 2])
+def test_forks_of_rows_with_a_page_that_does_not_exist_are_reported(number, entry):
+    """A full page's entry, and the last one's."""
+    p = Pair()
+    p.write([0], [10])
+    p.cache.page_table[0, entry] = number
+    p.cache.fork(_ints([0]), _ints([1]))
+    with pytest.raises(RuntimeError, match="does not exist"):
+        p.cache.check()
+    assert p.cache.page_table[0, entry] == number and int(p.cache.refs.sum()) <= 6
+
+
+@pytest.mark.parametrize("entry", [1, 2])
+def test_commits_with_a_page_that_does_not_exist_are_reported(entry):
+    """Where accepted rows would go to (position 7, page 1), and where they are (8 and 10, page 2): they stay."""
+    p = Pair()
+    p.write([0], [7])
+    p.cache.reserve(_ints([0]), _ints([5]))
+    before = p.cache.pool.clone()
+    p.cache.page_table[0, entry] = -5
+    p.cache.commit(_ints([0]), _ints([[1]]), _ints([1]))
+    with pytest.raises(RuntimeError, match="does not exist"):
+        p.cache.check()
+    assert torch.equal(p.cache.pool, before)
