@@ -872,9 +872,14 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeArgs& A, const Drafted& 
 // the end: one token's group (5 rows of 32 here) leaves the matrix cores idle,
 // but the bytes in flight, not the products, bound it.
 // Bound by HBM where contexts are long: 16 trees of 4-16 tokens over 9000-65000
-// positions, 40 heads of 8, dim 128, read 1.73 GB in 325 us, 5.3 TB/s; 64
-// single tokens over 2000-8000 5.06 TB/s. 8 trees of 1-33 tokens over 700-6000
-// positions take 27 us, 3.7 TB/s: two rounds of short parts.
+// positions, 40 heads of 8, dim 128, read 1.73 GB in 330 us, 5.2 TB/s; 64
+// single tokens over 2000-8000 5.1 TB/s. 8 trees of 1-33 tokens over 700-6000
+// positions take 27 us, 3.7 TB/s: 368 workgroups have rows and keys, fewer than
+// the 512 that run at a time, and each has ten tiles at most between its first
+// loads and its sums. Without masks, too, every block of rows takes all keys of
+// its sequence: right, but for a long stretch of a prompt over the cache twice
+// the products it needs (4096 rows over no context 521 us, packed prompts 204;
+// over 8000 positions 1285 and 852).
 // kPages: what of a tile never crosses a page, and so has one base address: 2
 // the tile, 1 the rows of one load (2 to 8), 0 a row. (With addresses made lane
 // by lane for pages of 16, 54 trees over 139-2238 positions took 155 us.)
@@ -1215,12 +1220,14 @@ constexpr int kMaxChunk = 8192;
 constexpr int kMaxSharedChunk = 4096;
 constexpr int kSlots = 256;         // workgroups of dealt-out keys that run at a time, one a CU
 constexpr int kFewParts = 16;       // at most so many are joined by DP / 4 threads a row
-// Workgroups of shared tiles, were all sequences the longest: two a CU, two and
-// a half rounds. Lengths that differ need the parts (16 trees of 18-33 tokens
-// over 200-8600 positions: 62 us, 86 with 1024, 116 with 512, 74 with 2048);
-// trees of one length would do with fewer (6 of 64 tokens over 8000: 113 us, 93
-// with 1024, 125 with 2048), which the host, that knows the longest alone,
-// cannot tell apart.
+// Workgroups of shared tiles, were all sequences the longest. It sets the keys
+// of a part; how many workgroups find rows and keys follows from the lengths (8
+// trees over 700-6000 positions: 368 of 1280) and the others return at once.
+// Chosen by what calls take: lengths that differ need the parts (16 trees of
+// 18-33 tokens over 200-8600 positions: 62 us, 86 with 1024, 116 with 512, 74
+// with 2048); trees of one length would do with fewer (6 of 64 tokens over 8000:
+// 113 us, 93 with 1024, 125 with 2048), which the host, that knows the longest
+// alone, cannot tell apart.
 constexpr int kSharedParts = 1280;
 
 // Rows of a workgroup. Up to 32 or 64 rows of a (sequence, head) go to every

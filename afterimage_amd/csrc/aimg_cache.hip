@@ -309,10 +309,11 @@ __global__ __launch_bounds__(kScan) void fork_plan_kernel(const ForkArgs A) {
 // Workgroup (pair, share of its rows to copy). The first share of a pair also
 // counts its references and writes its new row beside the table: a pair's
 // source may be another pair's branch, so no row changes before all were read.
-// Bound by what it writes (96 branches, 16 planes of 8 heads of 128: 95 MB
-// in 39.5 us; the sources' tails are read once and stay in the caches). Two,
-// four and eight times the rows a thread, or twice as many in flight, took
-// 0.2 to 2 us more.
+// 96 branches, 16 planes of 8 heads of 128: 95 MB written in 39.5 us, and 8 MB
+// read, for the sources' tails stay in the caches. That is half of what a copy
+// of as many bytes reaches (21 us), and what bounds it is not known. Two, four
+// and eight times the rows a thread, or twice as many in flight, took 0.2 to
+// 2 us more.
 __global__ __launch_bounds__(256) void fork_copy_kernel(const ForkArgs A) {
     const Cache& C = A.c;
     const int i = blockIdx.x;
@@ -414,8 +415,9 @@ constexpr int kPath = 128;  // rows of a path whose places are held at a time
 // A thread owns 16 bytes of one head in one plane and moves them for row after
 // row of its sequence's path. Accepted indices rise, so row i goes to a place
 // at or before its own and before every later source: four rows are read, then
-// written, and no other thread touches these bytes. Bound by HBM: 64 sequences,
-// 12 accepted rows in 80 planes of 8 heads of 128 move 126 MB in 24.5 us.
+// written, and no other thread touches these bytes. Bound by HBM: 64 sequences
+// of up to 12 accepted rows, 6 on average, in 80 planes of 8 heads of 128 read
+// 58 MB and write 58 in 25 us.
 __global__ __launch_bounds__(256) void commit_kernel(const CommitArgs A) {
     const Cache& C = A.c;
     __shared__ int64_t from[kPath], to[kPath];
