@@ -435,6 +435,13 @@ __device__ __forceinline__ int32_t part_rows_of(const Prompt& p, int32_t chunk) 
     return parts > 1 ? p.q_len * parts : 0;
 }
 
+// Whether a sequence's parts, from its place on, lie in the workspace. They do
+// unless offsets fall (sequences then lie over each other and need more rows than
+// there are); such a sequence is left out.
+__device__ __forceinline__ bool parts_fit(const PromptArgs& A, const Prompt& p, int32_t chunk, int32_t place) {
+    return place + part_rows_of(p, chunk) <= A.part_rows;
+}
+
 template <int kLanes>
 __device__ __forceinline__ int32_t sum_lanes(int32_t v) {
 #pragma unroll
@@ -538,9 +545,11 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
         chunk = __builtin_amdgcn_readfirstlane(part_keys<64>(A, lane));
         PromptPart p;
         if (!find_part(A, chunk, static_cast<int32_t>(blockIdx.x / A.kv_heads), lane, p)) return;
+        place = __builtin_amdgcn_readfirstlane(p.place);
+        if (!parts_fit(A, p.of, chunk, place)) return;
         q_begin = p.of.q_begin, q_len = p.of.q_len, k_begin = p.of.k_begin, k_len = p.of.k_len;
         rows = q_len * group, row0 = (p.tiles - 1 - p.tile) * BM;
-        split = p.part, place = p.place;
+        split = p.part;
     } else {
         const int slot = A.n_slots - 1 - static_cast<int>(blockIdx.x / A.kv_heads);
         const int lo = find_sequence(A.q_offsets, A.n_seqs, A.n_q, slot, lane, [&](int b, int first) { return first * group / BM + b; });
@@ -724,6 +733,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(const PromptArgs A) {
         for (int b = col; b < lo; b += kCols) place += part_rows_of(prompt_of(A, b), chunk);
         place = sum_lanes<kCols>(place);
     }
+    if (!parts_fit(A, p, chunk, place)) return;
     place += row - p.q_begin;
     join_parts<T, DP>(A.part_o, A.part_ml, static_cast<int64_t>(p.q_len) * A.heads, static_cast<int64_t>(place) * A.heads + head,
                       (keys - 1) / chunk + 1, col, A.dim, A.out + row * A.out_row + head * A.out_head,

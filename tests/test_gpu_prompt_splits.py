@@ -1,9 +1,11 @@
 """Prompts split along their keys: where their parts lie, and many sequences a call."""
+import ctypes
 import random
 
 import pytest
 import torch
 
+from afterimage_amd import _native
 from afterimage_amd.runtime.attention import prompt_attention
 from tests.attention_oracle import check
 from tests.test_gpu_prompt_attention import _case, _expected, _offsets
@@ -45,3 +47,24 @@ def test_many_short_sequences(seed):
     out = prompt_attention(q, k, v, _offsets(rows), _offsets(keys))
     o, bound, _ = _expected(q, k, v, rows, keys, 64 ** -0.5)
     check(out, o, bound)
+
+
+@pytest.mark.parametrize("q_offsets,k_offsets", [
+    ([0, 20, 0, 20], [0, 6000, 0, 6000]),
+    ([0, 20, 0, 20, -5, 999], [0, 6000, -9, 7000, 3, 6000]),
+    ([20, 0, 20, 0, 20], [0, 6000, 6000, 0, 6000]),
+])
+def test_offsets_that_fall_stay_within_the_workspace(q_offsets, k_offsets):
+    """Sequences over each other need more parts than were planned for: what lies past the workspace is not touched."""
+    q, k, v = _case([20], [6000], 8, 1, 64, torch.bfloat16)
+    out, n, seqs = torch.zeros_like(q), ctypes.c_size_t(), len(q_offsets) - 1
+    lib = _native.lib()
+    _native.check(lib.aimg_prompt_workspace_nbytes(20, 6000, 8, 1, 64, seqs, ctypes.byref(n)))
+    assert n.value > 0
+    guarded = torch.full((16 * n.value,), 77, dtype=torch.uint8, device="cuda")
+    at = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in (q_offsets, k_offsets)]
+    heads = [_native.AimgHeads(x.data_ptr(), x.shape[0], *x.stride()[:2], *x.shape[1:]) for x in (q, k, v, out)]
+    _native.check(lib.aimg_prompt_attention(*heads, at[0].data_ptr(), at[1].data_ptr(), seqs, _native.AIMG_BF16, 0.125, None,
+                                            guarded.data_ptr(), n.value, torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert bool((guarded[n.value:] == 77).all())
