@@ -125,6 +125,7 @@ __device__ __forceinline__ void load_to_lds(const void* from, lds_char* to) {
 template <int DP, int kRows>
 __device__ __forceinline__ void clear_past(int dim, lds_char* keys, int row0, int lane) {
     typedef Rows<DP> R;
+    asm volatile("" : "+v"(lane));  // its addresses are not worth registers in the loop over tiles
     const int r = row0 + lane % kRows;
     for (int x = dim / 8 + lane / kRows; x < R::kPieces; x += 64 / kRows)
         *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(keys + r * R::kBytes + ((x ^ R::key_place(r)) << 4)) = u32x4{0};
@@ -208,12 +209,10 @@ struct State {
             // one held stay in range: their sum, which is, tells. A row's own
             // sums (this lane's and that of the other half) decide for it
             // alone, so its bits do not depend on the wave's other rows.
-            float sum = 0.0f;
-            bool fits = false;
-            if (!__all(m[t] == -INFINITY)) {
-                sum = soften<NSUB>(s[t], p[t], c, m[t] == -INFINITY ? 0.0f : m[t] * c);
-                fits = sum <= kMostSum && m[t] != -INFINITY;
-            }
+            // (Against -inf, before a row's first visible key, they are infinite or NaN.)
+            float sum = INFINITY;
+            if (!__all(m[t] == -INFINITY)) sum = soften<NSUB>(s[t], p[t], c, m[t] * c);
+            const bool fits = sum <= kMostSum;
             if (__builtin_expect(!__all(fits), 0)) {
                 raise<NSUB>(t, s[t], c, fits);
                 sum = soften<NSUB>(s[t], p[t], c, m[t] == -INFINITY ? 0.0f : m[t] * c);
