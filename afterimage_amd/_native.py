@@ -14,7 +14,7 @@ from pathlib import Path
 import torch  # noqa: F401  (must be loaded before the library; see module doc)
 
 LIB_PATH = Path(__file__).resolve().parent / "libafterimage_decode.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 MAX_TENSORS = 32
 
 AIMG_OK = 0
@@ -25,6 +25,7 @@ AIMG_ERR_UNSUPPORTED = 4
 
 AIMG_BF16 = 0
 AIMG_FP16 = 1
+AIMG_FP32 = 2
 
 
 class NativeError(RuntimeError):
@@ -89,6 +90,17 @@ class AimgPages(ctypes.Structure):
     ]
 
 
+class AimgPageScales(ctypes.Structure):
+    """Mirror of ``aimg_page_scales``."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+    ]
+
+
 class AimgCache(ctypes.Structure):
     """Mirror of ``aimg_cache``."""
 
@@ -109,7 +121,35 @@ class AimgCache(ctypes.Structure):
     ]
 
 
+class AimgRotary(ctypes.Structure):
+    """Mirror of ``aimg_rotary``."""
+
+    _fields_ = [
+        ("cos", ctypes.c_void_p),
+        ("sin", ctypes.c_void_p),
+        ("n_positions", ctypes.c_int32),
+        ("half", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+    ]
+
+
+class AimgSampling(ctypes.Structure):
+    """Mirror of ``aimg_sampling``."""
+
+    _fields_ = [
+        ("temperatures", ctypes.c_void_p),
+        ("top_ks", ctypes.c_void_p),
+        ("top_ps", ctypes.c_void_p),
+        ("min_ps", ctypes.c_void_p),
+        ("temperature", ctypes.c_double),
+        ("top_p", ctypes.c_double),
+        ("min_p", ctypes.c_double),
+        ("top_k", ctypes.c_int32),
+    ]
+
+
 _HEADS = ctypes.POINTER(AimgHeads)
+_ROTARY = ctypes.POINTER(AimgRotary)
 _CACHE = ctypes.POINTER(AimgCache)
 _SIZE = ctypes.POINTER(ctypes.c_size_t)
 _PAGES = ctypes.POINTER(AimgPages)
@@ -165,10 +205,28 @@ _SIGNATURES = [
      [_HEADS, _PAGES, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
       ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
       ctypes.c_void_p]),
+    ("aimg_tree8_attention", ctypes.c_int,
+     [_HEADS, _PAGES, ctypes.POINTER(AimgPageScales), _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+      ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+      ctypes.c_void_p]),
     ("aimg_tree_masks", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p]),
     ("aimg_cache_append", ctypes.c_int,
      [_CACHE, ctypes.c_int, _HEADS, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    ("aimg_cache_append_rotated", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_int, _HEADS, _HEADS, _HEADS, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+      _ROTARY, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
+    ("aimg_cache_read", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, _HEADS, _HEADS,
+      ctypes.c_int, ctypes.c_void_p]),
+    ("aimg_cache8_fork", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    ("aimg_cache8_commit", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+      ctypes.c_void_p]),
+    ("aimg_cache8_compact", ctypes.c_int,
+     [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+      ctypes.c_void_p]),
     ("aimg_cache_advance", ctypes.c_int,
      [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     ("aimg_cache_reserve", ctypes.c_int,
@@ -183,6 +241,9 @@ _SIGNATURES = [
     ("aimg_cache_compact_workspace_nbytes", ctypes.c_int, [_CACHE, _SIZE]),
     ("aimg_cache_compact", ctypes.c_int,
      [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    ("aimg_sample", ctypes.c_int,
+     [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(AimgSampling),
+      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
 ]
 
 EXPORTED_SYMBOLS = tuple(name for name, _, _ in _SIGNATURES)

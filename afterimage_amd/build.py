@@ -67,7 +67,7 @@ def build(verbose: bool = False) -> Path:
     hipcc = _hipcc()
     inc = ["-I", str(INCLUDE), "-I", str(CSRC)]
     hip = [(CSRC / f"{name}.hip", BUILD_DIR / f"{name}.o", flags)
-           for name, flags in (("aimg_decode", []), ("aimg_attention", ATTENTION_FLAGS), ("aimg_cache", []))]
+           for name, flags in (("aimg_decode", []), ("aimg_attention", ATTENTION_FLAGS), ("aimg_cache", []), ("aimg_sample", []))]
     host_obj = BUILD_DIR / "aimg_host.o"
     cpu_obj = BUILD_DIR / "aimg_cpu.o"
     steps = [

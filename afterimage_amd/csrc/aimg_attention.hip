@@ -40,6 +40,7 @@ typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(8))) short s16x8;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
@@ -53,6 +54,14 @@ struct Bf16 {
     static __device__ uint32_t pack(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
     }
+    // Eight e4m3 elements times a power of two, exact.
+    static __device__ s16x8 from8(uint32_t a, uint32_t b, float scale) {
+        auto two = [](auto x) { return __builtin_bit_cast(uint32_t, x); };
+        return __builtin_bit_cast(s16x8, (u32x4{two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false)),
+                                                two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true)),
+                                                two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false)),
+                                                two(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true))}));
+    }
 };
 
 struct Fp16 {
@@ -62,6 +71,13 @@ struct Fp16 {
     }
     static __device__ uint32_t pack(float a, float b) {
         return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+    }
+    static __device__ s16x8 from8(uint32_t a, uint32_t b, float scale) {
+        auto two = [](auto x) { return __builtin_bit_cast(uint32_t, x); };
+        return __builtin_bit_cast(s16x8, (u32x4{two(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, false)),
+                                                two(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, scale, true)),
+                                                two(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, false)),
+                                                two(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, scale, true))}));
     }
 };
 
@@ -96,6 +112,20 @@ struct Rows {
     }
 };
 
+// Rows of a tile of 8-bit elements, pieces of 16. Keys: 16 rows at one x cover
+// all banks once (rows of 64 bytes take four places for each four rows). Values
+// are read by eight rows {0..3, 8..11} (+ 4) and two neighbouring pieces at a time.
+template <int DP>
+struct Rows8 {
+    static constexpr int kBytes = DP;
+    static constexpr int kPieces = DP / 16;
+    static constexpr int kPerLoad = 64 / kPieces;
+    static __device__ int key_place(int r) { return DP == 64 ? r >> 2 & 3 : DP == 128 ? r >> 1 & 7 : r & 15; }
+    static __device__ int value_place(int r) { return DP == 64 ? r >> 2 & 2 : DP == 128 ? (r & 2) | (r >> 1 & 4) : 2 * (r & 3) | (r & 8); }
+};
+
+constexpr int kBlock = 16;  // positions that share a scale in a cache of 8 bits
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // The larger of a lane's value and that of the same query in the wave's other half.
@@ -116,18 +146,22 @@ __device__ __forceinline__ void load_to_lds(const void* from, lds_char* to) {
                                      (__attribute__((address_space(3))) void*)to, 16, 0, 0);
 }
 
+__device__ __forceinline__ void load4_to_lds(const void* from, lds_char* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 4, 0, 0);
+}
+
 // Keys narrower than DP elements: the pieces past a row's last, which hold a
 // copy of it, become zeros in rows row0 .. row0 + kRows - 1 of the tile, that
 // the wave itself has loaded. (An infinite element of the copy would meet the
 // query's zeros there and make the score NaN. Lanes that sit those loads out
 // instead, over places cleared once: 32 trees of dim 96 over 2000-8000
 // positions 130 us.)
-template <int DP, int kRows>
-__device__ __forceinline__ void clear_past(int dim, lds_char* keys, int row0, int lane) {
-    typedef Rows<DP> R;
+template <typename R, int kRows>
+__device__ __forceinline__ void clear_past(int pieces, lds_char* keys, int row0, int lane) {
     asm volatile("" : "+v"(lane));  // its addresses are not worth registers in the loop over tiles
     const int r = row0 + lane % kRows;
-    for (int x = dim / 8 + lane / kRows; x < R::kPieces; x += 64 / kRows)
+    for (int x = pieces + lane / kRows; x < R::kPieces; x += 64 / kRows)
         *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(keys + r * R::kBytes + ((x ^ R::key_place(r)) << 4)) = u32x4{0};
 }
 
@@ -145,8 +179,21 @@ __device__ __forceinline__ void wait_loads() {
 }
 
 // One wave's softmax state and output of QT tiles of 32 queries.
-template <typename T, int DP, int QT>
+// k8: keys and values of 8 bits. A lane reads 16 elements of a key at a time,
+// which serve two steps of the first product (the queries are laid out
+// likewise); they enter it as they are, exact in either type, and a score is
+// multiplied by its key's scale. Values are multiplied by theirs as they become
+// bf16, which is exact whatever the queries' type: the second product is bf16's.
+template <typename T, int DP, int QT, bool k8 = false>
 struct State {
+    typedef std::conditional_t<k8, Bf16, T> P;  // of the second product
+    typedef std::conditional_t<k8, Rows8<DP>, Rows<DP>> R;
+    struct Scales {};
+    struct Scales8 {
+        const __attribute__((address_space(3))) float* at;  // a tile's keys' scales, then its values'
+        int blocks;
+    };
+    typedef std::conditional_t<k8, Scales8, Scales> TileScales;
     static constexpr int kSteps = DP / 16;   // steps of the first product
     static constexpr int kBlocks = DP / 32;  // blocks of output columns
     s16x8 q[QT][kSteps];
@@ -167,7 +214,7 @@ struct State {
     __device__ void load_query(int t, const uint16_t* row, int dim, int half) {
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-            const int x = 8 * (2 * k + half);
+            const int x = k8 ? 32 * (k / 2) + 16 * half + 8 * (k % 2) : 8 * (2 * k + half);
             const s16x8 v = *reinterpret_cast<const s16x8*>(row + (x < dim ? x : 0));
             q[t][k] = x < dim ? v : s16x8{0};
         }
@@ -178,20 +225,38 @@ struct State {
     // key 32 u + r; every key is seen otherwise.
     template <int NSUB, bool kMasked>
     __device__ __forceinline__ void step(const lds_char* keys, const lds_char* values, float c, int lane,
-                                         const uint32_t (&allow)[QT][NSUB]) {
-        typedef Rows<DP> R;
+                                         const uint32_t (&allow)[QT][NSUB], const TileScales& scales = {}) {
         const int half = lane >> 5;
         f32x16 s[QT][NSUB];
 #pragma unroll
         for (int u = 0; u < NSUB; ++u) {
             const int r = lane & 31;
             const lds_char* const row = keys + (32 * u + r) * R::kBytes;
+            if constexpr (k8) {
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                const s16x8 a = *reinterpret_cast<const __attribute__((address_space(3))) s16x8*>(
-                    row + (((2 * k + half) ^ R::key_place(r)) << 4));
+                for (int k = 0; k < kSteps; k += 2) {
+                    const u32x4 w = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
+                        row + (((k + half) ^ R::key_place(r)) << 4));
+                    const s16x8 a = T::from8(w[0], w[1], 1.0f), b = T::from8(w[2], w[3], 1.0f);
 #pragma unroll
-                for (int t = 0; t < QT; ++t) s[t][u] = T::mfma(a, q[t][k], k == 0 ? f32x16{0} : s[t][u]);
+                    for (int t = 0; t < QT; ++t) {
+                        s[t][u] = T::mfma(a, q[t][k], k == 0 ? f32x16{0} : s[t][u]);
+                        s[t][u] = T::mfma(b, q[t][k + 1], s[t][u]);
+                    }
+                }
+                const float low = scales.at[2 * u], high = scales.at[2 * u + 1];  // of keys 32 u + 0..15, 16..31
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[t][u][i] *= i < 8 ? low : high;
+            } else {
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const s16x8 a = *reinterpret_cast<const __attribute__((address_space(3))) s16x8*>(
+                        row + (((2 * k + half) ^ R::key_place(r)) << 4));
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) s[t][u] = T::mfma(a, q[t][k], k == 0 ? f32x16{0} : s[t][u]);
+                }
             }
         }
         s16x8 p[QT][NSUB][2];
@@ -219,9 +284,10 @@ struct State {
             }
             l[t] += sum;
         }
-        const int r = (lane & 15) >> 2;
+        // Of 8 bits: row j of {0..3, 8..11} by two lanes, 8 bytes each.
+        const int r = k8 ? (lane >> 1 & 3) + (lane & 8) : (lane & 15) >> 2;
         const lds_char* const first = values + (4 * half + r) * R::kBytes + (lane & 1) * 8;
-        const int piece = (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
+        const int piece = k8 ? lane >> 4 & 1 : (lane >> 4 & 1) * 2 + (lane >> 1 & 1);
         uint32_t odd = 0;
 #pragma unroll
         for (int u = 0; u < NSUB; ++u)
@@ -229,12 +295,12 @@ struct State {
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int d = 0; d < kBlocks; ++d) {
-                    s16x8 a = value(first, piece, r, u, k, d);
+                    s16x8 a = value(first, piece, r, u, k, d, scales);
                     if (kMasked) a = finite(a, odd);
 #pragma unroll
-                    for (int t = 0; t < QT; ++t) o[t][d] = T::mfma(a, p[t][u][k], o[t][d]);
+                    for (int t = 0; t < QT; ++t) o[t][d] = P::mfma(a, p[t][u][k], o[t][d]);
                 }
-        if (kMasked && __any(odd != 0)) add_infinite<NSUB>(first, piece, r, half, allow);
+        if (kMasked && __any(odd != 0)) add_infinite<NSUB>(first, piece, r, half, allow, scales);
     }
 
     // A lane's probabilities 2^(c s - mc), packed for the second product; returns their sum.
@@ -250,7 +316,7 @@ struct State {
                 for (int i = 0; i < 4; ++i) {
                     const float x = exp2_fast(fmaf(s[u][8 * k + 2 * i], c, -mc)), y = exp2_fast(fmaf(s[u][8 * k + 2 * i + 1], c, -mc));
                     sum += x + y;
-                    w[i] = T::pack(x, y);
+                    w[i] = P::pack(x, y);
                 }
                 p[u][k] = __builtin_bit_cast(s16x8, w);
             }
@@ -278,8 +344,13 @@ struct State {
     }
 
     // V^T of keys 32 u + 16 k + {0..3, 8..11} (+ 4 in the upper half) and block d of columns.
-    __device__ __forceinline__ s16x8 value(const lds_char* first, int piece, int r, int u, int k, int d) {
-        typedef Rows<DP> R;
+    __device__ __forceinline__ s16x8 value(const lds_char* first, int piece, int r, int u, int k, int d, const TileScales& scales) {
+        if constexpr (k8) {
+            typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+            lds_char* const at = const_cast<lds_char*>(first) + (32 * u + 16 * k) * R::kBytes + (((2 * d + piece) ^ R::value_place(r)) << 4);
+            const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)at);
+            return Bf16::from8(w[0], w[1], scales.at[scales.blocks + 2 * u + k]);
+        }
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
         lds_char* const at = const_cast<lds_char*>(first) + (32 * u + 16 * k) * R::kBytes + (((4 * d + piece) ^ R::value_place(r)) << 4);
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
@@ -294,7 +365,7 @@ struct State {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             // Adding the exponent's lowest bit to it carries into the sign's place where all its bits are set.
-            const uint32_t x = ((w[i] & T::kInf * 0x10001u) + (T::kInf & (0u - T::kInf)) * 0x10001u) & 0x80008000u;
+            const uint32_t x = ((w[i] & P::kInf * 0x10001u) + (P::kInf & (0u - P::kInf)) * 0x10001u) & 0x80008000u;
             odd |= x;
             w[i] &= ~((x - (x >> 15)) | x);
         }
@@ -306,7 +377,8 @@ struct State {
     // (Integer arithmetic on pairs throughout: as comparisons, this rare path
     // spilled scalar registers.)
     template <int NSUB>
-    __device__ __forceinline__ void add_infinite(const lds_char* first, int piece, int r, int half, const uint32_t (&allow)[QT][NSUB]) {
+    __device__ __forceinline__ void add_infinite(const lds_char* first, int piece, int r, int half, const uint32_t (&allow)[QT][NSUB],
+                                                 const TileScales& scales) {
         constexpr uint32_t kPair = 0x10001u, kTop = 0x8000u * kPair;
 #pragma nounroll
         for (int side = 0; side < 2; ++side) {
@@ -322,14 +394,14 @@ struct State {
                 for (int u = 0; u < NSUB; ++u)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        u32x4 v = __builtin_bit_cast(u32x4, value(first, piece, r, u, k, d));
+                        u32x4 v = __builtin_bit_cast(u32x4, value(first, piece, r, u, k, d, scales));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             // Top bits: at least inf; more (NaN); this sign. Then ones where they are set.
                             const uint32_t x = v[i] & ~kTop;
-                            const uint32_t big = x + (0x8000u - T::kInf) * kPair, nan = x + (0x7FFFu - T::kInf) * kPair;
+                            const uint32_t big = x + (0x8000u - P::kInf) * kPair, nan = x + (0x7FFFu - P::kInf) * kPair;
                             const uint32_t hit = big & (nan | ~(v[i] ^ sign)) & kTop;
-                            v[i] = ((hit - (hit >> 15)) | hit) & T::kOne * kPair;
+                            v[i] = ((hit - (hit >> 15)) | hit) & P::kOne * kPair;
                         }
 #pragma unroll
                         for (int t = 0; t < QT; ++t) {
@@ -338,10 +410,10 @@ struct State {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const int at = 8 * (i / 2) + 2 * (i % 2);
-                                w[i] = (static_cast<uint32_t>(__builtin_amdgcn_sbfe(bits, at, 1)) & T::kOne) |
-                                       (static_cast<uint32_t>(__builtin_amdgcn_sbfe(bits, at + 1, 1)) & T::kOne << 16);
+                                w[i] = (static_cast<uint32_t>(__builtin_amdgcn_sbfe(bits, at, 1)) & P::kOne) |
+                                       (static_cast<uint32_t>(__builtin_amdgcn_sbfe(bits, at + 1, 1)) & P::kOne << 16);
                             }
-                            n[t] = T::mfma(__builtin_bit_cast(s16x8, v), __builtin_bit_cast(s16x8, w), n[t]);
+                            n[t] = P::mfma(__builtin_bit_cast(s16x8, v), __builtin_bit_cast(s16x8, w), n[t]);
                         }
                     }
                 const float add = side ? -INFINITY : INFINITY;
@@ -609,7 +681,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void prompt_
     }
     auto arrived = [&](lds_char* to) __attribute__((always_inline)) {
         wait_loads<0>();
-        if (A.dim < DP) clear_past<DP, KT / NW>(A.dim, to, wave * (KT / NW), lane);
+        if (A.dim < DP) clear_past<R, KT / NW>(A.dim / 8, to, wave * (KT / NW), lane);
         __syncthreads();
     };
     arrived(shared);
@@ -809,7 +881,10 @@ int launch_prompt(PromptArgs& A, hipStream_t s) {
 // --------------------------------------------------------------------------
 
 struct TreeArgs {
-    const uint16_t *q, *k, *v;
+    const uint16_t* q;
+    const char *k, *v;
+    const float *k_scales, *v_scales;                // of a cache in 8 bits: [page][head][block], the last contiguous
+    int64_t scale_page, scale_head;                  // strides
     uint16_t* out;
     float* lse;
     const int32_t *table, *lengths, *seqs, *offsets;
@@ -892,18 +967,24 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeArgs& A, const Drafted& 
 // kPages: what of a tile never crosses a page, and so has one base address: 2
 // the tile, 1 the rows of one load (2 to 8), 0 a row. (With addresses made lane
 // by lane for pages of 16, 54 trees over 139-2238 positions took 155 us.)
-template <typename T, int DP, int QT, int NW, bool kShared, int kPages>
+// k8: a cache in 8 bits. Each wave brings its tile's scales along, a load of 4
+// bytes a lane into a place of its own.
+template <typename T, int DP, int QT, int NW, bool kShared, int kPages, bool k8>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_kernel(const TreeArgs A) {
-    typedef Rows<DP> R;
+    typedef State<T, DP, QT, k8> St;
+    typedef typename St::R R;
+    constexpr int kSize = k8 ? 1 : 2;  // bytes of an element
     constexpr int KT = kShared && DP <= 128 ? 64 : 32;
     constexpr int NSUB = KT / 32;
     constexpr int kTile = KT * R::kBytes;
     constexpr int kLoads = kTile / 1024 / (kShared ? NW : 1);  // loads a wave makes of K, and of V
+    constexpr int kBlocks = KT / kBlock;                       // of a tile
+    constexpr int kScales = k8 ? 2 * NW * 256 : 0;             // bytes of two tiles' scales for each wave
     constexpr int BM = 32 * QT * (kShared ? NW : 1);
     constexpr int kRow = DP + 4;  // floats of a row of sums in LDS: 16 bytes more than a multiple of all banks
     constexpr int kSums = kShared ? 0 : NW * 32 * QT * (kRow * 4 + 8);
     constexpr int kTiles = 4 * kTile * (kShared ? 1 : NW);
-    __shared__ __attribute__((aligned(1024))) char lds[kTiles > kSums ? kTiles : kSums];
+    __shared__ __attribute__((aligned(1024))) char lds[kTiles + kScales > kSums ? kTiles + kScales : kSums];
 
     const int group = A.heads / A.kv_heads;
     int id = blockIdx.x;
@@ -924,10 +1005,13 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
     const int half = lane >> 5;
     lds_char* const mine = (lds_char*)lds + (kShared ? 0 : wave * 4 * kTile);
 
-    const int pieces = A.dim / 8 - 1;
+    const int pieces = A.dim * kSize / 16 - 1;
     const int lane_row = lane / R::kPieces, lane_piece = lane % R::kPieces;
-    const uint32_t row_bytes = static_cast<uint32_t>(2 * A.slot_stride);
+    const uint32_t row_bytes = static_cast<uint32_t>(kSize * A.slot_stride);
     const int64_t head_at = kvh * A.kv_head_stride;
+    lds_char* const scales = (lds_char*)lds + kTiles + wave * 512;
+    const int lane_block = lane % kBlocks;
+    const float* const lane_scales = !k8 ? nullptr : (lane / kBlocks % 2 == 0 ? A.k_scales : A.v_scales) + kvh * A.scale_head;
     const int load0 = kShared ? wave * kLoads : 0;
     // A lane holds the number of page `first_page` + lane of the sequence, for
     // 64 pages at a time: a tile's page numbers then come out of a register,
@@ -940,7 +1024,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         held = static_cast<uint32_t>(id) < static_cast<uint32_t>(A.n_pages) ? id : 0;
     };
     // Keys past the last one repeat it; no row sees them.
-    auto issue = [&](int k0, lds_char* to) __attribute__((always_inline)) {
+    auto issue = [&](int k0, lds_char* to, lds_char* to_scales) __attribute__((always_inline)) {
         const int last = D.end - 1 - k0 < KT - 1 ? D.end - 1 - k0 : KT - 1;
         int32_t page, first, page_end, unused;
         page_of(A, k0, page, first);
@@ -948,7 +1032,15 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         if (page_end >= first_page + 64) hold(page);
         int64_t tile_at = 0;
         if (kPages == 2)
-            tile_at = 2 * (__builtin_amdgcn_readlane(held, page - first_page) * A.page_stride + first * A.slot_stride + head_at);
+            tile_at = kSize * (__builtin_amdgcn_readlane(held, page - first_page) * A.page_stride + first * A.slot_stride + head_at);
+        if constexpr (k8) {
+            // The scales of the blocks of keys k0 .., those past the last key's being its own.
+            const int at = kBlock * lane_block;
+            int32_t p, slot;
+            page_of(A, k0 + (at < last ? at : last), p, slot);
+            const int64_t id = __builtin_amdgcn_ds_bpermute(4 * (p - first_page), held);
+            load4_to_lds(lane_scales + (id * A.scale_page + slot / kBlock), to_scales);
+        }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int load = load0 + i;
@@ -961,17 +1053,17 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
                 const int row = r0 < last ? r0 : last;
                 int32_t p, slot;
                 page_of(A, k0 + row, p, slot);
-                at = 2 * (__builtin_amdgcn_readlane(held, p - first_page) * A.page_stride + slot * A.slot_stride + head_at);
+                at = kSize * (__builtin_amdgcn_readlane(held, p - first_page) * A.page_stride + slot * A.slot_stride + head_at);
                 from -= row;
             } else if (kPages == 0) {
                 int32_t p, slot;
                 page_of(A, k0 + from, p, slot);
                 const int64_t id = __builtin_amdgcn_ds_bpermute(4 * (p - first_page), held);
-                at = 2 * (id * A.page_stride + slot * A.slot_stride + head_at);
+                at = kSize * (id * A.page_stride + slot * A.slot_stride + head_at);
                 from = 0;
             }
-            load_to_lds(reinterpret_cast<const char*>(A.k) + at + (from * row_bytes + kp), to + load * 1024);
-            load_to_lds(reinterpret_cast<const char*>(A.v) + at + (from * row_bytes + vp), to + kTile + load * 1024);
+            load_to_lds(A.k + at + (from * row_bytes + kp), to + load * 1024);
+            load_to_lds(A.v + at + (from * row_bytes + vp), to + kTile + load * 1024);
         }
     };
 
@@ -984,9 +1076,9 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         int32_t page, unused;
         page_of(A, k0, page, unused);
         hold(page);
-        issue(k0, mine);
+        issue(k0, mine, scales);
     }
-    State<T, DP, QT> st;
+    St st;
     st.clear();
     int token[QT];
 #pragma unroll
@@ -998,24 +1090,26 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
     }
     auto arrived = [&](lds_char* to) __attribute__((always_inline)) {
         wait_loads<0>();
-        if (A.dim < DP) clear_past<DP, KT / NW>(A.dim, to, wave * (KT / NW), lane);
+        if (A.dim < DP) clear_past<R, KT / NW>(A.dim * kSize / 16, to, wave * (KT / NW), lane);
         __syncthreads();
     };
     if (kShared) arrived(mine);
     // Two tiles in turn.
-    auto tile = [&](auto masked, lds_char* __restrict__ next, lds_char* __restrict__ now) __attribute__((always_inline)) {
+    auto tile = [&](auto masked, lds_char* __restrict__ next, lds_char* __restrict__ now, lds_char* __restrict__ next_scales,
+                    lds_char* __restrict__ now_scales) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked)::value;
         const bool more = k0 + kStep < hi;
-        if (more) issue(k0 + kStep, next);
+        if (more) issue(k0 + kStep, next, next_scales);
         if (!kShared) {
-            // All but the 2 * kLoads loads just issued, the next tile's, have
-            // arrived. The tile's reads take their place from the wait, so
-            // that none can move before it.
+            // All but the loads just issued, the next tile's, have arrived. The
+            // tile's reads take their place from the wait, so that none can
+            // move before it.
             uint32_t zero = 0;
-            if (more) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(zero) : "n"(2 * kLoads) : "memory");
+            if (more) asm volatile("s_waitcnt vmcnt(%1)" : "+v"(zero) : "n"(2 * kLoads + (k8 ? 1 : 0)) : "memory");
             else asm volatile("s_waitcnt vmcnt(0)" : "+v"(zero) : : "memory");
             now += zero;
-            if (A.dim < DP) clear_past<DP, KT>(A.dim, now, 0, lane);
+            now_scales += zero;
+            if (A.dim < DP) clear_past<R, KT>(A.dim * kSize / 16, now, 0, lane);
         }
         if (!active) return;
         uint32_t allow[QT][NSUB] = {};
@@ -1025,14 +1119,17 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
 #pragma unroll
                 for (int u = 0; u < NSUB; ++u) allow[t][u] = seen_keys(A, D, D.row + token[t], token[t], k0 + 32 * u);
         }
-        st.template step<NSUB, kMasked>(now, now + kTile, A.c, lane, allow);
+        typename St::TileScales tile_scales;
+        if constexpr (k8) tile_scales = {reinterpret_cast<const __attribute__((address_space(3))) float*>(now_scales), kBlocks};
+        st.template step<NSUB, kMasked>(now, now + kTile, A.c, lane, allow, tile_scales);
     };
-    for (; k0 + KT <= D.context && k0 < hi; k0 += kStep, at ^= 2 * kTile) {
-        tile(std::integral_constant<bool, false>{}, mine + (at ^ 2 * kTile), mine + at);
+    uint32_t at_scales = 0;
+    for (; k0 + KT <= D.context && k0 < hi; k0 += kStep, at ^= 2 * kTile, at_scales ^= 256) {
+        tile(std::integral_constant<bool, false>{}, mine + (at ^ 2 * kTile), mine + at, scales + (at_scales ^ 256), scales + at_scales);
         if (kShared) arrived(mine + (at ^ 2 * kTile));
     }
-    for (; k0 < hi; k0 += kStep, at ^= 2 * kTile) {
-        tile(std::integral_constant<bool, true>{}, mine + (at ^ 2 * kTile), mine + at);
+    for (; k0 < hi; k0 += kStep, at ^= 2 * kTile, at_scales ^= 256) {
+        tile(std::integral_constant<bool, true>{}, mine + (at ^ 2 * kTile), mine + at, scales + (at_scales ^ 256), scales + at_scales);
         if (kShared) arrived(mine + (at ^ 2 * kTile));
     }
 
@@ -1269,17 +1366,17 @@ void plan_parts(TreeArgs& A, int64_t max_context) {
     A.n_splits = static_cast<int32_t>((longest + chunk - 1) / chunk);
 }
 
-template <typename T, int DP, int QT, int NW, bool kShared>
+template <typename T, int DP, int QT, int NW, bool kShared, bool k8>
 int launch_tree_as(TreeArgs& A, hipStream_t s) {
     const int64_t groups = static_cast<int64_t>(A.n_seqs) * A.kv_heads * A.row_blocks * A.n_splits;
     constexpr int KT = kShared && DP <= 128 ? 64 : 32;
     const dim3 grid(static_cast<uint32_t>(groups)), block(64 * NW);
     if (A.page_size % KT == 0)
-        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 2>), grid, block, 0, s, A);
-    else if (A.page_size % Rows<DP>::kPerLoad == 0)
-        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 1>), grid, block, 0, s, A);
-    else
-        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 0>), grid, block, 0, s, A);
+        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 2, k8>), grid, block, 0, s, A);
+    else if (k8 || A.page_size % Rows<DP>::kPerLoad == 0)  // pages of 8 bits: whole blocks of 16, the rows of a load or several loads'
+        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 1, k8>), grid, block, 0, s, A);
+    else if constexpr (!k8)
+        hipLaunchKernelGGL((tree_kernel<T, DP, QT, NW, kShared, 0, k8>), grid, block, 0, s, A);
     if (A.n_splits > kFewParts) {
         hipLaunchKernelGGL((tree_join_kernel<T, DP, true>), dim3(static_cast<uint32_t>(A.n_q) * A.heads), dim3(256), 0, s, A);
     } else if (A.n_splits > 1) {
@@ -1292,13 +1389,13 @@ int launch_tree_as(TreeArgs& A, hipStream_t s) {
     return AIMG_OK;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool k8>
 int launch_tree(TreeArgs& A, hipStream_t s) {
     const int per = tree_rows(A.dim, static_cast<int64_t>(A.max_drafts) * (A.heads / A.kv_heads));
-    if (per == 32) return launch_tree_as<T, DP, 1, DP == 256 ? 2 : 4, false>(A, s);
+    if (per == 32) return launch_tree_as<T, DP, 1, DP == 256 ? 2 : 4, false, k8>(A, s);
     if constexpr (DP < 256)
-        if (per == 64) return launch_tree_as<T, DP, 2, 4, false>(A, s);
-    return launch_tree_as<T, DP, 1, 4, true>(A, s);
+        if (per == 64) return launch_tree_as<T, DP, 2, 4, false, k8>(A, s);
+    return launch_tree_as<T, DP, 1, 4, true, k8>(A, s);
 }
 
 }  // namespace
@@ -1343,6 +1440,19 @@ int check_pages(const aimg_pages* p) {
         p->slot_stride % 8 != 0 || p->head_stride % 8 != 0 || p->page_stride < 0 || p->head_stride < 0 || p->slot_stride < 0 ||
         p->slot_stride > aimg::kMaxRowStride || p->table_stride < 0)
         return fail(AIMG_ERR_UNSUPPORTED, "pages: needs 16-byte aligned pointers and strides of whole 16 bytes, a position's at most 2^24 elements");
+    return AIMG_OK;
+}
+
+// What pages of 8-bit elements need besides.
+int check_page_scales(const aimg_pages* p, const aimg_page_scales* x) {
+    using aimg::fail;
+    if (p->dim % 16 != 0) return fail(AIMG_ERR_UNSUPPORTED, "pages: dim must be a multiple of 16 for 8 bits");
+    if (p->page_size % aimg::kBlock != 0) return fail(AIMG_ERR_UNSUPPORTED, "pages: page_size must be a multiple of 16 for 8 bits");
+    if (p->page_stride % 16 != 0 || p->slot_stride % 16 != 0 || p->head_stride % 16 != 0)
+        return fail(AIMG_ERR_UNSUPPORTED, "pages: needs strides of whole 16 bytes");
+    if (x->k == nullptr || x->v == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "scales: null pointer");
+    if ((reinterpret_cast<uintptr_t>(x->k) | reinterpret_cast<uintptr_t>(x->v)) % 4 != 0 || x->page_stride < 0 || x->head_stride < 0)
+        return fail(AIMG_ERR_UNSUPPORTED, "scales: needs 4-byte aligned pointers and strides that are not negative");
     return AIMG_OK;
 }
 
@@ -1468,14 +1578,17 @@ extern "C" int aimg_tree_workspace_nbytes(int64_t n_rows, int heads, int kv_head
     return AIMG_OK;
 }
 
-extern "C" int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_heads* out, const int32_t* seqs,
-                                   const int32_t* draft_offsets, int n_seqs, const int64_t* masks, int mask_words, int max_drafts,
-                                   int64_t max_context, int type, float scale, float* lse, void* workspace,
-                                   size_t workspace_nbytes, void* stream) {
+namespace {
+
+// Over a cache in 16 bits (scales null) or 8.
+int tree_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_page_scales* scales, const aimg_heads* out,
+                   const int32_t* seqs, const int32_t* draft_offsets, int n_seqs, const int64_t* masks, int mask_words, int max_drafts,
+                   int64_t max_context, int type, float scale, float* lse, void* workspace, size_t workspace_nbytes, void* stream) {
     using aimg::fail;
     int rc = check_heads(q, "q");
     if (rc == AIMG_OK) rc = check_heads(out, "out", INT64_MAX, true);
     if (rc == AIMG_OK) rc = check_pages(pages);
+    if (rc == AIMG_OK && scales != nullptr) rc = check_page_scales(pages, scales);
     if (rc == AIMG_OK) rc = check_scale(scale);
     if (rc != AIMG_OK) return rc;
     if (out->n_rows != q->n_rows || out->heads != q->heads || out->dim != q->dim)
@@ -1488,6 +1601,8 @@ extern "C" int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages,
     if (masks != nullptr && mask_words < 1) return fail(AIMG_ERR_INVALID_ARGUMENT, "mask_words must be >= 1");
     if (n_seqs == 0 || q->n_rows == 0) return AIMG_OK;
     if (seqs == nullptr || draft_offsets == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "null seqs or draft_offsets");
+    if (scales != nullptr)
+        a.k_scales = scales->k, a.v_scales = scales->v, a.scale_page = scales->page_stride, a.scale_head = scales->head_stride;
     const int64_t part_rows = q->n_rows * q->heads * a.n_splits;
     const int dp = aimg::padded_dim(q->dim);
     if (a.n_splits > 1 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
@@ -1496,8 +1611,8 @@ extern "C" int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages,
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + part_rows * dp);
     a.q = static_cast<const uint16_t*>(q->data);
-    a.k = static_cast<const uint16_t*>(pages->k);
-    a.v = static_cast<const uint16_t*>(pages->v);
+    a.k = static_cast<const char*>(pages->k);
+    a.v = static_cast<const char*>(pages->v);
     a.out = static_cast<uint16_t*>(out->data);
     a.lse = lse;
     a.table = pages->page_table, a.lengths = pages->lengths, a.seqs = seqs, a.offsets = draft_offsets;
@@ -1514,11 +1629,36 @@ extern "C" int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages,
     const hipStream_t s = static_cast<hipStream_t>(stream);
     return by_type(type, q->dim, [&](auto t, int dim) {
         typedef decltype(t) T;
-        if (dim <= 64) return aimg::launch_tree<T, 64>(a, s);
-        if (dim <= 128) return aimg::launch_tree<T, 128>(a, s);
-        return aimg::launch_tree<T, 256>(a, s);
+        if (scales != nullptr) {
+            if (dim <= 64) return aimg::launch_tree<T, 64, true>(a, s);
+            if (dim <= 128) return aimg::launch_tree<T, 128, true>(a, s);
+            return aimg::launch_tree<T, 256, true>(a, s);
+        }
+        if (dim <= 64) return aimg::launch_tree<T, 64, false>(a, s);
+        if (dim <= 128) return aimg::launch_tree<T, 128, false>(a, s);
+        return aimg::launch_tree<T, 256, false>(a, s);
     });
 }
+
+}  // namespace
+
+extern "C" int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_heads* out, const int32_t* seqs,
+                                   const int32_t* draft_offsets, int n_seqs, const int64_t* masks, int mask_words, int max_drafts,
+                                   int64_t max_context, int type, float scale, float* lse, void* workspace,
+                                   size_t workspace_nbytes, void* stream) {
+    return tree_attention(q, pages, nullptr, out, seqs, draft_offsets, n_seqs, masks, mask_words, max_drafts, max_context, type, scale,
+                          lse, workspace, workspace_nbytes, stream);
+}
+
+extern "C" int aimg_tree8_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_page_scales* scales, const aimg_heads* out,
+                                    const int32_t* seqs, const int32_t* draft_offsets, int n_seqs, const int64_t* masks, int mask_words,
+                                    int max_drafts, int64_t max_context, int type, float scale, float* lse, void* workspace,
+                                    size_t workspace_nbytes, void* stream) {
+    if (scales == nullptr) return aimg::fail(AIMG_ERR_INVALID_ARGUMENT, "scales is null");
+    return tree_attention(q, pages, scales, out, seqs, draft_offsets, n_seqs, masks, mask_words, max_drafts, max_context, type, scale, lse,
+                          workspace, workspace_nbytes, stream);
+}
+
 
 extern "C" int aimg_tree_masks(const int32_t* parents, const int32_t* draft_offsets, int n_seqs, int64_t n_rows, int mask_words,
                                int64_t* masks, void* stream) {

@@ -1,4 +1,5 @@
-// Pages of a key/value cache: appending rows, forking, reserving, releasing,
+// Pages of a key/value cache: appending rows (turned by their positions on the
+// way, where asked), reading them back, forking, reserving, releasing,
 // committing accepted drafts and compacting (gfx950).
 //
 // The page table, lengths, pages held and reference counts live on the GPU and
@@ -13,8 +14,17 @@
 // held, counts), for larger ones about 1 us more a round (compacting: 3). What
 // moves rows is a grid of its own, bound by HBM: 16 bytes a lane, whole rows
 // of a head at a time.
+//
+// A cache in 8 bits holds e4m3 values (4 bits of exponent, 3 of mantissa, no
+// infinity, up to 448) and a scale for each 16 positions of a page and head,
+// keys and values apart: element x stands for code * scale. A scale is the
+// smallest power of two, 2^-100 to 2^119, that brings the block's largest
+// element to at most 448, so the product is exact in bf16, and a block that
+// takes further rows is formed anew from what it stands for: where its scale
+// rises, only elements that fall below 2^-6 scales are rounded again.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -38,7 +48,19 @@ struct Cache {
     int32_t *table, *lengths, *held, *refs, *status;
     int64_t plane_bytes, page_bytes, head_bytes;
     int32_t planes, n_pages, kv_heads, page_size, row_bytes, max_seqs, max_pages, table_stride;
+    float* scales;        // of a cache in 8 bits: [planes][n_pages][kv_heads][blocks]; null in 16
+    int32_t blocks;       // of a page, kBlock positions each
 };
+
+constexpr int kBlock = 16;
+constexpr int kMaxDim8 = 256;
+constexpr float kMost8 = 448.0f;                 // 0.875 * 2^9
+constexpr int kLowExp = -100, kHighExp = 119;    // of scales
+
+// Where the scales of a page's head begin (of page 0, plane 0: C.scales).
+__device__ __forceinline__ int64_t scales_at(const Cache& C, int32_t plane, int32_t page, int32_t head) {
+    return ((static_cast<int64_t>(plane) * C.n_pages + page) * C.kv_heads + head) * C.blocks;
+}
 
 __device__ __forceinline__ void tell(const Cache& C, int32_t what) { atomicOr(C.status, what); }
 
@@ -185,6 +207,478 @@ __global__ __launch_bounds__(256) void advance_kernel(const Cache C, const int32
     if (more < 0) return tell(C, kBadIndex);
     if (to > static_cast<int64_t>(held_of(C, slot)) * C.page_size) return tell(C, kRowFull);
     C.lengths[slot] = static_cast<int32_t>(to);
+}
+
+// --------------------------------------------------------------------------
+// Rows turned by their positions on the way, and rows into blocks of 8 bits.
+// --------------------------------------------------------------------------
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+
+struct AsBf16 {
+    static __device__ f32x2 unpack(uint32_t w) { return f32x2{__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)}; }
+    static __device__ uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2)); }
+    // Two codes times a power of two, exact.
+    template <bool kUpper>
+    static __device__ uint32_t from8(uint32_t codes, float scale) {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, kUpper));
+    }
+};
+
+struct AsFp16 {
+    static __device__ f32x2 unpack(uint32_t w) { return __builtin_convertvector(__builtin_bit_cast(f16x2, w), f32x2); }
+    static __device__ uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2)); }
+    template <bool kUpper>
+    static __device__ uint32_t from8(uint32_t codes, float scale) {
+        const f32x2 x = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes), kUpper);
+        return pack(x[0] * scale, x[1] * scale);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x2 p = T::unpack(u[i]);
+        x[2 * i] = p[0], x[2 * i + 1] = p[1];
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return make_uint4(T::pack(x[0], x[1]), T::pack(x[2], x[3]), T::pack(x[4], x[5]), T::pack(x[6], x[7]));
+}
+
+__device__ __forceinline__ void read8(const float* p, float (&x)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+
+// (a, b) by the angle of (c, s): three roundings each, the products' and the
+// sum's, so that a row's values do not depend on what the compiler fuses where.
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+#pragma clang fp contract(off)
+    const float x = a * c - b * s, y = b * c + a * s;
+    a = x, b = y;
+}
+
+struct TurnArgs {
+    Cache c;
+    const uint16_t *q, *k, *v;
+    uint16_t* q_out;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;  // elements
+    const float *cos, *sin;   // [n_positions][half]
+    const int32_t *positions, *seqs, *offsets;
+    int32_t n_seqs, n_rows, heads, dim, half, n_positions;
+    int32_t plane;            // of the layer's keys; its values are in the next
+    uint32_t n_items;         // (block, head, keys or values) of a cache in 8 bits, a wave each
+    bool paired;
+};
+
+// How a row's pairs lie in its 16-byte pieces.
+constexpr int kHalves = 0;  // element i goes with i + half, 8 elements with 8 elements: half % 8 == 0
+constexpr int kPairs = 1;   // 2 i goes with 2 i + 1, in one piece: half % 4 == 0
+constexpr int kAny = 2;     // either, for every half: element by element
+
+// Rows of a call in place of offsets that may be any numbers.
+__device__ __forceinline__ int32_t row_bound(const int32_t* offsets, int b, int32_t n_rows) {
+    const int32_t x = offsets[b];
+    return x < 0 ? 0 : x > n_rows ? n_rows : x;
+}
+
+// The last sequence whose place is at most `at`.
+template <typename Place>
+__device__ __forceinline__ int last_before(int n_seqs, int64_t at, Place place) {
+    int lo = 0, hi = n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (place(mid) <= at) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Eight elements of a turned row from element x on, one by one.
+template <typename T>
+__device__ __forceinline__ void turn_any(const TurnArgs& A, const uint16_t* row, int x, int32_t position, float (&out)[8]) {
+    auto at = [&](int i) { return T::unpack(row[i])[0]; };
+    const int64_t angle = static_cast<int64_t>(position) * A.half;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e) {
+        const int i = x + e;
+        float a = at(i);
+        if (i < 2 * A.half) {
+            const bool second = A.paired ? i & 1 : i >= A.half;
+            const int j = A.paired ? i / 2 : second ? i - A.half : i;
+            float b = at(A.paired ? i ^ 1 : second ? i - A.half : i + A.half);
+            const float c = A.cos[angle + j], s = A.sin[angle + j];
+            if (second) {
+                turn(b, a, c, s);
+            } else {
+                turn(a, b, c, s);
+            }
+        }
+        out[e] = a;
+    }
+}
+
+// Eight elements of a turned row from element x on, a multiple of 8.
+template <typename T, int kMode>
+__device__ __forceinline__ void turned8(const TurnArgs& A, const uint16_t* row, int x, int32_t position, float (&out)[8]) {
+    if (kMode == kAny) return turn_any<T>(A, row, x, position, out);
+    unpack8<T>(get16(reinterpret_cast<const char*>(row + x)), out);
+    if (x >= 2 * A.half) return;
+    const int64_t angle = static_cast<int64_t>(position) * A.half;
+    float c[8], s[8];
+    if (kMode == kHalves) {
+        const bool second = x >= A.half;
+        const int first = second ? x - A.half : x;
+        float other[8];
+        unpack8<T>(get16(reinterpret_cast<const char*>(row + (second ? first : x + A.half))), other);
+        read8(A.cos + angle + first, c);
+        read8(A.sin + angle + first, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (second) {
+                turn(other[e], out[e], c[e], s[e]);
+            } else {
+                turn(out[e], other[e], c[e], s[e]);
+            }
+        }
+    } else {
+        const float4 c4 = *reinterpret_cast<const float4*>(A.cos + angle + x / 2), s4 = *reinterpret_cast<const float4*>(A.sin + angle + x / 2);
+        turn(out[0], out[1], c4.x, s4.x);
+        turn(out[2], out[3], c4.y, s4.y);
+        turn(out[4], out[5], c4.z, s4.z);
+        turn(out[6], out[7], c4.w, s4.w);
+    }
+}
+
+// One row's queries, and its keys and values where the cache is in 16 bits, by
+// a workgroup: a thread owns a pair of pieces (or a piece) of a head, keeps
+// their angles and steps over the heads. It reads its pieces before it writes
+// them, so the result may be q's own memory (kAny: the workgroup does).
+template <typename T, int kMode>
+__device__ __forceinline__ void turn_row(const TurnArgs& A, int32_t row) {
+    const Cache& C = A.c;
+    const int b = last_before(A.n_seqs, row, [&](int i) { return A.offsets[i]; });
+    const int32_t first = A.offsets[b];
+    if (row < first || row >= A.offsets[b + 1]) return;  // a row of no sequence
+    const int32_t slot = A.seqs[b];
+    auto wrong = [&](int32_t what) {
+        if (threadIdx.x == 0) tell(C, what);
+    };
+    if (!known(C, slot)) return wrong(kBadIndex);
+    const int64_t at = static_cast<int64_t>(length_of(C, slot)) + row - first;
+    const int64_t position = A.positions != nullptr ? A.positions[row] : at;
+    if (A.half > 0 && (position < 0 || position >= A.n_positions)) return wrong(kBadIndex);
+    char* to = nullptr;  // the row's place in head 0 of the layer's keys
+    if (C.scales == nullptr) {
+        const int64_t page = at / C.page_size;
+        if (page >= held_of(C, slot)) {
+            wrong(kRowFull);
+        } else {
+            const int32_t id = C.table[static_cast<int64_t>(slot) * C.table_stride + page];
+            if (id < 0 || id >= C.n_pages) wrong(kBadIndex);
+            else to = C.pool + A.plane * C.plane_bytes + id * C.page_bytes + at % C.page_size * C.row_bytes;
+        }
+    }
+    const int pairs = kMode == kHalves ? A.half / 8 : 0;
+    const int units = A.dim / 8 - pairs, step = 256 / units;
+    const int unit = static_cast<int>(threadIdx.x) % units, lane_head = static_cast<int>(threadIdx.x) / units;
+    const bool two = unit < pairs;
+    const int x = two ? 8 * unit : 8 * (unit + pairs), y = x + A.half;
+    const int all = A.heads + (to != nullptr ? 2 * C.kv_heads : 0);
+    auto from = [&](int h) {
+        return h < A.heads ? A.q + row * A.q_row + h * A.q_head
+               : h < A.heads + C.kv_heads ? A.k + row * A.k_row + (h - A.heads) * A.k_head : A.v + row * A.v_row + (h - A.heads - C.kv_heads) * A.v_head;
+    };
+    auto into = [&](int h) -> char* {
+        if (h < A.heads) return reinterpret_cast<char*>(A.q_out + row * A.out_row + h * A.out_head);
+        const bool value = h >= A.heads + C.kv_heads;
+        return to + (value ? C.plane_bytes : 0) + (h - A.heads - (value ? C.kv_heads : 0)) * C.head_bytes;
+    };
+    if constexpr (kMode == kAny) {
+        for (int h0 = 0; h0 < all; h0 += step) {
+            const int h = h0 + lane_head;
+            const bool mine = lane_head < step && h < all;
+            float out[8];
+            if (mine) {
+                if (h < A.heads + C.kv_heads) turn_any<T>(A, from(h), x, static_cast<int32_t>(position), out);
+                else unpack8<T>(get16(reinterpret_cast<const char*>(from(h) + x)), out);
+            }
+            __syncthreads();
+            if (mine) put16(into(h) + 2 * x, pack8<T>(out));
+        }
+    } else {
+        if (lane_head >= step) return;
+        const bool turns = kMode == kHalves ? two : x < 2 * A.half;
+        float c[8] = {}, s[8] = {};
+        if (turns) {
+            const int64_t angle = position * A.half + (kMode == kHalves ? x : x / 2);
+            if (kMode == kHalves) {
+                read8(A.cos + angle, c);
+                read8(A.sin + angle, s);
+            } else {
+                const float4 c4 = *reinterpret_cast<const float4*>(A.cos + angle), s4 = *reinterpret_cast<const float4*>(A.sin + angle);
+                c[0] = c4.x, c[1] = c4.y, c[2] = c4.z, c[3] = c4.w, s[0] = s4.x, s[1] = s4.y, s[2] = s4.z, s[3] = s4.w;
+            }
+        }
+        constexpr int kAhead = 2;  // heads whose pieces are on their way together
+        for (int h0 = lane_head; h0 < all; h0 += kAhead * step) {
+            uint4 a[kAhead], o[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const uint16_t* const p = from(h0 + i * step < all ? h0 + i * step : h0);
+                a[i] = get16(reinterpret_cast<const char*>(p + x));
+                if (kMode == kHalves && two) o[i] = get16(reinterpret_cast<const char*>(p + y));
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int h = h0 + i * step;
+                if (h >= all) continue;
+                if (turns && h < A.heads + C.kv_heads) {
+                    float u[8], w[8];
+                    unpack8<T>(a[i], u);
+                    if (kMode == kHalves) {
+                        unpack8<T>(o[i], w);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) turn(u[e], w[e], c[e], s[e]);
+                        o[i] = pack8<T>(w);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) turn(u[2 * e], u[2 * e + 1], c[e], s[e]);
+                    }
+                    a[i] = pack8<T>(u);
+                }
+                char* const d = into(h);
+                put16(d + 2 * x, a[i]);
+                if (kMode == kHalves && two) put16(d + 2 * y, o[i]);
+            }
+        }
+    }
+}
+
+// A block's pieces as a wave holds them: NP pieces of 8 elements a lane, piece
+// j * 64 + lane of the 16 rows' 2 * dim.
+template <int NP>
+struct Formed {
+    float x[NP][8];
+
+    // The exponent of the scale for these elements, by the whole wave.
+    __device__ __forceinline__ int exponent() const {
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float a = fabsf(x[j][e]);
+                top = a < INFINITY && a > top ? a : top;  // infinities and NaNs have no say
+            }
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+        const uint32_t bits = __float_as_uint(top);
+        // top = m 2^e with m in [1, 2): 448 = 1.75 * 2^8. (What is not normal lies below the lowest scale.)
+        const int e = static_cast<int>(bits >> 23) - 127 - ((bits & 0x7FFFFFu) <= 0x600000u ? 8 : 7);
+        return e < kLowExp ? kLowExp : e > kHighExp ? kHighExp : e;
+    }
+
+    // Piece j's codes for 1 / scale. Past 448 (at the highest scale alone) they stay there; infinities become NaN.
+    __device__ __forceinline__ uint2 codes(int j, float by) const {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = x[j][e] * by;
+            y[e] = fabsf(x[j][e]) < INFINITY ? fminf(fmaxf(v, -kMost8), kMost8) : NAN;
+        }
+        uint2 w;
+        w.x = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false), true);
+        w.y = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], 0, false), true);
+        return w;
+    }
+
+    __device__ __forceinline__ void hold(int j, uint2 w, float scale) {
+        const f32x2 p[4] = {__builtin_amdgcn_cvt_pk_f32_fp8(w.x, false), __builtin_amdgcn_cvt_pk_f32_fp8(w.x, true),
+                            __builtin_amdgcn_cvt_pk_f32_fp8(w.y, false), __builtin_amdgcn_cvt_pk_f32_fp8(w.y, true)};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[j][e] = p[e / 2][e % 2] * scale;
+    }
+
+    __device__ __forceinline__ void nothing(int j) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[j][e] = 0.0f;
+    }
+};
+
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }  // e in -126..127
+
+// One block of 16 positions of a head's keys or values that takes rows of the
+// call, by a wave: the rows it holds already (below the length) and the new
+// ones, their largest element, their codes. Sequence b's blocks are counted
+// from slot first_row / 16 + 2 b on: n rows lie in at most n / 16 + 2 blocks, so
+// no sums over the sequences are needed; the slots that are left over return.
+template <typename T, int kMode, int NP>
+__device__ __forceinline__ void form_block(const TurnArgs& A, uint32_t item, int lane) {
+    const Cache& C = A.c;
+    const int32_t which = item & 1, head = static_cast<int32_t>((item >> 1) % C.kv_heads), unit = static_cast<int32_t>((item >> 1) / C.kv_heads);
+    const int b = last_before(A.n_seqs, unit, [&](int i) { return row_bound(A.offsets, i, A.n_rows) / kBlock + 2 * static_cast<int64_t>(i); });
+    const int32_t first = row_bound(A.offsets, b, A.n_rows), n = row_bound(A.offsets, b + 1, A.n_rows) - first;
+    const int32_t i = unit - (first / kBlock + 2 * b);
+    if (n <= 0 || i < 0) return;
+    const int32_t slot = A.seqs[b];
+    auto wrong = [&](int32_t what) {
+        if (lane == 0) tell(C, what);
+    };
+    if (!known(C, slot)) return wrong(kBadIndex);
+    const int64_t length = length_of(C, slot), end = length + n, at = (length / kBlock + i) * kBlock;
+    if (at >= end) return;
+    const int64_t page = at / C.page_size;
+    if (page >= held_of(C, slot)) return wrong(kRowFull);
+    const int32_t id = C.table[static_cast<int64_t>(slot) * C.table_stride + page];
+    if (id < 0 || id >= C.n_pages) return wrong(kBadIndex);
+    const int32_t row0 = static_cast<int32_t>(at % C.page_size);
+    char* const codes = C.pool + (A.plane + which) * C.plane_bytes + id * C.page_bytes + head * C.head_bytes + row0 * C.row_bytes;
+    float* const scale = C.scales + scales_at(C, A.plane + which, id, head) + row0 / kBlock;
+    const int old = length > at ? static_cast<int>(length - at) : 0, rows = end - at < kBlock ? static_cast<int>(end - at) : kBlock;
+    const float held = old > 0 ? *scale : 0.0f;
+    const uint16_t* const from = which == 0 ? A.k + head * A.k_head : A.v + head * A.v_head;
+    const int64_t from_row = which == 0 ? A.k_row : A.v_row;
+    const int pieces = A.dim / 8;
+    Formed<NP> f;
+    uint32_t keep = 0;  // pieces that are written
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int r = (j * 64 + lane) / pieces, x = (j * 64 + lane) % pieces * 8;
+        if (r < old) {
+            f.hold(j, *reinterpret_cast<const uint2*>(codes + r * C.row_bytes + x), held);
+            keep |= 1u << j;
+        } else if (r < rows) {
+            const int32_t row = first + static_cast<int32_t>(at - length) + r;
+            const uint16_t* const p = from + row * from_row;
+            const int64_t position = A.half == 0 ? 0 : A.positions != nullptr ? A.positions[row] : at + r;
+            if (A.half > 0 && (position < 0 || position >= A.n_positions)) {
+                f.nothing(j);
+                bad = true;
+            } else {
+                if (which != 0 || A.half == 0) unpack8<T>(get16(reinterpret_cast<const char*>(p + x)), f.x[j]);
+                else turned8<T, kMode>(A, p, x, static_cast<int32_t>(position), f.x[j]);
+                keep |= 1u << j;
+            }
+        } else {
+            f.nothing(j);
+        }
+    }
+    if (bad) tell(C, kBadIndex);
+    const int e = f.exponent();
+    const float now = power_of_two(e), by = power_of_two(-e);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int r = (j * 64 + lane) / pieces, x = (j * 64 + lane) % pieces * 8;
+        if ((keep >> j & 1) == 0 || (r < old && now == held)) continue;
+        *reinterpret_cast<uint2*>(codes + r * C.row_bytes + x) = f.codes(j, by);
+    }
+    if (lane == 0) *scale = now;
+}
+
+// Blocks first, four a workgroup, then a workgroup a row. NP: 0 for a cache in 16 bits.
+template <typename T, int kMode, int NP>
+__global__ __launch_bounds__(256) void turn_kernel(const TurnArgs A) {
+    uint32_t group = blockIdx.x;
+    if constexpr (NP > 0) {
+        const uint32_t groups = (A.n_items + 3) / 4;
+        if (group < groups) {
+            const uint32_t item = __builtin_amdgcn_readfirstlane(group * 4 + (threadIdx.x >> 6));
+            if (item < A.n_items) form_block<T, kMode, NP>(A, item, threadIdx.x & 63);
+            return;
+        }
+        group -= groups;
+    }
+    turn_row<T, kMode>(A, static_cast<int32_t>(group));
+}
+
+// --------------------------------------------------------------------------
+// Rows out of pages.
+// --------------------------------------------------------------------------
+
+struct ReadArgs {
+    Cache c;
+    uint16_t *k, *v;
+    int64_t k_row, k_head, v_row, v_head;  // elements
+    const int32_t *seqs, *offsets, *starts;
+    int32_t n_seqs, n_rows, plane;
+};
+
+constexpr int kReadRows = 8;  // of a workgroup
+
+// Eight threads find where a workgroup's rows lie, then all move pieces of 8
+// elements: a thread keeps its place in a head and takes it from row after row.
+template <typename T, bool k8>
+__global__ __launch_bounds__(256) void read_kernel(const ReadArgs A) {
+    const Cache& C = A.c;
+    __shared__ int64_t place[kReadRows];   // bytes from a head's start in the pool; -1: not read
+    __shared__ int64_t scale[kReadRows];   // its block's scale of head 0, from the plane's first
+    const int32_t row0 = static_cast<int32_t>(blockIdx.x) * kReadRows;  // fewer than 2^31 rows
+    if (threadIdx.x < kReadRows) {
+        const int64_t row = static_cast<int64_t>(row0) + threadIdx.x;
+        int64_t found = -1, its_scale = 0;
+        if (row < A.n_rows) {
+            const int b = last_before(A.n_seqs, row, [&](int i) { return A.offsets[i]; });
+            const int64_t i = row - A.offsets[b];
+            if (i >= 0 && row < A.offsets[b + 1]) {
+                const int32_t slot = A.seqs[b];
+                const int64_t at = (A.starts != nullptr ? A.starts[b] : 0) + i;
+                if (!known(C, slot) || at < 0) {
+                    tell(C, kBadIndex);
+                } else if (at / C.page_size >= held_of(C, slot)) {
+                    tell(C, kRowFull);
+                } else {
+                    const int32_t id = C.table[static_cast<int64_t>(slot) * C.table_stride + at / C.page_size];
+                    if (id < 0 || id >= C.n_pages) {
+                        tell(C, kBadIndex);
+                    } else {
+                        found = id * C.page_bytes + at % C.page_size * C.row_bytes;
+                        if (k8) its_scale = scales_at(C, 0, id, 0) + at % C.page_size / kBlock;
+                    }
+                }
+            }
+        }
+        place[threadIdx.x] = found, scale[threadIdx.x] = its_scale;
+    }
+    __syncthreads();
+    constexpr int kBytes = k8 ? 8 : 16;  // of a piece in the cache
+    const int pieces = C.row_bytes / kBytes, all = 2 * C.kv_heads * pieces;
+    for (int t = threadIdx.x; t < all; t += 256) {
+        const int piece = t % pieces, h = t / pieces, which = h >= C.kv_heads ? 1 : 0, head = h - which * C.kv_heads;
+        const char* const from = C.pool + (A.plane + which) * C.plane_bytes + head * C.head_bytes + piece * kBytes;
+        const float* const scales = k8 ? C.scales + scales_at(C, A.plane + which, 0, head) : nullptr;
+        uint16_t* const to = which == 0 ? A.k + head * A.k_head + piece * 8 : A.v + head * A.v_head + piece * 8;
+        const int64_t to_row = which == 0 ? A.k_row : A.v_row;
+        uint4 v[kReadRows];
+        float f[kReadRows];
+#pragma unroll
+        for (int r = 0; r < kReadRows; ++r) {
+            if (place[r] < 0) continue;
+            if constexpr (k8) {
+                const uint2 w = *reinterpret_cast<const uint2*>(from + place[r]);
+                v[r].x = w.x, v[r].y = w.y;
+                f[r] = scales[scale[r]];
+            } else {
+                v[r] = get16(from + place[r]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kReadRows; ++r) {
+            if (place[r] < 0) continue;
+            uint4 w = v[r];
+            if constexpr (k8)
+                w = make_uint4(T::template from8<false>(v[r].x, f[r]), T::template from8<true>(v[r].x, f[r]),
+                               T::template from8<false>(v[r].y, f[r]), T::template from8<true>(v[r].y, f[r]));
+            put16(reinterpret_cast<char*>(to + (row0 + r) * to_row), w);
+        }
+    }
 }
 
 // --------------------------------------------------------------------------
@@ -377,6 +871,23 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(const ForkArgs A) {
     }
 }
 
+// The scales of the tails' blocks: a thread a scale and step. (A launch of its
+// own, for caches in 8 bits alone, before the rows change.)
+__global__ __launch_bounds__(256) void fork_scales_kernel(const ForkArgs A) {
+    const Cache& C = A.c;
+    const int i = blockIdx.x;
+    const int32_t page = A.fresh[i], len = A.lens[i], full = len / C.page_size, tail = len % C.page_size;
+    if (page < 0 || tail == 0) return;
+    const int32_t last = C.table[static_cast<int64_t>(A.src[i]) * C.table_stride + full];
+    if (last < 0 || last >= C.n_pages) return;
+    const uint32_t used = (tail + kBlock - 1) / kBlock, all = static_cast<uint32_t>(C.planes) * C.kv_heads * used;
+    for (uint32_t x = blockIdx.y * 256u + threadIdx.x; x < all; x += gridDim.y * 256u) {
+        const int32_t ph = static_cast<int32_t>(x / used), block = static_cast<int32_t>(x % used);
+        const int32_t plane = ph / C.kv_heads, head = ph % C.kv_heads;
+        C.scales[scales_at(C, plane, page, head) + block] = C.scales[scales_at(C, plane, last, head) + block];
+    }
+}
+
 __global__ __launch_bounds__(256) void fork_rows_kernel(const ForkArgs A) {
     const Cache& C = A.c;
     const int i = blockIdx.x;
@@ -466,6 +977,81 @@ __global__ __launch_bounds__(256) void commit_kernel(const CommitArgs A) {
             for (int x = 0; x < 4; ++x)
                 if (i + x < here && to[i + x] >= 0 && from[i + x] >= 0) put16(mine + to[i + x], v[x]);
         }
+    }
+}
+
+// The same for a cache in 8 bits, a wave a (plane, head): it takes the blocks
+// of the path in turn. A block into which a row moves is formed anew: its rows
+// below the length and those of the path, from wherever they lie, are held in
+// registers before any is written. Sources lie at or behind their own places,
+// so what one block writes no later block reads. A block with a place that is
+// no page's stays as it is.
+template <int NP>
+__global__ __launch_bounds__(256) void commit8_kernel(const CommitArgs A) {
+    const Cache& C = A.c;
+    const int b = blockIdx.y, lane = threadIdx.x & 63;
+    const int32_t slot = A.seqs[b];
+    if (!known(C, slot)) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) tell(C, kBadIndex);
+        return;
+    }
+    const int32_t len = length_of(C, slot), n = accepted_of(A, b, slot);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        const int32_t asked = A.counts[b];
+        if (n != asked) tell(C, asked < 0 || asked > A.most ? kBadIndex : kRowFull);
+        if (A.new_lengths != C.lengths) A.new_lengths[slot] = len + n;
+    }
+    const int32_t ph = static_cast<int32_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (ph >= C.planes * C.kv_heads) return;
+    const int32_t plane = ph / C.kv_heads, head = ph % C.kv_heads;
+    char* const mine = C.pool + plane * C.plane_bytes + head * C.head_bytes;
+    float* const scales = C.scales + scales_at(C, plane, 0, head);
+    const int64_t page_scales = static_cast<int64_t>(C.kv_heads) * C.blocks;
+    const int32_t* const row = C.table + static_cast<int64_t>(slot) * C.table_stride;
+    const int64_t most = static_cast<int64_t>(held_of(C, slot)) * C.page_size;
+    const int pieces = C.row_bytes / 8;
+    // Where a position lies: its row's bytes and its block's scale; false where it is no page's.
+    auto place = [&](int64_t at, int64_t& bytes, int64_t& scale) {
+        bytes = 0, scale = 0;
+        if (at < 0 || at >= most) return false;
+        const int32_t id = row[at / C.page_size], r = static_cast<int32_t>(at % C.page_size);
+        if (id < 0 || id >= C.n_pages) {
+            tell(C, kBadIndex);
+            return false;
+        }
+        bytes = id * C.page_bytes + r * C.row_bytes, scale = id * page_scales + r / kBlock;
+        return true;
+    };
+    for (int64_t at = len / kBlock * kBlock; at < static_cast<int64_t>(len) + n; at += kBlock) {
+        // Lane r < 16: row r of the block.
+        const int64_t i = at + (lane & 15) - len;  // index in the path; negative: held already
+        const int32_t x = i >= 0 && i < n ? A.accepted[static_cast<int64_t>(b) * A.most + i] : static_cast<int32_t>(i);
+        const bool used = i < n;
+        if (__ballot(used && x != i) == 0) continue;
+        int64_t from, from_scale, to, to_scale;
+        from = from_scale = 0;
+        const bool there = used && place(static_cast<int64_t>(len) + x, from, from_scale);
+        if (!place(at, to, to_scale) || __ballot(used && !there) != 0) continue;
+        const float its = there ? scales[from_scale] : 0.0f;
+        Formed<NP> f;
+        int rows = static_cast<int>(static_cast<int64_t>(len) + n - at);
+        rows = rows < kBlock ? rows : kBlock;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int r = (j * 64 + lane) / pieces, p = (j * 64 + lane) % pieces * 8;
+            const int64_t here = __shfl(from, r & 15);
+            const float scale = __shfl(its, r & 15);
+            if (r < rows) f.hold(j, *reinterpret_cast<const uint2*>(mine + here + p), scale);
+            else f.nothing(j);
+        }
+        const int e = f.exponent();
+        const float by = power_of_two(-e);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int r = (j * 64 + lane) / pieces, p = (j * 64 + lane) % pieces * 8;
+            if (r < rows) *reinterpret_cast<uint2*>(mine + to + r * C.row_bytes + p) = f.codes(j, by);
+        }
+        if (lane == 0) scales[to_scale] = power_of_two(e);
     }
 }
 
@@ -565,6 +1151,11 @@ __global__ __launch_bounds__(256) void compact_move_kernel(const CompactArgs A) 
             const int64_t x = static_cast<int64_t>(slice) * kSlice + j * 4096 + threadIdx.x * 16;
             if (x < C.page_bytes) put16(to + x, v[j]);
         }
+        if (C.scales != nullptr && slice == 0) {
+            const float* const f = C.scales + scales_at(C, plane, A.high[move], 0);
+            float* const t = C.scales + scales_at(C, plane, A.low[move], 0);
+            for (int32_t x = threadIdx.x; x < C.kv_heads * C.blocks; x += 256) t[x] = f[x];
+        }
     }
 }
 
@@ -594,7 +1185,20 @@ int take(const aimg_cache* c, Cache& C, bool pool) {
     if (reinterpret_cast<uintptr_t>(c->pool) % 16 != 0) return fail(AIMG_ERR_UNSUPPORTED, "cache: the pool must be 16-byte aligned");
     C = Cache{static_cast<char*>(c->pool), c->page_table, c->lengths, c->held, c->refs, c->status,
               page * c->n_pages, page, 2 * static_cast<int64_t>(c->page_size) * c->dim,
-              2 * c->n_layers, c->n_pages, c->kv_heads, c->page_size, 2 * c->dim, c->max_seqs, c->max_pages, c->max_pages};
+              2 * c->n_layers, c->n_pages, c->kv_heads, c->page_size, 2 * c->dim, c->max_seqs, c->max_pages, c->max_pages, nullptr, 0};
+    return AIMG_OK;
+}
+
+// The same for a cache in 8 bits, which has scales; in 16 where they are null.
+int take_as(const aimg_cache* c, float* scales, Cache& C) {
+    const int rc = take(c, C, true);
+    if (rc != AIMG_OK || scales == nullptr) return rc;
+    if (c->dim % 16 != 0 || c->dim > kMaxDim8)
+        return fail(AIMG_ERR_UNSUPPORTED, "cache: dim must be a multiple of 16 up to " + std::to_string(kMaxDim8) + " for 8 bits");
+    if (c->page_size % kBlock != 0) return fail(AIMG_ERR_UNSUPPORTED, "cache: page_size must be a multiple of 16 for 8 bits");
+    if (reinterpret_cast<uintptr_t>(scales) % 4 != 0) return fail(AIMG_ERR_UNSUPPORTED, "cache: the scales must be 4-byte aligned");
+    C.page_bytes /= 2, C.plane_bytes /= 2, C.head_bytes /= 2, C.row_bytes /= 2;
+    C.scales = scales, C.blocks = c->page_size / kBlock;
     return AIMG_OK;
 }
 
@@ -641,6 +1245,119 @@ extern "C" int aimg_cache_append(const aimg_cache* cache, int layer, const aimg_
     return aimg::launched();
 }
 
+namespace {
+
+// Rows of heads that a call reads or writes whole pieces of.
+int check_rows(const aimg_heads* x, const char* name, int heads, int dim) {
+    const std::string n(name);
+    if (x == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, n + " is null");
+    if (x->n_rows < 0 || x->n_rows > INT32_MAX - 8) return fail(AIMG_ERR_INVALID_ARGUMENT, n + ": n_rows must be in 0..2^31-9");
+    if (x->heads != heads || x->dim != dim || heads < 1)
+        return fail(AIMG_ERR_INVALID_ARGUMENT, n + " must have " + std::to_string(heads) + " heads of dim " + std::to_string(dim));
+    if (x->n_rows == 0) return AIMG_OK;
+    if (x->data == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, n + ": null data");
+    if (x->row_stride < 0 || x->head_stride < 0) return fail(AIMG_ERR_UNSUPPORTED, n + ": strides must not be negative");
+    if (reinterpret_cast<uintptr_t>(x->data) % 16 != 0 || (x->row_stride | x->head_stride) % 8 != 0)
+        return fail(AIMG_ERR_UNSUPPORTED, n + ": needs 16-byte aligned data and strides of whole 16 bytes");
+    return AIMG_OK;
+}
+
+int check_layer(const aimg_cache* cache, int layer) {
+    if (layer < 0 || layer >= cache->n_layers) return fail(AIMG_ERR_INVALID_ARGUMENT, "layer must be in 0.." + std::to_string(cache->n_layers - 1));
+    if (cache->dim > aimg::kMaxDim8) return fail(AIMG_ERR_UNSUPPORTED, "cache: dim must be at most " + std::to_string(aimg::kMaxDim8));
+    return AIMG_OK;
+}
+
+int check_type(int type) {
+    if (type != AIMG_BF16 && type != AIMG_FP16) return fail(AIMG_ERR_UNSUPPORTED, "type must be AIMG_BF16 or AIMG_FP16, got " + std::to_string(type));
+    return AIMG_OK;
+}
+
+template <typename T, int kMode>
+void launch_turn(const aimg::TurnArgs& a, hipStream_t s) {
+    const dim3 grid((a.n_items + 3) / 4 + static_cast<uint32_t>(a.c.scales == nullptr || a.q != nullptr ? a.n_rows : 0)), block(256);
+    if (a.c.scales == nullptr) hipLaunchKernelGGL((aimg::turn_kernel<T, kMode, 0>), grid, block, 0, s, a);
+    else if (a.dim <= 64) hipLaunchKernelGGL((aimg::turn_kernel<T, kMode, 2>), grid, block, 0, s, a);
+    else if (a.dim <= 128) hipLaunchKernelGGL((aimg::turn_kernel<T, kMode, 4>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((aimg::turn_kernel<T, kMode, 8>), grid, block, 0, s, a);
+}
+
+template <typename T>
+void launch_turn(const aimg::TurnArgs& a, hipStream_t s) {
+    const bool whole = (reinterpret_cast<uintptr_t>(a.cos) | reinterpret_cast<uintptr_t>(a.sin)) % 16 == 0;
+    if (a.half == 0 || (whole && a.paired && a.half % 4 == 0)) launch_turn<T, aimg::kPairs>(a, s);
+    else if (whole && !a.paired && a.half % 8 == 0) launch_turn<T, aimg::kHalves>(a, s);
+    else launch_turn<T, aimg::kAny>(a, s);
+}
+
+}  // namespace
+
+extern "C" int aimg_cache_append_rotated(const aimg_cache* cache, float* scales, int layer, const aimg_heads* q, const aimg_heads* k,
+                                         const aimg_heads* v, const aimg_heads* q_out, const int32_t* seqs, const int32_t* offsets,
+                                         int n_seqs, const aimg_rotary* rotary, const int32_t* positions, int type, void* stream) {
+    aimg::TurnArgs a{};
+    int rc = aimg::take_as(cache, scales, a.c);
+    if (rc == AIMG_OK) rc = aimg::check_seqs(n_seqs, seqs, offsets);
+    if (rc == AIMG_OK) rc = check_layer(cache, layer);
+    if (rc == AIMG_OK) rc = check_type(type);
+    if (rc == AIMG_OK) rc = check_rows(k, "k", cache->kv_heads, cache->dim);
+    if (rc == AIMG_OK) rc = check_rows(v, "v", cache->kv_heads, cache->dim);
+    if (rc == AIMG_OK && q != nullptr) rc = check_rows(q, "q", q->heads, cache->dim);
+    if (rc == AIMG_OK && q != nullptr) rc = check_rows(q_out, "q_out", q->heads, cache->dim);
+    if (rc != AIMG_OK) return rc;
+    if (v->n_rows != k->n_rows || (q != nullptr && (q->n_rows != k->n_rows || q_out->n_rows != k->n_rows)))
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "q, k, v and q_out must have the same rows");
+    if (rotary != nullptr) {
+        if (rotary->cos == nullptr || rotary->sin == nullptr || rotary->n_positions < 1)
+            return fail(AIMG_ERR_INVALID_ARGUMENT, "rotary: null tables or no positions");
+        if (rotary->half < 1 || 2 * static_cast<int64_t>(rotary->half) > cache->dim)
+            return fail(AIMG_ERR_INVALID_ARGUMENT, "rotary: half must be in 1..dim / 2, got " + std::to_string(rotary->half));
+        if ((reinterpret_cast<uintptr_t>(rotary->cos) | reinterpret_cast<uintptr_t>(rotary->sin)) % 4 != 0)
+            return fail(AIMG_ERR_UNSUPPORTED, "rotary: the tables must be 4-byte aligned");
+        a.cos = rotary->cos, a.sin = rotary->sin, a.n_positions = rotary->n_positions, a.half = rotary->half, a.paired = rotary->interleaved != 0;
+    }
+    const int64_t rows = k->n_rows;
+    if (n_seqs == 0 || rows == 0) return AIMG_OK;
+    const int64_t items = scales != nullptr ? (rows / aimg::kBlock + 2 * static_cast<int64_t>(n_seqs)) * cache->kv_heads * 2 : 0;
+    if (items > INT32_MAX || (items + 3) / 4 + rows > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "too many rows");
+    a.n_items = static_cast<uint32_t>(items);
+    if (q != nullptr) {
+        a.q = static_cast<const uint16_t*>(q->data), a.q_out = static_cast<uint16_t*>(q_out->data), a.heads = q->heads;
+        a.q_row = q->row_stride, a.q_head = q->head_stride, a.out_row = q_out->row_stride, a.out_head = q_out->head_stride;
+    }
+    a.k = static_cast<const uint16_t*>(k->data), a.v = static_cast<const uint16_t*>(v->data);
+    a.k_row = k->row_stride, a.k_head = k->head_stride, a.v_row = v->row_stride, a.v_head = v->head_stride;
+    a.positions = positions, a.seqs = seqs, a.offsets = offsets, a.n_seqs = n_seqs, a.n_rows = static_cast<int32_t>(rows);
+    a.dim = cache->dim, a.plane = 2 * layer;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (type == AIMG_BF16) launch_turn<aimg::AsBf16>(a, s);
+    else launch_turn<aimg::AsFp16>(a, s);
+    return aimg::launched();
+}
+
+extern "C" int aimg_cache_read(const aimg_cache* cache, float* scales, int layer, const int32_t* seqs, const int32_t* offsets,
+                               const int32_t* starts, int n_seqs, const aimg_heads* k, const aimg_heads* v, int type, void* stream) {
+    aimg::ReadArgs a{};
+    int rc = aimg::take_as(cache, scales, a.c);
+    if (rc == AIMG_OK) rc = aimg::check_seqs(n_seqs, seqs, offsets);
+    if (rc == AIMG_OK) rc = check_layer(cache, layer);
+    if (rc == AIMG_OK) rc = check_type(type);
+    if (rc == AIMG_OK) rc = check_rows(k, "k", cache->kv_heads, cache->dim);
+    if (rc == AIMG_OK) rc = check_rows(v, "v", cache->kv_heads, cache->dim);
+    if (rc != AIMG_OK) return rc;
+    if (v->n_rows != k->n_rows) return fail(AIMG_ERR_INVALID_ARGUMENT, "k and v must have the same rows");
+    if (n_seqs == 0 || k->n_rows == 0) return AIMG_OK;
+    a.k = static_cast<uint16_t*>(k->data), a.v = static_cast<uint16_t*>(v->data);
+    a.k_row = k->row_stride, a.k_head = k->head_stride, a.v_row = v->row_stride, a.v_head = v->head_stride;
+    a.seqs = seqs, a.offsets = offsets, a.starts = starts, a.n_seqs = n_seqs, a.n_rows = static_cast<int32_t>(k->n_rows), a.plane = 2 * layer;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const dim3 grid(aimg::blocks(k->n_rows, aimg::kReadRows)), block(256);
+    if (scales == nullptr) hipLaunchKernelGGL((aimg::read_kernel<aimg::AsBf16, false>), grid, block, 0, s, a);
+    else if (type == AIMG_BF16) hipLaunchKernelGGL((aimg::read_kernel<aimg::AsBf16, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((aimg::read_kernel<aimg::AsFp16, true>), grid, block, 0, s, a);
+    return aimg::launched();
+}
+
 extern "C" int aimg_cache_advance(const aimg_cache* cache, const int32_t* seqs, const int32_t* offsets, int n_seqs, void* stream) {
     aimg::Cache c;
     int rc = aimg::take(cache, c, false);
@@ -675,10 +1392,12 @@ extern "C" int aimg_cache_fork_workspace_nbytes(const aimg_cache* cache, int n_s
     return AIMG_OK;
 }
 
-extern "C" int aimg_cache_fork(const aimg_cache* cache, const int32_t* src, const int32_t* dst, int n_seqs, void* workspace,
-                               size_t workspace_nbytes, void* stream) {
+namespace {
+
+int fork(const aimg_cache* cache, float* scales, const int32_t* src, const int32_t* dst, int n_seqs, void* workspace,
+         size_t workspace_nbytes, void* stream) {
     aimg::ForkArgs a{};
-    int rc = aimg::take(cache, a.c, true);
+    int rc = aimg::take_as(cache, scales, a.c);
     if (rc == AIMG_OK) rc = aimg::check_seqs(n_seqs, src, dst);
     if (rc != AIMG_OK || n_seqs == 0) return rc;
     size_t need = 0;
@@ -692,14 +1411,34 @@ extern "C" int aimg_cache_fork(const aimg_cache* cache, const int32_t* src, cons
     // Shares of a pair: a thread moves up to four pieces of 16 bytes, in as many workgroups as a full tail takes.
     const int64_t pieces = static_cast<int64_t>(a.c.planes) * a.c.kv_heads * a.c.page_size * (a.c.row_bytes / 16);
     hipLaunchKernelGGL(aimg::fork_copy_kernel, dim3(static_cast<uint32_t>(n_seqs), aimg::blocks(pieces, 1024, 1024)), dim3(256), 0, s, a);
+    if (scales != nullptr) {
+        const int64_t most = static_cast<int64_t>(a.c.planes) * a.c.kv_heads * a.c.blocks;
+        hipLaunchKernelGGL(aimg::fork_scales_kernel, dim3(static_cast<uint32_t>(n_seqs), aimg::blocks(most, 256, 64)), dim3(256), 0, s, a);
+    }
     hipLaunchKernelGGL(aimg::fork_rows_kernel, dim3(static_cast<uint32_t>(n_seqs)), dim3(256), 0, s, a);
     return aimg::launched();
 }
 
-extern "C" int aimg_cache_commit(const aimg_cache* cache, const int32_t* seqs, const int32_t* accepted, int max_accepted,
-                                 const int32_t* counts, int n_seqs, int32_t* new_lengths, void* stream) {
+}  // namespace
+
+extern "C" int aimg_cache_fork(const aimg_cache* cache, const int32_t* src, const int32_t* dst, int n_seqs, void* workspace,
+                               size_t workspace_nbytes, void* stream) {
+    return fork(cache, nullptr, src, dst, n_seqs, workspace, workspace_nbytes, stream);
+}
+
+extern "C" int aimg_cache8_fork(const aimg_cache* cache, float* scales, const int32_t* src, const int32_t* dst, int n_seqs,
+                                void* workspace, size_t workspace_nbytes, void* stream) {
+    if (scales == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "scales is null");
+    return fork(cache, scales, src, dst, n_seqs, workspace, workspace_nbytes, stream);
+}
+
+namespace {
+
+// Of a cache in 16 bits (scales null) or 8.
+int commit(const aimg_cache* cache, float* scales, const int32_t* seqs, const int32_t* accepted, int max_accepted,
+           const int32_t* counts, int n_seqs, int32_t* new_lengths, void* stream) {
     aimg::CommitArgs a{};
-    int rc = aimg::take(cache, a.c, true);
+    int rc = aimg::take_as(cache, scales, a.c);
     if (rc == AIMG_OK) rc = aimg::check_seqs(n_seqs, seqs, counts);
     if (rc != AIMG_OK) return rc;
     if (max_accepted < 0) return fail(AIMG_ERR_INVALID_ARGUMENT, "max_accepted must be >= 0");
@@ -707,11 +1446,31 @@ extern "C" int aimg_cache_commit(const aimg_cache* cache, const int32_t* seqs, c
     if ((accepted == nullptr && max_accepted > 0) || new_lengths == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "null accepted or new_lengths");
     a.seqs = seqs, a.accepted = accepted, a.counts = counts, a.new_lengths = new_lengths, a.n_seqs = n_seqs, a.most = max_accepted;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t columns = static_cast<int64_t>(a.c.planes) * a.c.kv_heads * (a.c.row_bytes / 16);
-    hipLaunchKernelGGL(aimg::commit_kernel, dim3(aimg::blocks(columns, 256), static_cast<uint32_t>(n_seqs)), dim3(256), 0, s, a);
+    const int64_t heads = static_cast<int64_t>(a.c.planes) * a.c.kv_heads;
+    if (scales == nullptr) {
+        hipLaunchKernelGGL(aimg::commit_kernel, dim3(aimg::blocks(heads * (a.c.row_bytes / 16), 256), static_cast<uint32_t>(n_seqs)), dim3(256), 0, s, a);
+    } else {
+        const dim3 grid(aimg::blocks(heads, 4), static_cast<uint32_t>(n_seqs));
+        if (cache->dim <= 64) hipLaunchKernelGGL((aimg::commit8_kernel<2>), grid, dim3(256), 0, s, a);
+        else if (cache->dim <= 128) hipLaunchKernelGGL((aimg::commit8_kernel<4>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((aimg::commit8_kernel<8>), grid, dim3(256), 0, s, a);
+    }
     if (new_lengths == cache->lengths)
         hipLaunchKernelGGL(aimg::commit_lengths_kernel, dim3(aimg::blocks(n_seqs, 256)), dim3(256), 0, s, a);
     return aimg::launched();
+}
+
+}  // namespace
+
+extern "C" int aimg_cache_commit(const aimg_cache* cache, const int32_t* seqs, const int32_t* accepted, int max_accepted,
+                                 const int32_t* counts, int n_seqs, int32_t* new_lengths, void* stream) {
+    return commit(cache, nullptr, seqs, accepted, max_accepted, counts, n_seqs, new_lengths, stream);
+}
+
+extern "C" int aimg_cache8_commit(const aimg_cache* cache, float* scales, const int32_t* seqs, const int32_t* accepted, int max_accepted,
+                                  const int32_t* counts, int n_seqs, int32_t* new_lengths, void* stream) {
+    if (scales == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "scales is null");
+    return commit(cache, scales, seqs, accepted, max_accepted, counts, n_seqs, new_lengths, stream);
 }
 
 extern "C" int aimg_cache_compact_workspace_nbytes(const aimg_cache* cache, size_t* nbytes) {
@@ -720,10 +1479,12 @@ extern "C" int aimg_cache_compact_workspace_nbytes(const aimg_cache* cache, size
     return AIMG_OK;
 }
 
-extern "C" int aimg_cache_compact(const aimg_cache* cache, int32_t* new_table, int32_t* new_refs, int32_t* used, void* workspace,
-                                  size_t workspace_nbytes, void* stream) {
+namespace {
+
+int compact(const aimg_cache* cache, float* scales, int32_t* new_table, int32_t* new_refs, int32_t* used, void* workspace,
+            size_t workspace_nbytes, void* stream) {
     aimg::CompactArgs a{};
-    const int rc = aimg::take(cache, a.c, true);
+    const int rc = aimg::take_as(cache, scales, a.c);
     if (rc != AIMG_OK) return rc;
     size_t need = 0;
     aimg_cache_compact_workspace_nbytes(cache, &need);
@@ -738,4 +1499,17 @@ extern "C" int aimg_cache_compact(const aimg_cache* cache, int32_t* new_table, i
     const int64_t slices = (a.c.page_bytes + aimg::kSlice - 1) / aimg::kSlice;
     hipLaunchKernelGGL(aimg::compact_move_kernel, dim3(aimg::blocks(slices * a.c.planes * (a.c.n_pages / 2 + 1), 1, 2048)), dim3(256), 0, s, a);
     return aimg::launched();
+}
+
+}  // namespace
+
+extern "C" int aimg_cache_compact(const aimg_cache* cache, int32_t* new_table, int32_t* new_refs, int32_t* used, void* workspace,
+                                  size_t workspace_nbytes, void* stream) {
+    return compact(cache, nullptr, new_table, new_refs, used, workspace, workspace_nbytes, stream);
+}
+
+extern "C" int aimg_cache8_compact(const aimg_cache* cache, float* scales, int32_t* new_table, int32_t* new_refs, int32_t* used,
+                                   void* workspace, size_t workspace_nbytes, void* stream) {
+    if (scales == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "scales is null");
+    return compact(cache, scales, new_table, new_refs, used, workspace, workspace_nbytes, stream);
 }

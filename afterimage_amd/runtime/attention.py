@@ -25,6 +25,7 @@ _current_device = torch._C._cuda_getDevice
 _stream_handle = torch._C._cuda_getCurrentRawStream
 
 _TYPES = {torch.bfloat16: _native.AIMG_BF16, torch.float16: _native.AIMG_FP16}
+_BLOCK = 16  # positions that share a scale in a cache of 8 bits
 
 
 # The calls are short (a few microseconds of GPU time for one token), so the
@@ -183,8 +184,8 @@ def describe_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: tor
     index = k_pages.get_device()
     if index < 0:
         raise RuntimeError("the cache lives on the GPU only; got k_pages on %s" % k_pages.device)
-    if k_pages.dim() != 4 or k_pages.dtype not in _TYPES:
-        raise ValueError("k_pages must be a bf16 or fp16 [n_pages, kv_heads, page_size, dim] tensor")
+    if k_pages.dim() != 4 or (k_pages.dtype not in _TYPES and k_pages.dtype is not torch.float8_e4m3fn):
+        raise ValueError("k_pages must be a bf16, fp16 or float8_e4m3fn [n_pages, kv_heads, page_size, dim] tensor")
     shape, strides = k_pages.shape, k_pages.stride()
     if v_pages.shape != shape or v_pages.dtype is not k_pages.dtype or v_pages.stride() != strides or v_pages.get_device() != index:
         raise ValueError("v_pages must have k_pages' shape, type, strides and device")
@@ -197,10 +198,26 @@ def describe_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: tor
     n_pages, kv_heads, page_size, dim = shape
     page, head, slot, one = strides
     k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
-    if one != 1 or (page | head | slot) % 8 or (k_at | v_at) % 16:
+    if one != 1 or (page | head | slot) % (16 if k_pages.dtype is torch.float8_e4m3fn else 8) or (k_at | v_at) % 16:
         raise ValueError("k_pages and v_pages must be contiguous in their last dimension, their rows on 16-byte boundaries")
     return _native.AimgPages(k_at, v_at, page_table.data_ptr(), lengths.data_ptr(), page, slot, head, page_table.stride(0), n_pages,
                              page_size, kv_heads, dim, max_seqs, max_pages)
+
+
+def _page_scales(k_scales: torch.Tensor | None, v_scales: torch.Tensor | None, pages: _native.AimgPages,
+                 index: int) -> _native.AimgPageScales:
+    """The descriptor of the scales of pages in 8 bits."""
+    if pages.dim % 16 or pages.page_size % _BLOCK:
+        raise ValueError("pages in 8 bits: dim must be a multiple of 16 and page_size one of %d" % _BLOCK)
+    shape = (pages.n_pages, pages.kv_heads, pages.page_size // _BLOCK)
+    for x, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+        if x is None or x.dtype is not torch.float32 or x.shape != shape or x.get_device() != index \
+                or (x.stride(2) != 1 and shape[2] > 1):
+            raise ValueError("%s must be an fp32 %s tensor on cuda:%d, contiguous in its last dimension" % (name, list(shape), index))
+        forward_only(x, name)
+    if k_scales.stride() != v_scales.stride():
+        raise ValueError("v_scales must have k_scales' strides")
+    return _native.AimgPageScales(k_scales.data_ptr(), v_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -215,7 +232,8 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    lengths: torch.Tensor, seqs: torch.Tensor, draft_offsets: torch.Tensor,
                    masks: torch.Tensor | None = None, *, max_drafts: int, max_context: int | None = None,
                    scale: float | None = None, out: torch.Tensor | None = None,
-                   lse: torch.Tensor | None = None) -> torch.Tensor:
+                   lse: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
+                   v_scales: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of drafted tokens over a paged cache, on the current stream:
     the verification pass of drafted trees (afterimage/runtime/
     streaming_engine.py:2554-2556 runs step_k + 1 positions), and plain
@@ -235,6 +253,11 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     expect (all that the table can hold when not given), decides how the work is
     split, nothing else.
 
+    Pages of float8_e4m3fn come with their scales, fp32 [n_pages, kv_heads,
+    page_size / 16]: powers of two, which the elements of 16 positions of a
+    page and head are multiplied by (page_size and dim multiples of 16). q is
+    then bf16 or fp16, and probabilities are rounded to bf16.
+
     Returns out (q's shape and type; rows of no sequence, or past its first
     max_drafts, are not written); lse as in prompt_attention. Results do not
     vary between calls. No gradients, as there."""
@@ -242,8 +265,13 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     pages = describe_pages(k_pages, v_pages, page_table, lengths)
     forward_only(k_pages, "k_pages")
     forward_only(v_pages, "v_pages")
-    if k_pages.dtype is not q.dtype or k_pages.get_device() != index:
+    narrow = k_pages.dtype is torch.float8_e4m3fn
+    if (not narrow and k_pages.dtype is not q.dtype) or k_pages.get_device() != index:
         raise ValueError("k_pages must be %s on %s" % (q.dtype, q.device))
+    if narrow:
+        scales = _page_scales(k_scales, v_scales, pages, index)
+    elif k_scales is not None or v_scales is not None:
+        raise ValueError("k_scales and v_scales belong to pages of float8_e4m3fn")
     heads, kv_heads, dim = qd.heads, pages.kv_heads, qd.dim
     if pages.dim != dim or heads % kv_heads:
         raise ValueError("q's dim %d must be the pages' %d, its %d heads a multiple of their %d"
@@ -268,9 +296,25 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     out, od = _result(q, qd, out, index)
     nbytes = _tree_workspace_nbytes(n, heads, kv_heads, dim, n_seqs, max_drafts, max_context)
     work = _workspace(nbytes, q)
-    launch(_native.lib().aimg_tree_attention, index, qd, pages, od, seqs_at, at, n_seqs, masks_at, words, max_drafts, max_context,
-           kind, _scale(scale, dim), _lse(lse, q), work.data_ptr() if nbytes else None, nbytes)
+    rest = (od, seqs_at, at, n_seqs, masks_at, words, max_drafts, max_context, kind, _scale(scale, dim), _lse(lse, q),
+            work.data_ptr() if nbytes else None, nbytes)
+    if narrow:
+        launch(_native.lib().aimg_tree8_attention, index, qd, pages, scales, *rest)
+    else:
+        launch(_native.lib().aimg_tree_attention, index, qd, pages, *rest)
     return out
+
+
+def rotary_tables(positions: int, dim: int, base: float = 10000.0, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin [positions, dim / 2] (fp32) of the angles p * base ** (-2 i /
+    dim), for PagedKVCache.append_rotated: dim is the number of a head's
+    elements that turn. The angles are taken in 64 bits: in 32 those of far
+    positions are off by as much as their position times 2^-24."""
+    if positions < 1 or dim < 2 or dim % 2 or not base > 0.0:
+        raise ValueError("rotary_tables needs a position, an even dim and a positive base, got %d, %d and %r" % (positions, dim, base))
+    rate = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * rate
+    return angle.cos().float(), angle.sin().float()
 
 
 def tree_masks(parents: torch.Tensor, draft_offsets: torch.Tensor, max_drafts: int) -> torch.Tensor:

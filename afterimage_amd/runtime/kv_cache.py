@@ -14,6 +14,14 @@ lengths[s] positions and those to come; position j is row j % page_size of page
 page_table[s, j // page_size], the same page in every layer, for keys and for
 values. refs[p] slots hold page p. Free pages are given out lowest first, in the
 order of a call. A call names a slot once.
+
+A cache may hold its elements in 8 bits (torch.float8_e4m3fn), half the bytes
+that attention reads: a scale for each 16 positions of a page and head, keys and
+values apart, says what they stand for (value * scale). Scales are powers of
+two, the smallest that bring the largest of the 16 positions' elements to at
+most 448. Rows are rounded to nearest as they come in; where later rows raise
+the scale of their 16 positions, earlier elements below 2^-6 of it are rounded
+again. Infinities become NaN.
 """
 from __future__ import annotations
 
@@ -22,10 +30,12 @@ import ctypes
 import torch
 
 from .. import _native
-from .attention import forward_only, launch, tree_attention
+from .attention import _TYPES, forward_only, launch, tree_attention
 
 MAX_SEQS = 8192      # sequences of one call
 MAX_PAGES = (1 << 20) - 1
+BLOCK = 16           # positions that share a scale, in 8 bits
+MAX_DIM = 256        # of a cache in 8 bits, and of rows that are turned or read
 
 _PROBLEMS = ((1, "too few free pages"), (2, "positions past a sequence's pages or its row of the page table"),
              (4, "a slot, page, source or number of rows that does not exist"))
@@ -40,25 +50,28 @@ def _int32(x: torch.Tensor, name: str, shape: tuple, index: int) -> int:
 class PagedKVCache:
     """Pages of keys and values for every layer of a model, over tensors on one GPU:
 
-    pool        [n_layers, 2, n_pages, kv_heads, page_size, dim], bf16 or fp16
+    pool        [n_layers, 2, n_pages, kv_heads, page_size, dim], bf16, fp16 or
+                float8_e4m3fn (dim and page_size then multiples of 16)
     page_table  int32 [max_seqs, max_pages], -1 where a slot holds no page
     lengths     int32 [max_seqs], positions of each slot
     held        int32 [max_seqs], pages of each slot
     refs        int32 [n_pages], slots that hold each page
     status      int32 [1], what went wrong (see check)
+    scales      fp32 [n_layers, 2, n_pages, kv_heads, page_size / 16], of a pool
+                in 8 bits alone
 
     ``allocate`` makes an empty one. The tensors are used in place and are the
     cache's whole state. ``seqs``, ``src`` and ``dst`` below are slots: int32
     tensors on the GPU of at most 8192 entries."""
 
     def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, held: torch.Tensor,
-                 refs: torch.Tensor, status: torch.Tensor):
+                 refs: torch.Tensor, status: torch.Tensor, scales: torch.Tensor | None = None):
         index = pool.get_device()
         if index < 0:
             raise RuntimeError("the cache lives on the GPU only; got the pool on %s" % pool.device)
-        if pool.dim() != 6 or pool.shape[1] != 2 or pool.dtype not in (torch.bfloat16, torch.float16) \
+        if pool.dim() != 6 or pool.shape[1] != 2 or pool.dtype not in (torch.bfloat16, torch.float16, torch.float8_e4m3fn) \
                 or not pool.is_contiguous() or pool.numel() == 0:
-            raise ValueError("pool must be a contiguous bf16 or fp16 [n_layers, 2, n_pages, kv_heads, page_size, dim] tensor")
+            raise ValueError("pool must be a contiguous bf16, fp16 or float8_e4m3fn [n_layers, 2, n_pages, kv_heads, page_size, dim] tensor")
         if page_table.dim() != 2 or page_table.numel() == 0:
             raise ValueError("page_table must be a contiguous int32 [max_seqs, max_pages] tensor on cuda:%d" % index)
         self.n_layers, _, self.n_pages, self.kv_heads, self.page_size, self.dim = pool.shape
@@ -67,6 +80,18 @@ class PagedKVCache:
             raise ValueError("pool: dim must be a multiple of 8 and its memory 16-byte aligned")
         if self.n_pages > MAX_PAGES or self.max_pages * self.page_size >= 1 << 30:
             raise ValueError("pool: at most %d pages, and fewer than 2^30 positions a sequence" % MAX_PAGES)
+        self._scales_at = None
+        if pool.dtype is torch.float8_e4m3fn:
+            if self.dim % 16 or self.dim > MAX_DIM or self.page_size % BLOCK:
+                raise ValueError("pool: in 8 bits dim must be a multiple of 16 up to %d and page_size one of %d" % (MAX_DIM, BLOCK))
+            shape = (self.n_layers, 2, self.n_pages, self.kv_heads, self.page_size // BLOCK)
+            if scales is None or scales.dtype is not torch.float32 or scales.get_device() != index or scales.shape != shape \
+                    or not scales.is_contiguous():
+                raise ValueError("scales must be a contiguous fp32 %s tensor on cuda:%d" % (list(shape), index))
+            self._scales_at = scales.data_ptr()
+        elif scales is not None:
+            raise ValueError("scales belong to a pool of float8_e4m3fn")
+        self.scales = scales
         self._cache = _native.AimgCache(
             pool.data_ptr(), _int32(page_table, "page_table", (self.max_seqs, self.max_pages), index),
             _int32(lengths, "lengths", (self.max_seqs,), index), _int32(held, "held", (self.max_seqs,), index),
@@ -86,11 +111,13 @@ class PagedKVCache:
     @classmethod
     def allocate(cls, n_layers: int, n_pages: int, page_size: int, kv_heads: int, dim: int, max_seqs: int, max_pages: int,
                  dtype: torch.dtype = torch.bfloat16, device="cuda") -> "PagedKVCache":
-        """An empty cache. The pool's memory is not cleared."""
+        """An empty cache, of bf16, fp16 or float8_e4m3fn elements. The pool's memory is not cleared."""
         def ints(*shape, value=0):
             return torch.full(shape, value, dtype=torch.int32, device=device)
         pool = torch.empty((n_layers, 2, n_pages, kv_heads, page_size, dim), dtype=dtype, device=device)
-        return cls(pool, ints(max_seqs, max_pages, value=-1), ints(max_seqs), ints(max_seqs), ints(n_pages), ints(1))
+        scales = torch.empty((n_layers, 2, n_pages, kv_heads, page_size // BLOCK), dtype=torch.float32, device=device) \
+            if dtype is torch.float8_e4m3fn else None
+        return cls(pool, ints(max_seqs, max_pages, value=-1), ints(max_seqs), ints(max_seqs), ints(n_pages), ints(1), scales)
 
     def _seqs(self, x: torch.Tensor, name: str = "seqs") -> tuple[int, int]:
         """The address and the number of a call's slots."""
@@ -114,29 +141,119 @@ class PagedKVCache:
         at, n = self._seqs(seqs)
         launch(self._lib.aimg_cache_reserve, self._index, self._cache, at, _int32(tokens, "tokens", (n,), self._index), n)
 
-    def _rows(self, x: torch.Tensor, name: str) -> _native.AimgHeads:
-        if x.dim() != 3 or x.dtype is not self.pool.dtype or x.get_device() != self._index \
-                or x.shape[1:] != (self.kv_heads, self.dim):
-            raise ValueError("%s must be a %s [rows, %d, %d] tensor on %s"
-                             % (name, self.pool.dtype, self.kv_heads, self.dim, self.device))
+    def _heads(self, x: torch.Tensor, name: str, dtype: torch.dtype, heads: int) -> _native.AimgHeads:
+        if x.dim() != 3 or x.dtype is not dtype or x.get_device() != self._index or x.shape[1:] != (heads, self.dim):
+            raise ValueError("%s must be a %s [rows, %d, %d] tensor on %s" % (name, dtype, heads, self.dim, self.device))
         row, head, one = x.stride()
         if one != 1 or (row | head) % 8 or x.data_ptr() % 16:
             raise ValueError("%s must be contiguous in its last dimension, its rows and heads on 16-byte boundaries" % name)
         forward_only(x, name)
-        return _native.AimgHeads(x.data_ptr(), x.shape[0], row, head, x.shape[1], x.shape[2])
+        return _native.AimgHeads(x.data_ptr(), x.shape[0], row, head, heads, self.dim)
+
+    def _rows(self, x: torch.Tensor, name: str) -> _native.AimgHeads:
+        return self._heads(x, name, self.pool.dtype, self.kv_heads)
+
+    def _type(self, x: torch.Tensor, name: str) -> int:
+        """The number of the type of a call's rows: the pool's, or bf16 or fp16 for a pool in 8 bits."""
+        kind = _TYPES.get(x.dtype)
+        if kind is None or (self.scales is None and x.dtype is not self.pool.dtype):
+            raise ValueError("%s must be %s, got %s" % (name, self.pool.dtype if self.scales is None else "bf16 or fp16", x.dtype))
+        return kind
+
+    def _layer(self, layer: int) -> int:
+        if not 0 <= layer < self.n_layers:
+            raise ValueError("layer must be in 0..%d, got %d" % (self.n_layers - 1, layer))
+        return layer
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, offsets: torch.Tensor) -> None:
         """Rows offsets[b] .. offsets[b + 1] - 1 of k and v [rows, kv_heads,
         dim] into slot seqs[b]'s reserved pages, from its length on; lengths
-        stay (advance or commit moves them, once every layer has its rows)."""
-        kd, vd = self._rows(k, "k"), self._rows(v, "v")
-        if not 0 <= layer < self.n_layers:
-            raise ValueError("layer must be in 0..%d, got %d" % (self.n_layers - 1, layer))
+        stay (advance or commit moves them, once every layer has its rows). k
+        and v have the pool's type, bf16 or fp16 for one in 8 bits."""
+        if self.scales is not None:
+            kind = self._type(k, "k")
+            kd, vd = self._heads(k, "k", k.dtype, self.kv_heads), self._heads(v, "v", k.dtype, self.kv_heads)
+        else:
+            kd, vd = self._rows(k, "k"), self._rows(v, "v")
+        self._layer(layer)
         if k.shape != v.shape:
             raise ValueError("k and v must have one shape, got %s and %s" % (tuple(k.shape), tuple(v.shape)))
         at, n = self._seqs(seqs)
-        launch(self._lib.aimg_cache_append, self._index, self._cache, layer, kd, vd, at,
-               _int32(offsets, "offsets", (n + 1,), self._index), n)
+        offsets_at = _int32(offsets, "offsets", (n + 1,), self._index)
+        if self.scales is not None:
+            launch(self._lib.aimg_cache_append_rotated, self._index, self._cache, self._scales_at, layer, None, kd, vd, None, at,
+                   offsets_at, n, None, None, kind)
+        else:
+            launch(self._lib.aimg_cache_append, self._index, self._cache, layer, kd, vd, at, offsets_at, n)
+
+    def append_rotated(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor,
+                       offsets: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None, *,
+                       interleaved: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+        """append, with the rotation of q [rows, heads, dim] and k by their
+        positions on the way; returns the turned q (out where given, which may
+        be q itself but must not overlap it or k and v otherwise).
+
+        cos and sin: fp32 [positions, half], contiguous, half at most dim / 2
+        (attention.rotary_tables makes them): elements i and i + half of a row
+        at position p turn by the angle of cos[p, i] and sin[p, i], or elements
+        2 i and 2 i + 1 where interleaved; those from 2 half on stay. Row r's
+        position is positions[r] (int32 [rows]; a drafted token's is that of
+        its place in the tree), its place in the cache where not given. Rows
+        that are turned are rounded once, for a cache in 8 bits to its
+        elements. Rows of no sequence, or whose position the tables do not hold
+        (recorded), are not written to either; nor are keys and values that the
+        pages have no room for (recorded)."""
+        kind = self._type(q, "q")
+        if q.dim() != 3 or q.shape[1] < 1:
+            raise ValueError("q must be a %s [rows, heads, %d] tensor on %s" % (q.dtype, self.dim, self.device))
+        qd = self._heads(q, "q", q.dtype, q.shape[1])
+        kd, vd = self._heads(k, "k", q.dtype, self.kv_heads), self._heads(v, "v", q.dtype, self.kv_heads)
+        self._layer(layer)
+        if k.shape != v.shape or k.shape[0] != q.shape[0]:
+            raise ValueError("q, k and v must have the same rows, k and v one shape, got %s, %s and %s"
+                             % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+        if cos.dim() != 2 or cos.dtype is not torch.float32 or cos.get_device() != self._index or not cos.is_contiguous() \
+                or not 1 <= cos.shape[1] <= self.dim // 2 or cos.shape[0] < 1:
+            raise ValueError("cos must be a contiguous fp32 [positions, up to %d] tensor on cuda:%d" % (self.dim // 2, self._index))
+        if sin.shape != cos.shape or sin.dtype is not torch.float32 or sin.get_device() != self._index or not sin.is_contiguous():
+            raise ValueError("sin must have cos' shape, type and device")
+        at, n = self._seqs(seqs)
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif out.shape != q.shape:
+            raise ValueError("out must have q's shape %s" % (tuple(q.shape),))
+        od = self._heads(out, "out", q.dtype, q.shape[1])
+        launch(self._lib.aimg_cache_append_rotated, self._index, self._cache, self._scales_at, layer, qd, kd, vd, od, at,
+               _int32(offsets, "offsets", (n + 1,), self._index), n,
+               _native.AimgRotary(cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.shape[1], int(interleaved)),
+               None if positions is None else _int32(positions, "positions", (q.shape[0],), self._index), kind)
+        return out
+
+    def read(self, layer: int, seqs: torch.Tensor, offsets: torch.Tensor, rows: int, starts: torch.Tensor | None = None, *,
+             dtype: torch.dtype | None = None, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values of a layer as packed rows [rows, kv_heads, dim], as
+        prompt_attention takes them for a prompt that continues a context: rows
+        offsets[b] .. offsets[b + 1] - 1 (int32, on the GPU; ``rows`` is their
+        number) are positions starts[b] (int32, 0 where not given) and on of
+        slot seqs[b]. They may pass its length, not its pages. dtype: bf16 or
+        fp16 for a cache in 8 bits (bf16 where not given, and exact there), the
+        pool's otherwise. Rows of no sequence, or of no page (recorded), are
+        not written."""
+        dtype = dtype or (self.pool.dtype if self.scales is None else torch.bfloat16)
+        if dtype not in _TYPES or (self.scales is None and dtype is not self.pool.dtype):
+            raise ValueError("dtype must be %s, got %s" % (self.pool.dtype if self.scales is None else "bf16 or fp16", dtype))
+        self._layer(layer)
+        if rows < 0:
+            raise ValueError("rows must not be negative, got %d" % rows)
+        k, v = out or (torch.empty((rows, self.kv_heads, self.dim), dtype=dtype, device=self.device) for _ in range(2))
+        kd, vd = self._heads(k, "k", dtype, self.kv_heads), self._heads(v, "v", dtype, self.kv_heads)
+        if k.shape[0] != rows or v.shape[0] != rows:
+            raise ValueError("out must hold %d rows, got %d and %d" % (rows, k.shape[0], v.shape[0]))
+        at, n = self._seqs(seqs)
+        launch(self._lib.aimg_cache_read, self._index, self._cache, self._scales_at, layer, at,
+               _int32(offsets, "offsets", (n + 1,), self._index), None if starts is None else _int32(starts, "starts", (n,), self._index),
+               n, kd, vd, _TYPES[dtype])
+        return k, v
 
     def advance(self, seqs: torch.Tensor, offsets: torch.Tensor) -> None:
         """Slot seqs[b]'s length grows by offsets[b + 1] - offsets[b], the rows that were appended."""
@@ -146,6 +263,8 @@ class PagedKVCache:
     def attend(self, layer: int, q: torch.Tensor, seqs: torch.Tensor, draft_offsets: torch.Tensor,
                masks: torch.Tensor | None = None, **options) -> torch.Tensor:
         """tree_attention of q over one layer of this cache."""
+        if self.scales is not None:
+            options |= {"k_scales": self.scales[layer, 0], "v_scales": self.scales[layer, 1]}
         return tree_attention(q, self.keys(layer), self.values(layer), self.page_table, self.lengths, seqs, draft_offsets,
                               masks, **options)
 
@@ -163,7 +282,9 @@ class PagedKVCache:
             raise ValueError("accepted must be a contiguous int32 [%d, most] tensor on %s" % (n, self.device))
         most = accepted.shape[1]
         lengths = self.lengths if new_lengths is None else new_lengths
-        launch(self._lib.aimg_cache_commit, self._index, self._cache, at, _int32(accepted, "accepted", (n, most), self._index), most,
+        entry = (self._lib.aimg_cache_commit, self._index, self._cache) if self.scales is None else \
+            (self._lib.aimg_cache8_commit, self._index, self._cache, self._scales_at)
+        launch(*entry, at, _int32(accepted, "accepted", (n, most), self._index), most,
                _int32(counts, "counts", (n,), self._index), n, _int32(lengths, "new_lengths", (self.max_seqs,), self._index))
         return lengths
 
@@ -180,7 +301,10 @@ class PagedKVCache:
         # kept here would have to grow, and a captured graph or another stream
         # may still use the smaller one.
         work = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        launch(self._lib.aimg_cache_fork, self._index, self._cache, s, d, n, work.data_ptr(), nbytes)
+        if self.scales is None:
+            launch(self._lib.aimg_cache_fork, self._index, self._cache, s, d, n, work.data_ptr(), nbytes)
+        else:
+            launch(self._lib.aimg_cache8_fork, self._index, self._cache, self._scales_at, s, d, n, work.data_ptr(), nbytes)
 
     def release(self, seqs: torch.Tensor) -> None:
         """Empties the slots; pages that no other slot holds are free."""
@@ -195,8 +319,9 @@ class PagedKVCache:
         table = self.page_table if new_table is None else new_table
         refs = self.refs if new_refs is None else new_refs
         used = torch.empty_like(self._used)
-        launch(self._lib.aimg_cache_compact, self._index, self._cache,
-               _int32(table, "new_table", (self.max_seqs, self.max_pages), self._index),
+        entry = (self._lib.aimg_cache_compact, self._index, self._cache) if self.scales is None else \
+            (self._lib.aimg_cache8_compact, self._index, self._cache, self._scales_at)
+        launch(*entry, _int32(table, "new_table", (self.max_seqs, self.max_pages), self._index),
                _int32(refs, "new_refs", (self.n_pages,), self._index), used.data_ptr(), self._compact_work.data_ptr(),
                self._compact_work.shape[0])
         return used

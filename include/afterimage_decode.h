@@ -354,6 +354,27 @@ int aimg_tree_attention(const aimg_heads* q, const aimg_pages* pages, const aimg
                         int64_t max_context, int type, float scale, float* lse, void* workspace,
                         size_t workspace_nbytes, void* stream);
 
+/* The factors of pages of 8-bit elements (see the cache below): positions
+ * 16 i .. 16 i + 15 of head h of a page share k[page * page_stride + h *
+ * head_stride + i], and v's likewise (strides in floats, the same for both). */
+typedef struct aimg_page_scales {
+    const float* k;       /* device */
+    const float* v;
+    int64_t page_stride;
+    int64_t head_stride;
+} aimg_page_scales;
+
+/*
+ * aimg_tree_attention over a cache in 8 bits: pages of e4m3 elements (strides
+ * in elements, whole 16 bytes; dim and page_size multiples of 16), the factors
+ * powers of two. q and out are bf16 or fp16 (type). Keys enter the first
+ * product exactly, probabilities are rounded to bf16 for the second.
+ */
+int aimg_tree8_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_page_scales* scales, const aimg_heads* out,
+                         const int32_t* seqs, const int32_t* draft_offsets, int n_seqs, const int64_t* masks, int mask_words,
+                         int max_drafts, int64_t max_context, int type, float scale, float* lse, void* workspace,
+                         size_t workspace_nbytes, void* stream);
+
 /*
  * masks[row * mask_words + w] for n_rows drafted tokens from their parents:
  * parents[row] is the index, within its sequence, of an earlier drafted token,
@@ -405,6 +426,67 @@ typedef struct aimg_cache {
 int aimg_cache_append(const aimg_cache* cache, int layer, const aimg_heads* k, const aimg_heads* v, const int32_t* seqs,
                       const int32_t* offsets, int n_seqs, void* stream);
 
+/*
+ * A cache in 8 bits: the pool holds e4m3 elements (one byte: 4 bits of
+ * exponent, 3 of mantissa, no infinity), dim a multiple of 16 up to 256,
+ * page_size one of 16, and scales[n_layers][2][n_pages][kv_heads][page_size /
+ * 16] (floats, device) one factor for each 16 positions of a page and head: an
+ * element stands for its value times the factor. Factors are powers of two from
+ * 2^-100 to 2^119: the smallest that brings the largest of the block's rows to
+ * at most 448 (past that at the highest one, elements are held as 448 of it).
+ * Infinities and NaN are held as NaN and do not count. A block that a call adds
+ * rows to is formed anew from what its rows below the length stand for and
+ * those, rounded to nearest even. Where `scales` is an argument of a call for
+ * either, NULL means a cache in 16 bits.
+ */
+
+/* Tables of a rotation: element i < half of a position's row turns, with the
+ * element it is paired with, by the angle whose cosine and sine are
+ * cos[position * half + i] and sin[...]: (a, b) becomes (a c - b s, b c + a s).
+ * Pairs are i and i + half, or 2 i and 2 i + 1 where interleaved is not 0; the
+ * elements from 2 * half on stay. */
+typedef struct aimg_rotary {
+    const float* cos;     /* device: [n_positions][half] */
+    const float* sin;
+    int32_t n_positions;
+    int32_t half;         /* 1 .. dim / 2 */
+    int32_t interleaved;
+} aimg_rotary;
+
+/*
+ * aimg_cache_append with the rotation of q and k on the way (rotary NULL:
+ * none), into a cache in 16 bits or 8 (type: that of q, k and v; in 16 bits
+ * the pool's too). Row r turns by positions[r] (int32, device), by its position in
+ * the cache where positions is NULL; the turned q goes to q_out, which may be
+ * q (q NULL: none). Products and sums are fp32, rounded once. A row whose
+ * position the tables do not hold is left out and recorded (4); rows of no
+ * sequence are left out. Rows, heads and 16-byte pieces as for aimg_heads'
+ * inputs, q_out too; dim up to 256.
+ */
+int aimg_cache_append_rotated(const aimg_cache* cache, float* scales, int layer, const aimg_heads* q, const aimg_heads* k,
+                              const aimg_heads* v, const aimg_heads* q_out, const int32_t* seqs, const int32_t* offsets,
+                              int n_seqs, const aimg_rotary* rotary, const int32_t* positions, int type, void* stream);
+
+/*
+ * Rows offsets[b] .. offsets[b+1] - 1 of k and v (written, in 16 bits of the
+ * given type, which is the pool's where that has 16) become positions starts[b]
+ * .. (0 .. where starts is NULL) of slot seqs[b]. Positions past its length, in
+ * pages it holds, are read too; rows of no sequence, or of positions that no
+ * page holds (recorded), are left as they are.
+ */
+int aimg_cache_read(const aimg_cache* cache, float* scales, int layer, const int32_t* seqs, const int32_t* offsets,
+                    const int32_t* starts, int n_seqs, const aimg_heads* k, const aimg_heads* v, int type, void* stream);
+
+/* aimg_cache_fork, aimg_cache_commit and aimg_cache_compact of a cache in 8
+ * bits, with the same workspaces. A block into which an accepted row moves is
+ * formed anew; the others stay. */
+int aimg_cache8_fork(const aimg_cache* cache, float* scales, const int32_t* src, const int32_t* dst, int n_seqs,
+                     void* workspace, size_t workspace_nbytes, void* stream);
+int aimg_cache8_commit(const aimg_cache* cache, float* scales, const int32_t* seqs, const int32_t* accepted, int max_accepted,
+                       const int32_t* counts, int n_seqs, int32_t* new_lengths, void* stream);
+int aimg_cache8_compact(const aimg_cache* cache, float* scales, int32_t* new_table, int32_t* new_refs, int32_t* used,
+                        void* workspace, size_t workspace_nbytes, void* stream);
+
 /* Adds offsets[b+1] - offsets[b] to slot seqs[b]'s length: the rows that every
  * layer has appended (a difference below 0 is an error, 4). */
 int aimg_cache_advance(const aimg_cache* cache, const int32_t* seqs, const int32_t* offsets, int n_seqs, void* stream);
@@ -450,6 +532,44 @@ int aimg_cache_commit(const aimg_cache* cache, const int32_t* seqs, const int32_
 int aimg_cache_compact_workspace_nbytes(const aimg_cache* cache, size_t* nbytes);
 int aimg_cache_compact(const aimg_cache* cache, int32_t* new_table, int32_t* new_refs, int32_t* used, void* workspace,
                        size_t workspace_nbytes, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Tokens from logits.                                                       */
+/* ------------------------------------------------------------------------- */
+
+#define AIMG_FP32 2
+
+/* A row's settings: its entry of an array (device), or the number below for
+ * every row where the array is NULL. temperature: 0 (or less, or NaN) takes the
+ * largest logit's first token. top_k: 0 (or less) for none. top_p: 1 (or more)
+ * for none. min_p: 0 (or less) for none. */
+typedef struct aimg_sampling {
+    const float* temperatures;
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    double temperature;
+    double top_p;
+    double min_p;
+    int32_t top_k;
+} aimg_sampling;
+
+/*
+ * A token for each of n_rows rows of `vocab` logits (at most 2^18), rows
+ * row_stride elements apart, of type bf16, fp16 or fp32. A row's tokens stand
+ * in the order of falling logits, equal ones by rising index; with w = exp((x -
+ * max x) / temperature) those are kept that are among the first top_k, in the
+ * shortest prefix whose weights reach top_p times the first top_k's, and
+ * weigh at least min_p; one at least. tokens[row] is the first whose weights,
+ * summed along the order, pass uniforms[row] (in [0, 1); other numbers as the
+ * nearest there) times those of all that are kept, and logprobs[row] (where not
+ * NULL) the logarithm of its share of them: 0 at temperature 0. Logits of -inf or
+ * NaN are no tokens; a row without any other gives -1 and -inf. Weights below
+ * 2^-64 of the largest count as nothing, the others are sums of 2^-26 of
+ * themselves, in integers and doubles: results do not vary between calls.
+ */
+int aimg_sample(const void* logits, int64_t n_rows, int64_t row_stride, int vocab, int type, const float* uniforms,
+                const aimg_sampling* settings, int64_t* tokens, float* logprobs, void* stream);
 
 #ifdef __cplusplus
 }
