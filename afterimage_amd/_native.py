@@ -241,9 +241,10 @@ _SIGNATURES = [
     ("aimg_cache_compact_workspace_nbytes", ctypes.c_int, [_CACHE, _SIZE]),
     ("aimg_cache_compact", ctypes.c_int,
      [_CACHE, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    ("aimg_sample_workspace_nbytes", ctypes.c_int, [ctypes.c_int64, ctypes.c_int, _SIZE]),
     ("aimg_sample", ctypes.c_int,
      [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(AimgSampling),
-      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+      ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
 ]
 
 EXPORTED_SYMBOLS = tuple(name for name, _, _ in _SIGNATURES)

@@ -10,8 +10,9 @@
 // weights say in which bins the prefixes end and the draw falls, and only these
 // bins' tokens (a few hundred, mostly) are gathered and sorted.
 //
-// Sums. A token's place t = 64 log2(1 / w) is computed in 64 bits; its whole
-// part is its bin, and its weight against the bin's top is rounded to 2^-26. A
+// Sums. A token's place t = 64 log2(1 / w) is computed as a pair of floats (in
+// doubles a row of 151936 took 68 us, not 44); its whole part is its bin, and
+// its weight against the bin's top is rounded to 2^-26. A
 // bin's count and sum are integers in one 64-bit word, so a row's result does
 // not depend on the order of the atomics that add them; sums of bins are
 // doubles, in a fixed order. Tokens below 2^-64 of the largest weigh nothing.
@@ -20,6 +21,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "afterimage_decode.h"
 #include "aimg_internal.h"
@@ -27,16 +29,17 @@
 namespace aimg {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kPerOctave = 64;             // bins of a factor of 2
 constexpr int kBins = 4096;
 constexpr int kEach = kBins / kThreads;    // bins, and sorted tokens, of a thread
 constexpr int kList = 4096;                // tokens that are gathered and sorted
-constexpr int kCountShift = 45;            // of a bin's word: count above, sum of weights (in 2^-26) below
-constexpr uint64_t kSumMask = (uint64_t{1} << kCountShift) - 1;
+constexpr int kFew = 512;             // so many are sorted by counting
+constexpr int kCountShift = 45;            // of a bin's word: count above; below, what its tokens lack to the weight of its top, in 2^-26 of that
+constexpr uint64_t kLackMask = (uint64_t{1} << kCountShift) - 1;
 constexpr int kMaxVocab = 1 << 18;         // so that neither overflows
-constexpr float kUnit = 67108864.0f;       // 2^26
+constexpr uint32_t kUnits = 1u << 26;
 
 struct SampleArgs {
     const void* logits;
@@ -65,17 +68,19 @@ struct LogitFp32 {
     static __device__ float value(uint32_t x) { return __uint_as_float(x); }
 };
 
-// Calls f(index, logit) for logits thread, thread + step, .. of 16-byte pieces
-// (a row may begin and end anywhere; what lies outside whole pieces comes one by
-// one), each thread's by rising index. A NaN is -inf, which no token has.
-template <typename L, typename F>
-__device__ __forceinline__ void each_logit(const typename L::Element* row, int n, int thread, int threads, F f) {
+// Calls f(index of the first, logits) for 16-byte pieces thread, thread +
+// threads, .. of a row, each thread's by rising index. A row may begin and end
+// anywhere: what lies outside whole pieces comes one by one.
+template <typename L, int kAhead = 4, typename F>
+__device__ __forceinline__ void each_piece(const typename L::Element* row, int n, int thread, int threads, F f) {
     typedef typename L::Element E;
-    constexpr int kPiece = 16 / sizeof(E), kAhead = 4;
-    auto give = [&](int i, float x) { f(i, x != x ? -INFINITY : x); };
+    constexpr int kPiece = 16 / sizeof(E);
     int head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(E));
     if (head > n) head = n;
-    if (thread < head) give(thread, L::value(row[thread]));
+    if (thread < head) {
+        const float one[1] = {L::value(row[thread])};
+        f(thread, one);
+    }
     const int pieces = (n - head) / kPiece;
     for (int c0 = thread; c0 < pieces; c0 += kAhead * threads) {
         uint4 w[kAhead];
@@ -89,13 +94,26 @@ __device__ __forceinline__ void each_logit(const typename L::Element* row, int n
             const int c = c0 + j * threads;
             if (c >= pieces) break;
             const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+            float x[kPiece];
 #pragma unroll
-            for (int e = 0; e < kPiece; ++e)
-                give(head + c * kPiece + e, L::value(static_cast<E>(sizeof(E) == 2 ? u[e / 2] >> 16 * (e % 2) : u[e])));
+            for (int e = 0; e < kPiece; ++e) x[e] = L::value(static_cast<E>(sizeof(E) == 2 ? u[e / 2] >> 16 * (e % 2) : u[e]));
+            f(head + c * kPiece, x);
         }
     }
     const int done = head + pieces * kPiece;
-    if (done + thread < n) give(done + thread, L::value(row[done + thread]));  // fewer than a piece
+    if (done + thread < n) {  // fewer than a piece
+        const float one[1] = {L::value(row[done + thread])};
+        f(done + thread, one);
+    }
+}
+
+// The same with f(index, logit). (No comparison with a NaN holds, so a NaN is never taken.)
+template <typename L, typename F>
+__device__ __forceinline__ void each_logit(const typename L::Element* row, int n, int thread, int threads, F f) {
+    each_piece<L>(row, n, thread, threads, [&](int i, const auto& x) {
+#pragma unroll
+        for (int e = 0; e < static_cast<int>(sizeof(x) / sizeof(float)); ++e) f(i + e, x[e]);
+    });
 }
 
 // Unsigned numbers in the order of logits; equal ones for both zeros.
@@ -106,28 +124,118 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
-// A token's place: how far below the largest, 64 to a factor of 2. (max - x is
-// exact in 64 bits or rounds without changing the order; an infinite maximum
-// leaves its equals alone at 0.)
-struct Places {
-    double top, per;
-    __device__ __forceinline__ double of(float x) const { return static_cast<double>(x) == top ? 0.0 : (top - static_cast<double>(x)) * per; }
+// A token's place: how far below the largest, 64 to a factor of 2, as the whole
+// part `bin` and the rest f, which may leave [0, 1) by its rounding. What the
+// product loses in 32 bits goes into the rest, and so does what max - x loses,
+// for fp32 logits. (Logits of 16 bits lose nothing unless 2^16 apart, and then
+// 2^-25 of the difference at most.) Bins rise as the logits fall, for both
+// roundings keep the order. An infinite maximum leaves its equals alone at 0.
+struct Place {
+    float t;  // the bin's number and more; from kBins on, or NaN: no weight
+    float f;
+    __device__ __forceinline__ int bin() const { return static_cast<int>(t); }
+    __device__ __forceinline__ double exact() const { return static_cast<double>(bin()) + f; }
 };
 
-// 2^(-f / 64) in 2^-26, f in [0, 1): one minus its series in g = f ln 2 / 64 < 0.011, whose fourth term is below 2^-30.
-__device__ __forceinline__ uint32_t weight_in_bin(float f) {
-    const float g = f * (0.693147180559945f / kPerOctave);
-    const float less = g * (1.0f - g * (0.5f - g * (1.0f / 6.0f)));
-    return static_cast<uint32_t>(kUnit) - static_cast<uint32_t>(__float2int_rn(less * kUnit));
+template <typename L>
+struct Places {
+    float top, per, rest;  // per + rest: 64 log2(e) / temperature
+    bool endless;          // the top is infinite
+
+    __device__ __forceinline__ Place of(float x) const { return endless ? Place{x == top ? 0.0f : INFINITY, 0.0f} : of_finite(x); }
+
+    __device__ __forceinline__ Place of_finite(float x) const {
+#pragma clang fp contract(off)
+        const float d = top - x, t = d * per;
+        float f = fmaf(d, rest, fmaf(d, per, -t));
+        if constexpr (sizeof(typename L::Element) == 4) {
+            const float v = d - top;
+            f = fmaf((top - (d - v)) - (x + v), per, f);
+        }
+        return Place{t, __builtin_amdgcn_fractf(t) + f};
+    }
+
+    // Logits whose places may lie in bins first .. last (all that do, and some more).
+    __device__ __forceinline__ void span(int first, int last, float& low, float& high) const {
+        if (endless) {
+            low = high = top;
+            return;
+        }
+        const double by = per, room = 1e-6 * fabs(static_cast<double>(top)), far = (last + 1) / by * (1.0 + 1e-6), near = first / by * (1.0 - 1e-6);
+        low = static_cast<float>(top - far - room - 1e-6 * far);
+        high = static_cast<float>(top - near + room + 1e-6 * near);
+        if (first == 0 || !(high > low)) high = top;  // (nothing is above it; near is 0 / 0 where the temperature is infinite)
+    }
+};
+
+// Spans of logits, of which a piece's nearest to any says whether it holds one:
+// two instructions a logit and span, no masks.
+struct Spans {
+    float low[4], high[4], by[4], off[4];  // |x * by + off| <= 1 inside
+    float room = 1.0f;                     // 1 and the roundings of that
+    int n = 0;
+    bool exact = true;
+
+    __device__ __forceinline__ void add(float l, float h) {
+        const double mid = 0.5 * (static_cast<double>(l) + h), half = 0.5 * (static_cast<double>(h) - l);
+        const double to = half > 0.0 ? 1.0 / half : INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i == n) low[i] = l, high[i] = h, by[i] = static_cast<float>(to), off[i] = static_cast<float>(-mid * to);
+        ++n;
+        // x * by is off by 2^-24 of itself from by's rounding, and the sum by 2^-24 of off.
+        const float far = static_cast<float>(fabs(mid * to));
+        if (far < 1e5f) room = fmaxf(room, 1.0f + far * 1e-6f + 1e-6f);
+        else exact = false;  // NaN too: infinite ends, spans of nearly no width
+    }
+
+    template <int kSpans, int kPiece>
+    __device__ __forceinline__ bool any(const float (&x)[kPiece]) const {
+        if (!exact) {
+            bool in = false;
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) in |= holds<kSpans>(x[e]);
+            return in;
+        }
+        float least = INFINITY;
+#pragma unroll
+        for (int i = 0; i < kSpans; ++i) {
+            if (i > 1 && i >= n) break;
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) least = fminf(least, fabsf(fmaf(x[e], by[i], off[i])));
+        }
+        return least <= room;
+    }
+
+    template <int kSpans>
+    __device__ __forceinline__ bool holds(float x) const {
+        bool in = false;
+#pragma unroll
+        for (int i = 0; i < kSpans; ++i) in |= (i < 2 || i < n) && x >= low[i] && x <= high[i];
+        return in;
+    }
+};
+
+// What 2^(-f / 64) lacks to 1, in 2^-26 and rounded, for f in [0, 1]: its series
+// in g = f ln 2 / 64 < 0.011, whose fourth term is below 2^-30.
+__device__ __forceinline__ uint32_t lack_in_bin(float f) {
+    constexpr float g = 0.6931471805599453f / kPerOctave;
+    return static_cast<uint32_t>(fmaf(f, fmaf(f, fmaf(f, g * g * g / 6.0f * kUnits, -g * g / 2.0f * kUnits), g * kUnits), 0.5f));
 }
 
-__device__ __forceinline__ uint64_t word_of(double t) {
-    const int bin = static_cast<int>(t);
-    return uint64_t{1} << kCountShift | weight_in_bin(static_cast<float>(t - bin));
-}
+__device__ __forceinline__ uint64_t word_of(const Place& p) { return uint64_t{1} << kCountShift | lack_in_bin(p.f); }
+__device__ __forceinline__ int32_t count_of(uint64_t word) { return static_cast<int32_t>(word >> kCountShift); }
+__device__ __forceinline__ uint64_t units_of(uint64_t word) { return (word >> kCountShift) * kUnits - (word & kLackMask); }
 
-// What a unit of a bin's sum weighs.
-__device__ __forceinline__ double unit_of(int bin) { return exp2(-static_cast<double>(bin) / kPerOctave - 26.0); }
+// 2^(-i / 64), i < 64: a table that a workgroup makes once (exp2 for every bin took longer than their sums).
+struct Octave {
+    double part[kPerOctave];
+    __device__ __forceinline__ void make() {
+        if (threadIdx.x < kPerOctave) part[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / kPerOctave);
+    }
+    // What a unit of a bin's sum weighs.
+    __device__ __forceinline__ double unit(int bin) const { return ldexp(part[bin % kPerOctave], -26 - bin / kPerOctave); }
+};
 
 template <typename V>
 __device__ __forceinline__ V before_in_wave(V v, V& all) {
@@ -143,59 +251,6 @@ __device__ __forceinline__ V before_in_wave(V v, V& all) {
     return lane == 0 ? V(0) : e;
 }
 
-struct Shared {
-    uint64_t words[kBins];      // bins, then the gathered tokens: ~key above, index below
-    double weight[kBins + 1];   // of the bins before
-    int32_t count[kBins + 1];
-    uint64_t sums[kList];       // of the tokens before, in their bins' units
-    double wave_weight[kWaves];
-    uint64_t wave_best[kWaves];
-    int32_t wave_count[kWaves], wave_first[kWaves];
-    double end_weight[3], found_weight;
-    int32_t end_count[3], found[4], n, drawn;
-};
-
-// Sums over the bins before each, and of all.
-__device__ __forceinline__ void sum_bins(Shared& S) {
-    const int t = threadIdx.x, wave = t >> 6;
-    int32_t c[kEach], all_c;
-    double w[kEach], all_w;
-    int32_t my_c = 0;
-    double my_w = 0.0;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const uint64_t x = S.words[t * kEach + j];
-        c[j] = static_cast<int32_t>(x >> kCountShift);
-        w[j] = x == 0 ? 0.0 : static_cast<double>(x & kSumMask) * unit_of(t * kEach + j);
-        my_c += c[j], my_w += w[j];
-    }
-    int32_t at_c = before_in_wave(my_c, all_c);
-    double at_w = before_in_wave(my_w, all_w);
-    if ((t & 63) == 0) S.wave_count[wave] = all_c, S.wave_weight[wave] = all_w;
-    __syncthreads();
-    double base = 0.0;
-    for (int i = 0; i < wave; ++i) at_c += S.wave_count[i], base += S.wave_weight[i];
-    at_w += base;
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        S.count[t * kEach + j] = at_c, S.weight[t * kEach + j] = at_w;
-        at_c += c[j], at_w += w[j];
-    }
-    if (t == kThreads - 1) S.count[kBins] = at_c, S.weight[kBins] = at_w;
-    __syncthreads();
-}
-
-// The bin where a weight is reached (weight before < x <= with it) or passed (<=, <): one thread finds it.
-template <bool kPassed>
-__device__ __forceinline__ void find_weight(Shared& S, double x, int32_t* to) {
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int b = threadIdx.x * kEach + j;
-        const double low = S.weight[b], high = S.weight[b + 1];
-        if (kPassed ? low <= x && x < high : low < x && x <= high) *to = b;
-    }
-}
-
 // A row's settings. Numbers out of range mean the nearest in it: no rule, or the first token.
 struct Rules {
     bool greedy;
@@ -203,20 +258,178 @@ struct Rules {
     int32_t k;
 };
 
+__device__ __forceinline__ bool greedy(const SampleArgs& A, int row) {
+    return !((A.temperatures != nullptr ? A.temperatures[row] : A.temperature) > 0.0);
+}
+
 __device__ __forceinline__ Rules rules_of(const SampleArgs& A, int row) {
     Rules r;
     const double t = A.temperatures != nullptr ? A.temperatures[row] : A.temperature;
     const double p = A.top_ps != nullptr ? A.top_ps[row] : A.top_p, m = A.min_ps != nullptr ? A.min_ps[row] : A.min_p;
     const int32_t k = A.top_ks != nullptr ? A.top_ks[row] : A.top_k;
     const double u = A.uniforms[row];
-    r.greedy = !(t > 0.0);
+    r.greedy = greedy(A, row);
     r.per = r.greedy ? 0.0 : kPerOctave * 1.4426950408889634 / t;
-    if (r.per > 1e300) r.per = 1e300;
+    if (r.per > 1e30) r.per = 1e30;
     r.k = k > 0 ? k : INT32_MAX;
     r.p = p < 1.0 ? (p > 0.0 ? p : 0.0) : 1.0;
     r.min_t = m > 0.0 ? (m < 1.0 ? -kPerOctave * log2(m) : 0.0) : INFINITY;
     r.u = u > 0.0 ? (u < 1.0 ? u : 1.0 - 0x1p-53) : 0.0;
     return r;
+}
+
+// What a row's workgroup keeps in LDS. The words are the bins, later the
+// gathered tokens: ~key above, index below.
+struct Shared {
+    uint64_t words[kBins + 64];
+    Octave octave;
+    double wave_weight[kWaves], start[kThreads + 1];
+    uint64_t wave_best[kWaves];
+    int32_t wave_count[kWaves], wave_first[kWaves];
+    double found_low[6], found_high[6], end_weight[3], found_weight;
+    int32_t found[6], end_count[3], n, drawn, before_count, inside_count;
+    uint64_t inside;
+    int32_t rank[kFew];
+};
+
+// Tokens and weights before each bin, and of all: [kBins + 1].
+struct Sums {
+    double* weight;
+    int32_t* count;
+};
+
+// The bins where a row's prefixes may end (what the first k weigh is known to a
+// bin, so what p of it is lies in some range) and where its draw may fall; -1: none.
+struct Found {
+    int32_t bin_k, low_p, high_p, bin_m, low_u, high_u, last;
+    __device__ __forceinline__ bool wanted(int b) const {
+        return b == bin_k || (b >= low_p && b <= high_p) || b == bin_m || (b >= low_u && b <= high_u);
+    }
+};
+
+__device__ __forceinline__ double reached(double x, double all) { return x < 1e-300 ? 1e-300 : x > all ? all : x; }
+
+// The words' sums (into `to`, where it is not null) and those bins, by a workgroup.
+__device__ __forceinline__ Found find_bins(Shared& S, const Rules& R, const Sums& to) {
+    const int t = threadIdx.x, wave = t >> 6;
+    int32_t count[kEach + 1], all_c, my_c = 0;
+    double weight[kEach + 1], all_w, my_w = 0.0;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const uint64_t x = S.words[t * kEach + j];
+        count[j + 1] = count_of(x);
+        weight[j + 1] = static_cast<double>(units_of(x)) * S.octave.unit(t * kEach + j);
+        my_c += count[j + 1], my_w += weight[j + 1];
+    }
+    count[0] = before_in_wave(my_c, all_c);
+    weight[0] = before_in_wave(my_w, all_w);
+    if ((t & 63) == 0) S.wave_count[wave] = all_c, S.wave_weight[wave] = all_w;
+    if (t < 6) S.found[t] = -1, S.found_low[t] = S.found_high[t] = 0.0;
+    __syncthreads();
+    int32_t total_c = 0;
+    double base = 0.0, total = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (i == wave) count[0] += total_c, base = total;
+        total_c += S.wave_count[i], total += S.wave_weight[i];
+    }
+    weight[0] += base;
+    S.start[t] = weight[0];
+    if (t == 0) S.start[kThreads] = total;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        if (to.count != nullptr) to.count[t * kEach + j] = count[j], to.weight[t * kEach + j] = weight[j];
+        count[j + 1] += count[j];
+        weight[j + 1] = j + 1 < kEach ? weight[j] + weight[j + 1] : S.start[t + 1];  // where the next thread begins
+    }
+    if (t == 0 && to.count != nullptr) to.count[kBins] = total_c, to.weight[kBins] = total;
+    auto mark = [&](int i, int j) { S.found[i] = t * kEach + j, S.found_low[i] = weight[j], S.found_high[i] = weight[j + 1]; };
+    const int m = R.min_t < kBins ? static_cast<int>(R.min_t) : -1;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        if (R.k < total_c && count[j] < R.k && R.k <= count[j + 1]) mark(0, j);
+        if (t * kEach + j == m) mark(3, j);
+    }
+    __syncthreads();
+    Found f;
+    f.bin_k = S.found[0], f.bin_m = m;
+    double low = total, high = total;  // that the kept tokens weigh
+    if (f.bin_k >= 0) low = S.found_low[0], high = S.found_high[0];
+    if (R.p < 1.0) {
+        const double x = reached(R.p * low, total), y = reached(R.p * high, total);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            if (weight[j] < x && x <= weight[j + 1]) mark(1, j);
+            if (weight[j] < y && y <= weight[j + 1]) mark(2, j);
+        }
+    }
+    __syncthreads();
+    f.low_p = S.found[1], f.high_p = S.found[2];
+    int end = f.bin_k >= 0 ? f.bin_k : kBins - 1;
+    if (f.high_p >= 0) {
+        low = fmin(low, f.low_p >= 0 ? S.found_low[1] : 0.0), high = fmin(high, S.found_high[2]);
+        end = f.high_p < end ? f.high_p : end;
+    }
+    if (m >= 0) {
+        low = fmin(low, S.found_low[3]), high = fmin(high, S.found_high[3]);
+        if (m > end) f.bin_m = -1;  // min_p ends no prefix
+        else end = m;
+    }
+    const double x = R.u * low, y = R.u * high;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        if (weight[j] <= x && x < weight[j + 1]) mark(4, j);
+        if (weight[j] <= y && y < weight[j + 1]) mark(5, j);
+    }
+    __syncthreads();
+    f.low_u = S.found[4] < 0 ? 0 : S.found[4];
+    f.high_u = S.found[5] < 0 ? end : S.found[5];
+    f.last = f.bin_k > f.high_p ? f.bin_k : f.high_p;
+    f.last = f.high_u > f.last ? f.high_u : f.last;
+    f.last = f.bin_m > f.last ? f.bin_m : f.last;
+    return f;
+}
+
+// The tokens of those bins among logits thread, thread + threads, .. into the
+// words, which hold kList of them; S.n counts all. Their logits lie in four spans at most, which
+// are tested a piece at a time and first: a place takes ten times as long.
+template <typename L>
+__device__ __forceinline__ void gather(Shared& S, const typename L::Element* row, int n, int thread, int threads, const Places<L>& P, const Found& f) {
+    Spans spans{};
+    auto add = [&](int first, int to) {
+        float low, high;
+        P.span(first, to, low, high);
+        spans.add(low, high);
+    };
+    add(f.low_u, f.high_u);
+    if (f.high_p >= 0) add(f.low_p < 0 ? 0 : f.low_p, f.high_p);
+    if (f.bin_k >= 0) add(f.bin_k, f.bin_k);
+    if (f.bin_m >= 0) add(f.bin_m, f.bin_m);
+    auto take = [&](auto number) {
+        constexpr int kSpans = decltype(number)::value;
+        each_piece<L>(row, n, thread, threads, [&](int i, const auto& x) {
+            constexpr int kPiece = static_cast<int>(sizeof(x) / sizeof(float));
+            if (!spans.template any<kSpans>(x)) return;
+            uint32_t hits = 0;
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) hits |= spans.template holds<kSpans>(x[e]) ? 1u << e : 0u;
+            while (hits != 0) {
+                const int e = __builtin_ctz(hits);
+                hits &= hits - 1;
+                float v = x[0];
+#pragma unroll
+                for (int j = 1; j < kPiece; ++j) v = e == j ? x[j] : v;
+                const Place place = P.of(v);
+                if (!(place.t < f.last + 1 && f.wanted(place.bin()))) continue;
+                const int at = atomicAdd(&S.n, 1);
+                if (at < kList) S.words[at] = static_cast<uint64_t>(~key_of(v)) << 32 | static_cast<uint32_t>(i + e);
+            }
+        });
+    };
+    if (spans.n == 1) take(std::integral_constant<int, 1>{});
+    else if (spans.n == 2) take(std::integral_constant<int, 2>{});
+    else take(std::integral_constant<int, 4>{});
 }
 
 // How a prefix ends, or which token is drawn, where a bin holds more tokens
@@ -232,26 +445,22 @@ struct Equals {
 enum Goal { kCounted, kReached, kPassed };
 
 template <typename L, Goal kGoal>
-__device__ Equals narrow(const SampleArgs& A, Shared& S, const typename L::Element* row, const Places& P, int bin, int32_t k, double x) {
+__device__ Equals narrow(const SampleArgs& A, Shared& S, const Sums& B, const typename L::Element* row, const Places<L>& P, int bin, int32_t k, double x) {
     uint32_t low = 0, high = 0xFFFFFFFFu;
-    int32_t count = S.count[bin];
-    double weight = S.weight[bin];
-    const double unit = unit_of(bin);
-    __shared__ int32_t at;
-    __shared__ int32_t before_count, inside_count;
-    __shared__ double before_weight;
-    __shared__ uint64_t inside;
+    int32_t count = B.count[bin];
+    double weight = B.weight[bin];
+    const double unit = S.octave.unit(bin);
     for (;;) {
         int shift = 0;
         while (((high - low) >> shift) >= kBins) ++shift;
         __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += kThreads) S.words[i] = 0;
-        if (threadIdx.x == 0) at = -1;
+        if (threadIdx.x == 0) S.found[0] = -1;
         __syncthreads();
         each_logit<L>(row, A.vocab, threadIdx.x, kThreads, [&](int, float v) {
-            const double t = P.of(v);
+            const Place t = P.of(v);
             const uint32_t key = key_of(v);
-            if (t < kBins && static_cast<int>(t) == bin && key >= low && key <= high)
+            if (t.t < kBins && t.bin() == bin && key >= low && key <= high)
                 atomicAdd(reinterpret_cast<unsigned long long*>(&S.words[(high - key) >> shift]), word_of(t));
         });
         __syncthreads();
@@ -270,28 +479,29 @@ __device__ Equals narrow(const SampleArgs& A, Shared& S, const typename L::Eleme
         for (int j = 0; j < kEach; ++j) {
             const uint64_t one = S.words[threadIdx.x * kEach + j], next = sum + one;
             if (one != 0) {
-                const int32_t c0 = count + static_cast<int32_t>(sum >> kCountShift), c1 = count + static_cast<int32_t>(next >> kCountShift);
-                const double w0 = weight + static_cast<double>(sum & kSumMask) * unit;
+                const int32_t c0 = count + count_of(sum), c1 = count + count_of(next);
+                const double w0 = weight + static_cast<double>(units_of(sum)) * unit;
                 // The last part takes what rounding leaves over.
-                const double w1 = next == total ? INFINITY : weight + static_cast<double>(next & kSumMask) * unit;
+                const double w1 = next == total ? INFINITY : weight + static_cast<double>(units_of(next)) * unit;
                 const bool first = sum == 0;
                 const bool here = kGoal == kCounted ? c0 < k && (k <= c1 || next == total)
                                   : kGoal == kReached ? (first || w0 < x) && x <= w1 : (first || w0 <= x) && x < w1;
-                if (here) at = threadIdx.x * kEach + j, before_count = c0, before_weight = w0, inside = one, inside_count = c1 - c0;
+                if (here) S.found[0] = threadIdx.x * kEach + j, S.before_count = c0, S.found_weight = w0, S.inside = one, S.inside_count = c1 - c0;
             }
             sum = next;
         }
         __syncthreads();
+        const int32_t at = S.found[0];
         if (at < 0) {  // no token of the bin, which no caller asks for
             Equals none{0, count, 0, weight, 0.0};
             return none;
         }
-        count = before_count, weight = before_weight;
+        count = S.before_count, weight = S.found_weight;
         const uint32_t part = static_cast<uint32_t>(at);
         const uint32_t top = high - (part << shift), size = shift == 0 ? 1u : 1u << shift;
         const uint32_t bottom = top - low < size ? low : top - size + 1;
         if (shift == 0) {
-            Equals e{top, count, inside_count, weight, static_cast<double>(inside & kSumMask) / inside_count * unit};
+            Equals e{top, count, S.inside_count, weight, static_cast<double>(units_of(S.inside)) / S.inside_count * unit};
             __syncthreads();
             return e;
         }
@@ -326,54 +536,57 @@ __device__ int32_t index_of(const SampleArgs& A, Shared& S, const typename L::El
 
 // Where a row's prefixes end and its draw falls, one after the other.
 template <typename L>
-__device__ void resolve_large(const SampleArgs& A, Shared& S, const typename L::Element* row, const Places& P, const Rules& R, int bin_k, int bin_m,
-                              int32_t& token, double& weight, double& kept) {
-    int32_t most = S.count[kBins];
-    kept = S.weight[kBins];
+__device__ void resolve_large(const SampleArgs& A, Shared& S, const Sums& B, const typename L::Element* row, const Places<L>& P, const Rules& R,
+                              const Found& f, int32_t& token, double& weight, double& kept) {
+    const int bin_k = f.bin_k, bin_m = f.bin_m;
+    int32_t most = B.count[kBins];
+    kept = B.weight[kBins];
+    // The bin where a weight is reached (weight before < x <= with it) or passed (<=, <).
     auto find = [&](double x, bool passed) {
         __syncthreads();
-        if (threadIdx.x == 0) S.found[0] = -1;
+        if (threadIdx.x == 0) S.found[1] = -1;
         __syncthreads();
-        if (passed) find_weight<true>(S, x, &S.found[0]);
-        else find_weight<false>(S, x, &S.found[0]);
+        for (int b = threadIdx.x; b < kBins; b += kThreads) {
+            const double low = B.weight[b], high = B.weight[b + 1];
+            if (passed ? low <= x && x < high : low < x && x <= high) S.found[1] = b;
+        }
         __syncthreads();
-        return S.found[0];
+        return S.found[1];
     };
     if (bin_k >= 0) {
-        const Equals e = narrow<L, kCounted>(A, S, row, P, bin_k, R.k, 0.0);
+        const Equals e = narrow<L, kCounted>(A, S, B, row, P, bin_k, R.k, 0.0);
         most = R.k;
         kept = e.weight + (R.k - e.count) * e.each;
     }
     if (R.p < 1.0) {
-        double x = R.p * kept;
-        x = x < 1e-300 ? 1e-300 : x > S.weight[kBins] ? S.weight[kBins] : x;
+        const double x = reached(R.p * kept, B.weight[kBins]);
         const int b = find(x, false);
         if (b >= 0) {
-            const Equals e = narrow<L, kReached>(A, S, row, P, b, 0, x);
+            const Equals e = narrow<L, kReached>(A, S, B, row, P, b, 0, x);
             double n = ceil((x - e.weight) / e.each);
             n = n < 1.0 ? 1.0 : n > e.n ? e.n : n;
             if (e.count + static_cast<int32_t>(n) < most) most = e.count + static_cast<int32_t>(n), kept = e.weight + n * e.each;
         }
     }
-    if (bin_m >= 0 && S.count[bin_m] < most) {
+    if (bin_m >= 0 && B.count[bin_m] < most) {
         // The tokens of the bin that weigh enough.
         __syncthreads();
-        if (threadIdx.x == 0) S.sums[0] = 0;
+        if (threadIdx.x == 0) S.inside = 0;
         __syncthreads();
         uint64_t mine = 0;
         each_logit<L>(row, A.vocab, threadIdx.x, kThreads, [&](int, float v) {
-            const double t = P.of(v);
-            if (t < kBins && static_cast<int>(t) == bin_m && t <= R.min_t) mine += word_of(t);
+            const Place t = P.of(v);
+            if (t.t < kBins && t.bin() == bin_m && t.exact() <= R.min_t) mine += word_of(t);
         });
-        if (mine != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&S.sums[0]), mine);
+        if (mine != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&S.inside), mine);
         __syncthreads();
-        const int32_t n = S.count[bin_m] + static_cast<int32_t>(S.sums[0] >> kCountShift);
-        if (n < most) most = n, kept = S.weight[bin_m] + static_cast<double>(S.sums[0] & kSumMask) * unit_of(bin_m);
+        const int32_t n = B.count[bin_m] + count_of(S.inside);
+        if (n < most) most = n, kept = B.weight[bin_m] + static_cast<double>(units_of(S.inside)) * S.octave.unit(bin_m);
     }
     const double x = R.u * kept;
     int b = find(x, true);
-    if (b < 0) b = find(S.weight[kBins], false);
-    const Equals e = narrow<L, kPassed>(A, S, row, P, b < 0 ? 0 : b, 0, x);
+    if (b < 0) b = find(B.weight[kBins], false);
+    const Equals e = narrow<L, kPassed>(A, S, B, row, P, b < 0 ? 0 : b, 0, x);
     double j = floor((x - e.weight) / e.each);
     j = j < 0.0 ? 0.0 : j > e.n - 1 ? e.n - 1 : j;
     if (e.count + j > most - 1) j = most - 1 > e.count ? most - 1 - e.count : 0;
@@ -381,210 +594,227 @@ __device__ void resolve_large(const SampleArgs& A, Shared& S, const typename L::
     weight = e.each;
 }
 
-// A workgroup a row. Bound by the arithmetic on its tokens (64-bit places).
+// The largest logit's key, and of its tokens the first where asked, in one word; 0 where there is none.
 template <typename L>
-__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
-    __shared__ Shared S;
-    const int row_at = blockIdx.x, t = threadIdx.x, wave = t >> 6;
-    const typename L::Element* const row = static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride;
-    const Rules R = rules_of(A, row_at);
-
-    // The largest logit and its first token; the bins are empty meanwhile.
-    for (int i = t; i < kBins; i += kThreads) S.words[i] = 0;
+__device__ __forceinline__ uint64_t largest(const typename L::Element* row, int n, int thread, int threads, bool first) {
     float best = -INFINITY;
-    int32_t best_at = -1;
-    each_logit<L>(row, A.vocab, t, kThreads, [&](int i, float x) {
-        if (x > best || (x == best && i < best_at)) best = x, best_at = i;
-    });
-    uint64_t top = static_cast<uint64_t>(key_of(best)) << 32 | ~static_cast<uint32_t>(best_at);
-    if (best_at < 0) top = 0;
+    int32_t best_at = 0;
+    if (first) {
+        each_logit<L>(row, n, thread, threads, [&](int i, float x) {
+            if (x > best) best = x, best_at = i;
+        });
+    } else {
+        each_logit<L>(row, n, thread, threads, [&](int, float x) { best = fmaxf(best, x); });  // of a number and a NaN: the number
+    }
+    uint64_t top = best == -INFINITY ? 0 : static_cast<uint64_t>(key_of(best)) << 32 | ~static_cast<uint32_t>(best_at);
 #pragma unroll
     for (int x = 1; x < 64; x *= 2) {
         const uint64_t o = __shfl_xor(top, x);
         top = o > top ? o : top;
     }
-    if ((t & 63) == 0) S.wave_best[wave] = top;
-    __syncthreads();
-    for (int i = 0; i < kWaves; ++i) top = S.wave_best[i] > top ? S.wave_best[i] : top;
-    if (top == 0 || R.greedy) {
-        if (t == 0) {
-            A.tokens[row_at] = top == 0 ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(top));
-            if (A.logprobs != nullptr) A.logprobs[row_at] = top == 0 ? -INFINITY : 0.0f;
-        }
-        return;
+    return top;
+}
+
+template <typename L>
+__device__ __forceinline__ Places<L> places_of(uint64_t top, const Rules& R) {
+    // (The same in every lane, which the compiler cannot tell.)
+    const float per = static_cast<float>(R.per);
+    const float x = of_key(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(top >> 32)))));
+    return Places<L>{x, per, static_cast<float>(R.per - per), x == INFINITY};
+}
+
+// Tokens into their bins: kBins words, and one more for each lane, which takes
+// what has no place (a branch around the atomic for each token took twice as
+// long). Without top-p nothing asks for tokens that weigh less than min_p.
+template <typename L>
+__device__ __forceinline__ void fill_bins(const typename L::Element* row, int n, int thread, int threads, const Places<L>& P, const Rules& R, uint64_t* bins) {
+    const float end = R.p < 1.0 || !(R.min_t < kBins - 1) ? kBins : static_cast<float>(static_cast<int>(R.min_t) + 1);
+    const int nowhere = kBins + (threadIdx.x & 63);
+    auto fill = [&](auto place_of) {
+        each_logit<L>(row, n, thread, threads, [&](int, float x) {
+            const Place p = place_of(x);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&bins[p.t < end ? p.bin() : nowhere]), word_of(p));
+        });
+    };
+    if (P.endless) fill([&](float x) { return P.of(x); });
+    else fill([&](float x) { return P.of_finite(x); });
+}
+
+// The sorted tokens' places in the row's order, where its prefixes end, and the
+// draw, by the first wave alone or the workgroup.
+template <bool kWave>
+__device__ __forceinline__ void sync_as() {
+    if constexpr (kWave) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
     }
-    const Places P{static_cast<double>(of_key(static_cast<uint32_t>(top >> 32))), R.per};
+}
 
-    each_logit<L>(row, A.vocab, t, kThreads, [&](int, float x) {
-        const double place = P.of(x);
-        if (place < kBins) atomicAdd(reinterpret_cast<unsigned long long*>(&S.words[static_cast<int>(place)]), word_of(place));
-    });
-    __syncthreads();
-    sum_bins(S);
-
-    // The bins where the prefixes may end (what the first k weigh is known to a
-    // bin, so what p of it is lies in some range) and the draw may fall.
-    const int32_t all = S.count[kBins];
-    if (t < 4) S.found[t] = -1;
-    if (t < 3) S.end_count[t] = INT32_MAX;
-    if (t == 0) S.n = 0, S.drawn = 0;
-    __syncthreads();
-    if (R.k < all) {
+template <bool kWave, typename L>
+__device__ __forceinline__ void finish_as(Shared& S, const Sums& B, uint64_t* sums, const Places<L>& P, const Rules& R, int n, const Found& f, double& kept) {
+    const int t = threadIdx.x, wave = t >> 6;
+    const int32_t all = B.count[kBins];
+    const int bin_k = f.bin_k, bin_m = f.bin_m;
+    auto sync = [] { sync_as<kWave>(); };
+    // Each token's bin, weight and sums before it in its bin.
+    int bin_of[kEach];
+    uint32_t w[kEach];
+    bool weighs[kEach];  // at least min_p
+    int first[kEach];  // of its bin, in the list
+    uint64_t mine = 0, all_sum;
+    int start = -1, previous = -1;
+    if (t * kEach > 0 && t * kEach - 1 < n) previous = P.of(of_key(~static_cast<uint32_t>(S.words[t * kEach - 1] >> 32))).bin();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = t * kEach + j;
+        w[j] = 0, bin_of[j] = 0, first[j] = -1, weighs[j] = false;
+        if (i >= n) continue;
+        const Place place = P.of(of_key(~static_cast<uint32_t>(S.words[i] >> 32)));
+        bin_of[j] = place.bin(), weighs[j] = place.exact() <= R.min_t;
+        w[j] = kUnits - lack_in_bin(place.f);
+        if (bin_of[j] != previous) start = i;
+        first[j] = start, previous = bin_of[j];
+        mine += w[j];
+    }
+    uint64_t sum = before_in_wave(mine, all_sum);
+    // The last start at or before a thread's tokens: starts rise along the list.
+    int starts = start;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+        const int o = __shfl_up(starts, x);
+        if ((t & 63) >= x && o > starts) starts = o;
+    }
+    const int in_wave = __shfl_up(starts, 1);
+    int carried = (t & 63) == 0 ? -1 : in_wave;
+    if ((t & 63) == 63) S.wave_best[wave] = all_sum, S.wave_first[wave] = starts;
+    sync();
+    for (int i = 0; i < wave; ++i) {
+        sum += S.wave_best[i];
+        carried = S.wave_first[i] > carried ? S.wave_first[i] : carried;
+    }
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = t * kEach + j;
+        if (i >= n) break;
+        sums[i] = sum;
+        sum += w[j];
+        if (first[j] < 0) first[j] = carried;
+    }
+    sync();
+    // In the row's order: tokens before it, weights before and with it (the last
+    // of a bin ends where the next begins). Read once: the sums may lie in
+    // global memory.
+    int32_t rank[kEach];
+    double before[kEach], with[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+        const int i = t * kEach + j, bin = bin_of[j];
+        rank[j] = INT32_MAX - 1, before[j] = with[j] = INFINITY;
+        if (i >= n) continue;
+        const int32_t count = B.count[bin], next = B.count[bin + 1];
+        const double base = B.weight[bin], end = B.weight[bin + 1], unit = S.octave.unit(bin);
+        const uint64_t from = sums[i] - sums[first[j]];
+        rank[j] = count + i - first[j];
+        before[j] = base + static_cast<double>(from) * unit;
+        with[j] = rank[j] + 1 == next ? end : base + static_cast<double>(from + w[j]) * unit;
+    }
+    if (bin_k >= 0)
 #pragma unroll
         for (int j = 0; j < kEach; ++j)
-            if (S.count[t * kEach + j] < R.k && R.k <= S.count[t * kEach + j + 1]) S.found[0] = t * kEach + j;
-    }
-    __syncthreads();
-    const int bin_k = S.found[0];
-    const double low_k = bin_k >= 0 ? S.weight[bin_k] : S.weight[kBins], high_k = bin_k >= 0 ? S.weight[bin_k + 1] : S.weight[kBins];
-    auto reached = [&](double x) { return x < 1e-300 ? 1e-300 : x > S.weight[kBins] ? S.weight[kBins] : x; };
+            if (rank[j] == R.k - 1) S.end_count[0] = R.k, S.end_weight[0] = with[j];
+    sync();
     if (R.p < 1.0) {
-        find_weight<false>(S, reached(R.p * low_k), &S.found[1]);
-        find_weight<false>(S, reached(R.p * high_k), &S.found[2]);
+        const double x = reached(R.p * (bin_k >= 0 ? S.end_weight[0] : B.weight[kBins]), B.weight[kBins]);
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+            if (before[j] < x && x <= with[j]) S.end_count[1] = rank[j] + 1, S.end_weight[1] = with[j];
     }
-    __syncthreads();
-    const int low_p = S.found[1], high_p = S.found[2];
-    const int bin_m = R.min_t < kBins ? static_cast<int>(R.min_t) : -1;
-    int low_end = kBins - 1, high_end = kBins - 1;
-    auto ends = [&](int low, int high) {
-        if (high < 0) return;
-        low_end = low < low_end ? low : low_end, high_end = high < high_end ? high : high_end;
-    };
-    ends(bin_k, bin_k), ends(low_p, high_p), ends(bin_m, bin_m);
-    __syncthreads();
-    if (t < 2) S.found[t] = -1;
-    __syncthreads();
-    find_weight<true>(S, R.u * S.weight[low_end], &S.found[0]);
-    find_weight<true>(S, R.u * S.weight[high_end + 1], &S.found[1]);
-    __syncthreads();
-    const int low_u = S.found[0], high_u = S.found[1];
-
-    // Their tokens.
-    auto wanted = [&](int b) {
-        return b == bin_k || (b >= low_p && b <= high_p) || (b == bin_m && bin_m <= high_end) || (b >= low_u && b <= high_u);
-    };
-    int last = bin_k > high_p ? bin_k : high_p;
-    last = high_u > last ? high_u : last;
-    last = bin_m <= high_end && bin_m > last ? bin_m : last;
-    __syncthreads();
-    each_logit<L>(row, A.vocab, t, kThreads, [&](int i, float x) {
-        const double place = P.of(x);
-        if (place < last + 1 && wanted(static_cast<int>(place))) {
-            const int at = atomicAdd(&S.n, 1);
-            if (at < kList) S.words[at] = static_cast<uint64_t>(~key_of(x)) << 32 | static_cast<uint32_t>(i);
+    if (bin_m >= 0) {
+        if (t == 0) S.found[2] = B.count[bin_m];
+        sync();
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+            if (bin_of[j] == bin_m && weighs[j]) atomicMax(&S.found[2], rank[j] + 1);
+        sync();
+        if (t == 0 && S.found[2] == B.count[bin_m]) S.end_count[2] = S.found[2], S.end_weight[2] = B.weight[bin_m];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j)
+            if (bin_of[j] == bin_m && rank[j] + 1 == S.found[2]) S.end_count[2] = S.found[2], S.end_weight[2] = with[j];
+    }
+    if (t == 0) S.found[3] = 0;
+    sync();
+    int32_t most = all;
+    kept = B.weight[kBins];
+    for (int i = 0; i < 3; ++i)
+        if (S.end_count[i] < most) most = S.end_count[i], kept = S.end_weight[i];
+    const double x = R.u * kept;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+        if (rank[j] < most && before[j] <= x) atomicMax(&S.found[3], rank[j] + 1);
+    sync();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+        if (rank[j] + 1 == S.found[3]) {
+            S.drawn = static_cast<int32_t>(static_cast<uint32_t>(S.words[t * kEach + j]));
+            S.found_weight = static_cast<double>(w[j]) * S.octave.unit(bin_of[j]);
         }
-    });
-    __syncthreads();
-    const int n = S.n;
+    sync();
+}
+
+// The token, from the S.n gathered ones in the words. sums: room for kList numbers in LDS.
+template <typename L>
+__device__ __forceinline__ void finish(const SampleArgs& A, Shared& S, const Sums& B, uint64_t* sums, const typename L::Element* row, int row_at,
+                                       const Places<L>& P, const Rules& R, const Found& f, int n) {
+    const int t = threadIdx.x;
+    if (t < 3) S.end_count[t] = INT32_MAX;
     int32_t token = -1;
     double weight = 0.0, kept = 0.0;
-    if (n > kList || n == 0) {
-        resolve_large<L>(A, S, row, P, R, bin_k, bin_m, token, weight, kept);
+    if (n > kList || n < 1) {
+        resolve_large<L>(A, S, B, row, P, R, f, token, weight, kept);
     } else {
         int size = 64;
         while (size < n) size *= 2;
-        for (int i = n + t; i < size; i += kThreads) S.words[i] = ~uint64_t{0};
-        __syncthreads();
-        for (int span = 2; span <= size; span *= 2)
-            for (int gap = span / 2; gap > 0; gap /= 2) {
-                for (int i = t; i < size / 2; i += kThreads) {
-                    const int a = 2 * i - (i & (gap - 1)), b = a + gap;
-                    const uint64_t x = S.words[a], y = S.words[b];
-                    if ((x > y) == ((a & span) == 0)) S.words[a] = y, S.words[b] = x;
+        if (size <= kFew) {
+            // Few: a token's rank is the number of those before it, counted by kThreads / size threads for each.
+            const int e = t & (size - 1), parts = kThreads / size, part = t / size;
+            const uint64_t mine = e < n ? S.words[e] : 0;
+            if (t < size) S.rank[t] = 0;
+            __syncthreads();
+            int32_t rank = 0;
+            for (int i = part; i < n; i += 8 * parts) {  // eight reads on their way together
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int at = i + j * parts;
+                    const uint64_t other = S.words[at & (kList - 1)];
+                    rank += (at < n) & (other < mine) ? 1 : 0;
                 }
-                __syncthreads();
             }
-        // Each token's bin, weight and sums before it in its bin.
-        double place[kEach];
-        uint32_t w[kEach];
-        int first[kEach];  // of its bin, in the list
-        uint64_t mine = 0, all_sum;
-        int start = -1, previous = -1;
-        if (t * kEach > 0 && t * kEach - 1 < n) previous = static_cast<int>(P.of(of_key(~static_cast<uint32_t>(S.words[t * kEach - 1] >> 32))));
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int i = t * kEach + j;
-            w[j] = 0, place[j] = 0.0, first[j] = -1;
-            if (i >= n) continue;
-            place[j] = P.of(of_key(~static_cast<uint32_t>(S.words[i] >> 32)));
-            const int bin = static_cast<int>(place[j]);
-            w[j] = weight_in_bin(static_cast<float>(place[j] - bin));
-            if (bin != previous) start = i;
-            first[j] = start, previous = bin;
-            mine += w[j];
-        }
-        uint64_t sum = before_in_wave(mine, all_sum);
-        // The last start at or before a thread's tokens: starts rise along the list.
-        int starts = start;
-#pragma unroll
-        for (int x = 1; x < 64; x *= 2) {
-            const int o = __shfl_up(starts, x);
-            if ((t & 63) >= x && o > starts) starts = o;
-        }
-        const int in_wave = __shfl_up(starts, 1);
-        int carried = (t & 63) == 0 ? -1 : in_wave;
-        if ((t & 63) == 63) S.wave_best[wave] = all_sum, S.wave_first[wave] = starts;
-        __syncthreads();
-        for (int i = 0; i < wave; ++i) {
-            sum += S.wave_best[i];
-            carried = S.wave_first[i] > carried ? S.wave_first[i] : carried;
-        }
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const int i = t * kEach + j;
-            if (i >= n) break;
-            S.sums[i] = sum;
-            sum += w[j];
-            if (first[j] < 0) first[j] = carried;
-        }
-        __syncthreads();
-        // In the row's order: tokens before it, weights before and with it (the last of a bin ends where the next begins).
-        auto before = [&](int j) {
-            const int bin = static_cast<int>(place[j]);
-            return S.weight[bin] + static_cast<double>(S.sums[t * kEach + j] - S.sums[first[j]]) * unit_of(bin);
-        };
-        auto with = [&](int j) {
-            const int i = t * kEach + j, bin = static_cast<int>(place[j]);
-            if (S.count[bin] + i - first[j] + 1 == S.count[bin + 1]) return S.weight[bin + 1];
-            return S.weight[bin] + static_cast<double>(S.sums[i] - S.sums[first[j]] + w[j]) * unit_of(bin);
-        };
-        auto rank = [&](int j) { return S.count[static_cast<int>(place[j])] + t * kEach + j - first[j]; };
-        const int mine_n = n - t * kEach < kEach ? n - t * kEach : kEach;
-        if (bin_k >= 0)
-            for (int j = 0; j < mine_n; ++j)
-                if (rank(j) == R.k - 1) S.end_count[0] = R.k, S.end_weight[0] = with(j);
-        __syncthreads();
-        if (R.p < 1.0) {
-            const double x = reached(R.p * (bin_k >= 0 ? S.end_weight[0] : S.weight[kBins]));
-            for (int j = 0; j < mine_n; ++j)
-                if (before(j) < x && x <= with(j)) S.end_count[1] = rank(j) + 1, S.end_weight[1] = with(j);
-        }
-        if (bin_m >= 0 && bin_m <= high_end) {
-            if (t == 0) S.found[2] = S.count[bin_m];
+            if (e < n && rank > 0) atomicAdd(&S.rank[e], rank);
             __syncthreads();
-            for (int j = 0; j < mine_n; ++j)
-                if (static_cast<int>(place[j]) == bin_m && place[j] <= R.min_t) atomicMax(&S.found[2], rank(j) + 1);
+            if (t < n) S.words[S.rank[t]] = mine;
             __syncthreads();
-            if (t == 0 && S.found[2] == S.count[bin_m]) S.end_count[2] = S.found[2], S.end_weight[2] = S.weight[bin_m];
-            for (int j = 0; j < mine_n; ++j)
-                if (static_cast<int>(place[j]) == bin_m && rank(j) + 1 == S.found[2]) S.end_count[2] = S.found[2], S.end_weight[2] = with(j);
+        } else {
+            for (int i = n + t; i < size; i += kThreads) S.words[i] = ~uint64_t{0};
+            __syncthreads();
+            for (int span = 2; span <= size; span *= 2)
+                for (int gap = span / 2; gap > 0; gap /= 2) {
+                    for (int i = t; i < size / 2; i += kThreads) {
+                        const int a = 2 * i - (i & (gap - 1)), b = a + gap;
+                        const uint64_t x = S.words[a], y = S.words[b];
+                        if ((x > y) == ((a & span) == 0)) S.words[a] = y, S.words[b] = x;
+                    }
+                    __syncthreads();
+                }
         }
-        if (t == 0) S.found[3] = 0;
-        __syncthreads();
-        int32_t most = all;
-        kept = S.weight[kBins];
-        for (int i = 0; i < 3; ++i)
-            if (S.end_count[i] < most) most = S.end_count[i], kept = S.end_weight[i];
-        const double x = R.u * kept;
-        for (int j = 0; j < mine_n; ++j)
-            if (rank(j) < most && before(j) <= x) atomicMax(&S.found[3], rank(j) + 1);
-        __syncthreads();
-        for (int j = 0; j < mine_n; ++j)
-            if (rank(j) + 1 == S.found[3]) {
-                S.drawn = static_cast<int32_t>(static_cast<uint32_t>(S.words[t * kEach + j]));
-                S.found_weight = static_cast<double>(w[j]) * unit_of(static_cast<int>(place[j]));
-            }
-        __syncthreads();
+        // A wave alone needs no barriers.
+        if (n <= 64 * kEach) {
+            if (t >= 64) return;
+            finish_as<true, L>(S, B, sums, P, R, n, f, kept);
+        } else {
+            finish_as<false, L>(S, B, sums, P, R, n, f, kept);
+        }
         token = S.drawn, weight = S.found_weight;
     }
     if (t == 0) {
@@ -593,15 +823,228 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
     }
 }
 
+// A row without tokens, or whose largest logit decides.
+__device__ __forceinline__ bool decided(const SampleArgs& A, int row_at, uint64_t top, const Rules& R, bool writes) {
+    if (top != 0 && !R.greedy) return false;
+    if (writes) {
+        A.tokens[row_at] = top == 0 ? -1 : static_cast<int64_t>(~static_cast<uint32_t>(top));
+        if (A.logprobs != nullptr) A.logprobs[row_at] = top == 0 ? -INFINITY : 0.0f;
+    }
+    return true;
+}
+
+__device__ __forceinline__ void clear(Shared& S) {
+    S.octave.make();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) S.words[i] = 0;
+    if (threadIdx.x == 0) S.n = 0, S.drawn = 0;
+}
+
+__device__ __forceinline__ uint64_t largest_of_waves(Shared& S, uint64_t top) {
+    if ((threadIdx.x & 63) == 0) S.wave_best[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) top = S.wave_best[i] > top ? S.wave_best[i] : top;
+    return top;
+}
+
+// Many rows, or few logits: a workgroup a row.
+template <typename L>
+__global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
+    __shared__ Shared S;
+    __shared__ double weight[kBins + 1];
+    __shared__ int32_t count[kBins + 1];
+    __shared__ uint64_t sums[kList];
+    Sums B;
+    B.weight = weight, B.count = count;
+    const int row_at = blockIdx.x;
+    const typename L::Element* const row = static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride;
+    const Rules R = rules_of(A, row_at);
+    clear(S);
+    const uint64_t top = largest_of_waves(S, largest<L>(row, A.vocab, threadIdx.x, kThreads, R.greedy));
+    if (decided(A, row_at, top, R, threadIdx.x == 0)) return;
+    const Places<L> P = places_of<L>(top, R);
+    fill_bins<L>(row, A.vocab, threadIdx.x, kThreads, P, R, S.words);
+    __syncthreads();
+    const Found f = find_bins(S, R, B);
+    gather<L>(S, row, A.vocab, threadIdx.x, kThreads, P, f);
+    __syncthreads();
+    finish<L>(A, S, B, sums, row, row_at, P, R, f, S.n);
+}
+
+// Fewer rows: `n` workgroups a row, in four launches: the largest logit; the
+// bins; their tokens; by one workgroup, the draw. (Fewer, where the last
+// workgroup of a row to come goes on with what the others wrote, need fences
+// over all L2s: 64 rows 290 us.)
+struct Slices {
+    uint64_t* tops;      // [rows][n]
+    uint64_t* bins;      // [rows][kBins]
+    double* weight;      // [rows][kBins + 1]
+    uint64_t* list;      // [rows][kList]
+    Rules* rules;        // [rows]
+    Found* found;        // [rows]
+    int32_t* count;      // [rows][kBins + 1]
+    int32_t* gathered;   // [rows]
+    int32_t n;
+
+    __device__ __forceinline__ Sums sums(int row) const {
+        return Sums{weight + static_cast<int64_t>(row) * (kBins + 1), count + static_cast<int64_t>(row) * (kBins + 1)};
+    }
+};
+
+// (A row has at most 64 slices.)
+__device__ __forceinline__ uint64_t top_of(const Slices& W, int row) {
+    const int lane = threadIdx.x & 63;
+    uint64_t top = W.tops[static_cast<int64_t>(row) * W.n + (lane < W.n ? lane : 0)];
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+        const uint64_t o = __shfl_xor(top, x);
+        top = o > top ? o : top;
+    }
+    return top;
+}
+
+template <typename L>
+__global__ __launch_bounds__(kThreads) void sample_top_kernel(const SampleArgs A, const Slices W) {
+    __shared__ uint64_t best[kWaves];
+    const int row_at = blockIdx.y, t = threadIdx.x;
+    for (int i = blockIdx.x * kThreads + t; i < kBins; i += W.n * kThreads) W.bins[static_cast<int64_t>(row_at) * kBins + i] = 0;
+    if (blockIdx.x == 0 && t == 0) W.gathered[row_at] = 0, W.rules[row_at] = rules_of(A, row_at);
+    uint64_t top = largest<L>(static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride, A.vocab, blockIdx.x * kThreads + t,
+                              W.n * kThreads, greedy(A, row_at));
+    if ((t & 63) == 0) best[t >> 6] = top;
+    __syncthreads();
+    for (int i = 0; i < kWaves; ++i) top = best[i] > top ? best[i] : top;
+    if (t == 0) W.tops[static_cast<int64_t>(row_at) * W.n + blockIdx.x] = top;
+}
+
+template <typename L>
+__global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs A, const Slices W) {
+    __shared__ uint64_t words[kBins + 64];
+    const int row_at = blockIdx.y, t = threadIdx.x;
+    const typename L::Element* const row = static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride;
+    const Rules R = W.rules[row_at];
+    const uint64_t top = top_of(W, row_at);
+    if (decided(A, row_at, top, R, blockIdx.x == 0 && t == 0)) return;
+    for (int i = t; i < kBins; i += kThreads) words[i] = 0;
+    __syncthreads();
+    fill_bins<L>(row, A.vocab, blockIdx.x * kThreads + t, W.n * kThreads, places_of<L>(top, R), R, words);
+    __syncthreads();
+    uint64_t* const bins = W.bins + static_cast<int64_t>(row_at) * kBins;
+    for (int i = t; i < kBins; i += kThreads)
+        if (words[i] != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&bins[i]), words[i]);
+}
+
+// (Each workgroup looks at the bins for itself: a launch for that took 4 us more.)
+template <typename L>
+__global__ __launch_bounds__(kThreads) void sample_gather_kernel(const SampleArgs A, const Slices W) {
+    __shared__ Shared S;
+    const int row_at = blockIdx.y, t = threadIdx.x;
+    const typename L::Element* const row = static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride;
+    const Rules R = W.rules[row_at];
+    const uint64_t top = top_of(W, row_at);
+    if (decided(A, row_at, top, R, false)) return;
+    S.octave.make();
+    for (int i = t; i < kBins; i += kThreads) S.words[i] = W.bins[static_cast<int64_t>(row_at) * kBins + i];
+    if (t == 0) S.n = 0;
+    __syncthreads();
+    const Found f = find_bins(S, R, blockIdx.x == 0 ? W.sums(row_at) : Sums{nullptr, nullptr});
+    if (blockIdx.x == 0 && t == 0) W.found[row_at] = f;
+    gather<L>(S, row, A.vocab, blockIdx.x * kThreads + t, W.n * kThreads, places_of<L>(top, R), f);
+    __syncthreads();
+    // Its tokens to the row's.
+    uint64_t* const list = W.list + static_cast<int64_t>(row_at) * kList;
+    const int32_t n = S.n;
+    if (n == 0) return;
+    if (t == 0) S.rank[0] = atomicAdd(&W.gathered[row_at], n);
+    __syncthreads();
+    const int32_t at = S.rank[0];
+    for (int i = t; i < n && i < kList && at + i < kList; i += kThreads) list[at + i] = S.words[i];
+}
+
+template <typename L>
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs A, const Slices W) {
+    __shared__ Shared S;
+    __shared__ uint64_t sums[kList];
+    const int row_at = blockIdx.x, t = threadIdx.x;
+    const typename L::Element* const row = static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride;
+    const Rules R = W.rules[row_at];
+    const uint64_t top = top_of(W, row_at);
+    if (decided(A, row_at, top, R, false)) return;
+    const int32_t n = W.gathered[row_at];
+    S.octave.make();
+    for (int i = t; i < n && i < kList; i += kThreads) S.words[i] = W.list[static_cast<int64_t>(row_at) * kList + i];
+    __syncthreads();
+    finish<L>(A, S, W.sums(row_at), sums, row, row_at, places_of<L>(top, R), R, W.found[row_at], n);
+}
+
 }  // namespace
 }  // namespace aimg
 
+namespace aimg {
+namespace {
+
+// Workgroups a row; 0: one, in one launch. Logits that one workgroup reads as
+// fast as four launches follow each other (32000 of bf16: 29 us, 32 dealt out;
+// 50001: 35, 33; 151936: 54, 33), and rows that fill the card (256 rows of
+// 151936: 87 us, 99; 128: 85, 78), are not dealt out. Otherwise 512 in all: 64
+// rows in 8 each 58 us, in 4 61, in 16 65.
+int slices_of(int64_t n_rows, int vocab) {
+    if (n_rows < 1 || n_rows >= 192 || vocab < 40000) return 0;
+    const int64_t most = (vocab + 8191) / 8192, n = 512 / n_rows;
+    return static_cast<int>(n < 4 ? 4 : n < most ? n : most);
+}
+
+// Where a call's arrays lie in its workspace, those of 8 bytes first; returns its size.
+size_t slices_at(Slices& w, char* at, int64_t rows) {
+    const size_t tops = 8 * static_cast<size_t>(rows) * w.n, bins = 8 * static_cast<size_t>(rows) * kBins, weight = 8 * static_cast<size_t>(rows) * (kBins + 1);
+    const size_t list = 8 * static_cast<size_t>(rows) * kList, rules = sizeof(Rules) * rows, found = sizeof(Found) * rows, count = 4 * static_cast<size_t>(rows) * (kBins + 1);
+    w.tops = reinterpret_cast<uint64_t*>(at), w.bins = reinterpret_cast<uint64_t*>(at + tops), w.weight = reinterpret_cast<double*>(at + tops + bins);
+    w.list = reinterpret_cast<uint64_t*>(at + tops + bins + weight), w.rules = reinterpret_cast<Rules*>(at + tops + bins + weight + list);
+    at += tops + bins + weight + list + rules;
+    w.found = reinterpret_cast<Found*>(at), w.gathered = reinterpret_cast<int32_t*>(at + found);
+    w.count = reinterpret_cast<int32_t*>(at + found + 4 * rows);
+    return tops + bins + weight + list + rules + found + 4 * rows + count;
+}
+
+template <typename L>
+void launch_sample(const SampleArgs& a, int64_t n_rows, const Slices& w, hipStream_t s) {
+    const dim3 rows(static_cast<uint32_t>(n_rows)), slices(static_cast<uint32_t>(w.n), static_cast<uint32_t>(n_rows)), block(kThreads);
+    if (w.n == 0) {
+        hipLaunchKernelGGL((sample_kernel<L>), rows, block, 0, s, a);
+        return;
+    }
+    hipLaunchKernelGGL((sample_top_kernel<L>), slices, block, 0, s, a, w);
+    hipLaunchKernelGGL((sample_bins_kernel<L>), slices, block, 0, s, a, w);
+    hipLaunchKernelGGL((sample_gather_kernel<L>), slices, block, 0, s, a, w);
+    hipLaunchKernelGGL((sample_draw_kernel<L>), rows, block, 0, s, a, w);
+}
+
+int check_sample(int64_t n_rows, int vocab) {
+    if (n_rows < 0 || n_rows > INT32_MAX || vocab < 1) return fail(AIMG_ERR_INVALID_ARGUMENT, "sample: n_rows must be in 0..2^31-1 and vocab at least 1");
+    if (vocab > kMaxVocab) return fail(AIMG_ERR_UNSUPPORTED, "sample: vocab must be at most 2^18");
+    return AIMG_OK;
+}
+
+}  // namespace
+}  // namespace aimg
+
+extern "C" int aimg_sample_workspace_nbytes(int64_t n_rows, int vocab, size_t* nbytes) {
+    if (nbytes == nullptr) return aimg::fail(AIMG_ERR_INVALID_ARGUMENT, "nbytes is null");
+    const int rc = aimg::check_sample(n_rows, vocab);
+    if (rc != AIMG_OK) return rc;
+    aimg::Slices w{};
+    w.n = aimg::slices_of(n_rows, vocab);
+    *nbytes = w.n == 0 ? 0 : aimg::slices_at(w, nullptr, n_rows);
+    return AIMG_OK;
+}
+
 extern "C" int aimg_sample(const void* logits, int64_t n_rows, int64_t row_stride, int vocab, int type, const float* uniforms,
-                           const aimg_sampling* settings, int64_t* tokens, float* logprobs, void* stream) {
+                           const aimg_sampling* settings, int64_t* tokens, float* logprobs, void* workspace, size_t workspace_nbytes,
+                           void* stream) {
     using aimg::fail;
-    if (n_rows < 0 || n_rows > INT32_MAX || vocab < 1 || row_stride < 0)
-        return fail(AIMG_ERR_INVALID_ARGUMENT, "sample: n_rows must be in 0..2^31-1, vocab at least 1 and row_stride not negative");
-    if (vocab > aimg::kMaxVocab) return fail(AIMG_ERR_UNSUPPORTED, "sample: vocab must be at most 2^18");
+    const int rc = aimg::check_sample(n_rows, vocab);
+    if (rc != AIMG_OK) return rc;
+    if (row_stride < 0) return fail(AIMG_ERR_INVALID_ARGUMENT, "sample: row_stride must not be negative");
     if (type != AIMG_BF16 && type != AIMG_FP16 && type != AIMG_FP32)
         return fail(AIMG_ERR_UNSUPPORTED, "sample: type must be AIMG_BF16, AIMG_FP16 or AIMG_FP32, got " + std::to_string(type));
     if (settings == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "sample: settings is null");
@@ -609,16 +1052,20 @@ extern "C" int aimg_sample(const void* logits, int64_t n_rows, int64_t row_strid
     if (logits == nullptr || uniforms == nullptr || tokens == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "sample: null pointer");
     if (reinterpret_cast<uintptr_t>(logits) % (type == AIMG_FP32 ? 4 : 2) != 0 || reinterpret_cast<uintptr_t>(tokens) % 8 != 0)
         return fail(AIMG_ERR_UNSUPPORTED, "sample: logits and tokens must be aligned to their elements");
+    aimg::Slices w{};
+    w.n = aimg::slices_of(n_rows, vocab);
+    if (w.n > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 8 != 0 ||
+                    workspace_nbytes < aimg::slices_at(w, static_cast<char*>(workspace), n_rows)))
+        return fail(AIMG_ERR_INVALID_ARGUMENT, "the workspace is null, misaligned or below aimg_sample_workspace_nbytes");
     aimg::SampleArgs a{};
     a.logits = logits, a.row_stride = row_stride, a.uniforms = uniforms, a.vocab = vocab;
     a.temperatures = settings->temperatures, a.top_ks = settings->top_ks, a.top_ps = settings->top_ps, a.min_ps = settings->min_ps;
     a.temperature = settings->temperature, a.top_k = settings->top_k, a.top_p = settings->top_p, a.min_p = settings->min_p;
     a.tokens = tokens, a.logprobs = logprobs;
-    const dim3 grid(static_cast<uint32_t>(n_rows)), block(aimg::kThreads);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (type == AIMG_BF16) hipLaunchKernelGGL((aimg::sample_kernel<aimg::LogitBf16>), grid, block, 0, s, a);
-    else if (type == AIMG_FP16) hipLaunchKernelGGL((aimg::sample_kernel<aimg::LogitFp16>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((aimg::sample_kernel<aimg::LogitFp32>), grid, block, 0, s, a);
+    if (type == AIMG_BF16) aimg::launch_sample<aimg::LogitBf16>(a, n_rows, w, s);
+    else if (type == AIMG_FP16) aimg::launch_sample<aimg::LogitFp16>(a, n_rows, w, s);
+    else aimg::launch_sample<aimg::LogitFp32>(a, n_rows, w, s);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return fail(AIMG_ERR_HIP, std::string("kernel launch failed: ") + hipGetErrorString(err));
     return AIMG_OK;

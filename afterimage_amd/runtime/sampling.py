@@ -10,6 +10,9 @@ where a child is accepted if it is its parent's drawn token.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+
 import torch
 
 from .. import _native
@@ -24,6 +27,13 @@ def _vector(x: torch.Tensor, name: str, dtype: torch.dtype, rows: int, index: in
     if x.dtype is not dtype or x.shape != (rows,) or x.get_device() != index or not x.is_contiguous():
         raise ValueError("%s must be a contiguous %s [%d] tensor on cuda:%d" % (name, dtype, rows, index))
     return x.data_ptr()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_nbytes(rows: int, vocab: int) -> int:
+    nbytes = ctypes.c_size_t(0)
+    _native.check(_native.lib().aimg_sample_workspace_nbytes(rows, vocab, ctypes.byref(nbytes)))
+    return nbytes.value
 
 
 def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
@@ -70,6 +80,9 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float |
         out = torch.empty(rows, dtype=torch.int64, device=logits.device)
     out_at = _vector(out, "out", torch.int64, rows, index)
     logs = torch.empty(rows, dtype=torch.float32, device=logits.device) if logprobs else None
+    nbytes = _workspace_nbytes(rows, vocab)
+    # Held until the launches are made, from torch's allocator on the current stream.
+    work = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
     launch(_native.lib().aimg_sample, index, logits.data_ptr(), rows, logits.stride(0), vocab, kind, uniforms_at, settings, out_at,
-           logs.data_ptr() if logprobs else None)
+           logs.data_ptr() if logprobs else None, work.data_ptr() if nbytes else None, nbytes)
     return (out, logs) if logprobs else out

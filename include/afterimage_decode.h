@@ -567,9 +567,13 @@ typedef struct aimg_sampling {
  * NaN are no tokens; a row without any other gives -1 and -inf. Weights below
  * 2^-64 of the largest count as nothing, the others are sums of 2^-26 of
  * themselves, in integers and doubles: results do not vary between calls.
+ * aimg_sample_workspace_nbytes gives the device scratch memory a call needs
+ * (8-byte aligned; 0 for many rows or few logits): few rows are dealt out.
  */
+int aimg_sample_workspace_nbytes(int64_t n_rows, int vocab, size_t* nbytes);
 int aimg_sample(const void* logits, int64_t n_rows, int64_t row_stride, int vocab, int type, const float* uniforms,
-                const aimg_sampling* settings, int64_t* tokens, float* logprobs, void* stream);
+                const aimg_sampling* settings, int64_t* tokens, float* logprobs, void* workspace, size_t workspace_nbytes,
+                void* stream);
 
 #ifdef __cplusplus
 }

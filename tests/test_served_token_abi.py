@@ -60,7 +60,7 @@ def test_nothing_to_do_is_no_error():
     for entry in (lib.aimg_cache8_fork, ):
         assert entry(_cache(), AT, AT, AT, 0, None, 0, None) == OK
     assert lib.aimg_cache8_commit(_cache(), AT, AT, AT, 4, AT, 0, AT, None) == OK
-    assert lib.aimg_sample(None, 0, 10, 10, 0, None, _native.AimgSampling(), None, None, None) == OK
+    assert lib.aimg_sample(None, 0, 10, 10, 0, None, _native.AimgSampling(), None, None, None, 0, None) == OK
     assert _tree8(n=0) == OK
 
 
@@ -115,11 +115,13 @@ def test_attention_over_eight_bits_refuses(args, code, message):
     (dict(rows=-1), BAD, b"n_rows"), (dict(vocab=0), BAD, b"vocab"), (dict(vocab=(1 << 18) + 1), UNSUPPORTED, b"2^18"), (dict(stride=-1), BAD, b"row_stride"),
     (dict(kind=3), UNSUPPORTED, b"type"), (dict(logits=None), BAD, b"null"), (dict(uniforms=None), BAD, b"null"), (dict(tokens=None), BAD, b"null"),
     (dict(settings=None), BAD, b"settings"), (dict(logits=AT + 1), UNSUPPORTED, b"aligned"), (dict(tokens=AT + 4), UNSUPPORTED, b"aligned"),
-    (dict(logits=AT + 2, kind=2), UNSUPPORTED, b"aligned"),
+    (dict(logits=AT + 2, kind=2), UNSUPPORTED, b"aligned"), (dict(vocab=100000), BAD, b"workspace"), (dict(vocab=100000, work=AT, nbytes=100), BAD, b"workspace"),
+    (dict(vocab=100000, work=AT + 4, nbytes=1 << 20), BAD, b"workspace"),
 ])
 def test_sample_refuses(args, code, message):
-    a = dict(logits=AT, rows=2, stride=10, vocab=10, kind=0, uniforms=AT, settings=_native.AimgSampling(), tokens=AT) | args
-    assert _native.lib().aimg_sample(a["logits"], a["rows"], a["stride"], a["vocab"], a["kind"], a["uniforms"], a["settings"], a["tokens"], None, None) == code
+    a = dict(logits=AT, rows=2, stride=10, vocab=10, kind=0, uniforms=AT, settings=_native.AimgSampling(), tokens=AT, work=None, nbytes=0) | args
+    assert _native.lib().aimg_sample(a["logits"], a["rows"], a["stride"], a["vocab"], a["kind"], a["uniforms"], a["settings"], a["tokens"], None, a["work"], a["nbytes"],
+                                     None) == code
     assert message in _native.lib().aimg_last_error()
 
 
