@@ -35,7 +35,6 @@ constexpr int kPerOctave = 64;             // bins of a factor of 2
 constexpr int kBins = 4096;
 constexpr int kEach = kBins / kThreads;    // bins, and sorted tokens, of a thread
 constexpr int kList = 4096;                // tokens that are gathered and sorted
-constexpr int kFew = 512;             // so many are sorted by counting
 constexpr int kCountShift = 45;            // of a bin's word: count above; below, what its tokens lack to the weight of its top, in 2^-26 of that
 constexpr uint64_t kLackMask = (uint64_t{1} << kCountShift) - 1;
 constexpr int kMaxVocab = 1 << 18;         // so that neither overflows
@@ -289,7 +288,7 @@ struct Shared {
     double found_low[6], found_high[6], end_weight[3], found_weight;
     int32_t found[6], end_count[3], n, drawn, before_count, inside_count;
     uint64_t inside;
-    int32_t rank[kFew];
+    int32_t at;
 };
 
 // Tokens and weights before each bin, and of all: [kBins + 1].
@@ -309,7 +308,9 @@ struct Found {
 
 __device__ __forceinline__ double reached(double x, double all) { return x < 1e-300 ? 1e-300 : x > all ? all : x; }
 
-// The words' sums (into `to`, where it is not null) and those bins, by a workgroup.
+// The words' sums and those bins, by a workgroup. `to` (where not null) takes the
+// sums: of all bins, or of those wanted alone.
+template <bool kAll>
 __device__ __forceinline__ Found find_bins(Shared& S, const Rules& R, const Sums& to) {
     const int t = threadIdx.x, wave = t >> 6;
     int32_t count[kEach + 1], all_c, my_c = 0;
@@ -339,11 +340,11 @@ __device__ __forceinline__ Found find_bins(Shared& S, const Rules& R, const Sums
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-        if (to.count != nullptr) to.count[t * kEach + j] = count[j], to.weight[t * kEach + j] = weight[j];
+        if (kAll) to.count[t * kEach + j] = count[j], to.weight[t * kEach + j] = weight[j];
         count[j + 1] += count[j];
         weight[j + 1] = j + 1 < kEach ? weight[j] + weight[j + 1] : S.start[t + 1];  // where the next thread begins
     }
-    if (t == 0 && to.count != nullptr) to.count[kBins] = total_c, to.weight[kBins] = total;
+    if (kAll && t == 0) to.count[kBins] = total_c, to.weight[kBins] = total;
     auto mark = [&](int i, int j) { S.found[i] = t * kEach + j, S.found_low[i] = weight[j], S.found_high[i] = weight[j + 1]; };
     const int m = R.min_t < kBins ? static_cast<int>(R.min_t) : -1;
 #pragma unroll
@@ -388,6 +389,17 @@ __device__ __forceinline__ Found find_bins(Shared& S, const Rules& R, const Sums
     f.last = f.bin_k > f.high_p ? f.bin_k : f.high_p;
     f.last = f.high_u > f.last ? f.high_u : f.last;
     f.last = f.bin_m > f.last ? f.bin_m : f.last;
+    if (!kAll && to.count != nullptr) {
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const int b = t * kEach + j;
+            if (!f.wanted(b)) continue;
+            to.count[b] = count[j], to.weight[b] = weight[j];
+            to.count[b + 1] = count[j + 1], to.weight[b + 1] = weight[j + 1];
+        }
+        __syncthreads();  // the total's place follows the last bin's
+        if (t == 0) to.count[kBins] = total_c, to.weight[kBins] = total;
+    }
     return f;
 }
 
@@ -652,23 +664,23 @@ __device__ __forceinline__ void sync_as() {
     }
 }
 
-template <bool kWave, typename L>
+template <bool kWave, int kMine, typename L>
 __device__ __forceinline__ void finish_as(Shared& S, const Sums& B, uint64_t* sums, const Places<L>& P, const Rules& R, int n, const Found& f, double& kept) {
     const int t = threadIdx.x, wave = t >> 6;
     const int32_t all = B.count[kBins];
     const int bin_k = f.bin_k, bin_m = f.bin_m;
     auto sync = [] { sync_as<kWave>(); };
     // Each token's bin, weight and sums before it in its bin.
-    int bin_of[kEach];
-    uint32_t w[kEach];
-    bool weighs[kEach];  // at least min_p
-    int first[kEach];  // of its bin, in the list
+    int bin_of[kMine];
+    uint32_t w[kMine];
+    bool weighs[kMine];  // at least min_p
+    int first[kMine];  // of its bin, in the list
     uint64_t mine = 0, all_sum;
     int start = -1, previous = -1;
-    if (t * kEach > 0 && t * kEach - 1 < n) previous = P.of(of_key(~static_cast<uint32_t>(S.words[t * kEach - 1] >> 32))).bin();
+    if (t * kMine > 0 && t * kMine - 1 < n) previous = P.of(of_key(~static_cast<uint32_t>(S.words[t * kMine - 1] >> 32))).bin();
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int i = t * kEach + j;
+    for (int j = 0; j < kMine; ++j) {
+        const int i = t * kMine + j;
         w[j] = 0, bin_of[j] = 0, first[j] = -1, weighs[j] = false;
         if (i >= n) continue;
         const Place place = P.of(of_key(~static_cast<uint32_t>(S.words[i] >> 32)));
@@ -695,8 +707,8 @@ __device__ __forceinline__ void finish_as(Shared& S, const Sums& B, uint64_t* su
         carried = S.wave_first[i] > carried ? S.wave_first[i] : carried;
     }
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int i = t * kEach + j;
+    for (int j = 0; j < kMine; ++j) {
+        const int i = t * kMine + j;
         if (i >= n) break;
         sums[i] = sum;
         sum += w[j];
@@ -706,11 +718,11 @@ __device__ __forceinline__ void finish_as(Shared& S, const Sums& B, uint64_t* su
     // In the row's order: tokens before it, weights before and with it (the last
     // of a bin ends where the next begins). Read once: the sums may lie in
     // global memory.
-    int32_t rank[kEach];
-    double before[kEach], with[kEach];
+    int32_t rank[kMine];
+    double before[kMine], with[kMine];
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int i = t * kEach + j, bin = bin_of[j];
+    for (int j = 0; j < kMine; ++j) {
+        const int i = t * kMine + j, bin = bin_of[j];
         rank[j] = INT32_MAX - 1, before[j] = with[j] = INFINITY;
         if (i >= n) continue;
         const int32_t count = B.count[bin], next = B.count[bin + 1];
@@ -722,25 +734,25 @@ __device__ __forceinline__ void finish_as(Shared& S, const Sums& B, uint64_t* su
     }
     if (bin_k >= 0)
 #pragma unroll
-        for (int j = 0; j < kEach; ++j)
+        for (int j = 0; j < kMine; ++j)
             if (rank[j] == R.k - 1) S.end_count[0] = R.k, S.end_weight[0] = with[j];
     sync();
     if (R.p < 1.0) {
         const double x = reached(R.p * (bin_k >= 0 ? S.end_weight[0] : B.weight[kBins]), B.weight[kBins]);
 #pragma unroll
-        for (int j = 0; j < kEach; ++j)
+        for (int j = 0; j < kMine; ++j)
             if (before[j] < x && x <= with[j]) S.end_count[1] = rank[j] + 1, S.end_weight[1] = with[j];
     }
     if (bin_m >= 0) {
         if (t == 0) S.found[2] = B.count[bin_m];
         sync();
 #pragma unroll
-        for (int j = 0; j < kEach; ++j)
+        for (int j = 0; j < kMine; ++j)
             if (bin_of[j] == bin_m && weighs[j]) atomicMax(&S.found[2], rank[j] + 1);
         sync();
         if (t == 0 && S.found[2] == B.count[bin_m]) S.end_count[2] = S.found[2], S.end_weight[2] = B.weight[bin_m];
 #pragma unroll
-        for (int j = 0; j < kEach; ++j)
+        for (int j = 0; j < kMine; ++j)
             if (bin_of[j] == bin_m && rank[j] + 1 == S.found[2]) S.end_count[2] = S.found[2], S.end_weight[2] = with[j];
     }
     if (t == 0) S.found[3] = 0;
@@ -751,16 +763,53 @@ __device__ __forceinline__ void finish_as(Shared& S, const Sums& B, uint64_t* su
         if (S.end_count[i] < most) most = S.end_count[i], kept = S.end_weight[i];
     const double x = R.u * kept;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
+    for (int j = 0; j < kMine; ++j)
         if (rank[j] < most && before[j] <= x) atomicMax(&S.found[3], rank[j] + 1);
     sync();
 #pragma unroll
-    for (int j = 0; j < kEach; ++j)
+    for (int j = 0; j < kMine; ++j)
         if (rank[j] + 1 == S.found[3]) {
-            S.drawn = static_cast<int32_t>(static_cast<uint32_t>(S.words[t * kEach + j]));
+            S.drawn = static_cast<int32_t>(static_cast<uint32_t>(S.words[t * kMine + j]));
             S.found_weight = static_cast<double>(w[j]) * S.octave.unit(bin_of[j]);
         }
     sync();
+}
+
+// Up to kThreads words, in order: each wave sorts 64 in registers, and a word's
+// place is its own there plus the numbers of smaller ones in the other waves',
+// by bisection. (Counting all smaller words took 12 us for 352, not 2.)
+__device__ __forceinline__ void sort_few(Shared& S, int n) {
+    const int t = threadIdx.x, lane = t & 63, runs = (n + 63) / 64, mine = t >> 6;
+    uint64_t x = t < n ? S.words[t] : ~uint64_t{0};
+    if (mine < runs) {
+#pragma unroll 1
+        for (int span = 2; span <= 64; span *= 2)
+#pragma unroll 1
+            for (int gap = span / 2; gap > 0; gap /= 2) {
+                const uint64_t o = __shfl_xor(x, gap);
+                const bool low = ((lane & gap) == 0) == ((lane & span) == 0);
+                x = (x < o) == low ? x : o;
+            }
+        S.words[t] = x;
+    }
+    if (runs == 1) {
+        __syncthreads();
+        return;
+    }
+    __syncthreads();
+    int at = lane;
+    if (mine < runs)
+        for (int r = 0; r < runs; ++r) {
+            const uint64_t* const run = S.words + 64 * r;
+            int below = 0;
+#pragma unroll
+            for (int step = 32; step > 0; step /= 2) below += run[below + step - 1] < x ? step : 0;
+            below += run[below] < x ? 1 : 0;
+            at += r == mine ? 0 : below;
+        }
+    __syncthreads();
+    if (t < n || x != ~uint64_t{0}) S.words[at] = x;
+    __syncthreads();
 }
 
 // The token, from the S.n gathered ones in the words. sums: room for kList numbers in LDS.
@@ -774,28 +823,11 @@ __device__ __forceinline__ void finish(const SampleArgs& A, Shared& S, const Sum
     if (n > kList || n < 1) {
         resolve_large<L>(A, S, B, row, P, R, f, token, weight, kept);
     } else {
-        int size = 64;
-        while (size < n) size *= 2;
-        if (size <= kFew) {
-            // Few: a token's rank is the number of those before it, counted by kThreads / size threads for each.
-            const int e = t & (size - 1), parts = kThreads / size, part = t / size;
-            const uint64_t mine = e < n ? S.words[e] : 0;
-            if (t < size) S.rank[t] = 0;
-            __syncthreads();
-            int32_t rank = 0;
-            for (int i = part; i < n; i += 8 * parts) {  // eight reads on their way together
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int at = i + j * parts;
-                    const uint64_t other = S.words[at & (kList - 1)];
-                    rank += (at < n) & (other < mine) ? 1 : 0;
-                }
-            }
-            if (e < n && rank > 0) atomicAdd(&S.rank[e], rank);
-            __syncthreads();
-            if (t < n) S.words[S.rank[t]] = mine;
-            __syncthreads();
+        if (n <= kThreads) {
+            sort_few(S, n);
         } else {
+            int size = 2 * kThreads;
+            while (size < n) size *= 2;
             for (int i = n + t; i < size; i += kThreads) S.words[i] = ~uint64_t{0};
             __syncthreads();
             for (int span = 2; span <= size; span *= 2)
@@ -809,12 +841,10 @@ __device__ __forceinline__ void finish(const SampleArgs& A, Shared& S, const Sum
                 }
         }
         // A wave alone needs no barriers.
-        if (n <= 64 * kEach) {
-            if (t >= 64) return;
-            finish_as<true, L>(S, B, sums, P, R, n, f, kept);
-        } else {
-            finish_as<false, L>(S, B, sums, P, R, n, f, kept);
-        }
+        if (n <= 64 * kEach && t >= 64) return;
+        if (n <= 64) finish_as<true, 1, L>(S, B, sums, P, R, n, f, kept);
+        else if (n <= 64 * kEach) finish_as<true, kEach, L>(S, B, sums, P, R, n, f, kept);
+        else finish_as<false, kEach, L>(S, B, sums, P, R, n, f, kept);
         token = S.drawn, weight = S.found_weight;
     }
     if (t == 0) {
@@ -865,7 +895,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
     const Places<L> P = places_of<L>(top, R);
     fill_bins<L>(row, A.vocab, threadIdx.x, kThreads, P, R, S.words);
     __syncthreads();
-    const Found f = find_bins(S, R, B);
+    const Found f = find_bins<true>(S, R, B);
     gather<L>(S, row, A.vocab, threadIdx.x, kThreads, P, f);
     __syncthreads();
     finish<L>(A, S, B, sums, row, row_at, P, R, f, S.n);
@@ -947,7 +977,7 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(const SampleArg
     for (int i = t; i < kBins; i += kThreads) S.words[i] = W.bins[static_cast<int64_t>(row_at) * kBins + i];
     if (t == 0) S.n = 0;
     __syncthreads();
-    const Found f = find_bins(S, R, blockIdx.x == 0 ? W.sums(row_at) : Sums{nullptr, nullptr});
+    const Found f = find_bins<false>(S, R, blockIdx.x == 0 ? W.sums(row_at) : Sums{nullptr, nullptr});
     if (blockIdx.x == 0 && t == 0) W.found[row_at] = f;
     gather<L>(S, row, A.vocab, blockIdx.x * kThreads + t, W.n * kThreads, places_of<L>(top, R), f);
     __syncthreads();
@@ -955,9 +985,9 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(const SampleArg
     uint64_t* const list = W.list + static_cast<int64_t>(row_at) * kList;
     const int32_t n = S.n;
     if (n == 0) return;
-    if (t == 0) S.rank[0] = atomicAdd(&W.gathered[row_at], n);
+    if (t == 0) S.at = atomicAdd(&W.gathered[row_at], n);
     __syncthreads();
-    const int32_t at = S.rank[0];
+    const int32_t at = S.at;
     for (int i = t; i < n && i < kList && at + i < kList; i += kThreads) list[at + i] = S.words[i];
 }
 
@@ -972,7 +1002,13 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     if (decided(A, row_at, top, R, false)) return;
     const int32_t n = W.gathered[row_at];
     S.octave.make();
-    for (int i = t; i < n && i < kList; i += kThreads) S.words[i] = W.list[static_cast<int64_t>(row_at) * kList + i];
+    if (n <= kList) {
+        for (int i = t; i < n; i += kThreads) S.words[i] = W.list[static_cast<int64_t>(row_at) * kList + i];
+    } else {  // too many tokens to sort: every bin's sums are needed
+        for (int i = t; i < kBins; i += kThreads) S.words[i] = W.bins[static_cast<int64_t>(row_at) * kBins + i];
+        __syncthreads();
+        find_bins<true>(S, R, W.sums(row_at));
+    }
     __syncthreads();
     finish<L>(A, S, W.sums(row_at), sums, row, row_at, places_of<L>(top, R), R, W.found[row_at], n);
 }
