@@ -261,17 +261,27 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     Returns out (q's shape and type; rows of no sequence, or past its first
     max_drafts, are not written); lse as in prompt_attention. Results do not
     vary between calls. No gradients, as there."""
-    qd, index, kind = _query(q)
+    query = _query(q)
     pages = describe_pages(k_pages, v_pages, page_table, lengths)
     forward_only(k_pages, "k_pages")
     forward_only(v_pages, "v_pages")
-    narrow = k_pages.dtype is torch.float8_e4m3fn
-    if (not narrow and k_pages.dtype is not q.dtype) or k_pages.get_device() != index:
-        raise ValueError("k_pages must be %s on %s" % (q.dtype, q.device))
-    if narrow:
-        scales = _page_scales(k_scales, v_scales, pages, index)
+    scales = None
+    if k_pages.dtype is torch.float8_e4m3fn:
+        scales = _page_scales(k_scales, v_scales, pages, k_pages.get_device())
     elif k_scales is not None or v_scales is not None:
         raise ValueError("k_scales and v_scales belong to pages of float8_e4m3fn")
+    return attend(q, query, pages, scales, k_pages.dtype, k_pages.get_device(), seqs, draft_offsets, masks, max_drafts, max_context, scale, out, lse)
+
+
+def attend(q: torch.Tensor, query: tuple[_native.AimgHeads, int, int], pages: _native.AimgPages,
+           scales: _native.AimgPageScales | None, dtype: torch.dtype, device: int, seqs: torch.Tensor, draft_offsets: torch.Tensor,
+           masks: torch.Tensor | None = None, max_drafts: int = 0, max_context: int | None = None, scale: float | None = None,
+           out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
+    """tree_attention over described pages of this type on this GPU, for a
+    described q: a cache describes its layers once."""
+    qd, index, kind = query
+    if (scales is None and dtype is not q.dtype) or device != index:
+        raise ValueError("k_pages must be %s on %s" % (q.dtype, q.device))
     heads, kv_heads, dim = qd.heads, pages.kv_heads, qd.dim
     if pages.dim != dim or heads % kv_heads:
         raise ValueError("q's dim %d must be the pages' %d, its %d heads a multiple of their %d"
@@ -298,7 +308,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     work = _workspace(nbytes, q)
     rest = (od, seqs_at, at, n_seqs, masks_at, words, max_drafts, max_context, kind, _scale(scale, dim), _lse(lse, q),
             work.data_ptr() if nbytes else None, nbytes)
-    if narrow:
+    if scales is not None:
         launch(_native.lib().aimg_tree8_attention, index, qd, pages, scales, *rest)
     else:
         launch(_native.lib().aimg_tree_attention, index, qd, pages, *rest)

@@ -30,7 +30,7 @@ import ctypes
 import torch
 
 from .. import _native
-from .attention import _TYPES, forward_only, launch, tree_attention
+from .attention import _TYPES, _query, attend, describe_pages, forward_only, launch
 
 MAX_SEQS = 8192      # sequences of one call
 MAX_PAGES = (1 << 20) - 1
@@ -63,6 +63,8 @@ class PagedKVCache:
     ``allocate`` makes an empty one. The tensors are used in place and are the
     cache's whole state. ``seqs``, ``src`` and ``dst`` below are slots: int32
     tensors on the GPU of at most 8192 entries."""
+
+    scales: torch.Tensor | None = None
 
     def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, held: torch.Tensor,
                  refs: torch.Tensor, status: torch.Tensor, scales: torch.Tensor | None = None):
@@ -99,6 +101,13 @@ class PagedKVCache:
             self.n_layers, self.n_pages, self.kv_heads, self.page_size, self.dim, self.max_seqs, self.max_pages)
         self.device = pool.device
         self._index = index
+        # What attention is told of each layer. (Views of the tensors, and their checks, took 12 us of a call.)
+        self._described = []
+        for layer in range(self.n_layers):
+            pages = describe_pages(pool[layer, 0], pool[layer, 1], page_table, lengths)
+            at = None if scales is None else scales[layer]
+            self._described.append((pages, None if scales is None else _native.AimgPageScales(
+                at[0].data_ptr(), at[1].data_ptr(), at.stride(1), at.stride(2))))
         self._lib = _native.lib()
         self.pool, self.page_table, self.lengths, self.held, self.refs, self.status = \
             pool, page_table, lengths, held, refs, status
@@ -142,13 +151,16 @@ class PagedKVCache:
         launch(self._lib.aimg_cache_reserve, self._index, self._cache, at, _int32(tokens, "tokens", (n,), self._index), n)
 
     def _heads(self, x: torch.Tensor, name: str, dtype: torch.dtype, heads: int) -> _native.AimgHeads:
-        if x.dim() != 3 or x.dtype is not dtype or x.get_device() != self._index or x.shape[1:] != (heads, self.dim):
+        shape = x.shape
+        if len(shape) != 3 or x.dtype is not dtype or x.get_device() != self._index or shape[1] != heads or shape[2] != self.dim:
             raise ValueError("%s must be a %s [rows, %d, %d] tensor on %s" % (name, dtype, heads, self.dim, self.device))
         row, head, one = x.stride()
-        if one != 1 or (row | head) % 8 or x.data_ptr() % 16:
+        at = x.data_ptr()
+        if one != 1 or (row | head) % 8 or at % 16:
             raise ValueError("%s must be contiguous in its last dimension, its rows and heads on 16-byte boundaries" % name)
-        forward_only(x, name)
-        return _native.AimgHeads(x.data_ptr(), x.shape[0], row, head, heads, self.dim)
+        if x.requires_grad:
+            forward_only(x, name)
+        return _native.AimgHeads(at, shape[0], row, head, heads, self.dim)
 
     def _rows(self, x: torch.Tensor, name: str) -> _native.AimgHeads:
         return self._heads(x, name, self.pool.dtype, self.kv_heads)
@@ -203,30 +215,35 @@ class PagedKVCache:
         elements. Rows of no sequence, or whose position the tables do not hold
         (recorded), are not written to either; nor are keys and values that the
         pages have no room for (recorded)."""
-        kind = self._type(q, "q")
+        kind, dtype, index = self._type(q, "q"), q.dtype, self._index
         if q.dim() != 3 or q.shape[1] < 1:
-            raise ValueError("q must be a %s [rows, heads, %d] tensor on %s" % (q.dtype, self.dim, self.device))
-        qd = self._heads(q, "q", q.dtype, q.shape[1])
-        kd, vd = self._heads(k, "k", q.dtype, self.kv_heads), self._heads(v, "v", q.dtype, self.kv_heads)
+            raise ValueError("q must be a %s [rows, heads, %d] tensor on %s" % (dtype, self.dim, self.device))
+        heads = q.shape[1]
+        qd = self._heads(q, "q", dtype, heads)
+        kd, vd = self._heads(k, "k", dtype, self.kv_heads), self._heads(v, "v", dtype, self.kv_heads)
         self._layer(layer)
-        if k.shape != v.shape or k.shape[0] != q.shape[0]:
+        rows = qd.n_rows
+        if kd.n_rows != rows or vd.n_rows != rows:
             raise ValueError("q, k and v must have the same rows, k and v one shape, got %s, %s and %s"
                              % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-        if cos.dim() != 2 or cos.dtype is not torch.float32 or cos.get_device() != self._index or not cos.is_contiguous() \
-                or not 1 <= cos.shape[1] <= self.dim // 2 or cos.shape[0] < 1:
-            raise ValueError("cos must be a contiguous fp32 [positions, up to %d] tensor on cuda:%d" % (self.dim // 2, self._index))
-        if sin.shape != cos.shape or sin.dtype is not torch.float32 or sin.get_device() != self._index or not sin.is_contiguous():
+        table = cos.shape
+        if len(table) != 2 or cos.dtype is not torch.float32 or cos.get_device() != index or not cos.is_contiguous() \
+                or not 1 <= table[1] <= self.dim // 2 or table[0] < 1:
+            raise ValueError("cos must be a contiguous fp32 [positions, up to %d] tensor on cuda:%d" % (self.dim // 2, index))
+        if sin.shape != table or sin.dtype is not torch.float32 or sin.get_device() != index or not sin.is_contiguous():
             raise ValueError("sin must have cos' shape, type and device")
         at, n = self._seqs(seqs)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != q.shape:
-            raise ValueError("out must have q's shape %s" % (tuple(q.shape),))
-        od = self._heads(out, "out", q.dtype, q.shape[1])
-        launch(self._lib.aimg_cache_append_rotated, self._index, self._cache, self._scales_at, layer, qd, kd, vd, od, at,
-               _int32(offsets, "offsets", (n + 1,), self._index), n,
-               _native.AimgRotary(cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.shape[1], int(interleaved)),
-               None if positions is None else _int32(positions, "positions", (q.shape[0],), self._index), kind)
+            od = _native.AimgHeads(out.data_ptr(), rows, heads * self.dim, self.dim, heads, self.dim)
+        else:
+            od = self._heads(out, "out", dtype, heads)
+            if od.n_rows != rows:
+                raise ValueError("out must have q's shape %s" % (tuple(q.shape),))
+        launch(self._lib.aimg_cache_append_rotated, index, self._cache, self._scales_at, layer, qd, kd, vd, od, at,
+               _int32(offsets, "offsets", (n + 1,), index), n,
+               _native.AimgRotary(cos.data_ptr(), sin.data_ptr(), table[0], table[1], interleaved),
+               None if positions is None else _int32(positions, "positions", (rows,), index), kind)
         return out
 
     def read(self, layer: int, seqs: torch.Tensor, offsets: torch.Tensor, rows: int, starts: torch.Tensor | None = None, *,
@@ -263,10 +280,11 @@ class PagedKVCache:
     def attend(self, layer: int, q: torch.Tensor, seqs: torch.Tensor, draft_offsets: torch.Tensor,
                masks: torch.Tensor | None = None, **options) -> torch.Tensor:
         """tree_attention of q over one layer of this cache."""
-        if self.scales is not None:
-            options |= {"k_scales": self.scales[layer, 0], "v_scales": self.scales[layer, 1]}
-        return tree_attention(q, self.keys(layer), self.values(layer), self.page_table, self.lengths, seqs, draft_offsets,
-                              masks, **options)
+        if not -self.n_layers <= layer < self.n_layers:
+            raise IndexError("layer %d is out of range for %d layers" % (layer, self.n_layers))
+        pages, scales = self._described[layer]
+        forward_only(self.pool, "pool")
+        return attend(q, _query(q), pages, scales, self.pool.dtype, self._index, seqs, draft_offsets, masks, **options)
 
     def commit(self, seqs: torch.Tensor, accepted: torch.Tensor, counts: torch.Tensor,
                new_lengths: torch.Tensor | None = None) -> torch.Tensor:
