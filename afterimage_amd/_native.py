@@ -205,6 +205,8 @@ _SIGNATURES = [
      [_HEADS, _PAGES, _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int,
       ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
       ctypes.c_void_p]),
+    ("aimg_tree8_workspace_nbytes", ctypes.c_int,
+     [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, _SIZE]),
     ("aimg_tree8_attention", ctypes.c_int,
      [_HEADS, _PAGES, ctypes.POINTER(AimgPageScales), _HEADS, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
       ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,

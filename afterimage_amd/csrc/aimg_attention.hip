@@ -179,13 +179,16 @@ __device__ __forceinline__ void wait_loads() {
 }
 
 // One wave's softmax state and output of QT tiles of 32 queries.
-// k8: keys and values of 8 bits. A lane reads 16 elements of a key at a time,
-// which serve two steps of the first product (the queries are laid out
-// likewise); they enter it as they are, exact in either type, and a score is
-// multiplied by its key's scale. Values are multiplied by theirs as they become
-// bf16, which is exact whatever the queries' type: the second product is bf16's.
+// Keys and values of 8 bits become bf16 times their scales, which is exact;
+// for queries in fp16, keys become fp16 as they are, exact too, and scores are
+// multiplied by their keys' scales. Values are bf16 for either (their range may
+// pass fp16's), and fp16 queries' probabilities the sum of two bf16 numbers,
+// which 16 bits of them are in.
+// A lane reads 16 elements of such a key at a time, which serve two steps of the
+// first product (the queries are laid out likewise).
 template <typename T, int DP, int QT, bool k8 = false>
 struct State {
+    static constexpr bool kScaled = k8 && std::is_same_v<T, Fp16>;
     typedef std::conditional_t<k8, Bf16, T> P;  // of the second product
     typedef std::conditional_t<k8, Rows8<DP>, Rows<DP>> R;
     struct Scales {};
@@ -233,22 +236,18 @@ struct State {
             const int r = lane & 31;
             const lds_char* const row = keys + (32 * u + r) * R::kBytes;
             if constexpr (k8) {
+                const float scale = kScaled ? 1.0f : scales.at[2 * u + (r >> 4)];
 #pragma unroll
                 for (int k = 0; k < kSteps; k += 2) {
                     const u32x4 w = *reinterpret_cast<const __attribute__((address_space(3))) u32x4*>(
                         row + (((k + half) ^ R::key_place(r)) << 4));
-                    const s16x8 a = T::from8(w[0], w[1], 1.0f), b = T::from8(w[2], w[3], 1.0f);
+                    const s16x8 a = T::from8(w[0], w[1], scale), b = T::from8(w[2], w[3], scale);
 #pragma unroll
                     for (int t = 0; t < QT; ++t) {
                         s[t][u] = T::mfma(a, q[t][k], k == 0 ? f32x16{0} : s[t][u]);
                         s[t][u] = T::mfma(b, q[t][k + 1], s[t][u]);
                     }
                 }
-                const float low = scales.at[2 * u], high = scales.at[2 * u + 1];  // of keys 32 u + 0..15, 16..31
-#pragma unroll
-                for (int t = 0; t < QT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[t][u][i] *= i < 8 ? low : high;
             } else {
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
@@ -258,8 +257,15 @@ struct State {
                     for (int t = 0; t < QT; ++t) s[t][u] = T::mfma(a, q[t][k], k == 0 ? f32x16{0} : s[t][u]);
                 }
             }
+            if constexpr (kScaled) {
+                const float low = scales.at[2 * u], high = scales.at[2 * u + 1];  // of keys 32 u + 0..15, 16..31
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[t][u][i] *= i < 8 ? low : high;
+            }
         }
-        s16x8 p[QT][NSUB][2];
+        s16x8 p[QT][NSUB][2], rest[QT][kScaled ? NSUB : 1][2];
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             if (kMasked) {
@@ -276,11 +282,11 @@ struct State {
             // alone, so its bits do not depend on the wave's other rows.
             // (Against -inf, before a row's first visible key, they are infinite or NaN.)
             float sum = INFINITY;
-            if (!__all(m[t] == -INFINITY)) sum = soften<NSUB>(s[t], p[t], c, m[t] * c);
+            if (!__all(m[t] == -INFINITY)) sum = soften<NSUB>(s[t], p[t], rest[t], c, m[t] * c);
             const bool fits = sum <= kMostSum;
             if (__builtin_expect(!__all(fits), 0)) {
                 raise<NSUB>(t, s[t], c, fits);
-                sum = soften<NSUB>(s[t], p[t], c, m[t] == -INFINITY ? 0.0f : m[t] * c);
+                sum = soften<NSUB>(s[t], p[t], rest[t], c, m[t] == -INFINITY ? 0.0f : m[t] * c);
             }
             l[t] += sum;
         }
@@ -299,26 +305,34 @@ struct State {
                     if (kMasked) a = finite(a, odd);
 #pragma unroll
                     for (int t = 0; t < QT; ++t) o[t][d] = P::mfma(a, p[t][u][k], o[t][d]);
+                    if constexpr (kScaled) {
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) o[t][d] = P::mfma(a, rest[t][u][k], o[t][d]);
+                    }
                 }
         if (kMasked && __any(odd != 0)) add_infinite<NSUB>(first, piece, r, half, allow, scales);
     }
 
-    // A lane's probabilities 2^(c s - mc), packed for the second product; returns their sum.
+    // A lane's probabilities 2^(c s - mc), packed for the second product (and
+    // what that rounds off, where it is kept); returns their sum.
     template <int NSUB>
-    static __device__ __forceinline__ float soften(const f32x16 (&s)[NSUB], s16x8 (&p)[NSUB][2], float c, float mc) {
+    static __device__ __forceinline__ float soften(const f32x16 (&s)[NSUB], s16x8 (&p)[NSUB][2], s16x8 (&rest)[kScaled ? NSUB : 1][2], float c,
+                                                   float mc) {
         float sum = 0.0f;
 #pragma unroll
         for (int u = 0; u < NSUB; ++u)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                u32x4 w;
+                u32x4 w, v;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float x = exp2_fast(fmaf(s[u][8 * k + 2 * i], c, -mc)), y = exp2_fast(fmaf(s[u][8 * k + 2 * i + 1], c, -mc));
                     sum += x + y;
                     w[i] = P::pack(x, y);
+                    if (kScaled) v[i] = P::pack(x - __uint_as_float(w[i] << 16), y - __uint_as_float(w[i] & 0xFFFF0000u));
                 }
                 p[u][k] = __builtin_bit_cast(s16x8, w);
+                if (kScaled) rest[u][k] = __builtin_bit_cast(s16x8, v);
             }
         return sum;
     }
@@ -967,8 +981,13 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeArgs& A, const Drafted& 
 // kPages: what of a tile never crosses a page, and so has one base address: 2
 // the tile, 1 the rows of one load (2 to 8), 0 a row. (With addresses made lane
 // by lane for pages of 16, 54 trees over 139-2238 positions took 155 us.)
-// k8: a cache in 8 bits. Each wave brings its tile's scales along, a load of 4
-// bytes a lane into a place of its own.
+// k8: a cache in 8 bits, whose codes become elements in every wave that reads
+// them. Each wave brings its tile's scales along, a load of 4 bytes a lane into
+// a place of its own. Half the bytes leave the matrix and vector instructions of
+// shared tiles to bound it: 16 trees of 4-16 tokens over 9000-65000 positions
+// 313 us, 3.8 TB/s; 64 single tokens over 1900-8100 113 us, 4.8 TB/s. (Elements
+// formed once for all waves, in LDS, between two barriers: 391 us, not 330 with
+// the same parts; a lane's places in its loads worked out for every tile: 352.)
 template <typename T, int DP, int QT, int NW, bool kShared, int kPages, bool k8>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_kernel(const TreeArgs A) {
     typedef State<T, DP, QT, k8> St;
@@ -1023,6 +1042,27 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         const int32_t id = D.pages[at];
         held = static_cast<uint32_t>(id) < static_cast<uint32_t>(A.n_pages) ? id : 0;
     };
+    // The scales of the blocks of keys k0 .., those past the last key's being its own.
+    auto load_scales = [&](int k0, int last, lds_char* to) __attribute__((always_inline)) {
+        const int at = kBlock * lane_block;
+        int32_t p, slot;
+        page_of(A, k0 + (at < last ? at : last), p, slot);
+        const int64_t id = __builtin_amdgcn_ds_bpermute(4 * (p - first_page), held);
+        load4_to_lds(lane_scales + (id * A.scale_page + slot / kBlock), to);
+    };
+    // A lane's place in each of its loads.
+    uint32_t k_off[k8 ? kLoads : 1], v_off[k8 ? kLoads : 1];
+    const char* const k_head = A.k + kSize * head_at;
+    const char* const v_head = A.v + kSize * head_at;
+    if constexpr (k8) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = (load0 + i) * R::kPerLoad + lane_row;
+            const int kx = lane_piece ^ R::key_place(r), vx = lane_piece ^ R::value_place(r);
+            k_off[i] = lane_row * row_bytes + (kx < pieces ? kx : pieces) * 16;
+            v_off[i] = lane_row * row_bytes + (vx < pieces ? vx : pieces) * 16;
+        }
+    }
     // Keys past the last one repeat it; no row sees them.
     auto issue = [&](int k0, lds_char* to, lds_char* to_scales) __attribute__((always_inline)) {
         const int last = D.end - 1 - k0 < KT - 1 ? D.end - 1 - k0 : KT - 1;
@@ -1030,17 +1070,28 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_ke
         page_of(A, k0, page, first);
         page_of(A, k0 + last, page_end, unused);
         if (page_end >= first_page + 64) hold(page);
+        if (k8 && kPages > 0 && last == KT - 1) {
+            // A whole tile: uniform addresses, and offsets that a lane keeps.
+            const int32_t id = __builtin_amdgcn_readlane(held, page - first_page);
+            if (kPages == 2) load4_to_lds(lane_scales + (id * A.scale_page + static_cast<uint32_t>(first) / kBlock) + lane_block, to_scales);
+            else load_scales(k0, last, to_scales);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                int64_t from = id * A.page_stride + (first + (load0 + i) * R::kPerLoad) * A.slot_stride;
+                if (kPages == 1) {
+                    int32_t p, slot;
+                    page_of(A, k0 + (load0 + i) * R::kPerLoad, p, slot);
+                    from = __builtin_amdgcn_readlane(held, p - first_page) * A.page_stride + slot * A.slot_stride;
+                }
+                load_to_lds(k_head + from + k_off[i], to + (load0 + i) * 1024);
+                load_to_lds(v_head + from + v_off[i], to + kTile + (load0 + i) * 1024);
+            }
+            return;
+        }
         int64_t tile_at = 0;
         if (kPages == 2)
             tile_at = kSize * (__builtin_amdgcn_readlane(held, page - first_page) * A.page_stride + first * A.slot_stride + head_at);
-        if constexpr (k8) {
-            // The scales of the blocks of keys k0 .., those past the last key's being its own.
-            const int at = kBlock * lane_block;
-            int32_t p, slot;
-            page_of(A, k0 + (at < last ? at : last), p, slot);
-            const int64_t id = __builtin_amdgcn_ds_bpermute(4 * (p - first_page), held);
-            load4_to_lds(lane_scales + (id * A.scale_page + slot / kBlock), to_scales);
-        }
+        if constexpr (k8) load_scales(k0, last, to_scales);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int load = load0 + i;
@@ -1324,6 +1375,7 @@ constexpr int kMinChunk = 512;
 // (shared tiles, 16 trees over 9000-65000: 340 us, 427 with 8192).
 constexpr int kMaxChunk = 8192;
 constexpr int kMaxSharedChunk = 4096;
+constexpr int kMaxSharedChunk8 = 2048;  // of a cache in 8 bits: 16 trees over 9000-65000 313 us, 330 with 4096, 322 with 1024
 constexpr int kSlots = 256;         // workgroups of dealt-out keys that run at a time, one a CU
 constexpr int kFewParts = 16;       // at most so many are joined by DP / 4 threads a row
 // Workgroups of shared tiles, were all sequences the longest. It sets the keys
@@ -1344,7 +1396,7 @@ constexpr int kSharedParts = 1280;
 int tree_rows(int dim, int64_t rows) { return rows <= 32 ? 32 : rows <= 64 && dim <= 128 ? 64 : 128; }
 
 // Keys of a part and how many parts the longest sequence has.
-void plan_parts(TreeArgs& A, int64_t max_context) {
+void plan_parts(TreeArgs& A, int64_t max_context, bool narrow) {
     const int64_t rows = static_cast<int64_t>(A.max_drafts) * (A.heads / A.kv_heads);
     const int per = tree_rows(A.dim, rows);
     A.row_blocks = static_cast<int32_t>((rows + per - 1) / per);
@@ -1358,7 +1410,7 @@ void plan_parts(TreeArgs& A, int64_t max_context) {
         chunk = longest / (units > 0 && units < kSlots ? kSlots / units : 1) + 1;
     } else {
         chunk = longest * units / kSharedParts;
-        most = kMaxSharedChunk;
+        most = narrow ? kMaxSharedChunk8 : kMaxSharedChunk;
     }
     chunk = (chunk + 127) / 128 * 128;
     chunk = chunk < kMinChunk ? kMinChunk : chunk > most ? most : chunk;
@@ -1546,7 +1598,8 @@ extern "C" int aimg_prompt_attention(const aimg_heads* q, const aimg_heads* k, c
 namespace {
 
 // What the sizes of one tree attention call imply.
-int tree_sizes(aimg::TreeArgs& a, int64_t n_rows, int n_seqs, int heads, int kv_heads, int dim, int max_drafts, int64_t max_context) {
+int tree_sizes(aimg::TreeArgs& a, int64_t n_rows, int n_seqs, int heads, int kv_heads, int dim, int max_drafts, int64_t max_context,
+               bool narrow) {
     using aimg::fail;
     if (n_rows < 0 || n_rows > INT32_MAX || n_seqs < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || dim < 1 ||
         dim > aimg::kMaxDim || max_drafts < 1 || max_context < 0 || max_context > INT32_MAX)
@@ -1558,9 +1611,21 @@ int tree_sizes(aimg::TreeArgs& a, int64_t n_rows, int n_seqs, int heads, int kv_
     const int64_t blocks = (static_cast<int64_t>(a.max_drafts) * (heads / kv_heads) + 31) / 32;  // at least the row blocks
     if (static_cast<int64_t>(n_seqs) * kv_heads > INT32_MAX / blocks)
         return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and rows");
-    aimg::plan_parts(a, max_context);
+    aimg::plan_parts(a, max_context, narrow);
     if (static_cast<int64_t>(n_seqs) * kv_heads * a.row_blocks > INT32_MAX / a.n_splits)
         return fail(AIMG_ERR_UNSUPPORTED, "tree attention: too many sequences, heads and keys");
+    return AIMG_OK;
+}
+
+int tree_workspace(int64_t n_rows, int heads, int kv_heads, int dim, int n_seqs, int max_drafts, int64_t max_context, bool narrow,
+                   size_t* nbytes) {
+    using aimg::fail;
+    if (nbytes == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "nbytes is null");
+    aimg::TreeArgs a{};
+    const int rc = tree_sizes(a, n_rows, n_seqs, heads, kv_heads, dim, max_drafts, max_context, narrow);
+    if (rc != AIMG_OK) return rc;
+    const int64_t rows = n_rows * heads * a.n_splits;
+    *nbytes = a.n_splits > 1 ? static_cast<size_t>(rows) * (4 * aimg::padded_dim(dim) + 8) : 0;
     return AIMG_OK;
 }
 
@@ -1568,14 +1633,12 @@ int tree_sizes(aimg::TreeArgs& a, int64_t n_rows, int n_seqs, int heads, int kv_
 
 extern "C" int aimg_tree_workspace_nbytes(int64_t n_rows, int heads, int kv_heads, int dim, int n_seqs, int max_drafts,
                                           int64_t max_context, size_t* nbytes) {
-    using aimg::fail;
-    if (nbytes == nullptr) return fail(AIMG_ERR_INVALID_ARGUMENT, "nbytes is null");
-    aimg::TreeArgs a{};
-    const int rc = tree_sizes(a, n_rows, n_seqs, heads, kv_heads, dim, max_drafts, max_context);
-    if (rc != AIMG_OK) return rc;
-    const int64_t rows = n_rows * heads * a.n_splits;
-    *nbytes = a.n_splits > 1 ? static_cast<size_t>(rows) * (4 * aimg::padded_dim(dim) + 8) : 0;
-    return AIMG_OK;
+    return tree_workspace(n_rows, heads, kv_heads, dim, n_seqs, max_drafts, max_context, false, nbytes);
+}
+
+extern "C" int aimg_tree8_workspace_nbytes(int64_t n_rows, int heads, int kv_heads, int dim, int n_seqs, int max_drafts,
+                                           int64_t max_context, size_t* nbytes) {
+    return tree_workspace(n_rows, heads, kv_heads, dim, n_seqs, max_drafts, max_context, true, nbytes);
 }
 
 namespace {
@@ -1596,7 +1659,7 @@ int tree_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_page
     if (q->dim != pages->dim || q->heads % pages->kv_heads != 0)
         return fail(AIMG_ERR_INVALID_ARGUMENT, "q must have the pages' dim and a multiple of their heads");
     aimg::TreeArgs a{};
-    rc = tree_sizes(a, q->n_rows, n_seqs, q->heads, pages->kv_heads, q->dim, max_drafts, max_context);
+    rc = tree_sizes(a, q->n_rows, n_seqs, q->heads, pages->kv_heads, q->dim, max_drafts, max_context, scales != nullptr);
     if (rc != AIMG_OK) return rc;
     if (masks != nullptr && mask_words < 1) return fail(AIMG_ERR_INVALID_ARGUMENT, "mask_words must be >= 1");
     if (n_seqs == 0 || q->n_rows == 0) return AIMG_OK;

@@ -221,10 +221,11 @@ def _page_scales(k_scales: torch.Tensor | None, v_scales: torch.Tensor | None, p
 
 
 @functools.lru_cache(maxsize=1024)
-def _tree_workspace_nbytes(n: int, heads: int, kv_heads: int, dim: int, n_seqs: int, max_drafts: int, max_context: int) -> int:
+def _tree_workspace_nbytes(n: int, heads: int, kv_heads: int, dim: int, n_seqs: int, max_drafts: int, max_context: int,
+                           narrow: bool = False) -> int:
     nbytes = ctypes.c_size_t(0)
-    _native.check(_native.lib().aimg_tree_workspace_nbytes(n, heads, kv_heads, dim, n_seqs, max_drafts, max_context,
-                                                           ctypes.byref(nbytes)))
+    entry = _native.lib().aimg_tree8_workspace_nbytes if narrow else _native.lib().aimg_tree_workspace_nbytes
+    _native.check(entry(n, heads, kv_heads, dim, n_seqs, max_drafts, max_context, ctypes.byref(nbytes)))
     return nbytes.value
 
 
@@ -256,7 +257,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     Pages of float8_e4m3fn come with their scales, fp32 [n_pages, kv_heads,
     page_size / 16]: powers of two, which the elements of 16 positions of a
     page and head are multiplied by (page_size and dim multiples of 16). q is
-    then bf16 or fp16, and probabilities are rounded to bf16.
+    then bf16 or fp16; probabilities are rounded to bf16, for fp16 to 16 bits.
 
     Returns out (q's shape and type; rows of no sequence, or past its first
     max_drafts, are not written); lse as in prompt_attention. Results do not
@@ -304,7 +305,7 @@ def attend(q: torch.Tensor, query: tuple[_native.AimgHeads, int, int], pages: _n
     elif max_context < 0:
         raise ValueError("max_context must not be negative, got %d" % max_context)
     out, od = _result(q, qd, out, index)
-    nbytes = _tree_workspace_nbytes(n, heads, kv_heads, dim, n_seqs, max_drafts, max_context)
+    nbytes = _tree_workspace_nbytes(n, heads, kv_heads, dim, n_seqs, max_drafts, max_context, scales is not None)
     work = _workspace(nbytes, q)
     rest = (od, seqs_at, at, n_seqs, masks_at, words, max_drafts, max_context, kind, _scale(scale, dim), _lse(lse, q),
             work.data_ptr() if nbytes else None, nbytes)

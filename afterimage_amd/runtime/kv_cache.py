@@ -262,10 +262,17 @@ class PagedKVCache:
         self._layer(layer)
         if rows < 0:
             raise ValueError("rows must not be negative, got %d" % rows)
-        k, v = out or (torch.empty((rows, self.kv_heads, self.dim), dtype=dtype, device=self.device) for _ in range(2))
-        kd, vd = self._heads(k, "k", dtype, self.kv_heads), self._heads(v, "v", dtype, self.kv_heads)
-        if k.shape[0] != rows or v.shape[0] != rows:
-            raise ValueError("out must hold %d rows, got %d and %d" % (rows, k.shape[0], v.shape[0]))
+        if out is None:
+            both = torch.empty((2, rows, self.kv_heads, self.dim), dtype=dtype, device=self.device)
+            k, v = both.unbind(0)
+            row = self.kv_heads * self.dim
+            first = both.data_ptr()
+            kd, vd = (_native.AimgHeads(at, rows, row, self.dim, self.kv_heads, self.dim) for at in (first, first + 2 * rows * row))
+        else:
+            k, v = out
+            kd, vd = self._heads(k, "k", dtype, self.kv_heads), self._heads(v, "v", dtype, self.kv_heads)
+            if kd.n_rows != rows or vd.n_rows != rows:
+                raise ValueError("out must hold %d rows, got %d and %d" % (rows, kd.n_rows, vd.n_rows))
         at, n = self._seqs(seqs)
         launch(self._lib.aimg_cache_read, self._index, self._cache, self._scales_at, layer, at,
                _int32(offsets, "offsets", (n + 1,), self._index), None if starts is None else _int32(starts, "starts", (n,), self._index),

@@ -368,8 +368,11 @@ typedef struct aimg_page_scales {
  * aimg_tree_attention over a cache in 8 bits: pages of e4m3 elements (strides
  * in elements, whole 16 bytes; dim and page_size multiples of 16), the factors
  * powers of two. q and out are bf16 or fp16 (type). Keys enter the first
- * product exactly, probabilities are rounded to bf16 for the second.
+ * product exactly; probabilities are rounded to bf16 for the second where q is
+ * bf16, to a sum of two bf16 numbers (16 bits) where it is fp16.
  */
+int aimg_tree8_workspace_nbytes(int64_t n_rows, int heads, int kv_heads, int dim, int n_seqs, int max_drafts,
+                                int64_t max_context, size_t* nbytes);
 int aimg_tree8_attention(const aimg_heads* q, const aimg_pages* pages, const aimg_page_scales* scales, const aimg_heads* out,
                          const int32_t* seqs, const int32_t* draft_offsets, int n_seqs, const int64_t* masks, int mask_words,
                          int max_drafts, int64_t max_context, int type, float scale, float* lse, void* workspace,
