@@ -1,4 +1,4 @@
-"""Greedy decoding, then the same tokens out of one verified draft tree.
+"""Decoding, then the same tokens out of one verified draft tree.
 
 A small decoder-only model whose projections stay compressed on the GPU
 (decode_linear decodes each as it is used) runs the way a speculative engine
@@ -7,21 +7,29 @@ verifies them in one target pass):
 
   - the prompts of a batch go through prompt_attention, their keys and values
     into a PagedKVCache;
-  - each sequence is forked: the first branch decodes greedily, a token a pass;
+  - each sequence is forked: the first branch decodes, a token a pass: the
+    largest logit's, or one sampled with a random number for each position;
   - the other verifies a tree that holds those tokens among wrong guesses, in
-    one pass, and commits the path it accepts.
+    one pass, and commits the path it accepts: a child is accepted where it is
+    its parent's token by the same rule and random number, so that what is
+    accepted follows the model's distribution.
 
-Both branches hold the same tokens afterwards. Run as
-``python -m afterimage_amd.examples.verify_tree``.
+Both branches hold the same tokens afterwards. Queries and keys may be turned by
+their positions on their way into the cache, which may hold 16 bits or 8. Run as
+``python -m afterimage_amd.examples.verify_tree``: greedily with a cache in 16
+bits; with ``--sampled``, with sampling, rotation and a cache in 8.
 """
 from __future__ import annotations
 
+import sys
+
 import torch
 
-from ..runtime.attention import prompt_attention, tree_masks
+from ..runtime.attention import prompt_attention, rotary_tables, tree_masks
 from ..runtime.compressed_store import compress_layer
 from ..runtime.device import DeviceTensor, decode_linear
 from ..runtime.kv_cache import PagedKVCache
+from ..runtime.sampling import sample
 
 
 def _ints(values, device) -> torch.Tensor:
@@ -42,10 +50,11 @@ class Linear:
 
 
 class Model:
-    """Attention blocks with a residual, an embedding and an output projection, random weights."""
+    """Attention blocks with a residual, an embedding and an output projection, random weights. With positions, so many of
+    them have angles that queries and keys turn by."""
 
     def __init__(self, layers: int = 2, heads: int = 8, kv_heads: int = 2, dim: int = 64, vocab: int = 512, seed: int = 0,
-                 device="cuda"):
+                 device="cuda", positions: int = 0):
         g = torch.Generator().manual_seed(seed)
         self.heads, self.kv_heads, self.dim, self.device = heads, kv_heads, dim, torch.device(device)
         width = heads * dim
@@ -54,6 +63,7 @@ class Model:
                         "v": Linear(kv_heads * dim, width, g, device), "o": Linear(width, width, g, device)}
                        for _ in range(layers)]
         self.head = Linear(vocab, width, g, device)
+        self.rotary = rotary_tables(positions, dim, device=device) if positions else None
 
     def forward(self, tokens: torch.Tensor, attend) -> torch.Tensor:
         """Logits of each token; attend(layer, q, k, v) is the attention of one layer."""
@@ -66,41 +76,62 @@ class Model:
         return self.head(torch.nn.functional.rms_norm(x, (x.shape[1],)))
 
 
+class Choice:
+    """A token for each row of logits: the largest's, or sampled with the settings and a random number for each (sequence, position)."""
+
+    def __init__(self, sequences: int, positions: int, settings: dict | None, seed: int, device):
+        self.settings = settings
+        self.uniforms = torch.rand(sequences, positions, generator=torch.Generator().manual_seed(seed)).to(device)
+
+    def __call__(self, logits: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        if self.settings is None:
+            return logits.argmax(-1)
+        return sample(logits, self.uniforms[sequences, positions], **self.settings)
+
+
 def prefill(model: Model, cache: PagedKVCache, prompts: list[list[int]], slots: torch.Tensor) -> torch.Tensor:
-    """The prompts into their slots; returns each one's next token."""
+    """The prompts into their slots; returns the logits after each."""
     lengths = [len(p) for p in prompts]
     offsets = _ints([sum(lengths[:i]) for i in range(len(lengths) + 1)], model.device)
     cache.reserve(slots, _ints(lengths, model.device))
 
     def attend(layer, q, k, v):
-        cache.append(layer, k, v, slots, offsets)
+        if model.rotary is None:
+            cache.append(layer, k, v, slots, offsets)
+        else:  # the cache's rows are the turned ones, of the cache's precision
+            q = cache.append_rotated(layer, q, k, v, slots, offsets, *model.rotary)
+            k, v = cache.read(layer, slots, offsets, q.shape[0])
         return prompt_attention(q, k, v, offsets)
 
     logits = model.forward(torch.tensor(sum(prompts, []), device=model.device), attend)
     cache.advance(slots, offsets)
-    return logits[offsets[1:].long() - 1].argmax(-1)
+    return logits[offsets[1:].long() - 1]
 
 
 def verify(model: Model, cache: PagedKVCache, slots: torch.Tensor, tokens: torch.Tensor, offsets: torch.Tensor,
-           masks: torch.Tensor | None, most: int) -> torch.Tensor:
+           masks: torch.Tensor | None, most: int, positions: torch.Tensor | None = None) -> torch.Tensor:
     """Logits of drafted tokens, whose keys and values go past the slots' lengths."""
     cache.reserve(slots, offsets.diff())
 
     def attend(layer, q, k, v):
-        cache.append(layer, k, v, slots, offsets)
+        if model.rotary is None:
+            cache.append(layer, k, v, slots, offsets)
+        else:
+            q = cache.append_rotated(layer, q, k, v, slots, offsets, *model.rotary, positions)
         return cache.attend(layer, q, slots, offsets, masks, max_drafts=most)
 
     return model.forward(tokens, attend)
 
 
-def greedy(model: Model, cache: PagedKVCache, slots: torch.Tensor, tokens: torch.Tensor, steps: int) -> torch.Tensor:
+def decode(model: Model, cache: PagedKVCache, slots: torch.Tensor, tokens: torch.Tensor, steps: int, choose: Choice) -> torch.Tensor:
     """[sequences, steps + 1]: the given tokens and what follows them, a token a pass."""
     n = slots.shape[0]
     offsets = torch.arange(n + 1, dtype=torch.int32, device=model.device)
-    out = [tokens]
+    out, sequences = [tokens], torch.arange(n, device=model.device)
     for _ in range(steps):
-        out.append(verify(model, cache, slots, out[-1], offsets, None, 1).argmax(-1))
+        logits = verify(model, cache, slots, out[-1], offsets, None, 1)
         cache.advance(slots, offsets)
+        out.append(choose(logits, sequences, cache.lengths[slots.long()].long()))
     return torch.stack(out, 1)
 
 
@@ -114,18 +145,21 @@ def accept(tree: list[int], parents: list[int], best: list[int]) -> list[int]:
         path.append(child)
 
 
-def run(prompts=(37, 5, 130), steps: int = 5, wrong: int = 2, seed: int = 0, device="cuda") -> dict:
-    """Both ways of decoding; the tokens of each and the cache."""
-    model = Model(seed=seed, device=device)
+def run(prompts=(37, 5, 130), steps: int = 5, wrong: int = 2, seed: int = 0, device="cuda", dtype: torch.dtype = torch.bfloat16,
+        rotary: bool = False, settings: dict | None = None) -> dict:
+    """Both ways of decoding; the tokens of each and the cache. dtype: the cache's; settings: sample's, None for the largest logit."""
+    positions = max(prompts) + steps + 2
+    model = Model(seed=seed, device=device, positions=positions if rotary else 0)
     rng = torch.Generator().manual_seed(seed + 1)
     vocab, n = model.embedding.shape[0], len(prompts)
     texts = [torch.randint(vocab, (length,), generator=rng).tolist() for length in prompts]
-    cache = PagedKVCache.allocate(len(model.blocks), 64, 16, model.kv_heads, model.dim, 2 * n, 16, device=device)
+    cache = PagedKVCache.allocate(len(model.blocks), 64, 16, model.kv_heads, model.dim, 2 * n, 16, dtype, device)
+    choose = Choice(n, positions + 1, settings, seed + 2, device)
     slots = _ints(list(range(n)), device)
     branches = _ints(list(range(n, 2 * n)), device)
-    first = prefill(model, cache, texts, slots)
+    first = choose(prefill(model, cache, texts, slots), torch.arange(n, device=device), cache.lengths[:n].long())
     cache.fork(slots, branches)
-    decoded = greedy(model, cache, slots, first, steps)
+    decoded = decode(model, cache, slots, first, steps, choose)
     # A tree for each sequence: the decoded tokens in a row, wrong ones beside each.
     trees, parents = [], []
     for row in decoded.tolist():
@@ -142,7 +176,17 @@ def run(prompts=(37, 5, 130), steps: int = 5, wrong: int = 2, seed: int = 0, dev
     most = max(map(len, trees))
     offsets = _ints([sum(map(len, trees[:i])) for i in range(n + 1)], device)
     masks = tree_masks(_ints(sum(parents, []), device), offsets, most)
-    best = verify(model, cache, branches, torch.tensor(sum(trees, []), device=device), offsets, masks, most).argmax(-1).tolist()
+    # A drafted token's position is that of its place in the tree; what follows it comes after that.
+    depths = []
+    for up in parents:
+        depth = []
+        for p in up:
+            depth.append(0 if p < 0 else depth[p] + 1)
+        depths += depth
+    sequences = torch.tensor([b for b, t in enumerate(trees) for _ in t], device=device)
+    at = cache.lengths[branches.long()].long()[sequences] + torch.tensor(depths, device=device)
+    logits = verify(model, cache, branches, torch.tensor(sum(trees, []), device=device), offsets, masks, most, at.int())
+    best = choose(logits, sequences, at + 1).tolist()
     paths = []
     for b in range(n):
         at = int(offsets[b])
@@ -154,8 +198,11 @@ def run(prompts=(37, 5, 130), steps: int = 5, wrong: int = 2, seed: int = 0, dev
             "following": [best[int(offsets[b]) + p[-1]] for b, p in enumerate(paths)], "slots": slots, "branches": branches}
 
 
-def main() -> None:
-    got = run()
+SAMPLED = {"dtype": torch.float8_e4m3fn, "rotary": True, "settings": {"temperature": 0.8, "top_k": 40, "top_p": 0.95}}
+
+
+def main(sampled: bool = False) -> None:
+    got = run(**SAMPLED) if sampled else run()
     for b, (row, path) in enumerate(zip(got["decoded"].tolist(), got["accepted"])):
         print("sequence %d: decoded %s, accepted from its tree %s" % (b, row, path))
     cache = got["cache"]
@@ -164,4 +211,4 @@ def main() -> None:
 
 
 if __name__ == "__main__":
-    main()
+    main("--sampled" in sys.argv[1:])
