@@ -29,16 +29,14 @@
 namespace aimg {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWaves = kThreads / 64;
 constexpr int kPerOctave = 64;             // bins of a factor of 2
 constexpr int kBins = 4096;
-constexpr int kEach = kBins / kThreads;    // bins, and sorted tokens, of a thread
 constexpr int kList = 4096;                // tokens that are gathered and sorted
 constexpr int kCountShift = 45;            // of a bin's word: count above; below, what its tokens lack to the weight of its top, in 2^-26 of that
 constexpr uint64_t kLackMask = (uint64_t{1} << kCountShift) - 1;
 constexpr int kMaxVocab = 1 << 18;         // so that neither overflows
 constexpr uint32_t kUnits = 1u << 26;
+constexpr int64_t kMaxRows = 1 << 21;      // a launch's threads are counted in 32 bits
 
 struct SampleArgs {
     const void* logits;
@@ -279,7 +277,9 @@ __device__ __forceinline__ Rules rules_of(const SampleArgs& A, int row) {
 
 // What a row's workgroup keeps in LDS. The words are the bins, later the
 // gathered tokens: ~key above, index below.
+template <int kThreads>
 struct Shared {
+    static constexpr int kWaves = kThreads / 64;
     uint64_t words[kBins + 64];
     Octave octave;
     double wave_weight[kWaves], start[kThreads + 1];
@@ -310,8 +310,9 @@ __device__ __forceinline__ double reached(double x, double all) { return x < 1e-
 
 // The words' sums and those bins, by a workgroup. `to` (where not null) takes the
 // sums: of all bins, or of those wanted alone.
-template <bool kAll>
-__device__ __forceinline__ Found find_bins(Shared& S, const Rules& R, const Sums& to) {
+template <bool kAll, int kThreads>
+__device__ __forceinline__ Found find_bins(Shared<kThreads>& S, const Rules& R, const Sums& to) {
+    constexpr int kEach = kBins / kThreads, kWaves = kThreads / 64;
     const int t = threadIdx.x, wave = t >> 6;
     int32_t count[kEach + 1], all_c, my_c = 0;
     double weight[kEach + 1], all_w, my_w = 0.0;
@@ -406,8 +407,8 @@ __device__ __forceinline__ Found find_bins(Shared& S, const Rules& R, const Sums
 // The tokens of those bins among logits thread, thread + threads, .. into the
 // words, which hold kList of them; S.n counts all. Their logits lie in four spans at most, which
 // are tested a piece at a time and first: a place takes ten times as long.
-template <typename L>
-__device__ __forceinline__ void gather(Shared& S, const typename L::Element* row, int n, int thread, int threads, const Places<L>& P, const Found& f) {
+template <typename L, int kThreads>
+__device__ __forceinline__ void gather(Shared<kThreads>& S, const typename L::Element* row, int n, int thread, int threads, const Places<L>& P, const Found& f) {
     Spans spans{};
     auto add = [&](int first, int to) {
         float low, high;
@@ -456,8 +457,9 @@ struct Equals {
 
 enum Goal { kCounted, kReached, kPassed };
 
-template <typename L, Goal kGoal>
-__device__ Equals narrow(const SampleArgs& A, Shared& S, const Sums& B, const typename L::Element* row, const Places<L>& P, int bin, int32_t k, double x) {
+template <typename L, Goal kGoal, int kThreads>
+__device__ Equals narrow(const SampleArgs& A, Shared<kThreads>& S, const Sums& B, const typename L::Element* row, const Places<L>& P, int bin, int32_t k, double x) {
+    constexpr int kEach = kBins / kThreads, kWaves = kThreads / 64;
     uint32_t low = 0, high = 0xFFFFFFFFu;
     int32_t count = B.count[bin];
     double weight = B.weight[bin];
@@ -523,8 +525,8 @@ __device__ Equals narrow(const SampleArgs& A, Shared& S, const Sums& B, const ty
 }
 
 // The index of the j-th token with this key.
-template <typename L>
-__device__ int32_t index_of(const SampleArgs& A, Shared& S, const typename L::Element* row, uint32_t key, int32_t j) {
+template <typename L, int kThreads>
+__device__ int32_t index_of(const SampleArgs& A, Shared<kThreads>& S, const typename L::Element* row, uint32_t key, int32_t j) {
     const int each = (A.vocab + kThreads - 1) / kThreads, from = threadIdx.x * each < A.vocab ? threadIdx.x * each : A.vocab;
     const int to = from + each < A.vocab ? from + each : A.vocab;
     int32_t n = 0, all;
@@ -547,8 +549,8 @@ __device__ int32_t index_of(const SampleArgs& A, Shared& S, const typename L::El
 }
 
 // Where a row's prefixes end and its draw falls, one after the other.
-template <typename L>
-__device__ void resolve_large(const SampleArgs& A, Shared& S, const Sums& B, const typename L::Element* row, const Places<L>& P, const Rules& R,
+template <typename L, int kThreads>
+__device__ void resolve_large(const SampleArgs& A, Shared<kThreads>& S, const Sums& B, const typename L::Element* row, const Places<L>& P, const Rules& R,
                               const Found& f, int32_t& token, double& weight, double& kept) {
     const int bin_k = f.bin_k, bin_m = f.bin_m;
     int32_t most = B.count[kBins];
@@ -664,8 +666,8 @@ __device__ __forceinline__ void sync_as() {
     }
 }
 
-template <bool kWave, int kMine, typename L>
-__device__ __forceinline__ void finish_as(Shared& S, const Sums& B, uint64_t* sums, const Places<L>& P, const Rules& R, int n, const Found& f, double& kept) {
+template <bool kWave, int kMine, typename L, int kThreads>
+__device__ __forceinline__ void finish_as(Shared<kThreads>& S, const Sums& B, uint64_t* sums, const Places<L>& P, const Rules& R, int n, const Found& f, double& kept) {
     const int t = threadIdx.x, wave = t >> 6;
     const int32_t all = B.count[kBins];
     const int bin_k = f.bin_k, bin_m = f.bin_m;
@@ -778,7 +780,8 @@ __device__ __forceinline__ void finish_as(Shared& S, const Sums& B, uint64_t* su
 // Up to kThreads words, in order: each wave sorts 64 in registers, and a word's
 // place is its own there plus the numbers of smaller ones in the other waves',
 // by bisection. (Counting all smaller words took 12 us for 352, not 2.)
-__device__ __forceinline__ void sort_few(Shared& S, int n) {
+template <int kThreads>
+__device__ __forceinline__ void sort_few(Shared<kThreads>& S, int n) {
     const int t = threadIdx.x, lane = t & 63, runs = (n + 63) / 64, mine = t >> 6;
     uint64_t x = t < n ? S.words[t] : ~uint64_t{0};
     if (mine < runs) {
@@ -813,9 +816,10 @@ __device__ __forceinline__ void sort_few(Shared& S, int n) {
 }
 
 // The token, from the S.n gathered ones in the words. sums: room for kList numbers in LDS.
-template <typename L>
-__device__ __forceinline__ void finish(const SampleArgs& A, Shared& S, const Sums& B, uint64_t* sums, const typename L::Element* row, int row_at,
+template <typename L, int kThreads>
+__device__ __forceinline__ void finish(const SampleArgs& A, Shared<kThreads>& S, const Sums& B, uint64_t* sums, const typename L::Element* row, int row_at,
                                        const Places<L>& P, const Rules& R, const Found& f, int n) {
+    constexpr int kEach = kList / kThreads;  // tokens of a thread
     const int t = threadIdx.x;
     if (t < 3) S.end_count[t] = INT32_MAX;
     int32_t token = -1;
@@ -863,13 +867,16 @@ __device__ __forceinline__ bool decided(const SampleArgs& A, int row_at, uint64_
     return true;
 }
 
-__device__ __forceinline__ void clear(Shared& S) {
+template <int kThreads>
+__device__ __forceinline__ void clear(Shared<kThreads>& S) {
     S.octave.make();
     for (int i = threadIdx.x; i < kBins; i += kThreads) S.words[i] = 0;
     if (threadIdx.x == 0) S.n = 0, S.drawn = 0;
 }
 
-__device__ __forceinline__ uint64_t largest_of_waves(Shared& S, uint64_t top) {
+template <int kThreads>
+__device__ __forceinline__ uint64_t largest_of_waves(Shared<kThreads>& S, uint64_t top) {
+    constexpr int kWaves = kThreads / 64;
     if ((threadIdx.x & 63) == 0) S.wave_best[threadIdx.x >> 6] = top;
     __syncthreads();
 #pragma unroll
@@ -878,9 +885,9 @@ __device__ __forceinline__ uint64_t largest_of_waves(Shared& S, uint64_t top) {
 }
 
 // Many rows, or few logits: a workgroup a row.
-template <typename L>
+template <typename L, int kThreads>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
-    __shared__ Shared S;
+    __shared__ Shared<kThreads> S;
     __shared__ double weight[kBins + 1];
     __shared__ int32_t count[kBins + 1];
     __shared__ uint64_t sums[kList];
@@ -905,6 +912,8 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
 // bins; their tokens; by one workgroup, the draw. (Fewer, where the last
 // workgroup of a row to come goes on with what the others wrote, need fences
 // over all L2s: 64 rows 290 us.)
+constexpr int kSliceThreads = 512;
+
 struct Slices {
     uint64_t* tops;      // [rows][n]
     uint64_t* bins;      // [rows][kBins]
@@ -934,52 +943,52 @@ __device__ __forceinline__ uint64_t top_of(const Slices& W, int row) {
 }
 
 template <typename L>
-__global__ __launch_bounds__(kThreads) void sample_top_kernel(const SampleArgs A, const Slices W) {
-    __shared__ uint64_t best[kWaves];
+__global__ __launch_bounds__(kSliceThreads) void sample_top_kernel(const SampleArgs A, const Slices W) {
+    __shared__ uint64_t best[kSliceThreads / 64];
     const int row_at = blockIdx.y, t = threadIdx.x;
-    for (int i = blockIdx.x * kThreads + t; i < kBins; i += W.n * kThreads) W.bins[static_cast<int64_t>(row_at) * kBins + i] = 0;
+    for (int i = blockIdx.x * kSliceThreads + t; i < kBins; i += W.n * kSliceThreads) W.bins[static_cast<int64_t>(row_at) * kBins + i] = 0;
     if (blockIdx.x == 0 && t == 0) W.gathered[row_at] = 0, W.rules[row_at] = rules_of(A, row_at);
-    uint64_t top = largest<L>(static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride, A.vocab, blockIdx.x * kThreads + t,
-                              W.n * kThreads, greedy(A, row_at));
+    uint64_t top = largest<L>(static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride, A.vocab, blockIdx.x * kSliceThreads + t,
+                              W.n * kSliceThreads, greedy(A, row_at));
     if ((t & 63) == 0) best[t >> 6] = top;
     __syncthreads();
-    for (int i = 0; i < kWaves; ++i) top = best[i] > top ? best[i] : top;
+    for (int i = 0; i < kSliceThreads / 64; ++i) top = best[i] > top ? best[i] : top;
     if (t == 0) W.tops[static_cast<int64_t>(row_at) * W.n + blockIdx.x] = top;
 }
 
 template <typename L>
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs A, const Slices W) {
+__global__ __launch_bounds__(kSliceThreads) void sample_bins_kernel(const SampleArgs A, const Slices W) {
     __shared__ uint64_t words[kBins + 64];
     const int row_at = blockIdx.y, t = threadIdx.x;
     const typename L::Element* const row = static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride;
     const Rules R = W.rules[row_at];
     const uint64_t top = top_of(W, row_at);
     if (decided(A, row_at, top, R, blockIdx.x == 0 && t == 0)) return;
-    for (int i = t; i < kBins; i += kThreads) words[i] = 0;
+    for (int i = t; i < kBins; i += kSliceThreads) words[i] = 0;
     __syncthreads();
-    fill_bins<L>(row, A.vocab, blockIdx.x * kThreads + t, W.n * kThreads, places_of<L>(top, R), R, words);
+    fill_bins<L>(row, A.vocab, blockIdx.x * kSliceThreads + t, W.n * kSliceThreads, places_of<L>(top, R), R, words);
     __syncthreads();
     uint64_t* const bins = W.bins + static_cast<int64_t>(row_at) * kBins;
-    for (int i = t; i < kBins; i += kThreads)
+    for (int i = t; i < kBins; i += kSliceThreads)
         if (words[i] != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&bins[i]), words[i]);
 }
 
 // (Each workgroup looks at the bins for itself: a launch for that took 4 us more.)
 template <typename L>
-__global__ __launch_bounds__(kThreads) void sample_gather_kernel(const SampleArgs A, const Slices W) {
-    __shared__ Shared S;
+__global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(const SampleArgs A, const Slices W) {
+    __shared__ Shared<kSliceThreads> S;
     const int row_at = blockIdx.y, t = threadIdx.x;
     const typename L::Element* const row = static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride;
     const Rules R = W.rules[row_at];
     const uint64_t top = top_of(W, row_at);
     if (decided(A, row_at, top, R, false)) return;
     S.octave.make();
-    for (int i = t; i < kBins; i += kThreads) S.words[i] = W.bins[static_cast<int64_t>(row_at) * kBins + i];
+    for (int i = t; i < kBins; i += kSliceThreads) S.words[i] = W.bins[static_cast<int64_t>(row_at) * kBins + i];
     if (t == 0) S.n = 0;
     __syncthreads();
     const Found f = find_bins<false>(S, R, blockIdx.x == 0 ? W.sums(row_at) : Sums{nullptr, nullptr});
     if (blockIdx.x == 0 && t == 0) W.found[row_at] = f;
-    gather<L>(S, row, A.vocab, blockIdx.x * kThreads + t, W.n * kThreads, places_of<L>(top, R), f);
+    gather<L>(S, row, A.vocab, blockIdx.x * kSliceThreads + t, W.n * kSliceThreads, places_of<L>(top, R), f);
     __syncthreads();
     // Its tokens to the row's.
     uint64_t* const list = W.list + static_cast<int64_t>(row_at) * kList;
@@ -988,12 +997,12 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(const SampleArg
     if (t == 0) S.at = atomicAdd(&W.gathered[row_at], n);
     __syncthreads();
     const int32_t at = S.at;
-    for (int i = t; i < n && i < kList && at + i < kList; i += kThreads) list[at + i] = S.words[i];
+    for (int i = t; i < n && i < kList && at + i < kList; i += kSliceThreads) list[at + i] = S.words[i];
 }
 
 template <typename L>
-__global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs A, const Slices W) {
-    __shared__ Shared S;
+__global__ __launch_bounds__(kSliceThreads) void sample_draw_kernel(const SampleArgs A, const Slices W) {
+    __shared__ Shared<kSliceThreads> S;
     __shared__ uint64_t sums[kList];
     const int row_at = blockIdx.x, t = threadIdx.x;
     const typename L::Element* const row = static_cast<const typename L::Element*>(A.logits) + row_at * A.row_stride;
@@ -1003,9 +1012,9 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
     const int32_t n = W.gathered[row_at];
     S.octave.make();
     if (n <= kList) {
-        for (int i = t; i < n; i += kThreads) S.words[i] = W.list[static_cast<int64_t>(row_at) * kList + i];
+        for (int i = t; i < n; i += kSliceThreads) S.words[i] = W.list[static_cast<int64_t>(row_at) * kList + i];
     } else {  // too many tokens to sort: every bin's sums are needed
-        for (int i = t; i < kBins; i += kThreads) S.words[i] = W.bins[static_cast<int64_t>(row_at) * kBins + i];
+        for (int i = t; i < kBins; i += kSliceThreads) S.words[i] = W.bins[static_cast<int64_t>(row_at) * kBins + i];
         __syncthreads();
         find_bins<true>(S, R, W.sums(row_at));
     }
@@ -1019,13 +1028,20 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(const SampleArgs 
 namespace aimg {
 namespace {
 
-// Workgroups a row; 0: one, in one launch. Logits that one workgroup reads as
-// fast as four launches follow each other (32000 of bf16: 29 us, 32 dealt out;
-// 50001: 35, 33; 151936: 54, 33), and rows that fill the card (256 rows of
-// 151936: 87 us, 99; 128: 85, 78), are not dealt out. Otherwise 512 in all: 64
-// rows in 8 each 58 us, in 4 61, in 16 65.
+// Threads of a row's only workgroup: 1024 where its logits are many, which are
+// read and put into bins faster by more waves; else 512, since what comes after
+// the bins costs more barriers' time the more waves there are. (32000 logits of
+// 16 bits: 27.2 us with 512, 27.4 with 1024; 4096: 17.9 and 21.6; 256 rows of
+// 151936: 107 and 90. 256 rows of 32000 in fp32: 44.0 and 39.1.)
+constexpr int64_t kWideBytes = 96 << 10;
+
+// Workgroups a row; 0: one, in one launch. Four launches cost some 7 us more, and
+// each workgroup looks at all bins, so several pay for long rows and while they
+// fill the chip: of 65536 logits with top_p 0.9, 1 row took 36 us by one
+// workgroup and 28 by eight, 37 rows 42 and 39 (by four), 100 rows 52 and 53; of
+// 50001, 37 rows 39 and 38; of 151936, 100 rows 77 and 79.
 int slices_of(int64_t n_rows, int vocab) {
-    if (n_rows < 1 || n_rows >= 192 || vocab < 40000) return 0;
+    if (n_rows < 1 || n_rows >= 96 || vocab < 65536) return 0;
     const int64_t most = (vocab + 8191) / 8192, n = 512 / n_rows;
     return static_cast<int>(n < 4 ? 4 : n < most ? n : most);
 }
@@ -1044,9 +1060,10 @@ size_t slices_at(Slices& w, char* at, int64_t rows) {
 
 template <typename L>
 void launch_sample(const SampleArgs& a, int64_t n_rows, const Slices& w, hipStream_t s) {
-    const dim3 rows(static_cast<uint32_t>(n_rows)), slices(static_cast<uint32_t>(w.n), static_cast<uint32_t>(n_rows)), block(kThreads);
+    const dim3 rows(static_cast<uint32_t>(n_rows)), slices(static_cast<uint32_t>(w.n), static_cast<uint32_t>(n_rows)), block(kSliceThreads);
     if (w.n == 0) {
-        hipLaunchKernelGGL((sample_kernel<L>), rows, block, 0, s, a);
+        if (static_cast<int64_t>(a.vocab) * sizeof(typename L::Element) < kWideBytes) hipLaunchKernelGGL((sample_kernel<L, 512>), rows, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((sample_kernel<L, 1024>), rows, dim3(1024), 0, s, a);
         return;
     }
     hipLaunchKernelGGL((sample_top_kernel<L>), slices, block, 0, s, a, w);
@@ -1056,8 +1073,8 @@ void launch_sample(const SampleArgs& a, int64_t n_rows, const Slices& w, hipStre
 }
 
 int check_sample(int64_t n_rows, int vocab) {
-    if (n_rows < 0 || n_rows > INT32_MAX || vocab < 1) return fail(AIMG_ERR_INVALID_ARGUMENT, "sample: n_rows must be in 0..2^31-1 and vocab at least 1");
-    if (vocab > kMaxVocab) return fail(AIMG_ERR_UNSUPPORTED, "sample: vocab must be at most 2^18");
+    if (n_rows < 0 || vocab < 1) return fail(AIMG_ERR_INVALID_ARGUMENT, "sample: n_rows must not be negative and vocab at least 1");
+    if (vocab > kMaxVocab || n_rows > kMaxRows) return fail(AIMG_ERR_UNSUPPORTED, "sample: vocab must be at most 2^18 and n_rows 2^21");
     return AIMG_OK;
 }
 

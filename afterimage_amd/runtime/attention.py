@@ -35,7 +35,7 @@ _BLOCK = 16  # positions that share a scale in a cache of 8 bits
 def forward_only(x: torch.Tensor, name: str) -> None:
     """Refuses a tensor whose gradient autograd would expect."""
     if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("%s requires a gradient, and attention has no backward pass: detach it, or call under torch.no_grad()" % name)
+        raise RuntimeError("%s requires a gradient, and this call has no backward pass: detach it, or call under torch.no_grad()" % name)
 
 
 def _heads(x: torch.Tensor, name: str, dtype: torch.dtype, index: int, unit: int = 8) -> _native.AimgHeads:

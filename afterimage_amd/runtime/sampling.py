@@ -19,6 +19,7 @@ from .. import _native
 from .attention import forward_only, launch
 
 MAX_VOCAB = 1 << 18
+MAX_ROWS = 1 << 21
 
 _TYPES = {torch.bfloat16: _native.AIMG_BF16, torch.float16: _native.AIMG_FP16, torch.float32: _native.AIMG_FP32}
 
@@ -40,7 +41,7 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float |
            top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
            logprobs: bool = False, out: torch.Tensor | None = None):
     """A token for each row of logits [rows, vocab] (bf16, fp16 or fp32, any
-    row stride, vocab up to 2^18), from uniforms [rows] (fp32, in [0, 1)).
+    row stride, vocab up to 2^18, up to 2^21 rows), from uniforms [rows] (fp32, in [0, 1)).
 
     A row's tokens stand in the order of falling logits, equal ones by rising
     index, and weigh w = exp((x - max) / temperature). Kept are those among the
@@ -55,8 +56,8 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float |
     Returns int64 tokens [rows] (out where given), with logprobs the
     logarithms (fp32) of the tokens' shares of the sums kept besides. Logits of
     -inf or NaN are no tokens; a row without any other gives -1 (and -inf).
-    Results do not vary between calls. No gradients: logits that require one
-    are refused outside torch.no_grad()."""
+    Results do not vary between calls. No gradients: logits or settings that
+    require one are refused outside torch.no_grad()."""
     index, kind = logits.get_device(), _TYPES.get(logits.dtype)
     if index < 0:
         raise RuntimeError("sample runs on the GPU only; got logits on %s" % logits.device)
@@ -65,11 +66,14 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, *, temperature: float |
     rows, vocab = logits.shape
     if vocab > MAX_VOCAB:
         raise ValueError("logits: vocab must be at most %d, got %d" % (MAX_VOCAB, vocab))
+    if rows > MAX_ROWS:
+        raise ValueError("logits: at most %d rows, got %d" % (MAX_ROWS, rows))
     forward_only(logits, "logits")
     settings = _native.AimgSampling(temperature=1.0, top_p=1.0)
     for name, value, dtype, least, most in (("temperature", temperature, torch.float32, 0.0, None), ("top_k", top_k, torch.int32, 0, None),
                                             ("top_p", top_p, torch.float32, 0.0, 1.0), ("min_p", min_p, torch.float32, 0.0, 1.0)):
         if isinstance(value, torch.Tensor):
+            forward_only(value, name)
             setattr(settings, name + "s", _vector(value, name, dtype, rows, index))
         elif not value >= least or (most is not None and value > most):
             raise ValueError("%s must be %s, got %r" % (name, "at least 0" if most is None else "in 0..1", value))

@@ -558,8 +558,8 @@ typedef struct aimg_sampling {
 } aimg_sampling;
 
 /*
- * A token for each of n_rows rows of `vocab` logits (at most 2^18), rows
- * row_stride elements apart, of type bf16, fp16 or fp32. A row's tokens stand
+ * A token for each of n_rows (at most 2^21) rows of `vocab` logits (at most
+ * 2^18), row_stride elements apart, of type bf16, fp16 or fp32. A row's tokens stand
  * in the order of falling logits, equal ones by rising index; with w = exp((x -
  * max x) / temperature) those are kept that are among the first top_k, in the
  * shortest prefix whose weights reach top_p times the first top_k's, and

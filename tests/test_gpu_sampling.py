@@ -33,20 +33,12 @@ def define(x, u, t, k, p, m):
     w = torch.where(x == x[0], 1.0, torch.exp((x - x[0]) / t))
     if k > 0:
         w[k:] = 0
-    if m > 0:
-        w = w * (w >= min(m, 1.0))
-        n_m = int((w > 0).sum())
-        full = torch.where(x == x[0], 1.0, torch.exp((x - x[0]) / t))
-        if k > 0:
-            full[k:] = 0
-    else:
-        n_m, full = int((w > 0).sum()), w
-    cum = full.cumsum(0)
-    total = float(cum[-1])
+    cum = w.cumsum(0)
+    heavy = int((w >= min(m, 1.0)).sum()) if m > 0 else int((w > 0).sum())
     ends = []
     for move in (-NEAR, NEAR):
-        n = int((cum - full < (max(p, 0.0) + move) * total).sum()) if p < 1 else len(w)
-        ends.append(max(1, min(n, n_m)))
+        n = int((cum - w < (max(p, 0.0) + move) * float(cum[-1])).sum()) if p < 1 else len(w)
+        ends.append(max(1, min(n, heavy)))
     low, high = (float(cum[n - 1]) for n in ends)
     first = int((cum <= u * low - NEAR * high).sum())
     last = min(int((cum <= u * high + NEAR * high).sum()), ends[1] - 1)

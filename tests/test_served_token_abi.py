@@ -112,7 +112,7 @@ def test_attention_over_eight_bits_refuses(args, code, message):
 
 
 @pytest.mark.parametrize("args,code,message", [
-    (dict(rows=-1), BAD, b"n_rows"), (dict(vocab=0), BAD, b"vocab"), (dict(vocab=(1 << 18) + 1), UNSUPPORTED, b"2^18"), (dict(stride=-1), BAD, b"row_stride"),
+    (dict(rows=-1), BAD, b"n_rows"), (dict(vocab=0), BAD, b"vocab"), (dict(vocab=(1 << 18) + 1), UNSUPPORTED, b"2^18"), (dict(rows=(1 << 21) + 1), UNSUPPORTED, b"2^21"), (dict(stride=-1), BAD, b"row_stride"),
     (dict(kind=3), UNSUPPORTED, b"type"), (dict(logits=None), BAD, b"null"), (dict(uniforms=None), BAD, b"null"), (dict(tokens=None), BAD, b"null"),
     (dict(settings=None), BAD, b"settings"), (dict(logits=AT + 1), UNSUPPORTED, b"aligned"), (dict(tokens=AT + 4), UNSUPPORTED, b"aligned"),
     (dict(logits=AT + 2, kind=2), UNSUPPORTED, b"aligned"), (dict(vocab=100000), BAD, b"workspace"), (dict(vocab=100000, work=AT, nbytes=100), BAD, b"workspace"),
