@@ -291,7 +291,7 @@ __device__ __forceinline__ int32_t row_bound(const int32_t* offsets, int b, int3
 
 // The last sequence whose place is at most `at`, by the whole wave: its lanes
 // look at 64 sequences at once (steps one after the other cost a memory latency
-// each: 64 single tokens took 9.5 us, not 7).
+// each: 64 single tokens' append took 9.2 us, not 8.9).
 template <typename Place>
 __device__ __forceinline__ int last_before(int n_seqs, int64_t at, Place place) {
     const int lane = threadIdx.x & 63;
@@ -589,7 +589,11 @@ __device__ __forceinline__ void form_block(const TurnArgs& A, uint32_t item, int
     if (lane == 0) *scale = now;
 }
 
-// Blocks first, four a workgroup, then a workgroup a row. NP: 0 for a cache in 16 bits.
+// Blocks first, four a workgroup, then a workgroup a row. NP: 0 for a cache in
+// 16 bits. Many rows are bound by HBM: 16384 rows of 40 heads and 2 * 8 of 128,
+// 478 MB read and written in 88 us, 5.4 TB/s; 8192 rows into 8 bits, 223 MB in 45
+// to 53 us. A token is bound by its reads that wait for each other (its sequence,
+// slot, length, page, block): one 5 us, 64 in sequences of their own 9.
 template <typename T, int kMode, int NP>
 __global__ __launch_bounds__(256) void turn_kernel(const TurnArgs A) {
     uint32_t group = blockIdx.x;
@@ -620,7 +624,10 @@ struct ReadArgs {
 constexpr int kReadRows = 8;  // of a workgroup
 
 // Eight threads find where a workgroup's rows lie, then all move pieces of 8
-// elements: a thread keeps its place in a head and takes it from row after row.
+// elements: a thread keeps its place in a head and takes it from row after row,
+// eight pieces on their way at once. Bound by HBM: 23912 rows of 2 * 8 heads of
+// 128 from 8 bits, 147 MB read and written in 36 us, 4.1 TB/s; 16384 rows of 16
+// bits that were just written, 134 MB in 23 us.
 template <typename T, bool k8>
 __global__ __launch_bounds__(256) void read_kernel(const ReadArgs A) {
     const Cache& C = A.c;
@@ -880,7 +887,8 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(const ForkArgs A) {
 }
 
 // The scales of the tails' blocks: a thread a scale and step. (A launch of its
-// own, for caches in 8 bits alone, before the rows change.)
+// own, for caches in 8 bits alone, before the rows change: 5 us for 96 branches
+// in 80 planes, beside the rows' 111.)
 __global__ __launch_bounds__(256) void fork_scales_kernel(const ForkArgs A) {
     const Cache& C = A.c;
     const int i = blockIdx.x;
@@ -993,7 +1001,10 @@ __global__ __launch_bounds__(256) void commit_kernel(const CommitArgs A) {
 // below the length and those of the path, from wherever they lie, are held in
 // registers before any is written. Sources lie at or behind their own places,
 // so what one block writes no later block reads. A block with a place that is
-// no page's stays as it is.
+// no page's stays as it is. 64 sequences of up to 12 accepted rows, 6 on average,
+// in 80 planes of 8 heads of 128: 53 us; in 16 bits, where rows move without a
+// look at their elements, 14. (Eight heads a wave, which finds the places once:
+// 66; rows not written that stay as they are: 57.)
 template <int NP>
 __global__ __launch_bounds__(256) void commit8_kernel(const CommitArgs A) {
     const Cache& C = A.c;
