@@ -464,7 +464,7 @@ struct Equals {
 enum Goal { kCounted, kReached, kPassed };
 
 template <typename L, Goal kGoal, int kThreads>
-__device__ Equals narrow(const SampleArgs& A, Shared<kThreads>& S, const Sums& B, const typename L::Element* row, const Places<L>& P, int bin, int32_t k, double x) {
+__device__ __forceinline__ Equals narrow(const SampleArgs& A, Shared<kThreads>& S, const Sums& B, const typename L::Element* row, const Places<L>& P, int bin, int32_t k, double x) {
     constexpr int kEach = kBins / kThreads, kWaves = kThreads / 64;
     uint32_t low = 0, high = 0xFFFFFFFFu;
     int32_t count = B.count[bin];
@@ -532,7 +532,7 @@ __device__ Equals narrow(const SampleArgs& A, Shared<kThreads>& S, const Sums& B
 
 // The index of the j-th token with this key.
 template <typename L, int kThreads>
-__device__ int32_t index_of(const SampleArgs& A, Shared<kThreads>& S, const typename L::Element* row, uint32_t key, int32_t j) {
+__device__ __forceinline__ int32_t index_of(const SampleArgs& A, Shared<kThreads>& S, const typename L::Element* row, uint32_t key, int32_t j) {
     const int each = (A.vocab + kThreads - 1) / kThreads, from = threadIdx.x * each < A.vocab ? threadIdx.x * each : A.vocab;
     const int to = from + each < A.vocab ? from + each : A.vocab;
     int32_t n = 0, all;
@@ -556,7 +556,7 @@ __device__ int32_t index_of(const SampleArgs& A, Shared<kThreads>& S, const type
 
 // Where a row's prefixes end and its draw falls, one after the other.
 template <typename L, int kThreads>
-__device__ void resolve_large(const SampleArgs& A, Shared<kThreads>& S, const Sums& B, const typename L::Element* row, const Places<L>& P, const Rules& R,
+__device__ __forceinline__ void resolve_large(const SampleArgs& A, Shared<kThreads>& S, const Sums& B, const typename L::Element* row, const Places<L>& P, const Rules& R,
                               const Found& f, int32_t& token, double& weight, double& kept) {
     const int bin_k = f.bin_k, bin_m = f.bin_m;
     int32_t most = B.count[kBins];
