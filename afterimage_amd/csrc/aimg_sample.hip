@@ -17,11 +17,12 @@
 // atomics that add them; sums of bins are doubles, in a fixed order. Tokens
 // below 2^-64 of the largest weigh nothing.
 //
-// A row is read three times, from HBM once. 256 rows of 151936 logits of 16 bits
-// (78 MB, 15 us at a copy's rate): 70 us, of which the largest takes the 15, the
-// bins 18 (some twenty instructions and an atomic in LDS a token), the gather 13
-// and the steps between them, which wait for each other, the rest. 64 rows with
-// settings of their own, by several workgroups each: 57 us; one row 28.
+// A row is read three times. 256 rows of 151936 logits of 16 bits (78 MB a time,
+// 15 us at a copy's rate): 56 us. The largest takes HBM's time for them; the bins
+// (some twenty instructions and an atomic in LDS a token) and the gather are
+// instructions, 42% of a SIMD's cycles, LDS 25%; the steps between them wait for
+// each other. 64 rows with settings of their own, by several workgroups each: 46
+// us; one row 24.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -914,8 +915,8 @@ __device__ __forceinline__ uint64_t largest_of_waves(Shared<kThreads>& S, uint64
     return top;
 }
 
-// Many rows, or few logits: a workgroup a row. 256 rows of 151936 70 us, 37 of
-// 50001 in fp32 28, one of 4096 18.
+// Many rows, or few logits: a workgroup a row. 256 rows of 151936 56 us, 37 of
+// 50001 in fp32 24, one of 4096 13.
 template <typename L, int kThreads>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
     __shared__ Shared<kThreads> S;
@@ -941,7 +942,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
 
 // Fewer rows: `n` workgroups a row, in four launches: the largest logit; the
 // bins; their tokens; by one workgroup, the draw. One row of 151936 in 19 slices
-// 3.4, 4.3, 12.4 and 8.4 us, 64 rows in 8 slices 6.4, 11.1, 24.1 and 15.4: from
+// 3.2, 4.4, 12.1 and 5.4 us, 64 rows in 4 slices 8.6, 10.4, 17.8 and 10.7: from
 // the gather on, sums over the bins and steps of a sort that wait for each
 // other, not HBM (0.06 and 4 us). (Fewer launches, where the last
 // workgroup of a row to come goes on with what the others wrote, need fences
@@ -1063,20 +1064,25 @@ namespace aimg {
 namespace {
 
 // Threads of a row's only workgroup: 1024 where its logits are many, which are
-// read and put into bins faster by more waves; else 512, since what comes after
-// the bins costs more barriers' time the more waves there are. (32000 logits of
-// 16 bits: 27.2 us with 512, 27.4 with 1024; 4096: 17.9 and 21.6; 256 rows of
-// 151936: 107 and 90. 256 rows of 32000 in fp32: 44.0 and 39.1.)
-constexpr int64_t kWideBytes = 96 << 10;
+// read and put into bins faster by more waves; else 512, since barriers cost
+// more the more waves there are. (256 rows with top_p 0.9, by 512 and by 1024:
+// of 4096 logits of 16 bits 13.8 us and 15.2, 16384 20.4 and 20.2, 32000 25.7
+// and 23.8, 151936 85.7 and 63.9; of 16384 in fp32 18.3 and 18.2, 32000 31.3 and
+// 25.7.)
+constexpr int64_t kWideBytes = 48 << 10;
 
-// Workgroups a row; 0: one, in one launch. Four launches cost some 7 us more, and
-// each workgroup looks at all bins, so several pay for long rows and while they
-// fill the chip: of 65536 logits with top_p 0.9, 1 row took 36 us by one
-// workgroup and 28 by eight, 37 rows 42 and 39 (by four), 100 rows 52 and 53; of
-// 50001, 37 rows 39 and 38; of 151936, 100 rows 77 and 79.
+// Workgroups a row; 0: one, in one launch. Four launches, and bins that each
+// workgroup looks at for itself, pay where rows are long and do not fill the
+// chip. Of 151936 logits, with all kept and with top_p 0.9, by one workgroup and
+// by several: 1 row 33 and 42 us, 22 and 27 by 16; 16 rows 44 and 46, 34 and 34 by
+// 8; 48 rows 43 and 49, 42 and 44 by 4; 64 rows 45 and 52, 45 and 59 by 4, in fp32
+// 56 and 66, 51 and 55, and 55 and 46 where rows have settings of their own; 96 in
+// fp32 60 and 67, 60 and 65. Of 100000: 1
+// row 27 and 33, 21 and 27; 37 rows 34 and 37, 35 and 37. Of 65536, 1 row: 22 and
+// 26, 21 and 25.
 int slices_of(int64_t n_rows, int vocab) {
-    if (n_rows < 1 || n_rows >= 96 || vocab < 65536) return 0;
-    const int64_t most = (vocab + 8191) / 8192, n = 512 / n_rows;
+    if (n_rows < 1 || n_rows > 64 || vocab < 90000) return 0;
+    const int64_t most = (vocab + 8191) / 8192, n = 256 / n_rows;
     return static_cast<int>(n < 4 ? 4 : n < most ? n : most);
 }
 
