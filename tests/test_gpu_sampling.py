@@ -92,6 +92,14 @@ def test_large_vocabularies(dtype):
             compare(x, u, t, k, p, m)
 
 
+@pytest.mark.parametrize("rows", [64, 65])
+def test_many_rows_of_a_large_vocabulary(rows):
+    """On both sides of where a row's work is dealt out."""
+    x, u = inputs(rows, 90001, torch.bfloat16, seed=rows)
+    for t, k, p, m in [(1.0, 0, 0.9, 0.0), (0.8, 50, 0.95, 0.01)]:
+        compare(x, u, t, k, p, m)
+
+
 def test_settings_of_their_own_for_each_row():
     x, u = inputs(40, 3001, torch.float32, seed=4)
     g = torch.Generator().manual_seed(4)
@@ -136,7 +144,7 @@ def test_ruled_out_tokens(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("vocab", [9000, 151936])
+@pytest.mark.parametrize("vocab", [9000, 60000, 151936])
 def test_many_equal_logits(dtype, vocab):
     """A bin holds more tokens than are sorted: equal logits, few values, very high temperatures."""
     g = torch.Generator(device="cuda").manual_seed(vocab)
