@@ -622,6 +622,7 @@ struct ReadArgs {
 };
 
 constexpr int kReadRows = 8;  // of a workgroup
+constexpr int64_t kMostGroups = (1 << 24) - 1;  // of 256 threads, which a launch counts in 32 bits
 
 // Eight threads find where a workgroup's rows lie, then all move pieces of 8
 // elements: a thread keeps its place in a head and takes it from row after row,
@@ -1338,7 +1339,7 @@ extern "C" int aimg_cache_append_rotated(const aimg_cache* cache, float* scales,
     const int64_t rows = k->n_rows;
     if (n_seqs == 0 || rows == 0) return AIMG_OK;
     const int64_t items = scales != nullptr ? (rows / aimg::kBlock + 2 * static_cast<int64_t>(n_seqs)) * cache->kv_heads * 2 : 0;
-    if (items > INT32_MAX || (items + 3) / 4 + rows > INT32_MAX) return fail(AIMG_ERR_UNSUPPORTED, "too many rows");
+    if (items > INT32_MAX || (items + 3) / 4 + rows > aimg::kMostGroups) return fail(AIMG_ERR_UNSUPPORTED, "too many rows");
     a.n_items = static_cast<uint32_t>(items);
     if (q != nullptr) {
         a.q = static_cast<const uint16_t*>(q->data), a.q_out = static_cast<uint16_t*>(q_out->data), a.heads = q->heads;
@@ -1366,6 +1367,7 @@ extern "C" int aimg_cache_read(const aimg_cache* cache, float* scales, int layer
     if (rc != AIMG_OK) return rc;
     if (v->n_rows != k->n_rows) return fail(AIMG_ERR_INVALID_ARGUMENT, "k and v must have the same rows");
     if (n_seqs == 0 || k->n_rows == 0) return AIMG_OK;
+    if ((k->n_rows + aimg::kReadRows - 1) / aimg::kReadRows > aimg::kMostGroups) return fail(AIMG_ERR_UNSUPPORTED, "too many rows");
     a.k = static_cast<uint16_t*>(k->data), a.v = static_cast<uint16_t*>(v->data);
     a.k_row = k->row_stride, a.k_head = k->head_stride, a.v_row = v->row_stride, a.v_head = v->head_stride;
     a.seqs = seqs, a.offsets = offsets, a.starts = starts, a.n_seqs = n_seqs, a.n_rows = static_cast<int32_t>(k->n_rows), a.plane = 2 * layer;

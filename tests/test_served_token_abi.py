@@ -46,6 +46,7 @@ def _append(cache=None, scales=None, layer=0, q="", k=None, v=None, out=None, se
     (dict(cache=_cache(dim=72), scales=AT), UNSUPPORTED, b"multiple of 16"), (dict(cache=_cache(page_size=24), scales=AT), UNSUPPORTED, b"page_size"),
     (dict(scales=AT + 2), UNSUPPORTED, b"4-byte"), (dict(cache=_cache(dim=272), scales=AT), UNSUPPORTED, b"up to 256"),
     (dict(q=None, k=_heads(n=(1 << 31) - 9), n=1, scales=AT), UNSUPPORTED, b"too many rows"),
+    (dict(q=_heads(n=1 << 24, heads=4), k=_heads(n=1 << 24)), UNSUPPORTED, b"too many rows"),
 ])
 def test_append_rotated_refuses(args, code, message):
     assert _append(**args) == code
@@ -67,6 +68,7 @@ def test_nothing_to_do_is_no_error():
 @pytest.mark.parametrize("args,code,message", [
     (dict(layer=5), BAD, b"layer"), (dict(k=_heads(heads=1)), BAD, b"k must have"), (dict(v=_heads(n=3)), BAD, b"same rows"), (dict(kind=7), UNSUPPORTED, b"type"),
     (dict(k=_heads(row=4)), UNSUPPORTED, b"16 bytes"), (dict(scales=AT, cache=_cache(page_size=8)), UNSUPPORTED, b"page_size"), (dict(n=-2), BAD, b"n_seqs"),
+    (dict(k=_heads(n=(1 << 27) + 1), v=_heads(n=(1 << 27) + 1)), UNSUPPORTED, b"too many rows"),
 ])
 def test_read_refuses(args, code, message):
     a = dict(cache=_cache(), scales=None, layer=0, k=_heads(), v=_heads(), n=1, kind=0) | args
