@@ -232,6 +232,9 @@ class PagedKVCache:
             raise ValueError("cos must be a contiguous fp32 [positions, up to %d] tensor on cuda:%d" % (self.dim // 2, index))
         if sin.shape != table or sin.dtype is not torch.float32 or sin.get_device() != index or not sin.is_contiguous():
             raise ValueError("sin must have cos' shape, type and device")
+        if cos.requires_grad or sin.requires_grad:
+            forward_only(cos, "cos")
+            forward_only(sin, "sin")
         at, n = self._seqs(seqs)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)

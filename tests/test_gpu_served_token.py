@@ -245,6 +245,8 @@ def test_refusals():
         wide.read(0, slots, offsets, 2, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="no backward"):
         turned(q=q.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="sin requires"):
+        turned(sin=sin.clone().requires_grad_())
     with pytest.raises(ValueError, match="scales"):
         PagedKVCache(cache.pool, cache.page_table, cache.lengths, cache.held, cache.refs, cache.status)
     with pytest.raises(ValueError, match="scales"):
@@ -262,5 +264,7 @@ def test_refusals():
     for logits, text in ((x.double(), "bf16"), (x.t(), "contiguous"), (x[0], "rows"), (torch.zeros(1, (1 << 18) + 1, device="cuda"), "vocab")):
         with pytest.raises(ValueError, match=text):
             sample(logits, u)
+    with pytest.raises(RuntimeError, match="no backward"):
+        sample(x, u, temperature=torch.ones(2, device="cuda").requires_grad_())
     with pytest.raises(RuntimeError, match="no backward"):
         sample(x.requires_grad_(), u)
