@@ -568,8 +568,9 @@ typedef struct aimg_sampling {
  * nearest there) times those of all that are kept, and logprobs[row] (where not
  * NULL) the logarithm of its share of them: 0 at temperature 0. Logits of -inf or
  * NaN are no tokens; a row without any other gives -1 and -inf. Weights below
- * 2^-64 of the largest count as nothing, the others are sums of 2^-26 of
- * themselves, in integers and doubles: results do not vary between calls.
+ * 2^-64 of the largest (at any temperature those of logits 2^128 below it) count
+ * as nothing, the others are sums of 2^-26 of themselves, in integers and
+ * doubles: results do not vary between calls.
  * aimg_sample_workspace_nbytes gives the device scratch memory a call needs
  * (8-byte aligned; 0 for many rows or few logits): few rows are dealt out.
  */
