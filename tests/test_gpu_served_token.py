@@ -181,6 +181,26 @@ def test_two_graphs_and_two_streams_at_once():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(a, want[0])
 
 
+def test_long_rows_sampled_from_a_graph():
+    """Rows that several workgroups share: every replay starts from its own inputs, whatever eager calls ran in between."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, u = torch.empty(3, 100000, device="cuda", dtype=torch.bfloat16), torch.empty(3, device="cuda")
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    x.normal_(generator=g), u.uniform_(generator=g)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        sample(x, u, top_p=0.9)
+    torch.cuda.current_stream().wait_stream(stream)
+    with torch.cuda.graph(graph):
+        tokens, logs = sample(x, u, top_p=0.9, logprobs=True)
+    for spread in (2.5, 1e-3, 0.0, 4.0, 2.5):
+        x.normal_(generator=g).mul_(spread), u.uniform_(generator=g)
+        graph.replay()
+        want, want_logs = sample(x, u, top_p=0.9, logprobs=True)
+        torch.cuda.synchronize()
+        assert torch.equal(tokens, want) and torch.equal(logs, want_logs)
+
+
 def test_calls_on_another_stream():
     g = torch.Generator().manual_seed(5)
     tables = rotary_tables(64, DIM)
