@@ -1076,10 +1076,9 @@ constexpr int64_t kWideBytes = 48 << 10;
 // chip. Of 151936 logits, with all kept and with top_p 0.9, by one workgroup and
 // by several: 1 row 33 and 42 us, 22 and 27 by 16; 16 rows 44 and 46, 34 and 34 by
 // 8; 48 rows 43 and 49, 42 and 44 by 4; 64 rows 45 and 52, 45 and 59 by 4, in fp32
-// 56 and 66, 51 and 55, and 55 and 46 where rows have settings of their own; 96 in
-// fp32 60 and 67, 60 and 65. Of 100000: 1
-// row 27 and 33, 21 and 27; 37 rows 34 and 37, 35 and 37. Of 65536, 1 row: 22 and
-// 26, 21 and 25.
+// 56 and 66, 51 and 55; with settings of its own for each row 55 by one and 46 by
+// 4; 96 rows in fp32 60 and 67, 60 and 65. Of 100000: 1 row 27 and 33, 21 and 27;
+// 37 rows 34 and 37, 35 and 37. Of 65536, 1 row: 22 and 26, 21 and 25.
 int slices_of(int64_t n_rows, int vocab) {
     if (n_rows < 1 || n_rows > 64 || vocab < 90000) return 0;
     const int64_t most = (vocab + 8191) / 8192, n = 256 / n_rows;
