@@ -11,8 +11,8 @@
 // bins' tokens (a few hundred, mostly) are gathered and sorted.
 //
 // Sums. A token's place t = 64 log2(1 / w) is computed as a pair of floats
-// (doubles run at half the rate); its whole part is its bin, and its weight
-// against the bin's top is rounded to 2^-26. A bin's count and sum are integers
+// (doubles run at half the rate); the first's whole part is its bin, and its
+// weight against the bin's top, by both, is rounded to 2^-26. A bin's count and sum are integers
 // in one 64-bit word, so a row's result does not depend on the order of the
 // atomics that add them; sums of bins are doubles, in a fixed order. Tokens
 // below 2^-64 of the largest weigh nothing.
@@ -39,10 +39,12 @@ namespace {
 constexpr int kPerOctave = 64;             // bins of a factor of 2
 constexpr int kBins = 4096;
 constexpr int kList = 4096;                // tokens that are gathered and sorted
-constexpr int kCountShift = 45;            // of a bin's word: count above; below, what its tokens lack to the weight of its top, in 2^-26 of that
+constexpr double kStray = 0x1p-10;         // a token's place lies less than this outside its bin (see Place)
+constexpr int kCountShift = 45;            // of a bin's word: count above; below, what its tokens lack to kMostUnits, in 2^-26 of the weight of its top
 constexpr uint64_t kLackMask = (uint64_t{1} << kCountShift) - 1;
 constexpr int kMaxVocab = 1 << 18;         // so that neither overflows
 constexpr uint32_t kUnits = 1u << 26;
+constexpr uint32_t kMostUnits = kUnits + 1024;  // a token that lies kStray above its bin weighs 710 units more than the bin's top
 constexpr int64_t kMaxRows = 1 << 21;      // a launch's threads are counted in 32 bits
 
 struct SampleArgs {
@@ -153,11 +155,15 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
 // A token's place: how far below the largest, 64 to a factor of 2, as the whole
-// part `bin` and the rest f, which may leave [0, 1) by its rounding. What the
-// product loses in 32 bits goes into the rest, and so does what max - x loses,
-// for fp32 logits. (Logits of 16 bits lose nothing unless 2^16 apart, and then
-// 2^-25 of the difference at most.) Bins rise as the logits fall, for both
-// roundings keep the order. An infinite maximum leaves its equals alone at 0.
+// part `bin` of t, its value in 32 bits, and the rest f. What the product loses
+// in 32 bits goes into the rest, and so does what max - x loses, for fp32
+// logits: half a step of t (2^-13 below 4096) and 2^-24 of t for the difference's
+// rounding and the factor's each, less than kStray together, by which f may lie
+// outside [0, 1). (Of 16 bits, bf16 logits lose nothing unless 2^16 apart in
+// size and fp16 unless 2^13, and then 2^-24 of the difference at most.) Bins rise
+// as the logits fall, for both roundings keep the order; on which side of a
+// border between two bins a place this near to it lies, they do not say. An
+// infinite maximum leaves its equals alone at 0.
 struct Place {
     float t;  // the bin's number and more; from kBins on, or NaN: no weight
     float f;
@@ -244,16 +250,17 @@ struct Spans {
     }
 };
 
-// What 2^(-f / 64) lacks to 1, in 2^-26 and rounded, for f in [0, 1]: its series
-// in g = f ln 2 / 64 < 0.011, whose fourth term is below 2^-30.
+// What 2^(-f / 64) lacks to kMostUnits, in 2^-26 and rounded, for f in [-kStray,
+// 1 + kStray], where it is above 0: the series of 1 - 2^(-f / 64) in g = f ln 2 / 64 < 0.011,
+// whose fourth term is below 2^-30.
 __device__ __forceinline__ uint32_t lack_in_bin(float f) {
     constexpr float g = 0.6931471805599453f / kPerOctave;
-    return static_cast<uint32_t>(fmaf(f, fmaf(f, fmaf(f, g * g * g / 6.0f * kUnits, -g * g / 2.0f * kUnits), g * kUnits), 0.5f));
+    return static_cast<uint32_t>(fmaf(f, fmaf(f, fmaf(f, g * g * g / 6.0f * kUnits, -g * g / 2.0f * kUnits), g * kUnits), kMostUnits - kUnits + 0.5f));
 }
 
-__device__ __forceinline__ uint64_t word_of(const Place& p) { return uint64_t{1} << kCountShift | lack_in_bin(p.f); }
+__device__ __forceinline__ uint64_t word_of(float f) { return uint64_t{1} << kCountShift | lack_in_bin(f); }
 __device__ __forceinline__ int32_t count_of(uint64_t word) { return static_cast<int32_t>(word >> kCountShift); }
-__device__ __forceinline__ uint64_t units_of(uint64_t word) { return (word >> kCountShift) * kUnits - (word & kLackMask); }
+__device__ __forceinline__ uint64_t units_of(uint64_t word) { return (word >> kCountShift) * kMostUnits - (word & kLackMask); }
 
 // 2^(-i / 64), i < 64: a table that a workgroup makes once (exp2 for every bin took longer than their sums).
 struct Octave {
@@ -316,8 +323,8 @@ struct Shared {
     double wave_weight[kWaves], start[kThreads + 1];
     uint64_t wave_best[kWaves];
     int32_t wave_count[kWaves], wave_first[kWaves];
-    double found_low[6], found_high[6], end_weight[3], found_weight;
-    int32_t found[6], end_count[3], n, drawn, before_count, inside_count;
+    double found_low[7], found_high[7], end_weight[3], found_weight;
+    int32_t found[7], end_count[3], n, drawn, before_count, inside_count;
     uint64_t inside;
     int32_t at;
 };
@@ -329,11 +336,12 @@ struct Sums {
 };
 
 // The bins where a row's prefixes may end (what the first k weigh is known to a
-// bin, so what p of it is lies in some range) and where its draw may fall; -1: none.
+// bin, so what p of it is lies in some range; tokens next to min_p's border may
+// lie in either of two bins) and where its draw may fall; -1: none.
 struct Found {
-    int32_t bin_k, low_p, high_p, bin_m, low_u, high_u, last;
+    int32_t bin_k, low_p, high_p, low_m, high_m, low_u, high_u, last;
     __device__ __forceinline__ bool wanted(int b) const {
-        return b == bin_k || (b >= low_p && b <= high_p) || b == bin_m || (b >= low_u && b <= high_u);
+        return b == bin_k || (b >= low_p && b <= high_p) || (b >= low_m && b <= high_m) || (b >= low_u && b <= high_u);
     }
 };
 
@@ -357,7 +365,7 @@ __device__ __forceinline__ Found find_bins(Shared<kThreads>& S, const Rules& R, 
     count[0] = before_in_wave(my_c, all_c);
     weight[0] = before_in_wave(my_w, all_w);
     if ((t & 63) == 0) S.wave_count[wave] = all_c, S.wave_weight[wave] = all_w;
-    if (t < 6) S.found[t] = -1, S.found_low[t] = S.found_high[t] = 0.0;
+    if (t < 7) S.found[t] = -1, S.found_low[t] = S.found_high[t] = 0.0;
     __syncthreads();
     int32_t total_c = 0;
     double base = 0.0, total = 0.0;
@@ -378,15 +386,20 @@ __device__ __forceinline__ Found find_bins(Shared<kThreads>& S, const Rules& R, 
     }
     if (kAll && t == 0) to.count[kBins] = total_c, to.weight[kBins] = total;
     auto mark = [&](int i, int j) { S.found[i] = t * kEach + j, S.found_low[i] = weight[j], S.found_high[i] = weight[j + 1]; };
-    const int m = R.min_t < kBins ? static_cast<int>(R.min_t) : -1;
+    Found f;
+    f.low_m = 0, f.high_m = -1;
+    if (R.min_t < kBins) {
+        f.low_m = R.min_t > kStray ? static_cast<int>(R.min_t - kStray) : 0;
+        f.high_m = R.min_t + kStray < kBins ? static_cast<int>(R.min_t + kStray) : kBins - 1;
+    }
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
         if (R.k < total_c && count[j] < R.k && R.k <= count[j + 1]) mark(0, j);
-        if (t * kEach + j == m) mark(3, j);
+        if (t * kEach + j == f.low_m) mark(3, j);
+        if (t * kEach + j == f.high_m) mark(6, j);
     }
     __syncthreads();
-    Found f;
-    f.bin_k = S.found[0], f.bin_m = m;
+    f.bin_k = S.found[0];
     double low = total, high = total;  // that the kept tokens weigh
     if (f.bin_k >= 0) low = S.found_low[0], high = S.found_high[0];
     if (R.p < 1.0) {
@@ -404,10 +417,10 @@ __device__ __forceinline__ Found find_bins(Shared<kThreads>& S, const Rules& R, 
         low = fmin(low, f.low_p >= 0 ? S.found_low[1] : 0.0), high = fmin(high, S.found_high[2]);
         end = f.high_p < end ? f.high_p : end;
     }
-    if (m >= 0) {
-        low = fmin(low, S.found_low[3]), high = fmin(high, S.found_high[3]);
-        if (m > end) f.bin_m = -1;  // min_p ends no prefix
-        else end = m;
+    if (f.high_m >= 0) {
+        low = fmin(low, S.found_low[3]), high = fmin(high, S.found_high[6]);
+        if (f.low_m > end) f.high_m = -1;  // min_p ends no prefix
+        else end = f.high_m < end ? f.high_m : end;
     }
     const double x = R.u * low, y = R.u * high;
 #pragma unroll
@@ -420,7 +433,7 @@ __device__ __forceinline__ Found find_bins(Shared<kThreads>& S, const Rules& R, 
     f.high_u = S.found[5] < 0 ? end : S.found[5];
     f.last = f.bin_k > f.high_p ? f.bin_k : f.high_p;
     f.last = f.high_u > f.last ? f.high_u : f.last;
-    f.last = f.bin_m > f.last ? f.bin_m : f.last;
+    f.last = f.high_m > f.last ? f.high_m : f.last;
     if (!kAll && to.count != nullptr) {
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
@@ -449,7 +462,7 @@ __device__ __forceinline__ void gather(Shared<kThreads>& S, const typename L::El
     add(f.low_u, f.high_u);
     if (f.high_p >= 0) add(f.low_p < 0 ? 0 : f.low_p, f.high_p);
     if (f.bin_k >= 0) add(f.bin_k, f.bin_k);
-    if (f.bin_m >= 0) add(f.bin_m, f.bin_m);
+    if (f.high_m >= 0) add(f.low_m, f.high_m);
     auto take = [&](auto number) {
         constexpr int kSpans = decltype(number)::value;
         auto test = [&](const auto& x) { return spans.template any<kSpans>(x); };
@@ -506,7 +519,7 @@ __device__ __forceinline__ Equals narrow(const SampleArgs& A, Shared<kThreads>& 
             const Place t = P.of(v);
             const uint32_t key = key_of(v);
             if (t.t < kBins && t.bin() == bin && key >= low && key <= high)
-                atomicAdd(reinterpret_cast<unsigned long long*>(&S.words[(high - key) >> shift]), word_of(t));
+                atomicAdd(reinterpret_cast<unsigned long long*>(&S.words[(high - key) >> shift]), word_of(t.f));
         });
         __syncthreads();
         // The parts' sums before each, by one thread after the other: a part's
@@ -583,7 +596,7 @@ __device__ __forceinline__ int32_t index_of(const SampleArgs& A, Shared<kThreads
 template <typename L, int kThreads>
 __device__ __forceinline__ void resolve_large(const SampleArgs& A, Shared<kThreads>& S, const Sums& B, const typename L::Element* row, const Places<L>& P, const Rules& R,
                               const Found& f, int32_t& token, double& weight, double& kept) {
-    const int bin_k = f.bin_k, bin_m = f.bin_m;
+    const int bin_k = f.bin_k;
     int32_t most = B.count[kBins];
     kept = B.weight[kBins];
     // The bin where a weight is reached (weight before < x <= with it) or passed (<=, <).
@@ -613,20 +626,24 @@ __device__ __forceinline__ void resolve_large(const SampleArgs& A, Shared<kThrea
             if (e.count + static_cast<int32_t>(n) < most) most = e.count + static_cast<int32_t>(n), kept = e.weight + n * e.each;
         }
     }
-    if (bin_m >= 0 && B.count[bin_m] < most) {
-        // The tokens of the bin that weigh enough.
-        __syncthreads();
-        if (threadIdx.x == 0) S.inside = 0;
-        __syncthreads();
-        uint64_t mine = 0;
-        each_logit<L>(row, A.vocab, threadIdx.x, kThreads, [&](int, float v) {
-            const Place t = P.of(v);
-            if (t.t < kBins && t.bin() == bin_m && t.exact() <= R.min_t) mine += word_of(t);
-        });
-        if (mine != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&S.inside), mine);
-        __syncthreads();
-        const int32_t n = B.count[bin_m] + count_of(S.inside);
-        if (n < most) most = n, kept = B.weight[bin_m] + static_cast<double>(units_of(S.inside)) * S.octave.unit(bin_m);
+    if (f.high_m >= 0 && B.count[f.low_m] < most) {
+        // The tokens of its bins that weigh enough.
+        int32_t n = B.count[f.low_m];
+        double with = B.weight[f.low_m];
+        for (int bin = f.low_m; bin <= f.high_m; ++bin) {
+            __syncthreads();
+            if (threadIdx.x == 0) S.inside = 0;
+            __syncthreads();
+            uint64_t mine = 0;
+            each_logit<L>(row, A.vocab, threadIdx.x, kThreads, [&](int, float v) {
+                const Place t = P.of(v);
+                if (t.t < kBins && t.bin() == bin && t.exact() <= R.min_t) mine += word_of(t.f);
+            });
+            if (mine != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&S.inside), mine);
+            __syncthreads();
+            n += count_of(S.inside), with += static_cast<double>(units_of(S.inside)) * S.octave.unit(bin);
+        }
+        if (n < most) most = n, kept = with;
     }
     const double x = R.u * kept;
     int b = find(x, true);
@@ -673,12 +690,13 @@ __device__ __forceinline__ Places<L> places_of(uint64_t top, const Rules& R) {
 // long). Without top-p nothing asks for tokens that weigh less than min_p.
 template <typename L>
 __device__ __forceinline__ void fill_bins(const typename L::Element* row, int n, int thread, int threads, const Places<L>& P, const Rules& R, uint64_t* bins) {
-    const float end = R.p < 1.0 || !(R.min_t < kBins - 1) ? kBins : static_cast<float>(static_cast<int>(R.min_t) + 1);
+    const float end = R.p < 1.0 || !(R.min_t < kBins - 1) ? kBins : static_cast<float>(static_cast<int>(R.min_t + kStray) + 1);
     const int nowhere = kBins + (threadIdx.x & 63);
     auto fill = [&](auto place_of) {
         each_logit<L>(row, n, thread, threads, [&](int, float x) {
             const Place p = place_of(x);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&bins[p.t < end ? p.bin() : nowhere]), word_of(p));
+            const bool in = p.t < end;  // (f may be any number where not, and none that an integer holds)
+            atomicAdd(reinterpret_cast<unsigned long long*>(&bins[in ? p.bin() : nowhere]), word_of(in ? p.f : 0.0f));
         });
     };
     if (P.endless) fill([&](float x) { return P.of(x); });
@@ -701,7 +719,7 @@ template <bool kWave, int kMine, typename L, int kThreads>
 __device__ __forceinline__ void finish_as(Shared<kThreads>& S, const Sums& B, uint64_t* sums, const Places<L>& P, const Rules& R, int n, const Found& f, double& kept) {
     const int t = threadIdx.x, wave = t >> 6;
     const int32_t all = B.count[kBins];
-    const int bin_k = f.bin_k, bin_m = f.bin_m;
+    const int bin_k = f.bin_k;
     auto sync = [] { sync_as<kWave>(); };
     // Each token's bin, weight and sums before it in its bin.
     int bin_of[kMine];
@@ -718,7 +736,7 @@ __device__ __forceinline__ void finish_as(Shared<kThreads>& S, const Sums& B, ui
         if (i >= n) continue;
         const Place place = P.of(of_key(~static_cast<uint32_t>(S.words[i] >> 32)));
         bin_of[j] = place.bin(), weighs[j] = place.exact() <= R.min_t;
-        w[j] = kUnits - lack_in_bin(place.f);
+        w[j] = kMostUnits - lack_in_bin(place.f);
         if (bin_of[j] != previous) start = i;
         first[j] = start, previous = bin_of[j];
         mine += w[j];
@@ -776,17 +794,17 @@ __device__ __forceinline__ void finish_as(Shared<kThreads>& S, const Sums& B, ui
         for (int j = 0; j < kMine; ++j)
             if (before[j] < x && x <= with[j]) S.end_count[1] = rank[j] + 1, S.end_weight[1] = with[j];
     }
-    if (bin_m >= 0) {
-        if (t == 0) S.found[2] = B.count[bin_m];
+    if (f.high_m >= 0) {
+        if (t == 0) S.found[2] = B.count[f.low_m];
         sync();
 #pragma unroll
         for (int j = 0; j < kMine; ++j)
-            if (bin_of[j] == bin_m && weighs[j]) atomicMax(&S.found[2], rank[j] + 1);
+            if (bin_of[j] >= f.low_m && bin_of[j] <= f.high_m && weighs[j]) atomicMax(&S.found[2], rank[j] + 1);
         sync();
-        if (t == 0 && S.found[2] == B.count[bin_m]) S.end_count[2] = S.found[2], S.end_weight[2] = B.weight[bin_m];
+        if (t == 0 && S.found[2] == B.count[f.low_m]) S.end_count[2] = S.found[2], S.end_weight[2] = B.weight[f.low_m];
 #pragma unroll
         for (int j = 0; j < kMine; ++j)
-            if (bin_of[j] == bin_m && rank[j] + 1 == S.found[2]) S.end_count[2] = S.found[2], S.end_weight[2] = with[j];
+            if (bin_of[j] >= f.low_m && bin_of[j] <= f.high_m && rank[j] + 1 == S.found[2]) S.end_count[2] = S.found[2], S.end_weight[2] = with[j];
     }
     if (t == 0) S.found[3] = 0;
     sync();
