@@ -41,6 +41,10 @@ _PROBLEMS = ((1, "too few free pages"), (2, "positions past a sequence's pages o
              (4, "a slot, page, source or number of rows that does not exist"))
 
 
+# What steps use of the cache's state is handed on by address.
+_TENSORS = frozenset(("pool", "page_table", "lengths", "held", "refs", "status", "scales"))
+
+
 def _int32(x: torch.Tensor, name: str, shape: tuple, index: int) -> int:
     if x.dtype is not torch.int32 or x.get_device() != index or x.shape != shape or not x.is_contiguous():
         raise ValueError("%s must be a contiguous int32 %s tensor on cuda:%d" % (name, list(shape), index))
@@ -61,8 +65,10 @@ class PagedKVCache:
                 in 8 bits alone
 
     ``allocate`` makes an empty one. The tensors are used in place and are the
-    cache's whole state. ``seqs``, ``src`` and ``dst`` below are slots: int32
-    tensors on the GPU of at most 8192 entries."""
+    cache's whole state. Another tensor of the same shape and type may be put
+    in an attribute's place: every step uses it from then on (captured graphs
+    go on with the one they were captured with). ``seqs``, ``src`` and ``dst``
+    below are slots: int32 tensors on the GPU of at most 8192 entries."""
 
     scales: torch.Tensor | None = None
 
@@ -93,7 +99,8 @@ class PagedKVCache:
             self._scales_at = scales.data_ptr()
         elif scales is not None:
             raise ValueError("scales belong to a pool of float8_e4m3fn")
-        self.scales = scales
+        self.pool, self.page_table, self.lengths, self.held, self.refs, self.status, self.scales = \
+            pool, page_table, lengths, held, refs, status, scales
         self._cache = _native.AimgCache(
             pool.data_ptr(), _int32(page_table, "page_table", (self.max_seqs, self.max_pages), index),
             _int32(lengths, "lengths", (self.max_seqs,), index), _int32(held, "held", (self.max_seqs,), index),
@@ -109,13 +116,43 @@ class PagedKVCache:
             self._described.append((pages, None if scales is None else _native.AimgPageScales(
                 at[0].data_ptr(), at[1].data_ptr(), at.stride(1), at.stride(2))))
         self._lib = _native.lib()
-        self.pool, self.page_table, self.lengths, self.held, self.refs, self.status = \
-            pool, page_table, lengths, held, refs, status
         nbytes = ctypes.c_size_t(0)
         _native.check(self._lib.aimg_cache_compact_workspace_nbytes(self._cache, ctypes.byref(nbytes)))
         # Scratch memory of compact, of one size and so kept as long as the cache: calls change one cache and run in order.
         self._compact_work = torch.empty(nbytes.value, dtype=torch.uint8, device=self.device)
         self._used = torch.empty((), dtype=torch.int32, device=self.device)
+
+    def __setattr__(self, name: str, value) -> None:
+        if name in _TENSORS and "_described" in self.__dict__:
+            self._replace(name, value)
+        object.__setattr__(self, name, value)
+
+    def _replace(self, name: str, x) -> None:
+        """Checks a tensor that takes an attribute's place, and moves the addresses that the steps hand on to it."""
+        old = self.__dict__[name]
+        if old is None or not isinstance(x, torch.Tensor) or x.shape != old.shape or x.dtype is not old.dtype or x.get_device() != self._index \
+                or not x.is_contiguous() or x.data_ptr() % (16 if name == "pool" else 4):
+            raise ValueError("%s must %s" % (name, "stay None: the pool has 16 bits" if old is None else "stay a contiguous %s %s tensor on %s%s" % (
+                old.dtype, list(old.shape), self.device, ", its memory 16-byte aligned" if name == "pool" else "")))
+        at = x.data_ptr()
+        # (Descriptors of this cache's own: a copy of the object shares the ones it was copied with.)
+        if name == "scales":
+            self._scales_at = at
+        else:
+            self._cache = _native.AimgCache.from_buffer_copy(self._cache)
+            setattr(self._cache, name, at)
+        if name in ("held", "refs", "status"):
+            return
+        described = [(_native.AimgPages.from_buffer_copy(pages), None if scales is None else _native.AimgPageScales.from_buffer_copy(scales))
+                     for pages, scales in self._described]
+        for layer, (pages, scales) in enumerate(described):
+            if name in ("page_table", "lengths"):
+                setattr(pages, name, at)
+            else:
+                one = pages if name == "pool" else scales
+                one.k = at + layer * x.stride(0) * x.element_size()
+                one.v = one.k + x.stride(1) * x.element_size()
+        self._described = described
 
     @classmethod
     def allocate(cls, n_layers: int, n_pages: int, page_size: int, kv_heads: int, dim: int, max_seqs: int, max_pages: int,
