@@ -271,12 +271,13 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         scales = _page_scales(k_scales, v_scales, pages, k_pages.get_device())
     elif k_scales is not None or v_scales is not None:
         raise ValueError("k_scales and v_scales belong to pages of float8_e4m3fn")
-    return attend(q, query, pages, scales, k_pages.dtype, k_pages.get_device(), seqs, draft_offsets, masks, max_drafts, max_context, scale, out, lse)
+    return attend(q, query, pages, scales, k_pages.dtype, k_pages.get_device(), seqs, draft_offsets, masks,
+                  max_drafts=max_drafts, max_context=max_context, scale=scale, out=out, lse=lse)
 
 
 def attend(q: torch.Tensor, query: tuple[_native.AimgHeads, int, int], pages: _native.AimgPages,
            scales: _native.AimgPageScales | None, dtype: torch.dtype, device: int, seqs: torch.Tensor, draft_offsets: torch.Tensor,
-           masks: torch.Tensor | None = None, max_drafts: int = 0, max_context: int | None = None, scale: float | None = None,
+           masks: torch.Tensor | None = None, *, max_drafts: int, max_context: int | None = None, scale: float | None = None,
            out: torch.Tensor | None = None, lse: torch.Tensor | None = None) -> torch.Tensor:
     """tree_attention over described pages of this type on this GPU, for a
     described q: a cache describes its layers once."""

@@ -326,7 +326,7 @@ class PagedKVCache:
 
     def attend(self, layer: int, q: torch.Tensor, seqs: torch.Tensor, draft_offsets: torch.Tensor,
                masks: torch.Tensor | None = None, **options) -> torch.Tensor:
-        """tree_attention of q over one layer of this cache."""
+        """tree_attention of q over one layer of this cache; options are its keyword arguments (max_drafts is needed)."""
         if not -self.n_layers <= layer < self.n_layers:
             raise IndexError("layer %d is out of range for %d layers" % (layer, self.n_layers))
         pages, scales = self._described[layer]
