@@ -6,8 +6,9 @@ The reference leaves attention to the model's own forward pass
 products a program runs between the q/k/v projections whose weights it decodes
 and the output projection. Elements are bf16 or fp16; scores, softmax
 statistics and sums are fp32. Work is ordered on the current stream and nothing
-here synchronises. There is no backward pass: inputs that require a gradient are
-refused while gradients are recorded.
+here synchronises. There is no backward pass and none in forward mode: inputs
+that require a gradient are refused while gradients are recorded, and those with
+a tangent.
 """
 from __future__ import annotations
 
@@ -16,6 +17,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -33,9 +35,13 @@ _BLOCK = 16  # positions that share a scale in a cache of 8 bits
 # device, shapes and strides taken apart once, descriptors built once a call.
 
 def forward_only(x: torch.Tensor, name: str) -> None:
-    """Refuses a tensor whose gradient autograd would expect."""
+    """Refuses a tensor whose gradient, or derivative in forward mode, autograd would expect."""
     if x.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("%s requires a gradient, and this call has no backward pass: detach it, or call under torch.no_grad()" % name)
+    # (The level is asked first, for it costs nothing where there is none.)
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(x).tangent is not None:
+        raise RuntimeError("%s has a tangent, and this call has no derivative in forward mode: pass its primal, or call under "
+                           "torch.inference_mode()" % name)
 
 
 def _heads(x: torch.Tensor, name: str, dtype: torch.dtype, index: int, unit: int = 8) -> _native.AimgHeads:

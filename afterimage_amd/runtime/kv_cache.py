@@ -195,8 +195,7 @@ class PagedKVCache:
         at = x.data_ptr()
         if one != 1 or (row | head) % 8 or at % 16:
             raise ValueError("%s must be contiguous in its last dimension, its rows and heads on 16-byte boundaries" % name)
-        if x.requires_grad:
-            forward_only(x, name)
+        forward_only(x, name)
         return _native.AimgHeads(at, shape[0], row, head, heads, self.dim)
 
     def _rows(self, x: torch.Tensor, name: str) -> _native.AimgHeads:
@@ -269,9 +268,8 @@ class PagedKVCache:
             raise ValueError("cos must be a contiguous fp32 [positions, up to %d] tensor on cuda:%d" % (self.dim // 2, index))
         if sin.shape != table or sin.dtype is not torch.float32 or sin.get_device() != index or not sin.is_contiguous():
             raise ValueError("sin must have cos' shape, type and device")
-        if cos.requires_grad or sin.requires_grad:
-            forward_only(cos, "cos")
-            forward_only(sin, "sin")
+        forward_only(cos, "cos")
+        forward_only(sin, "sin")
         at, n = self._seqs(seqs)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
