@@ -1091,14 +1091,26 @@ constexpr int64_t kWideBytes = 48 << 10;
 
 // Workgroups a row; 0: one, in one launch. Four launches, and bins that each
 // workgroup looks at for itself, pay where rows are long and do not fill the
-// chip. Of 151936 logits, with all kept and with top_p 0.9, by one workgroup and
-// by several: 1 row 33 and 42 us, 22 and 27 by 16; 16 rows 44 and 46, 34 and 34 by
-// 8; 48 rows 43 and 49, 42 and 44 by 4; 64 rows 45 and 52, 45 and 59 by 4, in fp32
-// 56 and 66, 51 and 55; with settings of its own for each row 55 by one and 46 by
-// 4; 96 rows in fp32 60 and 67, 60 and 65. Of 100000: 1 row 27 and 33, 21 and 27;
-// 37 rows 34 and 37, 35 and 37. Of 65536, 1 row: 22 and 26, 21 and 25.
-int slices_of(int64_t n_rows, int vocab) {
-    if (n_rows < 1 || n_rows > 64 || vocab < 90000) return 0;
+// chip. What a row costs goes by its tokens and, for a quarter of it in 16 bits
+// and half in 32, by its bytes; that is compared with a number that rises with
+// the rows, twice as fast where four workgroups a row are more than the 256 CUs.
+// Several workgroups' time by one's, for rows with all kept, top_p 0.9, top-k 50
+// and top_p 0.95, and settings of their own (us by one, with all kept):
+//   bf16, 65536 logits: 1 row 0.91 - 1.0 (25), 12 rows 1.02 - 1.08 (28), 64 1.12 - 1.21 (30)
+//   bf16, 90112: 8 rows 0.87 - 0.94 (31), 32 0.95 - 1.03 (34), 64 1.03 - 1.10 (36)
+//   bf16, 151936: 1 row 0.61 - 0.65 (38), 64 0.87 - 1.04 (49), 72 1.00 - 1.18 (49)
+//   bf16, 262144: 64 rows 0.76 - 0.89 (74), 96 0.87 - 1.03 (77), 192 1.16 - 1.24 (86)
+//   fp32, 50001: 1 row 0.95 - 1.01 (22), 8 1.02 - 1.06 (24)
+//   fp32, 65536: 8 rows 0.94 - 0.98 (29), 40 1.07 - 1.14 (31)
+//   fp32, 151936: 64 rows 0.83 - 0.93 (61), 80 0.92 - 0.95 (62), 128 1.04 - 1.13 (63)
+//   fp32, 262144: 128 rows 0.93 - 1.01 (113), 192 1.08 - 1.11 (128)
+// Of 994 such measurements, 65536 to 262144 logits (50001 in fp32) and 1 to 256 rows, it
+// chooses what takes over 5% longer in 12, 18% at most.
+constexpr int64_t kDealtLeast = 90000, kDealtRow = 640, kDealtManyRow = 2700, kOneEachRows = 64;
+
+int slices_of(int64_t n_rows, int vocab, int element_bytes) {
+    const int64_t cost = static_cast<int64_t>(vocab) * (8 + element_bytes) / 8;
+    if (n_rows < 1 || cost < (n_rows <= kOneEachRows ? kDealtLeast + kDealtRow * n_rows : kDealtManyRow * n_rows)) return 0;
     const int64_t most = (vocab + 8191) / 8192, n = 256 / n_rows;
     return static_cast<int>(n < 4 ? 4 : n < most ? n : most);
 }
@@ -1143,7 +1155,7 @@ extern "C" int aimg_sample_workspace_nbytes(int64_t n_rows, int vocab, size_t* n
     const int rc = aimg::check_sample(n_rows, vocab);
     if (rc != AIMG_OK) return rc;
     aimg::Slices w{};
-    w.n = aimg::slices_of(n_rows, vocab);
+    w.n = aimg::slices_of(n_rows, vocab, 4);  // whatever the logits' type: more are dealt out in 32 bits, to as many workgroups
     *nbytes = w.n == 0 ? 0 : aimg::slices_at(w, nullptr, n_rows);
     return AIMG_OK;
 }
@@ -1163,7 +1175,7 @@ extern "C" int aimg_sample(const void* logits, int64_t n_rows, int64_t row_strid
     if (reinterpret_cast<uintptr_t>(logits) % (type == AIMG_FP32 ? 4 : 2) != 0 || reinterpret_cast<uintptr_t>(tokens) % 8 != 0)
         return fail(AIMG_ERR_UNSUPPORTED, "sample: logits and tokens must be aligned to their elements");
     aimg::Slices w{};
-    w.n = aimg::slices_of(n_rows, vocab);
+    w.n = aimg::slices_of(n_rows, vocab, type == AIMG_FP32 ? 4 : 2);
     if (w.n > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 8 != 0 ||
                     workspace_nbytes < aimg::slices_at(w, static_cast<char*>(workspace), n_rows)))
         return fail(AIMG_ERR_INVALID_ARGUMENT, "the workspace is null, misaligned or below aimg_sample_workspace_nbytes");

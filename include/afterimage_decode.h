@@ -571,8 +571,9 @@ typedef struct aimg_sampling {
  * 2^-64 of the largest (at any temperature those of logits 2^128 below it) count
  * as nothing, the others are sums of 2^-26 of themselves, in integers and
  * doubles: results do not vary between calls.
- * aimg_sample_workspace_nbytes gives the device scratch memory a call needs
- * (8-byte aligned; 0 for many rows or few logits): few rows are dealt out.
+ * aimg_sample_workspace_nbytes gives the device scratch memory that a call of
+ * these sizes needs for logits of any type (8-byte aligned; 0 for many rows or
+ * few logits): few long rows are dealt out to several workgroups each.
  */
 int aimg_sample_workspace_nbytes(int64_t n_rows, int vocab, size_t* nbytes);
 int aimg_sample(const void* logits, int64_t n_rows, int64_t row_stride, int vocab, int type, const float* uniforms,
