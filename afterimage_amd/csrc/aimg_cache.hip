@@ -21,7 +21,8 @@
 // smallest power of two, 2^-100 to 2^119, that brings the block's largest
 // element to at most 448, so the product is exact in bf16, and a block that
 // takes further rows is formed anew from what it stands for: where its scale
-// rises, only elements that fall below 2^-6 scales are rounded again.
+// rises, only elements that fall below 2^-6 scales are rounded again (and stay
+// so where the rows that raised it were drafts, and rejected).
 #include <hip/hip_runtime.h>
 
 #include <cmath>

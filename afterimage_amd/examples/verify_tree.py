@@ -14,8 +14,11 @@ verifies them in one target pass):
     its parent's token by the same rule and random number, so that what is
     accepted follows the model's distribution.
 
-Both branches hold the same tokens afterwards. Queries and keys may be turned by
-their positions on their way into the cache, which may hold 16 bits or 8. Run as
+Both branches hold the same tokens afterwards where the cache has 16 bits and no
+two logits are nearer than the passes' roundings. Queries and keys may be turned
+by their positions on their way into the cache, which may hold 16 bits or 8; in 8
+its 16 positions share a scale, so rows are rounded with the drafts beside them,
+and the branches may part. Run as
 ``python -m afterimage_amd.examples.verify_tree``: greedily with a cache in 16
 bits; with ``--sampled``, with sampling, rotation and a cache in 8.
 """

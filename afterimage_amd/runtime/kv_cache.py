@@ -21,7 +21,9 @@ values apart, says what they stand for (value * scale). Scales are powers of
 two, the smallest that bring the largest of the 16 positions' elements to at
 most 448. Rows are rounded to nearest as they come in; where later rows raise
 the scale of their 16 positions, earlier elements below 2^-6 of it are rounded
-again. Infinities become NaN.
+again, by at most 2^-10 of it. Drafted rows are such rows, and what they round
+stays rounded where they are rejected: what a sequence holds in 8 bits depends,
+by that much, on what was drafted. Infinities become NaN.
 """
 from __future__ import annotations
 

@@ -439,7 +439,9 @@ int aimg_cache_append(const aimg_cache* cache, int layer, const aimg_heads* k, c
  * at most 448 (past that at the highest one, elements are held as 448 of it).
  * Infinities and NaN are held as NaN and do not count. A block that a call adds
  * rows to is formed anew from what its rows below the length stand for and
- * those, rounded to nearest even. Where `scales` is an argument of a call for
+ * those, rounded to nearest even: where its factor rises, elements of earlier
+ * rows below 2^-6 of it change by up to 2^-10 of it, and stay so if the rows
+ * are drafts that no commit accepts. Where `scales` is an argument of a call for
  * either, NULL means a cache in 16 bits.
  */
 
