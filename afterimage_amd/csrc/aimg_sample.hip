@@ -252,10 +252,12 @@ struct Spans {
 
 // What 2^(-f / 64) lacks to kMostUnits, in 2^-26 and rounded, for f in [-kStray,
 // 1 + kStray], where it is above 0: the series of 1 - 2^(-f / 64) in g = f ln 2 / 64 < 0.011,
-// whose fourth term is below 2^-30.
+// whose fourth term is below 2^-30. The sum with 2^23 is the rounded number in
+// its last 23 bits (of an f that is anywhere else or NaN, some number).
 __device__ __forceinline__ uint32_t lack_in_bin(float f) {
     constexpr float g = 0.6931471805599453f / kPerOctave;
-    return static_cast<uint32_t>(fmaf(f, fmaf(f, fmaf(f, g * g * g / 6.0f * kUnits, -g * g / 2.0f * kUnits), g * kUnits), kMostUnits - kUnits + 0.5f));
+    const float x = fmaf(f, fmaf(f, fmaf(f, g * g * g / 6.0f * kUnits, -g * g / 2.0f * kUnits), g * kUnits), 0x1p23f + (kMostUnits - kUnits));
+    return __float_as_uint(x) & 0x7FFFFFu;
 }
 
 __device__ __forceinline__ uint64_t word_of(float f) { return uint64_t{1} << kCountShift | lack_in_bin(f); }
@@ -695,8 +697,7 @@ __device__ __forceinline__ void fill_bins(const typename L::Element* row, int n,
     auto fill = [&](auto place_of) {
         each_logit<L>(row, n, thread, threads, [&](int, float x) {
             const Place p = place_of(x);
-            const bool in = p.t < end;  // (f may be any number where not, and none that an integer holds)
-            atomicAdd(reinterpret_cast<unsigned long long*>(&bins[in ? p.bin() : nowhere]), word_of(in ? p.f : 0.0f));
+            atomicAdd(reinterpret_cast<unsigned long long*>(&bins[p.t < end ? p.bin() : nowhere]), word_of(p.f));
         });
     };
     if (P.endless) fill([&](float x) { return P.of(x); });
