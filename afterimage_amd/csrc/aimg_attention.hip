@@ -983,11 +983,15 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeArgs& A, const Drafted& 
 // by lane for pages of 16, 54 trees over 139-2238 positions took 155 us.)
 // k8: a cache in 8 bits, whose codes become elements in every wave that reads
 // them. Each wave brings its tile's scales along, a load of 4 bytes a lane into
-// a place of its own. Half the bytes leave the matrix and vector instructions of
-// shared tiles to bound it: 16 trees of 4-16 tokens over 9000-65000 positions
-// 313 us, 3.8 TB/s; 64 single tokens over 1900-8100 113 us, 4.8 TB/s. (Elements
+// a place of its own. 64 single tokens over 1900-8100 positions 113 us, 4.8 TB/s.
+// Shared tiles, 16 trees of 4-16 tokens over 9000-65000 313 us, 3.8 TB/s: matrix
+// units 19% and vector instructions 28% of the cycles, for the workgroups' rows
+// follow from the largest tree (128, 80 of them used) and of the waves, by their
+// keys, 48% hold rows of their sequence; the others load and wait. (Elements
 // formed once for all waves, in LDS, between two barriers: 391 us, not 330 with
 // the same parts; a lane's places in its loads worked out for every tile: 352.)
+// Of dim 64, 96 and 256 (16 heads of 4), 64 single tokens 4.9, 3.8 and 2.6 TB/s,
+// over 16 bits 4.7, 4.5 and 4.3.
 template <typename T, int DP, int QT, int NW, bool kShared, int kPages, bool k8>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DP <= 128 ? 2 : 1) void tree_kernel(const TreeArgs A) {
     typedef State<T, DP, QT, k8> St;
@@ -1375,7 +1379,11 @@ constexpr int kMinChunk = 512;
 // (shared tiles, 16 trees over 9000-65000: 340 us, 427 with 8192).
 constexpr int kMaxChunk = 8192;
 constexpr int kMaxSharedChunk = 4096;
-constexpr int kMaxSharedChunk8 = 2048;  // of a cache in 8 bits: 16 trees over 9000-65000 313 us, 330 with 4096, 322 with 1024
+// Of a cache in 8 bits: 16 trees over 9000-65000 313 us, 330 with 4096, 322 with
+// 1024. Of 48 shapes (bf16 and fp16, dims 64 to 256, 1 to 48 trees of up to 16 to 64
+// tokens over 4000 to 65000 positions) it takes 2% longer than the best of 1024 to
+// 8192 on average and 22% at most (dim 64); 1024 5% and 34%, 4096 7% and 61%.
+constexpr int kMaxSharedChunk8 = 2048;
 constexpr int kSlots = 256;         // workgroups of dealt-out keys that run at a time, one a CU
 constexpr int kFewParts = 16;       // at most so many are joined by DP / 4 threads a row
 // Workgroups of shared tiles, were all sequences the longest. It sets the keys

@@ -282,7 +282,7 @@ struct TurnArgs {
 // How a row's pairs lie in its 16-byte pieces.
 constexpr int kHalves = 0;  // element i goes with i + half, 8 elements with 8 elements: half % 8 == 0
 constexpr int kPairs = 1;   // 2 i goes with 2 i + 1, in one piece: half % 4 == 0
-constexpr int kAny = 2;     // either, for every half: element by element
+constexpr int kAny = 2;     // either, for every half: element by element (8192 rows of 40 and 2 * 8 heads of 128, half 50, 164-207 us; pieces, half 64, 37-41)
 
 // Rows of a call in place of offsets that may be any numbers.
 __device__ __forceinline__ int32_t row_bound(const int32_t* offsets, int b, int32_t n_rows) {

@@ -18,11 +18,12 @@
 // below 2^-64 of the largest weigh nothing.
 //
 // A row is read three times. 256 rows of 151936 logits of 16 bits (78 MB a time,
-// 15 us at a copy's rate): 56 us. The largest takes HBM's time for them; the bins
-// (some twenty instructions and an atomic in LDS a token) and the gather are
-// instructions, 42% of a SIMD's cycles, LDS 25%; the steps between them wait for
-// each other. 64 rows with settings of their own, by several workgroups each: 46
-// us; one row 24.
+// 15 us at a copy's rate): 57 us, in which 234 MB come past the L2, 4.1 TB/s, four
+// fifths of a copy's rate. The bins' some twenty instructions and an atomic in LDS
+// a token go beside that (42% of a SIMD's cycles, LDS 25%), and as a CU's LDS
+// holds one workgroup, no other row's loads go beside a row's barriers. 64 rows
+// with settings of their own, by several workgroups each: 46 to 57 us, by how many
+// tokens the settings ask for; one row 24; temperature 0 15 for 256 rows.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -494,7 +495,10 @@ __device__ __forceinline__ void gather(Shared<kThreads>& S, const typename L::El
 // How a prefix ends, or which token is drawn, where a bin holds more tokens
 // than are gathered (equal logits by the thousand, very high temperatures): the
 // bin's keys are binned again, 4096 at a time, until one key is left. It ends
-// after at most three passes over the row.
+// after at most three passes over the row, for each border and the draw, by one
+// workgroup. bf16 logits around 20 with a deviation of 1 do that, since some 7500
+// of 151936 are equal: 256 rows with all kept 306 us (around 0: 66), with top_p
+// 0.9 520 (103), 64 rows 266 (64), one 170-240 (29-43); with top-k 50 65 (53).
 struct Equals {
     uint32_t key;
     int32_t count, n;      // tokens before the equals, and the equals
@@ -934,8 +938,8 @@ __device__ __forceinline__ uint64_t largest_of_waves(Shared<kThreads>& S, uint64
     return top;
 }
 
-// Many rows, or few logits: a workgroup a row. 256 rows of 151936 56 us, 37 of
-// 50001 in fp32 24, one of 4096 13.
+// Many rows, or few logits: a workgroup a row. 256 rows of 151936 57 us, 37 of
+// 50001 in fp32 24.5, one of 4096 13.
 template <typename L, int kThreads>
 __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
     __shared__ Shared<kThreads> S;
@@ -961,7 +965,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleArgs A) {
 
 // Fewer rows: `n` workgroups a row, in four launches: the largest logit; the
 // bins; their tokens; by one workgroup, the draw. One row of 151936 in 19 slices
-// 3.2, 4.4, 12.1 and 5.4 us, 64 rows in 4 slices 8.6, 10.4, 17.8 and 10.7: from
+// 3.4, 4.3, 11.6 and 5.8 us, 64 rows in 4 slices 8.6, 10.4, 17.8 and 11.3: from
 // the gather on, sums over the bins and steps of a sort that wait for each
 // other, not HBM (0.06 and 4 us). (Fewer launches, where the last
 // workgroup of a row to come goes on with what the others wrote, need fences
