@@ -160,8 +160,10 @@ __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k &
 // in 32 bits goes into the rest, and so does what max - x loses, for fp32
 // logits: half a step of t (2^-13 below 4096) and 2^-24 of t for the difference's
 // rounding and the factor's each, less than kStray together, by which f may lie
-// outside [0, 1). (Of 16 bits, bf16 logits lose nothing unless 2^16 apart in
-// size and fp16 unless 2^13, and then 2^-24 of the difference at most.) Bins rise
+// outside [0, 1). (max - x loses nothing of bf16 logits unless their sizes are
+// 2^16 apart, nor of fp16 ones unless 2^13, and then 2^-24 of itself at most,
+// which weighs as much of (max - x) / T and is left: what takes it up would cost
+// five instructions a token, 256 rows of 151936 60.1 us, not 57.6.) Bins rise
 // as the logits fall, for both roundings keep the order; on which side of a
 // border between two bins a place this near to it lies, they do not say. An
 // infinite maximum leaves its equals alone at 0.
@@ -1096,12 +1098,12 @@ constexpr int64_t kWideBytes = 48 << 10;
 
 // Workgroups a row; 0: one, in one launch. Four launches, and bins that each
 // workgroup looks at for itself, pay where rows are long and do not fill the
-// chip. What a row costs goes by its tokens and, for a quarter of it in 16 bits
-// and half in 32, by its bytes; that is compared with a number that rises with
-// the rows, twice as fast where four workgroups a row are more than the 256 CUs.
+// chip. What a row costs goes by its tokens and an eighth of its bytes; that is
+// compared with a number that rises with the rows, and faster where four
+// workgroups a row are more than the 256 CUs.
 // Several workgroups' time by one's, for rows with all kept, top_p 0.9, top-k 50
 // and top_p 0.95, and settings of their own (us by one, with all kept):
-//   bf16, 65536 logits: 1 row 0.91 - 1.0 (25), 12 rows 1.02 - 1.08 (28), 64 1.12 - 1.21 (30)
+//   bf16, 65536 logits: 1 row 0.91 - 0.99 (23), 12 rows 1.02 - 1.08 (28), 64 1.12 - 1.21 (30)
 //   bf16, 90112: 8 rows 0.87 - 0.94 (31), 32 0.95 - 1.03 (34), 64 1.03 - 1.10 (36)
 //   bf16, 151936: 1 row 0.61 - 0.65 (38), 64 0.87 - 1.04 (49), 72 1.00 - 1.18 (49)
 //   bf16, 262144: 64 rows 0.76 - 0.89 (74), 96 0.87 - 1.03 (77), 192 1.16 - 1.24 (86)
@@ -1109,8 +1111,8 @@ constexpr int64_t kWideBytes = 48 << 10;
 //   fp32, 65536: 8 rows 0.94 - 0.98 (29), 40 1.07 - 1.14 (31)
 //   fp32, 151936: 64 rows 0.83 - 0.93 (61), 80 0.92 - 0.95 (62), 128 1.04 - 1.13 (63)
 //   fp32, 262144: 128 rows 0.93 - 1.01 (113), 192 1.08 - 1.11 (128)
-// Of 994 such measurements, 65536 to 262144 logits (50001 in fp32) and 1 to 256 rows, it
-// chooses what takes over 5% longer in 12, 18% at most.
+// Of 994 such measurements, of 50001 to 262144 logits and 1 to 256 rows, it chooses
+// what takes over 5% longer in 12, 11% at most.
 constexpr int64_t kDealtLeast = 90000, kDealtRow = 640, kDealtManyRow = 2700, kOneEachRows = 64;
 
 int slices_of(int64_t n_rows, int vocab, int element_bytes) {

@@ -572,7 +572,9 @@ typedef struct aimg_sampling {
  * NaN are no tokens; a row without any other gives -1 and -inf. Weights below
  * 2^-64 of the largest (at any temperature those of logits 2^128 below it) count
  * as nothing, the others are sums of 2^-26 of themselves, in integers and
- * doubles: results do not vary between calls.
+ * doubles: results do not vary between calls. (A bf16 logit 2^16 times smaller
+ * or larger in size than the largest, or an fp16 one 2^13 times, weighs besides
+ * by up to 2^-24 (max x - x) / temperature of itself more or less.)
  * aimg_sample_workspace_nbytes gives the device scratch memory that a call of
  * these sizes needs for logits of any type (8-byte aligned; 0 for many rows or
  * few logits): few long rows are dealt out to several workgroups each.
